@@ -54,6 +54,14 @@
  *                               in intent_quant_attention_reference() intent_quant_attention.py:56-84
  *                               (intent_quant.py:221-312), float32 K and V
  *   iak_fake_quant_blocks_workspace (no counterpart: sizes the optional split of long blocks)
+ *   iak_mx_append_tokens,       (no counterpart: the reference quantises whole blocks, intent_quant.py:221-312;
+ *   iak_mx_read_tokens           these write and read single tokens of a microscaled 4-bit cache)
+ *   iak_mx_attention,           (no counterpart: attention of one or several query tokens per sequence over
+ *   iak_mx_attention_workspace   that cache)
+ *   iak_grow_sequences,         (no counterpart: KVMemoryManager hands out pages on the host and shares none,
+ *   iak_fork_sequences,          kv_memory_manager.py:145-231; these keep page tables, lengths and reference
+ *   iak_free_sequences,          counts on the device)
+ *   iak_compact_pages, iak_copy_pages, iak_sequences_workspace, iak_compact_pages_workspace
  *   iak_status_string           (no counterpart: the reference raises ValueError/RuntimeError in Python)
  */
 #ifndef IAK_H
@@ -609,6 +617,159 @@ iak_status iak_fake_quant_blocks_workspace(const iak_fake_quant_blocks_args* arg
 
 iak_status iak_fake_quant_blocks(const iak_fake_quant_blocks_args* args, void* workspace, size_t workspace_bytes,
                                  void* stream);
+
+/*
+ * Microscaled 4-bit (MXFP4) token cache. Pages of 16 tokens of one KV head, as the
+ * decode's pools: codes [num_pages, 16, head_dim / 2] bytes (channel 2j in the low half of
+ * byte j; a code is sign << 3 | e2m1 magnitude 0, .5, 1, 1.5, 2, 3, 4, 6) and scale bytes
+ * [num_pages, 16, head_dim / 32], one per token and 32 channels:
+ *   value = code * 2^(clamp(scale, 104, 140) - 127);  scale 255: the block is NaN.
+ * The clamp (2^-23 .. 2^13) makes every value a float16 number, and whatever bytes lie in
+ * tokens that nobody wrote finite ones. head_dim 64 or 128, page_size 16.
+ *
+ * Row (b, h) of page_table [batch, num_kv_heads, table_width] lists its pages in token
+ * order; valid_tokens [batch, num_kv_heads] counts its tokens (clamped to 0 ..
+ * 16 * table_width). The newest n tokens of a sequence are its last: with q_lens [batch]
+ * (NULL: count for all; clamped to 0 .. count) token i < q_lens[b] is number
+ * valid_tokens[b, h] - q_lens[b] + i of row (b, h). Page ids outside [0, num_pages) hold
+ * no tokens.
+ */
+
+/* Write (append) or read the newest tokens: k, v [batch, count, num_kv_heads, head_dim]
+ * (dtype IAK_DTYPE_*), element strides, unit channel stride.
+ * Append rounds a block x of 32 channels as the microscaling standard does:
+ *   e = clamp(floor(log2(max|x|)) - 2, -23, 13), scale = e + 127,
+ *   code = round to nearest even of x / 2^e, at most 6; a block that holds an infinity or a
+ *   NaN: scale 255, codes 0.
+ * It writes bytes of the addressed tokens only; tokens without a page are left out. Two
+ * tokens that address one slot race. Read gives the values (exact in every dtype), and
+ * zeros for tokens without a page and for i >= q_lens[b]. */
+typedef struct {
+  int32_t batch, count, num_kv_heads, head_dim, page_size, table_width;
+  int64_t num_pages;
+  void* k; int64_t k_stride_b, k_stride_t, k_stride_h;
+  void* v; int64_t v_stride_b, v_stride_t, v_stride_h;
+  int32_t dtype;
+  const int32_t* page_table;
+  const int32_t* valid_tokens;
+  const int32_t* q_lens;
+  void* k_codes; void* k_scales; void* v_codes; void* v_scales;
+} iak_mx_tokens_args;
+
+iak_status iak_mx_append_tokens(const iak_mx_tokens_args* args, void* stream);
+iak_status iak_mx_read_tokens(const iak_mx_tokens_args* args, void* stream);
+
+/* Attention over the cache: q, out [batch, q_len, num_q_heads, head_dim] (element strides,
+ * unit inner stride). Query i < q_lens[b] (as above, q_len for count) of head h reads row
+ * (b, h / (num_q_heads / num_kv_heads)) and sees, with causal = 1, the tokens up to its own
+ * (numbers below valid_tokens - q_lens[b] + i + 1), else all of the row's:
+ *   out = softmax(sm_scale * q . k) v over them, 0 where there are none and for
+ *   i >= q_lens[b].
+ * A token with a NaN block makes every query that sees it NaN, as does a query that is
+ * not finite itself; tokens that a query does not see never reach it. Products run on the
+ * matrix cores in float16 (queries scaled by a power of two per row, so that neither range
+ * nor, for float16 and bfloat16 queries, bits are lost; K and V exact; weights rounded to
+ * 11 bits) with float32 sums; float32 queries and their weights are split in two (22 bits).
+ * splits: parts a row's tokens are divided into (0: automatic). The parts meet in the
+ * workspace (iak_mx_attention_workspace bytes, 16-byte aligned; 0: not needed); calls that
+ * share one on different streams race. */
+typedef struct {
+  int32_t batch, q_len, num_q_heads, num_kv_heads, head_dim, page_size, table_width;
+  int64_t num_pages;
+  const void* q; int32_t q_dtype; int64_t q_stride_b, q_stride_t, q_stride_h;
+  void* out; int32_t out_dtype; int64_t out_stride_b, out_stride_t, out_stride_h;
+  const int32_t* page_table;
+  const int32_t* valid_tokens;
+  const int32_t* q_lens;
+  const void* k_codes; const void* k_scales; const void* v_codes; const void* v_scales;
+  float sm_scale;
+  int32_t causal;
+  int32_t splits;
+} iak_mx_attention_args;
+
+iak_status iak_mx_attention_workspace(const iak_mx_attention_args* args, size_t* bytes);
+iak_status iak_mx_attention(const iak_mx_attention_args* args, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* One array with a row per page: page p is the row_bytes bytes at base + p * row_bytes. */
+typedef struct {
+  void* base;
+  int64_t row_bytes;
+} iak_page_array;
+#define IAK_MAX_PAGE_ARRAYS 24
+
+/* Copy pages: row src[i] of every array to row dst[i], i < count (int32 on the device).
+ * Pairs with an id outside [0, num_pages) are left out. The dst ids are distinct and none
+ * of them is a src of another pair (such pairs race). Async on `stream`. */
+typedef struct {
+  int32_t num_arrays;
+  iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
+  int64_t num_pages;
+  int32_t count;
+  const int32_t* src;
+  const int32_t* dst;
+} iak_copy_pages_args;
+iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
+
+/* Sequences over shared pages. refs [num_pages] counts the table entries (and other owners)
+ * that hold a page; a page with refs <= 0 is free. page_table [num_seqs, rows_per_seq,
+ * table_width], valid_tokens [num_seqs, rows_per_seq]: entries 0 .. ceil(valid / page_size)
+ * - 1 of a row are in use. All int32, on the device, changed in place.
+ *   iak_free_sequences  lets go of every page of sequences seqs[0 .. count-1]: refs - 1 per
+ *       entry, the entries become -1 and the lengths 0. Indices outside [0, num_seqs) are
+ *       left out, one listed twice is freed once.
+ *   iak_grow_sequences  sequence seqs[i] gets new_tokens[i] more tokens in each of its rows:
+ *       entries for them come from the free pages, the lowest id first, in the order of
+ *       (i, row, entry), with refs = 1.
+ *   iak_fork_sequences  sequence seqs[i], which has no tokens, becomes a copy of parents[i]:
+ *       it shares the parent's pages (refs + 1), except that a last page which is not full
+ *       is copied (every array) into a free page, chosen in the order of (i, row).
+ * Grow and fork do all of it or nothing and say which in missing[0]: 0 done; n > 0: n more
+ * free pages would be needed; -1: an index outside [0, num_seqs) or listed twice among
+ * seqs, a negative new_tokens, a row longer than its table, a forked sequence with tokens, or
+ * one that is also a parent. Results do not depend on timing. Workspace:
+ * iak_sequences_workspace bytes, 16-byte aligned (free needs none). */
+typedef struct {
+  int32_t num_seqs, rows_per_seq, table_width, page_size;
+  int64_t num_pages;
+  int32_t* page_table;
+  int32_t* valid_tokens;
+  int32_t* refs;
+  int32_t count;
+  const int32_t* seqs;
+  const int32_t* parents;      /* fork */
+  const int32_t* new_tokens;   /* grow */
+  int32_t* missing;            /* grow, fork */
+  int32_t num_arrays;          /* fork */
+  iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
+} iak_sequences_args;
+
+iak_status iak_sequences_workspace(const iak_sequences_args* args, size_t* bytes);
+iak_status iak_free_sequences(const iak_sequences_args* args, void* stream);
+iak_status iak_grow_sequences(const iak_sequences_args* args, void* workspace, size_t workspace_bytes, void* stream);
+iak_status iak_fork_sequences(const iak_sequences_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Compaction: with L pages in use (refs > 0), those with ids >= L move to the free ids
+ * below L, the highest to the lowest: page_map [num_pages] is the new id of every page (-1:
+ * free), out_refs [num_pages] the counts by new id, out_table [num_rows, table_width] the
+ * table with its entries in use mapped (the others as they are). The arrays' rows are
+ * copied in place; old rows keep their bytes, and page_table and refs stay as they are, so
+ * work that still reads the old table finds its pages. No output may overlap an input. */
+typedef struct {
+  int32_t num_rows, table_width, page_size;
+  int64_t num_pages;
+  const int32_t* page_table;
+  const int32_t* valid_tokens;   /* [num_rows] */
+  const int32_t* refs;
+  int32_t* out_table;
+  int32_t* out_refs;
+  int32_t* page_map;
+  int32_t num_arrays;
+  iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
+} iak_compact_pages_args;
+
+iak_status iak_compact_pages_workspace(const iak_compact_pages_args* args, size_t* bytes);
+iak_status iak_compact_pages(const iak_compact_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,467 @@
+// Pages handed out, shared, given back and moved, on the device (gfx950): page tables, row
+// lengths and reference counts stay there, so a serving loop needs no answer on the host.
+//
+// Which page a row gets does not depend on timing: free pages are ranked by id (counts per
+// 1,024 pages, then a rank within them), rows by their place in the call, and rank meets
+// rank. Reference counts change by integer atomics, whose order leaves no trace.
+//
+//   grow, fork   plan_kernel   free pages per 1,024 ids; one workgroup checks the call and
+//                              sums what its rows need
+//                rank_kernel   the free ids in order, as many as are needed; the verdict
+//                apply_kernel  a workgroup per row: entries, counts, the copied last page
+//   free         free_kernel   a workgroup per row
+//   compact      plan_kernel, compact_rank_kernel (which page goes where),
+//                compact_apply_kernel (pages copied, table, counts and map written)
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "iak.h"
+#include "iak_internal.h"
+#include "iak_device.h"
+
+namespace iak {
+
+namespace {
+
+constexpr int PAGE_GROUP = 1024;       // page ids a workgroup counts or ranks
+constexpr int POOL_THREADS = 256;
+constexpr int PLAN_THREADS = 1024;
+
+struct PageArrays {
+  int n;
+  iak_page_array a[IAK_MAX_PAGE_ARRAYS];
+};
+
+// Row `src` of every array to row `dst`, by the workgroup.
+__device__ __forceinline__ void copy_page(const PageArrays& p, int64_t src, int64_t dst) {
+  for (int k = 0; k < p.n; ++k) {
+    const int64_t bytes = p.a[k].row_bytes;
+    char* base = reinterpret_cast<char*>(p.a[k].base);
+    const char* from = base + src * bytes;
+    char* to = base + dst * bytes;
+    const uint64_t low = reinterpret_cast<uintptr_t>(base) | (uint64_t)bytes;
+    if ((low & 15u) == 0) {
+      for (int64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x)
+        reinterpret_cast<u4*>(to)[i] = reinterpret_cast<const u4*>(from)[i];
+    } else if ((low & 3u) == 0) {
+      for (int64_t i = threadIdx.x; i < bytes / 4; i += blockDim.x)
+        reinterpret_cast<uint32_t*>(to)[i] = reinterpret_cast<const uint32_t*>(from)[i];
+    } else {
+      for (int64_t i = threadIdx.x; i < bytes; i += blockDim.x) to[i] = from[i];
+    }
+  }
+}
+
+__global__ __launch_bounds__(POOL_THREADS) void copy_pages_kernel(const PageArrays p, int64_t num_pages, int count,
+                                                                  const int32_t* src, const int32_t* dst) {
+  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+    const int64_t s = src[i], d = dst[i];
+    if (s < 0 || s >= num_pages || d < 0 || d >= num_pages || s == d) continue;   // uniform
+    copy_page(p, s, d);
+  }
+}
+
+// --------------------------------------------------------------------------- //
+// Sums over a workgroup. Every thread of it calls them.
+// --------------------------------------------------------------------------- //
+
+// Sum of `x` over the threads before this one; `total`: over all. WAVES waves.
+template <int WAVES> __device__ __forceinline__ int scan_before(int x, int& total) {
+  __shared__ int wave_sum[WAVES];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(s, o, 64);
+    if (lane >= o) s += y;
+  }
+  __syncthreads();                      // the last call's sums have been read
+  if (lane == 63) wave_sum[w] = s;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k) {
+    if (k < w) before += wave_sum[k];
+    total += wave_sum[k];
+  }
+  return before + s - x;
+}
+
+// Sums of counts[0 .. at - 1] and of counts[0 .. n - 1].
+template <int WAVES> __device__ __forceinline__ void sum_groups(const int32_t* counts, int at, int n, int& before, int& all) {
+  int x = 0, y = 0;
+  for (int k = threadIdx.x; k < n; k += 64 * WAVES) {
+    const int v = counts[k];
+    y += v;
+    if (k < at) x += v;
+  }
+  scan_before<WAVES>(x, before);
+  scan_before<WAVES>(y, all);
+}
+
+// --------------------------------------------------------------------------- //
+// Grow and fork
+// --------------------------------------------------------------------------- //
+
+enum { SEQ_GROW = 0, SEQ_FORK = 1 };
+
+struct SeqArgs {
+  int num_seqs, R, W, PSZ;             // rows per sequence, table width, tokens per page
+  int64_t NP;
+  int32_t* table; int32_t* valid; int32_t* refs;
+  int count;
+  const int32_t* seqs; const int32_t* parents; const int32_t* new_tokens;
+  int32_t* missing;
+  int groups;                          // ceil(NP / PAGE_GROUP)
+  int32_t* head;                       // [0] pages needed, [1] the call is refused
+  int32_t* group_free;                 // [groups] free pages
+  int32_t* marks;                      // [num_seqs] 1: listed in seqs
+  int32_t* first;                      // [count * R] pages of the rows before
+  int32_t* list;                       // [NP] free ids in order
+  PageArrays arrays;
+};
+
+__device__ __forceinline__ int used_entries(int tokens, int page_size, int width) {
+  if (tokens <= 0) return 0;
+  const int64_t n = ((int64_t)tokens + page_size - 1) / page_size;
+  return n < width ? (int)n : width;
+}
+
+// Whether a forked row gets a page of its own: its parent's last page is not full.
+__device__ __forceinline__ bool ragged_last(const SeqArgs& a, int64_t parent_row, int& n, int64_t& page) {
+  const int tokens = a.valid[parent_row];
+  n = used_entries(tokens, a.PSZ, a.W);
+  if (n == 0 || (int64_t)n * a.PSZ <= tokens) return false;
+  page = a.table[parent_row * a.W + n - 1];
+  return page >= 0 && page < a.NP;
+}
+
+__device__ __forceinline__ int count_free(const int32_t* refs, int64_t NP, int group) {
+  int n = 0;
+  for (int k = threadIdx.x; k < PAGE_GROUP; k += blockDim.x) {
+    const int64_t id = (int64_t)group * PAGE_GROUP + k;
+    n += id < NP && refs[id] <= 0;
+  }
+  return n;
+}
+
+template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
+  constexpr int WAVES = PLAN_THREADS / 64;
+  if ((int)blockIdx.x < a.groups) {
+    int total;
+    scan_before<WAVES>(count_free(a.refs, a.NP, blockIdx.x), total);
+    if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
+    return;
+  }
+  // the last workgroup: is the call sound, and what does it need
+  __shared__ int refused;
+  if (threadIdx.x == 0) refused = 0;
+  for (int k = threadIdx.x; k < a.num_seqs; k += PLAN_THREADS) a.marks[k] = 0;
+  __threadfence_block();
+  __syncthreads();
+  bool bad = false;
+  for (int k = threadIdx.x; k < a.count; k += PLAN_THREADS) {
+    const int s = a.seqs[k];
+    if (s < 0 || s >= a.num_seqs) { bad = true; continue; }
+    if (atomicAdd(&a.marks[s], 1) != 0) bad = true;
+    if constexpr (KIND == SEQ_GROW) {
+      if (a.new_tokens[k] < 0) bad = true;
+    } else {
+      const int p = a.parents[k];
+      if (p < 0 || p >= a.num_seqs) bad = true;
+      for (int h = 0; h < a.R; ++h) if (a.valid[(int64_t)s * a.R + h] != 0) bad = true;
+    }
+  }
+  if (bad) refused = 1;
+  __threadfence_block();
+  __syncthreads();
+  const bool sound = !refused;          // before anyone sets it again: the branches below are uniform
+  __syncthreads();
+  int64_t total = 0;
+  const int rows = a.count * a.R;
+  if (sound) {
+    if constexpr (KIND == SEQ_FORK) {
+      for (int k = threadIdx.x; k < a.count; k += PLAN_THREADS)
+        if (a.marks[a.parents[k]] != 0) refused = 1;
+    }
+    for (int k0 = 0; k0 < rows; k0 += PLAN_THREADS) {
+      const int k = k0 + threadIdx.x;
+      int need = 0;
+      if (k < rows) {
+        const int j = k / a.R, h = k - j * a.R;
+        if constexpr (KIND == SEQ_GROW) {
+          const int old = a.valid[(int64_t)a.seqs[j] * a.R + h];
+          const int64_t tokens = (int64_t)(old < 0 ? 0 : old) + a.new_tokens[j];
+          if (tokens > (int64_t)a.W * a.PSZ) refused = 1;
+          else need = used_entries((int)tokens, a.PSZ, a.W) - used_entries(old, a.PSZ, a.W);
+        } else {
+          int n;
+          int64_t page;
+          need = ragged_last(a, (int64_t)a.parents[j] * a.R + h, n, page);
+        }
+      }
+      int all;
+      const int before = scan_before<WAVES>(need, all);
+      if (k < rows) a.first[k] = (int)(total + before > 0x7FFFFFFF ? 0x7FFFFFFF : total + before);
+      total += all;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.head[0] = (int)(total > 0x7FFFFFFF ? 0x7FFFFFFF : total);
+    a.head[1] = refused;
+  }
+}
+
+__global__ __launch_bounds__(POOL_THREADS) void seq_rank_kernel(const SeqArgs a) {
+  constexpr int WAVES = POOL_THREADS / 64;
+  int before, all;
+  sum_groups<WAVES>(a.group_free, blockIdx.x, a.groups, before, all);
+  const int need = a.head[0];
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.missing[0] = a.head[1] ? -1 : (need > all ? need - all : 0);
+  if (before >= need) return;                                    // uniform
+  for (int k0 = 0; k0 < PAGE_GROUP; k0 += POOL_THREADS) {
+    const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + k0 + threadIdx.x;
+    const bool free_page = id < a.NP && a.refs[id] <= 0;
+    int total;
+    const int rank = before + scan_before<WAVES>(free_page, total);
+    if (free_page) a.list[rank] = (int)id;
+    before += total;
+  }
+}
+
+template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_kernel(const SeqArgs a) {
+  if (a.missing[0] != 0) return;
+  const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
+  const int64_t row = (int64_t)a.seqs[j] * a.R + h;
+  int32_t* entries = a.table + row * a.W;
+  const int first = a.first[k];
+  if constexpr (KIND == SEQ_GROW) {
+    const int old = a.valid[row] < 0 ? 0 : a.valid[row], tokens = old + a.new_tokens[j];
+    const int have = used_entries(old, a.PSZ, a.W), want = used_entries(tokens, a.PSZ, a.W);
+    for (int e = have + threadIdx.x; e < want; e += POOL_THREADS) {
+      const int id = a.list[first + e - have];
+      entries[e] = id;
+      a.refs[id] = 1;
+    }
+    __syncthreads();                                             // every thread has read the old length
+    if (threadIdx.x == 0) a.valid[row] = tokens;
+  } else {
+    const int64_t parent = (int64_t)a.parents[j] * a.R + h;
+    const int32_t* from = a.table + parent * a.W;
+    int n;
+    int64_t last;
+    const bool own_page = ragged_last(a, parent, n, last);
+    const int shared = own_page ? n - 1 : n;
+    for (int e = threadIdx.x; e < shared; e += POOL_THREADS) {
+      const int id = from[e];
+      entries[e] = id;
+      if (id >= 0 && id < a.NP) atomicAdd(&a.refs[id], 1);
+    }
+    if (own_page) {
+      const int id = a.list[first];
+      if (threadIdx.x == 0) { entries[n - 1] = id; a.refs[id] = 1; }
+      copy_page(a.arrays, last, id);
+    }
+    if (threadIdx.x == 0) a.valid[row] = a.valid[parent];
+  }
+}
+
+// A workgroup per (listed sequence, row). The length is taken by one exchange, so that a
+// sequence listed twice is freed once.
+__global__ __launch_bounds__(POOL_THREADS) void seq_free_kernel(const SeqArgs a) {
+  __shared__ int tokens;
+  const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
+  const int s = a.seqs[j];
+  if (s < 0 || s >= a.num_seqs) return;
+  const int64_t row = (int64_t)s * a.R + h;
+  if (threadIdx.x == 0) tokens = atomicExch(&a.valid[row], 0);
+  __syncthreads();
+  const int n = used_entries(tokens, a.PSZ, a.W);
+  int32_t* entries = a.table + row * a.W;
+  for (int e = threadIdx.x; e < n; e += POOL_THREADS) {
+    const int id = entries[e];
+    if (id >= 0 && id < a.NP) atomicSub(&a.refs[id], 1);
+    entries[e] = -1;
+  }
+}
+
+// --------------------------------------------------------------------------- //
+// Compaction
+// --------------------------------------------------------------------------- //
+
+struct CompactArgs {
+  int64_t rows; int W, PSZ;
+  int64_t NP;
+  const int32_t* table; const int32_t* valid; const int32_t* refs;
+  int32_t* out_table; int32_t* out_refs; int32_t* page_map;
+  int groups;
+  int32_t* group_free;   // [groups]
+  int32_t* head;         // [0] pages in use, [1] moves
+  int32_t* order;        // [NP] of a page in use past the end: the move it is
+  int32_t* hole;         // [NP / 2 + 1] where move j goes
+  int32_t* mover;        // [NP / 2 + 1] what move j moves
+  int move_groups;       // workgroups that copy pages
+  PageArrays arrays;
+};
+
+__global__ __launch_bounds__(POOL_THREADS) void compact_count_kernel(const CompactArgs a) {
+  int total;
+  scan_before<POOL_THREADS / 64>(count_free(a.refs, a.NP, blockIdx.x), total);
+  if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
+}
+
+// With L pages in use: the free ids below L are the holes in order, and the page in use that
+// is r-th of all goes, where its id is L or more, to hole L - 1 - r.
+__global__ __launch_bounds__(POOL_THREADS) void compact_rank_kernel(const CompactArgs a) {
+  constexpr int WAVES = POOL_THREADS / 64;
+  int before, all;
+  sum_groups<WAVES>(a.group_free, blockIdx.x, a.groups, before, all);
+  const int64_t L = a.NP - all;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.head[0] = (int)L;
+    if (all == 0) a.head[1] = 0;
+  }
+  for (int k0 = 0; k0 < PAGE_GROUP; k0 += POOL_THREADS) {
+    const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + k0 + threadIdx.x;
+    const bool in = id < a.NP, free_page = in && a.refs[id] <= 0;
+    int total;
+    const int free_before = before + scan_before<WAVES>(free_page, total);
+    before += total;
+    if (in && id == L) a.head[1] = free_before;
+    if (free_page && id < L) a.hole[free_before] = (int)id;
+    if (in && !free_page && id >= L) {
+      const int move = (int)(L - 1 - (id - free_before));
+      a.mover[move] = (int)id;
+      a.order[id] = move;
+    }
+  }
+}
+
+__device__ __forceinline__ int moved_to(const CompactArgs& a, int id, int L) {
+  return id < L ? id : a.hole[a.order[id]];
+}
+
+__global__ __launch_bounds__(POOL_THREADS) void compact_apply_kernel(const CompactArgs a) {
+  const int L = a.head[0];
+  if ((int)blockIdx.x < a.move_groups) {
+    const int moves = a.head[1];
+    for (int j = blockIdx.x; j < moves; j += a.move_groups) copy_page(a.arrays, a.mover[j], a.hole[j]);
+    return;
+  }
+  const int64_t step = (int64_t)(gridDim.x - a.move_groups) * POOL_THREADS;
+  const int64_t at = (int64_t)(blockIdx.x - a.move_groups) * POOL_THREADS + threadIdx.x;
+  for (int64_t id = at; id < a.NP; id += step) {
+    const int r = a.refs[id];
+    const bool live = r > 0;
+    const int to = live ? moved_to(a, (int)id, L) : -1;
+    a.page_map[id] = to;
+    if (live) a.out_refs[to] = r;
+    if (id >= L) a.out_refs[id] = 0;
+  }
+  for (int64_t k = at; k < a.rows * a.W; k += step) {
+    const int64_t row = k / a.W;
+    const int e = (int)(k - row * a.W);
+    const int id = a.table[k];
+    const bool used = e < used_entries(a.valid[row], a.PSZ, a.W) && id >= 0 && id < a.NP;
+    a.out_table[k] = used ? (a.refs[id] > 0 ? moved_to(a, id, L) : -1) : id;
+  }
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
+  SeqArgs s;
+  s.num_seqs = a.num_seqs; s.R = a.rows_per_seq; s.W = a.table_width; s.PSZ = a.page_size; s.NP = a.num_pages;
+  s.table = a.page_table; s.valid = a.valid_tokens; s.refs = a.refs;
+  s.count = a.count; s.seqs = a.seqs; s.parents = a.parents; s.new_tokens = a.new_tokens; s.missing = a.missing;
+  s.groups = (int)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
+  s.arrays.n = a.num_arrays;
+  for (int k = 0; k < a.num_arrays; ++k) s.arrays.a[k] = a.arrays[k];
+  char* p = reinterpret_cast<char*>(workspace);
+  auto take = [&](size_t ints) { int32_t* r = reinterpret_cast<int32_t*>(p); p += up256(4 * ints); return r; };
+  if (p) {
+    s.head = take(2);
+    s.group_free = take((size_t)s.groups);
+    s.marks = take((size_t)s.num_seqs);
+    s.first = take((size_t)a.count * a.rows_per_seq);
+    s.list = take((size_t)a.num_pages);
+  }
+  return s;
+}
+
+template <int KIND> hipError_t launch_seq(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
+  const SeqArgs s = seq_args(a, workspace);
+  hipLaunchKernelGGL(seq_plan_kernel<KIND>, dim3(s.groups + 1), dim3(PLAN_THREADS), 0, stream, s);
+  hipLaunchKernelGGL(seq_rank_kernel, dim3(s.groups > 0 ? s.groups : 1), dim3(POOL_THREADS), 0, stream, s);
+  if (a.count > 0)
+    hipLaunchKernelGGL(seq_apply_kernel<KIND>, dim3(a.count * a.rows_per_seq), dim3(POOL_THREADS), 0, stream, s);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_copy_pages(const iak_copy_pages_args& a, hipStream_t stream) {
+  PageArrays p;
+  p.n = a.num_arrays;
+  for (int k = 0; k < a.num_arrays; ++k) p.a[k] = a.arrays[k];
+  const int grid = a.count < 65536 ? a.count : 65536;
+  hipLaunchKernelGGL(copy_pages_kernel, dim3(grid), dim3(POOL_THREADS), 0, stream, p, a.num_pages, a.count, a.src, a.dst);
+  return hipGetLastError();
+}
+
+size_t sequences_workspace(const iak_sequences_args& a) {
+  const size_t groups = (size_t)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
+  return up256(8) + up256(4 * groups) + up256(4 * (size_t)a.num_seqs) + up256(4 * (size_t)a.count * a.rows_per_seq) +
+         up256(4 * (size_t)a.num_pages);
+}
+
+hipError_t launch_free_sequences(const iak_sequences_args& a, hipStream_t stream) {
+  const SeqArgs s = seq_args(a, nullptr);
+  hipLaunchKernelGGL(seq_free_kernel, dim3(a.count * a.rows_per_seq), dim3(POOL_THREADS), 0, stream, s);
+  return hipGetLastError();
+}
+hipError_t launch_grow_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
+  return launch_seq<SEQ_GROW>(a, workspace, stream);
+}
+hipError_t launch_fork_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
+  return launch_seq<SEQ_FORK>(a, workspace, stream);
+}
+
+size_t compact_workspace(const iak_compact_pages_args& a) {
+  const size_t groups = (size_t)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP), np = (size_t)a.num_pages;
+  return up256(8) + up256(4 * groups) + up256(4 * np) + 2 * up256(4 * (np / 2 + 1));
+}
+
+hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace, hipStream_t stream) {
+  CompactArgs c;
+  c.rows = a.num_rows; c.W = a.table_width; c.PSZ = a.page_size; c.NP = a.num_pages;
+  c.table = a.page_table; c.valid = a.valid_tokens; c.refs = a.refs;
+  c.out_table = a.out_table; c.out_refs = a.out_refs; c.page_map = a.page_map;
+  c.groups = (int)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
+  c.arrays.n = a.num_arrays;
+  for (int k = 0; k < a.num_arrays; ++k) c.arrays.a[k] = a.arrays[k];
+  const size_t np = (size_t)a.num_pages;
+  char* p = reinterpret_cast<char*>(workspace);
+  auto take = [&](size_t ints) { int32_t* r = reinterpret_cast<int32_t*>(p); p += up256(4 * ints); return r; };
+  c.head = take(2);
+  c.group_free = take((size_t)c.groups);
+  c.order = take(np);
+  c.hole = take(np / 2 + 1);
+  c.mover = take(np / 2 + 1);
+  const int64_t moves = a.num_pages / 2 + 1;
+  c.move_groups = a.num_arrays > 0 ? (int)(moves < 4096 ? moves : 4096) : 0;
+  const int64_t items = a.num_pages > (int64_t)a.num_rows * a.table_width ? a.num_pages : (int64_t)a.num_rows * a.table_width;
+  const int64_t rest = (items + POOL_THREADS - 1) / POOL_THREADS;
+  if (a.num_pages > 0) {
+    hipLaunchKernelGGL(compact_count_kernel, dim3(c.groups), dim3(POOL_THREADS), 0, stream, c);
+    hipLaunchKernelGGL(compact_rank_kernel, dim3(c.groups), dim3(POOL_THREADS), 0, stream, c);
+  }
+  hipLaunchKernelGGL(compact_apply_kernel, dim3((uint32_t)(c.move_groups + (rest < 4096 ? rest : 4096))), dim3(POOL_THREADS), 0,
+                     stream, c);
+  return hipGetLastError();
+}
+
+}  // namespace iak

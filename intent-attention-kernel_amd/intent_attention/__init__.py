@@ -46,6 +46,15 @@ from .mla_core import LatentPools, mla_paged_decode
 from .triton_mla_decode import mla_decode_triton
 from .quantize import fake_int8_pages_device, quantize_pages
 from .page_tables import build_page_tables, routing_to_kernel_tensors
+from .mxfp4 import (
+    MxFp4Plan,
+    MxFp4Pools,
+    append_mxfp4_tokens,
+    make_mxfp4_plan,
+    mxfp4_paged_attention,
+    read_mxfp4_tokens,
+)
+from .page_sharing import compact_pages, copy_pages, fork_sequences, free_sequences, grow_sequences
 from .kv_memory_manager import KVMemoryManager, PageFormatPolicy, PageState, PageStorageFormat
 from .prefetch import BlockPrefetcher, get_prefetch_stream, get_prefetcher, launch_prefetch_pages, reset_prefetcher
 from .triton_adaptive_format_attention import (
@@ -74,6 +83,8 @@ __all__ = [
     "LatentPools", "mla_paged_decode", "mla_decode_triton",
     "quantize_pages", "fake_int8_pages_device",
     "build_page_tables", "routing_to_kernel_tensors",
+    "MxFp4Plan", "MxFp4Pools", "append_mxfp4_tokens", "make_mxfp4_plan", "mxfp4_paged_attention", "read_mxfp4_tokens",
+    "compact_pages", "copy_pages", "fork_sequences", "free_sequences", "grow_sequences",
     "KVMemoryManager", "PageFormatPolicy", "PageState", "PageStorageFormat",
     "BlockPrefetcher", "get_prefetch_stream", "get_prefetcher", "launch_prefetch_pages", "reset_prefetcher",
     "AdaptiveFormatKernelConfig", "AdaptivePageFormat", "adaptive_format_decode_attention_reference_dispatch",

@@ -190,6 +190,78 @@ class DenseAttentionArgs(ctypes.Structure):
     ]
 
 
+class MxTokensArgs(ctypes.Structure):
+    """Mirror of ``iak_mx_tokens_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("count", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32), ("page_size", c_i32),
+        ("table_width", c_i32),
+        ("num_pages", c_i64),
+        ("k", c_void_p), ("k_stride_b", c_i64), ("k_stride_t", c_i64), ("k_stride_h", c_i64),
+        ("v", c_void_p), ("v_stride_b", c_i64), ("v_stride_t", c_i64), ("v_stride_h", c_i64),
+        ("dtype", c_i32),
+        ("page_table", c_void_p), ("valid_tokens", c_void_p), ("q_lens", c_void_p),
+        ("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+    ]
+
+
+class MxAttentionArgs(ctypes.Structure):
+    """Mirror of ``iak_mx_attention_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("q_len", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("page_size", c_i32), ("table_width", c_i32),
+        ("num_pages", c_i64),
+        ("q", c_void_p), ("q_dtype", c_i32), ("q_stride_b", c_i64), ("q_stride_t", c_i64), ("q_stride_h", c_i64),
+        ("out", c_void_p), ("out_dtype", c_i32), ("out_stride_b", c_i64), ("out_stride_t", c_i64),
+        ("out_stride_h", c_i64),
+        ("page_table", c_void_p), ("valid_tokens", c_void_p), ("q_lens", c_void_p),
+        ("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+        ("sm_scale", c_float), ("causal", c_i32), ("splits", c_i32),
+    ]
+
+
+MAX_PAGE_ARRAYS = 24   # IAK_MAX_PAGE_ARRAYS
+
+
+class PageArray(ctypes.Structure):
+    """Mirror of ``iak_page_array`` (include/iak.h)."""
+
+    _fields_ = [("base", c_void_p), ("row_bytes", c_i64)]
+
+
+class CopyPagesArgs(ctypes.Structure):
+    """Mirror of ``iak_copy_pages_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("num_arrays", c_i32), ("arrays", PageArray * MAX_PAGE_ARRAYS), ("num_pages", c_i64), ("count", c_i32),
+        ("src", c_void_p), ("dst", c_void_p),
+    ]
+
+
+class SequencesArgs(ctypes.Structure):
+    """Mirror of ``iak_sequences_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("num_seqs", c_i32), ("rows_per_seq", c_i32), ("table_width", c_i32), ("page_size", c_i32),
+        ("num_pages", c_i64),
+        ("page_table", c_void_p), ("valid_tokens", c_void_p), ("refs", c_void_p),
+        ("count", c_i32), ("seqs", c_void_p), ("parents", c_void_p), ("new_tokens", c_void_p), ("missing", c_void_p),
+        ("num_arrays", c_i32), ("arrays", PageArray * MAX_PAGE_ARRAYS),
+    ]
+
+
+class CompactPagesArgs(ctypes.Structure):
+    """Mirror of ``iak_compact_pages_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("num_rows", c_i32), ("table_width", c_i32), ("page_size", c_i32), ("num_pages", c_i64),
+        ("page_table", c_void_p), ("valid_tokens", c_void_p), ("refs", c_void_p),
+        ("out_table", c_void_p), ("out_refs", c_void_p), ("page_map", c_void_p),
+        ("num_arrays", c_i32), ("arrays", PageArray * MAX_PAGE_ARRAYS),
+    ]
+
+
 EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_paged_decode_workspace", "iak_paged_decode",
             "iak_mla_decode_workspace", "iak_mla_decode", "iak_quantize_pages",
@@ -199,7 +271,10 @@ EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_pack_entry_records", "iak_dense_attention", "iak_dense_attention_indexed", "iak_dense_attention_workspace",
             "iak_mla_decode_rows_workspace", "iak_fake_quant_blocks",
             "iak_fake_quant_blocks_workspace", "iak_timing_event_create", "iak_timing_event_record",
-            "iak_timing_event_elapsed", "iak_timing_event_destroy")
+            "iak_timing_event_elapsed", "iak_timing_event_destroy",
+            "iak_mx_append_tokens", "iak_mx_read_tokens", "iak_mx_attention_workspace", "iak_mx_attention",
+            "iak_copy_pages", "iak_sequences_workspace", "iak_free_sequences", "iak_grow_sequences",
+            "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages")
 NOALLOC_SCRATCH_BYTES = 16 << 20   # IAK_NOALLOC_SCRATCH_BYTES
 
 _lib: Optional[ctypes.CDLL] = None
@@ -284,6 +359,21 @@ def load() -> ctypes.CDLL:
     lib.iak_dense_attention_workspace.argtypes = [ctypes.POINTER(DenseAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
     lib.iak_pack_entry_records.restype = ctypes.c_int
     lib.iak_pack_entry_records.argtypes = [ctypes.POINTER(PagedDecodeArgs), c_void_p, c_void_p]
+    size_p = ctypes.POINTER(ctypes.c_size_t)
+    for name, args in (("iak_mx_append_tokens", (MxTokensArgs, c_void_p)),
+                       ("iak_mx_read_tokens", (MxTokensArgs, c_void_p)),
+                       ("iak_mx_attention_workspace", (MxAttentionArgs, size_p)),
+                       ("iak_mx_attention", (MxAttentionArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_copy_pages", (CopyPagesArgs, c_void_p)),
+                       ("iak_sequences_workspace", (SequencesArgs, size_p)),
+                       ("iak_free_sequences", (SequencesArgs, c_void_p)),
+                       ("iak_grow_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_fork_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_compact_pages_workspace", (CompactPagesArgs, size_p)),
+                       ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p))):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(args[0]), *args[1:]]
     ver = lib.iak_abi_version()
     if ver != ABI_VERSION:
         _load_error = f"libiak.so ABI version {ver} != expected {ABI_VERSION}; rebuild the library"
@@ -452,3 +542,53 @@ def dense_attention(args: DenseAttentionArgs, stream: int, workspace: int = 0, w
                     kv_index: int = 0) -> None:
     check(load().iak_dense_attention_indexed(ctypes.byref(args), kv_index or None, workspace or None, workspace_bytes,
                                              stream or None))
+
+
+def mx_append_tokens(args: MxTokensArgs, stream: int) -> None:
+    check(load().iak_mx_append_tokens(ctypes.byref(args), stream or None))
+
+
+def mx_read_tokens(args: MxTokensArgs, stream: int) -> None:
+    check(load().iak_mx_read_tokens(ctypes.byref(args), stream or None))
+
+
+def mx_attention_workspace(args: MxAttentionArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_mx_attention_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def mx_attention(args: MxAttentionArgs, stream: int, workspace: int = 0, workspace_bytes: int = 0) -> None:
+    check(load().iak_mx_attention(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))
+
+
+def copy_pages(args: CopyPagesArgs, stream: int) -> None:
+    check(load().iak_copy_pages(ctypes.byref(args), stream or None))
+
+
+def sequences_workspace(args: SequencesArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_sequences_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def free_sequences(args: SequencesArgs, stream: int) -> None:
+    check(load().iak_free_sequences(ctypes.byref(args), stream or None))
+
+
+def grow_sequences(args: SequencesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
+    check(load().iak_grow_sequences(ctypes.byref(args), workspace, workspace_bytes, stream or None))
+
+
+def fork_sequences(args: SequencesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
+    check(load().iak_fork_sequences(ctypes.byref(args), workspace, workspace_bytes, stream or None))
+
+
+def compact_pages_workspace(args: CompactPagesArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_compact_pages_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def compact_pages(args: CompactPagesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
+    check(load().iak_compact_pages(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))

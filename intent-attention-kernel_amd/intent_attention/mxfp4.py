@@ -1,0 +1,251 @@
+"""A microscaled 4-bit (MXFP4) token cache on the MI355X: tokens written one by one,
+and attention of one or several query tokens per sequence over them
+(``iak_mx_append_tokens``, ``iak_mx_read_tokens``, ``iak_mx_attention``, include/iak.h).
+
+The decode's INT4 pages (``PagePools``) carry one scale per page and channel group, so a
+page is written whole. Here every token has its own scales, one per 32 channels: a
+serving loop appends each new token as it comes, at 4.25 bits a value.
+
+* ``MxFp4Pools`` -- pages of 16 tokens of one KV head: e2m1 codes and e8m0 scale bytes;
+* ``append_mxfp4_tokens(k, v, pools, page_table, valid_tokens)`` -- quantises the newest
+  tokens of every sequence into their pages, ``read_mxfp4_tokens`` gives them back;
+* ``mxfp4_paged_attention(q, pools, page_table, valid_tokens)`` -- attention of the
+  newest tokens: a decode step (q [B, Hq, D]), drafted tokens or a prompt chunk
+  (q [B, L, Hq, D], causal); ``make_mxfp4_plan`` checks the arguments once for many runs.
+
+All of them take the same page table [B, Hkv, W] and ``valid_tokens`` [B, Hkv], the tokens
+each row holds INCLUDING the newest ones: append first, then attend. With ``q_lens`` [B]
+sequence b has q_lens[b] new tokens, the first of the batch's L; the rest is padding (not
+written by append, zero from read and attention).
+
+The values: per block of 32 channels e = clamp(floor(log2 max|x|) - 2, -23, 13) and codes
+rounded to the nearest even of x / 2^e, at most 6 in magnitude (the OCP microscaling
+conversion; the clamp keeps every value a float16 number, the largest 49,152). A block
+with an infinity or a NaN is stored as NaN and makes every query that sees its token NaN.
+
+Device tensors only, inference only (no autograd history). The table, the lengths and the
+pages are read on the stream the call is made on.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass, fields
+from typing import Dict, Optional, Tuple
+
+import torch
+
+from . import _native as N
+from .decode_core import PAGE_SIZE, _DT, _check_pool, _ptr, current_stream_handle, require_device
+
+BLOCK = 32          # channels per scale
+
+
+@dataclass
+class MxFp4Pools:
+    """K and V pages of the cache: codes [NP, 16, D/2] uint8 (channel 2j in the low half of
+    byte j) and scale bytes [NP, 16, D/32] uint8, D = 64 or 128."""
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, num_pages: int, head_dim: int, device) -> "MxFp4Pools":
+        """Pools of ``num_pages`` pages whose every value is 0."""
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+        codes, scales = ((num_pages, PAGE_SIZE, head_dim // 2), (num_pages, PAGE_SIZE, head_dim // BLOCK))
+        return cls(*(torch.zeros(s, dtype=torch.uint8, device=device) for s in (codes, scales, codes, scales)))
+
+    def tensors(self) -> Dict[str, torch.Tensor]:
+        return {f.name: getattr(self, f.name) for f in fields(self)}
+
+
+def _check_cache(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor,
+                 q_lens: Optional[torch.Tensor], B: int, D: int) -> Tuple[int, int, int]:
+    """(Hkv, W, NP) of the pools and the metadata, or ValueError."""
+    if page_table.dim() != 3 or page_table.shape[0] != B or page_table.dtype != torch.int32:
+        raise ValueError(f"page_table must be int32 [{B}, Hkv, W], got {page_table.dtype} {tuple(page_table.shape)}")
+    Hkv, W = page_table.shape[1], page_table.shape[2]
+    if valid_tokens.shape != (B, Hkv) or valid_tokens.dtype != torch.int32:
+        raise ValueError(f"valid_tokens must be int32 [{B}, {Hkv}], got {valid_tokens.dtype} "
+                         f"{tuple(valid_tokens.shape)}")
+    if q_lens is not None and (q_lens.shape != (B,) or q_lens.dtype != torch.int32):
+        raise ValueError(f"q_lens must be int32 [{B}], got {q_lens.dtype} {tuple(q_lens.shape)}")
+    if D not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    NP = pools.k_codes.shape[0] if pools.k_codes.dim() else -1
+    for name, t in pools.tensors().items():
+        _check_pool(name, t, NP, (PAGE_SIZE, D // 2 if name.endswith("codes") else D // BLOCK), (torch.uint8,))
+    return Hkv, W, NP
+
+
+def _on(device: torch.device):
+    """A guard that makes ``device`` current, where it is not."""
+    return torch.cuda.device(device) if device.index not in (None, torch.cuda.current_device()) else _HERE
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _tokens_args(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor,
+                 valid_tokens: torch.Tensor, q_lens: Optional[torch.Tensor]):
+    """The argument block of append and read, and the tensors it points into."""
+    B, L, Hkv, D = k.shape
+    heads, W, NP = _check_cache(pools, page_table, valid_tokens, q_lens, B, D)
+    if heads != Hkv:
+        raise ValueError(f"page_table has {heads} KV heads, k has {Hkv}")
+    page_table, valid_tokens = page_table.contiguous(), valid_tokens.contiguous()
+    q_lens = None if q_lens is None else q_lens.contiguous()
+    a = N.MxTokensArgs()
+    a.batch, a.count, a.num_kv_heads, a.head_dim, a.page_size, a.table_width, a.num_pages = B, L, Hkv, D, PAGE_SIZE, W, NP
+    a.k, (a.k_stride_b, a.k_stride_t, a.k_stride_h, _) = k.data_ptr(), k.stride()
+    a.v, (a.v_stride_b, a.v_stride_t, a.v_stride_h, _) = v.data_ptr(), v.stride()
+    a.dtype = _DT[k.dtype]
+    a.page_table, a.valid_tokens, a.q_lens = page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens)
+    a.k_codes, a.k_scales = pools.k_codes.data_ptr(), pools.k_scales.data_ptr()
+    a.v_codes, a.v_scales = pools.v_codes.data_ptr(), pools.v_scales.data_ptr()
+    return a, (page_table, valid_tokens, q_lens)
+
+
+def append_mxfp4_tokens(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor,
+                        valid_tokens: torch.Tensor, *, q_lens: Optional[torch.Tensor] = None) -> None:
+    """Quantise the newest tokens' ``k``, ``v`` [B, L, Hkv, D] (float16, bfloat16 or float32,
+    one dtype, any strides) into the pools: token i < q_lens[b] (default L) of sequence b is
+    number valid_tokens[b, h] - q_lens[b] + i of row (b, h). Tokens before 0, past the table
+    or on a page id outside the pools are left out; nothing else of the pools is written.
+    Rows that share a page (``fork_sequences`` shares full pages only) must not both append
+    to it."""
+    if k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"k and v must have one shape [B, L, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype not in _DT or v.dtype != k.dtype:
+        raise ValueError(f"k and v must both be float16, bfloat16 or float32, got {k.dtype} and {v.dtype}")
+    extra = () if q_lens is None else (q_lens,)
+    dev = require_device(k, v, page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit token cache")
+    k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
+    a, keep = _tokens_args(k, v, pools, page_table, valid_tokens, q_lens)
+    with _on(dev):
+        N.mx_append_tokens(a, current_stream_handle(dev))
+    torch.autograd.graph.increment_version(tuple(pools.tensors().values()))   # written through raw pointers
+
+
+def read_mxfp4_tokens(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor, count: int, *,
+                      q_lens: Optional[torch.Tensor] = None,
+                      dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V [B, count, Hkv, D] of the newest ``count`` tokens of every row (with ``q_lens``:
+    of the newest q_lens[b], then zeros) as the cache holds them, exactly in every dtype;
+    tokens that do not exist are zero."""
+    if dtype not in _DT:
+        raise ValueError(f"dtype must be float16, bfloat16 or float32, got {dtype}")
+    if count < 0:
+        raise ValueError(f"count must not be negative, got {count}")
+    extra = () if q_lens is None else (q_lens,)
+    dev = require_device(page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit token cache")
+    if page_table.dim() != 3 or pools.k_codes.dim() != 3:
+        raise ValueError(f"page_table must be [B, Hkv, W] and codes [NP, {PAGE_SIZE}, D/2], got "
+                         f"{tuple(page_table.shape)} and {tuple(pools.k_codes.shape)}")
+    shape = (page_table.shape[0], int(count), page_table.shape[1], 2 * pools.k_codes.shape[2])
+    k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    a, keep = _tokens_args(k, v, pools, page_table, valid_tokens, q_lens)
+    with _on(dev):
+        N.mx_read_tokens(a, current_stream_handle(dev))
+    return k, v
+
+
+class MxFp4Plan:
+    """Checked launch arguments plus workspace (``run`` is one C call on the current stream;
+    the tensors are held so their memory stays valid). The plan reads the query, the pools,
+    the table and the lengths as they are at each run and writes ``out``; its workspace is
+    its own, so runs of one plan must not overlap, runs of two plans may."""
+
+    def __init__(self, args: N.MxAttentionArgs, device: torch.device, out: torch.Tensor, keep=()) -> None:
+        self.args = args
+        self.device = device
+        self.out = out
+        self._keep = keep
+        self.workspace_bytes = N.mx_attention_workspace(args)
+        self._ws = (torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+                    if self.workspace_bytes else None)
+        self._ws_ptr = self._ws.data_ptr() if self._ws is not None else 0
+
+    def run(self, stream: Optional[int] = None) -> None:
+        """Launch on ``stream`` (default: torch's current stream)."""
+        s = current_stream_handle(self.device) if stream is None else stream
+        with _on(self.device):
+            N.mx_attention(self.args, s, self._ws_ptr, self.workspace_bytes)
+
+
+def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor, *,
+                    q_lens: Optional[torch.Tensor] = None, causal: bool = True, sm_scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    splits: int = 0) -> MxFp4Plan:
+    """Check the arguments of ``mxfp4_paged_attention`` once, for repeated runs over the same
+    tensors. The plan reads the tensors in place: page_table, valid_tokens and q_lens must be
+    contiguous, q (and ``out``) have a unit last stride."""
+    extra = tuple(t for t in (q_lens, out) if t is not None)
+    dev = require_device(q, page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit cache attention")
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must have shape [B, Hq, D] or [B, L, Hq, D], got {tuple(q.shape)}")
+    q4 = q.unsqueeze(1) if q.dim() == 3 else q
+    B, L, Hq, D = q4.shape
+    if q.dtype not in _DT:
+        raise ValueError(f"q dtype {q.dtype} is not float16 / bfloat16 / float32")
+    Hkv, W, NP = _check_cache(pools, page_table, valid_tokens, q_lens, B, D)
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"query heads {Hq} must be a multiple of page-table heads {Hkv}")
+    for name, t in (("page_table", page_table), ("valid_tokens", valid_tokens), ("q_lens", q_lens)):
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if q.stride(-1) != 1:
+        raise ValueError("q must have a unit last stride")
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
+    elif out.shape != q.shape or out.stride(-1) != 1:
+        raise ValueError(f"out must have q's shape {tuple(q.shape)} and a unit last stride, got {tuple(out.shape)}")
+    if out.dtype not in _DT or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out dtype {out.dtype} is not {out_dtype or 'float16 / bfloat16 / float32'}")
+    o4 = out.unsqueeze(1) if out.dim() == 3 else out
+    a = N.MxAttentionArgs()
+    a.batch, a.q_len, a.num_q_heads, a.num_kv_heads, a.head_dim = B, L, Hq, Hkv, D
+    a.page_size, a.table_width, a.num_pages = PAGE_SIZE, W, NP
+    a.q, a.q_dtype, (a.q_stride_b, a.q_stride_t, a.q_stride_h, _) = q.data_ptr(), _DT[q.dtype], q4.stride()
+    a.out, a.out_dtype, (a.out_stride_b, a.out_stride_t, a.out_stride_h, _) = out.data_ptr(), _DT[out.dtype], o4.stride()
+    a.page_table, a.valid_tokens, a.q_lens = page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens)
+    a.k_codes, a.k_scales = pools.k_codes.data_ptr(), pools.k_scales.data_ptr()
+    a.v_codes, a.v_scales = pools.v_codes.data_ptr(), pools.v_scales.data_ptr()
+    a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    a.causal, a.splits = int(bool(causal)), int(splits)
+    return MxFp4Plan(a, dev, out, keep=(q, page_table, valid_tokens, q_lens, *pools.tensors().values()))
+
+
+def mxfp4_paged_attention(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor,
+                          *, q_lens: Optional[torch.Tensor] = None, causal: bool = True,
+                          sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                          out_dtype: Optional[torch.dtype] = None, splits: int = 0) -> torch.Tensor:
+    """Attention of the newest tokens over the cache.
+
+    q [B, Hq, D] (one token per sequence) or [B, L, Hq, D], float16, bfloat16 or float32.
+    Query i < q_lens[b] (default L) of head h reads row (b, h // (Hq // Hkv)) of the table and
+    sees its tokens up to its own, number valid_tokens - q_lens[b] + i, or with
+    ``causal=False`` all valid_tokens: out = softmax(sm_scale q . k) v, sm_scale = 1 / sqrt(D)
+    by default; zeros where a query sees nothing and for i >= q_lens[b]. ``splits``: parts
+    the rows' tokens are divided into (0: automatic). Returns ``out``, shaped as q."""
+    page_table, valid_tokens = page_table.contiguous(), valid_tokens.contiguous()
+    q_lens = None if q_lens is None else q_lens.contiguous()
+    if q.dim() and q.stride(-1) != 1:
+        q = q.contiguous()
+    plan = make_mxfp4_plan(q, pools, page_table, valid_tokens, q_lens=q_lens, causal=causal, sm_scale=sm_scale, out=out,
+                           out_dtype=out_dtype, splits=splits)
+    plan.run()
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return plan.out

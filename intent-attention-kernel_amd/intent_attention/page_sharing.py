@@ -1,0 +1,220 @@
+"""Pages of a KV cache handed out, shared, given back and moved, on the MI355X
+(``iak_grow_sequences``, ``iak_fork_sequences``, ``iak_free_sequences``,
+``iak_compact_pages``, ``iak_copy_pages``, include/iak.h).
+
+The state is three int32 tensors on the device, which a program keeps beside its pools
+(``PagePools``, ``LatentPools``, ``MxFp4Pools``, or any tensors with a row per page):
+
+  page_table    [B, R, W]  the pages of row (b, r): R = KV heads for K/V pools; a latent
+                           table [B, W] is passed as [B, 1, W]
+  valid_tokens  [B, R]     the tokens of each row; its first ceil(valid / 16) entries are in use
+  refs          [NP]       how many table entries (and other owners) hold a page; 0: free
+
+* ``grow_sequences`` makes room for new tokens: pages for them, the lowest free ids first;
+* ``fork_sequences`` makes empty sequences copies of others: full pages are shared, a last
+  page with room is copied, so that both may append;
+* ``free_sequences`` lets sequences go;
+* ``compact_pages`` moves the pages in use to the lowest ids and returns the new table;
+* ``copy_pages`` copies pages from id to id.
+
+Nothing waits for the device. Which page goes where is a function of the arguments alone.
+``grow_sequences`` and ``fork_sequences`` do all of a call or nothing of it, and return an
+int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
+of range or listed twice, a negative count, a row longer than its table, a forked sequence
+that has tokens or is itself a parent).
+"""
+from __future__ import annotations
+
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as N
+from .decode_core import PAGE_SIZE, PagePools, current_stream_handle, require_device
+from .mla_core import LatentPools
+from .mxfp4 import MxFp4Pools, _on
+
+Pools = Union[PagePools, LatentPools, MxFp4Pools, torch.Tensor, Sequence[torch.Tensor]]
+Indices = Union[torch.Tensor, Sequence[int]]
+
+
+def _pool_tensors(pools: Optional[Pools]) -> List[torch.Tensor]:
+    """The tensors of the pools, each once (K and V may be one pool)."""
+    if pools is None:
+        return []
+    if isinstance(pools, torch.Tensor):
+        ts: Iterable[torch.Tensor] = (pools,)
+    elif isinstance(pools, (PagePools, LatentPools, MxFp4Pools)):
+        ts = pools.tensors().values()
+    else:
+        ts = pools
+    seen, out = set(), []
+    for t in ts:
+        if (t.data_ptr(), t.numel() * t.element_size()) not in seen:
+            seen.add((t.data_ptr(), t.numel() * t.element_size()))
+            out.append(t)
+    return out
+
+
+def _fill_arrays(a, tensors: List[torch.Tensor], NP: int) -> None:
+    if len(tensors) > N.MAX_PAGE_ARRAYS:
+        raise ValueError(f"at most {N.MAX_PAGE_ARRAYS} pool tensors, got {len(tensors)}")
+    n = 0
+    for t in tensors:
+        if not t.is_contiguous() or t.dim() == 0 or NP == 0 or t.numel() % NP or t.shape[0] % NP:
+            if NP == 0 and t.numel() == 0:
+                continue
+            raise ValueError(f"every pool tensor must be contiguous with a row for each of {NP} pages, "
+                             f"got {tuple(t.shape)}")
+        row = t.numel() // NP * t.element_size()
+        if row:
+            a.arrays[n].base, a.arrays[n].row_bytes = t.data_ptr(), row
+            n += 1
+    a.num_arrays = n
+
+
+def _check_state(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor) -> Tuple[int, int, int, int]:
+    if page_table.dim() != 3 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise ValueError(f"page_table must be contiguous int32 [B, R, W], got {page_table.dtype} "
+                         f"{tuple(page_table.shape)}")
+    B, R, W = page_table.shape
+    if valid_tokens.shape != (B, R) or valid_tokens.dtype != torch.int32 or not valid_tokens.is_contiguous():
+        raise ValueError(f"valid_tokens must be contiguous int32 [{B}, {R}], got {valid_tokens.dtype} "
+                         f"{tuple(valid_tokens.shape)}")
+    if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous():
+        raise ValueError(f"refs must be contiguous int32 [num_pages], got {refs.dtype} {tuple(refs.shape)}")
+    if R == 0:
+        raise ValueError("page_table has no rows per sequence")
+    return B, R, W, refs.shape[0]
+
+
+def _indices(name: str, x: Indices, device: torch.device, count: Optional[int] = None) -> torch.Tensor:
+    """int32 [n] on the device; a list of ints is uploaded."""
+    if isinstance(x, torch.Tensor):
+        if x.dim() != 1 or x.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32 [n], got {x.dtype} {tuple(x.shape)}")
+        if x.device != device:
+            raise ValueError(f"{name} must be on {device}, got {x.device}")
+        x = x.contiguous()
+    else:
+        vals = [int(v) for v in x]
+        if any(not -2 ** 31 <= v < 2 ** 31 for v in vals):
+            raise ValueError(f"{name} must be int32 values")
+        x = torch.tensor(vals, dtype=torch.int32, device=device)
+    if count is not None and x.shape[0] != count:
+        raise ValueError(f"{name} must have {count} entries, got {x.shape[0]}")
+    return x
+
+
+def _sequences(what: str, page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
+               pools: Optional[Pools] = None):
+    tensors = _pool_tensors(pools)
+    dev = require_device(page_table, valid_tokens, refs, *tensors, what=what)
+    B, R, W, NP = _check_state(page_table, valid_tokens, refs)
+    seqs = _indices("seqs", seqs, dev)
+    a = N.SequencesArgs()
+    a.num_seqs, a.rows_per_seq, a.table_width, a.page_size, a.num_pages = B, R, W, PAGE_SIZE, NP
+    a.page_table, a.valid_tokens, a.refs = page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr()
+    a.count, a.seqs = seqs.shape[0], seqs.data_ptr()
+    _fill_arrays(a, tensors, NP)
+    return a, dev, seqs, tensors
+
+
+def _written(*tensors: torch.Tensor) -> None:
+    torch.autograd.graph.increment_version(tensors)     # written through raw pointers
+
+
+def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor]) -> torch.Tensor:
+    if missing is None:
+        missing = torch.empty(1, dtype=torch.int32, device=dev)
+    elif missing.shape != (1,) or missing.dtype != torch.int32 or missing.device != dev:
+        raise ValueError(f"missing must be int32 [1] on {dev}, got {missing.dtype} {tuple(missing.shape)}")
+    a.missing = missing.data_ptr()
+    size = N.sequences_workspace(a)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        launch(a, current_stream_handle(dev), ws.data_ptr(), size)
+    return missing
+
+
+def grow_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
+                   new_tokens: Indices, *, missing: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Room for ``new_tokens[i]`` more tokens in every row of sequence ``seqs[i]``: the table
+    entries they need get free pages (the lowest ids first, in the order of i, row, entry),
+    refs 1, and valid_tokens grows. All or nothing; returns ``missing`` (module docstring)."""
+    a, dev, seqs, _ = _sequences("page allocation", page_table, valid_tokens, refs, seqs)
+    new_tokens = _indices("new_tokens", new_tokens, dev, seqs.shape[0])
+    a.new_tokens = new_tokens.data_ptr()
+    missing = _planned(N.grow_sequences, a, dev, missing)
+    _written(page_table, valid_tokens, refs, missing)
+    return missing
+
+
+def fork_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, parents: Indices,
+                   children: Indices, pools: Optional[Pools] = None, *,
+                   missing: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sequence ``children[i]``, which has no tokens, becomes a copy of ``parents[i]``: it shares
+    the parent's pages (refs + 1), except that a last page which is not full is copied, in
+    every tensor of ``pools``, to a free page. All or nothing; returns ``missing``
+    (module docstring). A parent may be listed many times."""
+    a, dev, children, tensors = _sequences("page sharing", page_table, valid_tokens, refs, children, pools)
+    parents = _indices("parents", parents, dev, children.shape[0])
+    a.parents = parents.data_ptr()
+    missing = _planned(N.fork_sequences, a, dev, missing)
+    _written(page_table, valid_tokens, refs, missing, *tensors)
+    return missing
+
+
+def free_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices) -> None:
+    """Let go of every page of sequences ``seqs``: refs - 1 for each entry in use, the entries
+    become -1 and the lengths 0. Indices outside the table are left out, one listed twice is
+    freed once."""
+    a, dev, seqs, _ = _sequences("page sharing", page_table, valid_tokens, refs, seqs)
+    with _on(dev):
+        N.free_sequences(a, current_stream_handle(dev))
+    _written(page_table, valid_tokens, refs)
+
+
+def compact_pages(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor,
+                  pools: Optional[Pools] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(new page_table, new refs, page_map): with L pages in use, those with ids >= L move to
+    the free ids below L (the highest to the lowest), in place in every tensor of ``pools``.
+    page_map [NP] int32 is the new id of every page, -1 for free ones: owners other than the
+    table look theirs up in it. The arguments' table and refs stay as they are and the moved
+    pages' old rows keep their bytes, so what was queued with the old table still finds them
+    until their ids are handed out again."""
+    tensors = _pool_tensors(pools)
+    dev = require_device(page_table, valid_tokens, refs, *tensors, what="page compaction")
+    B, R, W, NP = _check_state(page_table, valid_tokens, refs)
+    table, new_refs, page_map = torch.empty_like(page_table), torch.empty_like(refs), torch.empty_like(refs)
+    a = N.CompactPagesArgs()
+    a.num_rows, a.table_width, a.page_size, a.num_pages = B * R, W, PAGE_SIZE, NP
+    a.page_table, a.valid_tokens, a.refs = page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr()
+    a.out_table, a.out_refs, a.page_map = table.data_ptr(), new_refs.data_ptr(), page_map.data_ptr()
+    _fill_arrays(a, tensors, NP)
+    size = N.compact_pages_workspace(a)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        N.compact_pages(a, current_stream_handle(dev), ws.data_ptr(), size)
+    if tensors:
+        _written(*tensors)
+    return table, new_refs, page_map
+
+
+def copy_pages(pools: Pools, src: Indices, dst: Indices, *, num_pages: Optional[int] = None) -> None:
+    """Page ``src[i]`` of every pool tensor to page ``dst[i]``. Pairs with an id outside the pools
+    are left out. The dst ids must be distinct, and none of them a src of another pair.
+    ``num_pages``: the pages of the pools (default: the first tensor's rows)."""
+    tensors = _pool_tensors(pools)
+    if not tensors:
+        raise ValueError("no pool tensor given")
+    dev = require_device(*tensors, what="page copy")
+    NP = tensors[0].shape[0] if num_pages is None else int(num_pages)
+    src = _indices("src", src, dev)
+    dst = _indices("dst", dst, dev, src.shape[0])
+    a = N.CopyPagesArgs()
+    a.num_pages, a.count, a.src, a.dst = NP, src.shape[0], src.data_ptr(), dst.data_ptr()
+    _fill_arrays(a, tensors, NP)
+    with _on(dev):
+        N.copy_pages(a, current_stream_handle(dev))
+    _written(*tensors)
