@@ -23,6 +23,15 @@ iak_status fail(iak_status st, const char* fmt, ...) {
   return st;
 }
 
+}  // namespace
+
+namespace iak {
+iak_status report(iak_status st, const char* text);   // mx_internal.h: the error text for entry points in other files
+iak_status report(iak_status st, const char* text) { return fail(st, "%s", text); }
+}  // namespace iak
+
+namespace {
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 const char* tag_name(int t) {
@@ -371,147 +380,6 @@ iak_status scratch_address(int dev, void** out) {
   }
   *out = g_scratch_ptr[dev];
   return IAK_OK;
-}
-
-// --------------------------------------------------------------------------- //
-// 4-bit token cache and page sharing
-// --------------------------------------------------------------------------- //
-
-iak_status launched(hipError_t e, const char* what) {
-  return e == hipSuccess ? IAK_OK : fail(IAK_EHIP, "%s launch: %s", what, hipGetErrorString(e));
-}
-
-// what the 4-bit cache's entry points have in common
-iak_status validate_mx_cache(int batch, int count, int kv_heads, int head_dim, int page_size, int width, int64_t num_pages) {
-  if (batch < 0 || count < 0 || kv_heads <= 0 || width < 0 || num_pages < 0)
-    return fail(IAK_EINVAL, "negative or zero size (batch=%d, tokens=%d, num_kv_heads=%d, table_width=%d, num_pages=%lld)", batch,
-                count, kv_heads, width, (long long)num_pages);
-  if (head_dim != 64 && head_dim != 128) return fail(IAK_ENOTSUP, "head_dim %d is not supported (64 or 128)", head_dim);
-  if (page_size != 16) return fail(IAK_ENOTSUP, "page_size %d is not supported (16)", page_size);
-  if (num_pages > 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)num_pages);
-  if (width > 0x7FFFFFF) return fail(IAK_EINVAL, "table_width %d: a row's tokens exceed int32", width);
-  return IAK_OK;
-}
-
-iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
-  if (!a) return fail(IAK_EINVAL, "args is NULL");
-  iak_status st = validate_mx_cache(a->batch, a->count, a->num_kv_heads, a->head_dim, a->page_size, a->table_width, a->num_pages);
-  if (st != IAK_OK) return st;
-  if (a->dtype < 0 || a->dtype > 2) return fail(IAK_EINVAL, "bad dtype %d", a->dtype);
-  if (a->batch == 0 || a->count == 0) return IAK_OK;
-  // one thread per 8 channels, fewer than 2^32 of them in a launch
-  if ((double)a->batch * a->count * a->num_kv_heads * (a->head_dim / 8) > 4.0e9)
-    return fail(IAK_EINVAL, "too many tokens for one call (%d x %d x %d heads)", a->batch, a->count, a->num_kv_heads);
-  if (!a->k || !a->v) return fail(IAK_EINVAL, "k/v is NULL");
-  if (!a->page_table && a->table_width > 0) return fail(IAK_EINVAL, "page_table is NULL");
-  if (!a->valid_tokens) return fail(IAK_EINVAL, "valid_tokens is NULL");
-  if (a->num_pages > 0 && (!a->k_codes || !a->k_scales || !a->v_codes || !a->v_scales))
-    return fail(IAK_EINVAL, "a code or scale pool is NULL");
-  if ((reinterpret_cast<uintptr_t>(a->k_codes) | reinterpret_cast<uintptr_t>(a->v_codes)) & 3u)
-    return fail(IAK_EINVAL, "code pools must be 4-byte aligned");
-  return IAK_OK;
-}
-
-struct MxPlan {
-  int G, tiles, splits, chunk;
-  int64_t items;
-  size_t ws_m, ws_l, ws_acc, total;
-};
-
-iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
-  if (!a) return fail(IAK_EINVAL, "args is NULL");
-  iak_status st = validate_mx_cache(a->batch, a->q_len, a->num_kv_heads, a->head_dim, a->page_size, a->table_width, a->num_pages);
-  if (st != IAK_OK) return st;
-  if (a->num_q_heads <= 0 || a->num_q_heads % a->num_kv_heads != 0)
-    return fail(IAK_EINVAL, "num_q_heads %d is not a multiple of num_kv_heads %d", a->num_q_heads, a->num_kv_heads);
-  if (a->q_dtype < 0 || a->q_dtype > 2 || a->out_dtype < 0 || a->out_dtype > 2)
-    return fail(IAK_EINVAL, "bad q/out dtype (%d, %d)", a->q_dtype, a->out_dtype);
-  if (!std::isfinite(a->sm_scale)) return fail(IAK_EINVAL, "sm_scale is not finite");
-  if (a->causal != 0 && a->causal != 1) return fail(IAK_EINVAL, "causal must be 0 or 1, got %d", a->causal);
-  if (a->splits < 0) return fail(IAK_EINVAL, "splits %d is negative", a->splits);
-  *p = MxPlan{};
-  p->G = a->num_q_heads / a->num_kv_heads;
-  if (a->batch == 0 || a->q_len == 0) return IAK_OK;
-  if (!a->q || !a->out) return fail(IAK_EINVAL, "q/out is NULL");
-  if (!a->page_table && a->table_width > 0) return fail(IAK_EINVAL, "page_table is NULL");
-  if (!a->valid_tokens) return fail(IAK_EINVAL, "valid_tokens is NULL");
-  if (a->num_pages > 0 && (!a->k_codes || !a->k_scales || !a->v_codes || !a->v_scales))
-    return fail(IAK_EINVAL, "a code or scale pool is NULL");
-  if (!aligned16(a->k_codes) || !aligned16(a->v_codes)) return fail(IAK_EINVAL, "code pools must be 16-byte aligned");
-  const int64_t rows = (int64_t)a->q_len * p->G;
-  if (rows > 0x3FFFFFFF) return fail(IAK_EINVAL, "q_len %d x %d heads per KV head is too long", a->q_len, p->G);
-  p->tiles = (int)((rows + 15) / 16);
-  const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
-  if (tiles > 3.0e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
-  const int W = a->table_width > 0 ? a->table_width : 1;
-  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(4096.0 / tiles);
-  if (splits > (W + 3) / 4) splits = (W + 3) / 4;
-  if (splits < 1) splits = 1;
-  while (splits > 1 && tiles * splits > 6.0e7) splits /= 2;
-  p->chunk = (int)((W + splits - 1) / splits);
-  if (p->chunk & 1) ++p->chunk;
-  p->splits = (W + p->chunk - 1) / p->chunk;
-  p->items = (int64_t)tiles * p->splits;
-  if (p->splits > 1) {
-    const size_t slots = (size_t)p->items * 16;
-    p->ws_m = 0;
-    p->ws_l = round_up(4 * slots);
-    p->ws_acc = p->ws_l + round_up(4 * slots);
-    p->total = p->ws_acc + round_up(4 * slots * (size_t)a->head_dim);
-  }
-  return IAK_OK;
-}
-
-iak_status validate_arrays(int n, const iak_page_array* arrays, int64_t num_pages) {
-  if (n < 0 || n > IAK_MAX_PAGE_ARRAYS) return fail(IAK_EINVAL, "num_arrays %d outside [0, %d]", n, IAK_MAX_PAGE_ARRAYS);
-  for (int k = 0; k < n; ++k) {
-    if (arrays[k].row_bytes <= 0 || arrays[k].row_bytes > (1LL << 31))
-      return fail(IAK_EINVAL, "array %d: row_bytes %lld", k, (long long)arrays[k].row_bytes);
-    if (!arrays[k].base && num_pages > 0) return fail(IAK_EINVAL, "array %d is NULL", k);
-  }
-  return IAK_OK;
-}
-
-bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-
-iak_status validate_sequences(const iak_sequences_args* a) {
-  if (!a) return fail(IAK_EINVAL, "args is NULL");
-  if (a->num_seqs < 0 || a->rows_per_seq <= 0 || a->table_width < 0 || a->page_size <= 0 || a->num_pages < 0 || a->count < 0)
-    return fail(IAK_EINVAL, "bad size (num_seqs=%d, rows_per_seq=%d, table_width=%d, page_size=%d, num_pages=%lld, count=%d)",
-                a->num_seqs, a->rows_per_seq, a->table_width, a->page_size, (long long)a->num_pages, a->count);
-  if (a->num_pages > 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)a->num_pages);
-  if ((double)a->table_width * a->page_size > 2147483647.0)
-    return fail(IAK_EINVAL, "table_width %d x page_size %d: a row's tokens exceed int32", a->table_width, a->page_size);
-  // one workgroup of 256 threads per listed row
-  if ((double)a->count * a->rows_per_seq > 1.6e7) return fail(IAK_EINVAL, "too many rows for one call (%d x %d)", a->count, a->rows_per_seq);
-  if (a->count > 0 && !a->seqs) return fail(IAK_EINVAL, "seqs is NULL");
-  if (a->num_seqs > 0 && (!a->valid_tokens || (!a->page_table && a->table_width > 0)))
-    return fail(IAK_EINVAL, "page_table/valid_tokens is NULL");
-  if (a->num_pages > 0 && !a->refs) return fail(IAK_EINVAL, "refs is NULL");
-  if (!aligned4(a->page_table) || !aligned4(a->valid_tokens) || !aligned4(a->refs) || !aligned4(a->seqs))
-    return fail(IAK_EINVAL, "int32 arrays must be 4-byte aligned");
-  return IAK_OK;
-}
-
-// grow and fork: `null`: the name of an argument they need and did not get
-iak_status validate_planned(const iak_sequences_args* a, const char* null, const void* workspace, size_t workspace_bytes) {
-  if (null) return fail(IAK_EINVAL, "%s is NULL", null);
-  if (!a->missing) return fail(IAK_EINVAL, "missing is NULL");
-  const size_t need = iak::sequences_workspace(*a);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
-    return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", need, workspace_bytes, workspace);
-  return IAK_OK;
-}
-
-iak_status validate_compact(const iak_compact_pages_args* a) {
-  if (!a) return fail(IAK_EINVAL, "args is NULL");
-  if (a->num_rows < 0 || a->table_width < 0 || a->page_size <= 0 || a->num_pages < 0 || a->num_pages > 0x7FFFFFFFLL)
-    return fail(IAK_EINVAL, "bad size (num_rows=%d, table_width=%d, page_size=%d, num_pages=%lld)", a->num_rows, a->table_width,
-                a->page_size, (long long)a->num_pages);
-  if (a->num_pages > 0 && (!a->refs || !a->out_refs || !a->page_map)) return fail(IAK_EINVAL, "refs, out_refs or page_map is NULL");
-  if ((int64_t)a->num_rows * a->table_width > 0 && (!a->page_table || !a->out_table || !a->valid_tokens))
-    return fail(IAK_EINVAL, "page_table, out_table or valid_tokens is NULL");
-  return validate_arrays(a->num_arrays, a->arrays, a->num_pages);
 }
 
 }  // namespace
@@ -1090,115 +958,6 @@ iak_status iak_build_page_tables(const iak_page_table_args* a, void* stream) {
   const hipError_t e = iak::launch_page_tables(*a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(IAK_EHIP, "kernel launch failed: %s", hipGetErrorString(e));
   return IAK_OK;
-}
-
-iak_status iak_mx_append_tokens(const iak_mx_tokens_args* a, void* stream) {
-  iak_status st = validate_mx_tokens(a);
-  if (st != IAK_OK) return st;
-  if (a->batch == 0 || a->count == 0) return IAK_OK;
-  return launched(iak::launch_mx_append(*a, reinterpret_cast<hipStream_t>(stream)), "append");
-}
-
-iak_status iak_mx_read_tokens(const iak_mx_tokens_args* a, void* stream) {
-  iak_status st = validate_mx_tokens(a);
-  if (st != IAK_OK) return st;
-  if (a->batch == 0 || a->count == 0) return IAK_OK;
-  return launched(iak::launch_mx_read(*a, reinterpret_cast<hipStream_t>(stream)), "read");
-}
-
-iak_status iak_mx_attention_workspace(const iak_mx_attention_args* args, size_t* bytes) {
-  if (!bytes) return fail(IAK_EINVAL, "bytes is NULL");
-  MxPlan p;
-  iak_status st = validate_mx_attention(args, &p);
-  if (st != IAK_OK) return st;
-  *bytes = p.total;
-  return IAK_OK;
-}
-
-iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  MxPlan p;
-  iak_status st = validate_mx_attention(a, &p);
-  if (st != IAK_OK) return st;
-  if (a->batch == 0 || a->q_len == 0) return IAK_OK;
-  if (p.total > 0 && (!workspace || workspace_bytes < p.total || !aligned16(workspace)))
-    return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", p.total, workspace_bytes, workspace);
-  iak::MxAttn k;
-  k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
-  k.W = a->table_width; k.NP = a->num_pages;
-  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.items = p.items;
-  k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
-  k.q_vec = aligned16(a->q) && (a->q_stride_b | a->q_stride_t | a->q_stride_h) % (a->q_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
-  k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;
-  k.out_vec = aligned16(a->out) && (a->out_stride_b | a->out_stride_t | a->out_stride_h) % (a->out_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
-  k.table = a->page_table; k.valid = a->valid_tokens; k.q_lens = a->q_lens;
-  k.k_codes = reinterpret_cast<const uint8_t*>(a->k_codes); k.k_scales = reinterpret_cast<const uint8_t*>(a->k_scales);
-  k.v_codes = reinterpret_cast<const uint8_t*>(a->v_codes); k.v_scales = reinterpret_cast<const uint8_t*>(a->v_scales);
-  k.score_mult = a->sm_scale * 1.44269504088896340736f;
-  k.causal = a->causal;
-  char* ws = reinterpret_cast<char*>(workspace);
-  k.ws_m = reinterpret_cast<float*>(ws + p.ws_m);
-  k.ws_l = reinterpret_cast<float*>(ws + p.ws_l);
-  k.ws_acc = reinterpret_cast<float*>(ws + p.ws_acc);
-  return launched(iak::launch_mx_attention(k, reinterpret_cast<hipStream_t>(stream)), "4-bit cache attention");
-}
-
-iak_status iak_copy_pages(const iak_copy_pages_args* a, void* stream) {
-  if (!a) return fail(IAK_EINVAL, "args is NULL");
-  if (a->num_pages < 0 || a->num_pages > 0x7FFFFFFFLL || a->count < 0)
-    return fail(IAK_EINVAL, "bad size (num_pages=%lld, count=%d)", (long long)a->num_pages, a->count);
-  iak_status st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
-  if (st != IAK_OK) return st;
-  if (a->count == 0 || a->num_arrays == 0 || a->num_pages == 0) return IAK_OK;
-  if (!a->src || !a->dst) return fail(IAK_EINVAL, "src/dst is NULL");
-  return launched(iak::launch_copy_pages(*a, reinterpret_cast<hipStream_t>(stream)), "page copy");
-}
-
-iak_status iak_sequences_workspace(const iak_sequences_args* a, size_t* bytes) {
-  if (!bytes) return fail(IAK_EINVAL, "bytes is NULL");
-  iak_status st = validate_sequences(a);
-  if (st != IAK_OK) return st;
-  *bytes = iak::sequences_workspace(*a);
-  return IAK_OK;
-}
-
-iak_status iak_free_sequences(const iak_sequences_args* a, void* stream) {
-  iak_status st = validate_sequences(a);
-  if (st != IAK_OK) return st;
-  if (a->count == 0 || a->num_seqs == 0) return IAK_OK;
-  return launched(iak::launch_free_sequences(*a, reinterpret_cast<hipStream_t>(stream)), "free sequences");
-}
-
-iak_status iak_grow_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  iak_status st = validate_sequences(a);
-  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->new_tokens ? "new_tokens" : nullptr, workspace, workspace_bytes);
-  if (st != IAK_OK) return st;
-  return launched(iak::launch_grow_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "grow sequences");
-}
-
-iak_status iak_fork_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  iak_status st = validate_sequences(a);
-  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->parents ? "parents" : nullptr, workspace, workspace_bytes);
-  if (st == IAK_OK) st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
-  if (st != IAK_OK) return st;
-  return launched(iak::launch_fork_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "fork sequences");
-}
-
-iak_status iak_compact_pages_workspace(const iak_compact_pages_args* a, size_t* bytes) {
-  if (!bytes) return fail(IAK_EINVAL, "bytes is NULL");
-  iak_status st = validate_compact(a);
-  if (st != IAK_OK) return st;
-  *bytes = iak::compact_workspace(*a);
-  return IAK_OK;
-}
-
-iak_status iak_compact_pages(const iak_compact_pages_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  iak_status st = validate_compact(a);
-  if (st != IAK_OK) return st;
-  if (a->num_pages == 0 && (int64_t)a->num_rows * a->table_width == 0) return IAK_OK;
-  const size_t need = iak::compact_workspace(*a);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
-    return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", need, workspace_bytes, workspace);
-  return launched(iak::launch_compact_pages(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "compact pages");
 }
 
 }  // extern "C"

@@ -133,41 +133,6 @@ hipError_t launch_transcode(const iak_transcode_args& a, hipStream_t stream);
 
 hipError_t launch_prefetch(const iak_prefetch_args& a, hipStream_t stream);
 
-// Kernel-side arguments of the 4-bit cache's attention (built from iak_mx_attention_args).
-struct MxAttn {
-  int B, L, Hq, Hkv, G, D, W;
-  int64_t NP;
-  int tiles;      // tiles of 16 query rows (query token * G + head of the group) per KV row
-  int splits;     // parts of `chunk` table entries (even, when there are several) per tile
-  int chunk;
-  int64_t items;  // B * Hkv * tiles * splits
-
-  const void* q; int q_dtype; int q_vec; int64_t qsb, qst, qsh;          // *_vec: rows lie on 16 bytes
-  void* out; int out_dtype; int out_vec; int64_t osb, ost, osh;
-  const int32_t* table;
-  const int32_t* valid;
-  const int32_t* q_lens;   // may be null
-  const uint8_t* k_codes; const uint8_t* k_scales; const uint8_t* v_codes; const uint8_t* v_scales;
-  float score_mult;        // sm_scale * log2(e)
-  int causal;
-
-  float* ws_m;             // [B, Hkv, tiles, splits, 16]
-  float* ws_l;
-  float* ws_acc;           // [B, Hkv, tiles, splits, 16, D]
-};
-
-hipError_t launch_mx_append(const iak_mx_tokens_args& a, hipStream_t stream);
-hipError_t launch_mx_read(const iak_mx_tokens_args& a, hipStream_t stream);
-hipError_t launch_mx_attention(const MxAttn& a, hipStream_t stream);
-
-hipError_t launch_copy_pages(const iak_copy_pages_args& a, hipStream_t stream);
-size_t sequences_workspace(const iak_sequences_args& a);
-hipError_t launch_free_sequences(const iak_sequences_args& a, hipStream_t stream);
-hipError_t launch_grow_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream);
-hipError_t launch_fork_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream);
-size_t compact_workspace(const iak_compact_pages_args& a);
-hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace, hipStream_t stream);
-
 }  // namespace iak
 
 #endif

@@ -7,7 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "iak_internal.h"
+#include "iak_device.h"
+#include "mx_internal.h"
 
 namespace iak {
 

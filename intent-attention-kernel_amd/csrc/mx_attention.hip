@@ -19,7 +19,7 @@
 #include <stdint.h>
 
 #include "iak.h"
-#include "iak_internal.h"
+#include "mx_internal.h"
 #include "mx_format.h"
 #include "mx_attention.h"
 

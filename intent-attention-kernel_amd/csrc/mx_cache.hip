@@ -13,7 +13,7 @@
 #include <stdint.h>
 
 #include "iak.h"
-#include "iak_internal.h"
+#include "mx_internal.h"
 #include "mx_format.h"
 
 namespace iak {

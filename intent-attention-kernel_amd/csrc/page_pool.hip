@@ -17,7 +17,7 @@
 #include <stdint.h>
 
 #include "iak.h"
-#include "iak_internal.h"
+#include "mx_internal.h"
 #include "iak_device.h"
 
 namespace iak {
