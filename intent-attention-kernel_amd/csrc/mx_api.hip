@@ -60,7 +60,7 @@ iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
 }
 
 struct MxPlan {
-  int G, tiles, splits, chunk;
+  int G, tiles, splits, chunk, waves;
   int64_t items;
   size_t ws_m, ws_l, ws_acc, total;
 };
@@ -89,15 +89,17 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   if (rows > 0x3FFFFFFF) return fail(IAK_EINVAL, "q_len %d x %d heads per KV head is too long", a->q_len, p->G);
   p->tiles = (int)((rows + 15) / 16);
   const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
-  if (tiles > 3.0e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
+  if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
   const int W = a->table_width > 0 ? a->table_width : 1;
-  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(4096.0 / tiles);
-  if (splits > (W + 3) / 4) splits = (W + 3) / 4;
+  // about 2,048 workgroups of four waves (two for each place on the card), of at least 32
+  // entries each; a row of few entries is one workgroup's, of sixteen waves when the grid is small
+  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(2048.0 / tiles);
+  if (splits > (W + 31) / 32) splits = (W + 31) / 32;
   if (splits < 1) splits = 1;
-  while (splits > 1 && tiles * splits > 6.0e7) splits /= 2;
+  while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
-  if (p->chunk & 1) ++p->chunk;
   p->splits = (W + p->chunk - 1) / p->chunk;
+  p->waves = p->splits == 1 && tiles < 512 && W > 8 ? 16 : 4;
   p->items = (int64_t)tiles * p->splits;
   if (p->splits > 1) {
     const size_t slots = (size_t)p->items * 16;
@@ -196,7 +198,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   iak::MxAttn k;
   k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
-  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.items = p.items;
+  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.waves = p.waves; k.items = p.items;
   k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
   k.q_vec = aligned16(a->q) && (a->q_stride_b | a->q_stride_t | a->q_stride_h) % (a->q_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
   k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;

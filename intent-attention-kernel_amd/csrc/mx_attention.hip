@@ -1,8 +1,9 @@
 // Attention of one or several query tokens per sequence over the microscaled 4-bit cache,
 // for gfx950:  out = softmax(sm_scale q . k) v  over the tokens that a query sees.
 //
-// A wave takes a tile of 16 query rows that share a KV head (row = query token * G + head of
-// the group) and one split of the head's table entries, two pages (32 tokens) a step.
+// A workgroup takes a tile of 16 query rows that share a KV head (row = query token * G +
+// head of the group) and one split of the head's table entries; its waves share the entries
+// out in pairs of pages (32 tokens), one pair a step, and their sums meet in LDS at the end.
 // Lane = c + 16 g (c = lane % 16, g = lane / 16):
 //   scores  S^T[16 tok x 16 rows] = K . Q^T, v_mfma_f32_16x16x32_f16. A lane loads token c's
 //           codes of channels (D/4) g .. : its 16 bytes are one scale block (D = 128), so one
@@ -27,7 +28,9 @@ namespace iak {
 
 namespace {
 
-constexpr int MX_WAVES = 4;
+#ifndef MXOCC
+#define MXOCC 3
+#endif
 constexpr float P_SHIFT = 6.0f;          // weights <= 2^(6 + RESCALE_SLACK) = 2^14
 constexpr float M_NONE = -3.402823466e38f;
 
@@ -44,26 +47,30 @@ template <int D> __device__ __forceinline__ int v_chunk(int t, int ch) {
 template <int D> struct MxPair {   // two pages as a lane loads them
   uint32_t k[2][D / 32], v[2][D / 32];
   uint32_t ks[2], vs[2];
+  int id[2];                       // wave-uniform; -1: no page
 };
 
 template <int D>
-__device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, const int (&id)[2], int c, int g) {
+__device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0, int id1, int c, int g) {
+  r.id[0] = id0;
+  r.id[1] = id1;
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    const int64_t page = id[p] < 0 ? 0 : id[p];
-    const int64_t code = (page * PS + c) * (D / 2) + g * (D / 8);
-    const int64_t sc = (page * PS + c) * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK;
+    const int64_t page = r.id[p] < 0 ? 0 : r.id[p];
+    const uint32_t code = c * (D / 2) + g * (D / 8), sc = c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK;
+    const uint8_t* kc = a.k_codes + page * (PS * D / 2);
+    const uint8_t* vc = a.v_codes + page * (PS * D / 2);
     if constexpr (D == 128) {
-      const u4 k = *reinterpret_cast<const u4*>(a.k_codes + code), v = *reinterpret_cast<const u4*>(a.v_codes + code);
+      const u4 k = *reinterpret_cast<const u4*>(kc + code), v = *reinterpret_cast<const u4*>(vc + code);
 #pragma unroll
       for (int i = 0; i < 4; ++i) { r.k[p][i] = k[i]; r.v[p][i] = v[i]; }
     } else {
-      const u2 k = *reinterpret_cast<const u2*>(a.k_codes + code), v = *reinterpret_cast<const u2*>(a.v_codes + code);
+      const u2 k = *reinterpret_cast<const u2*>(kc + code), v = *reinterpret_cast<const u2*>(vc + code);
 #pragma unroll
       for (int i = 0; i < 2; ++i) { r.k[p][i] = k[i]; r.v[p][i] = v[i]; }
     }
-    r.ks[p] = a.k_scales[sc];
-    r.vs[p] = a.v_scales[sc];
+    r.ks[p] = (a.k_scales + page * (PS * D / MX_BLOCK))[sc];
+    r.vs[p] = (a.v_scales + page * (PS * D / MX_BLOCK))[sc];
   }
 }
 
@@ -86,15 +93,17 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
   else out4(reinterpret_cast<__bf16*>(a.out) + at, a.out_vec, x);
 }
 
-template <int D, bool QF32>
-__global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) {
-  __shared__ u4 vt[MX_WAVES][2 * PS * D / 8];
+// Entry i of the wave's own, of those that the workgroup's NW waves share out in pairs.
+template <int NW> __device__ __forceinline__ int wave_entry(int w, int i) { return 2 * (w + NW * (i >> 1)) + (i & 1); }
+
+template <int D, bool QF32, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows_kernel(const MxAttn a) {
+  __shared__ u4 vt[NW][2 * PS * D / 8];                          // V rows; at the end the waves' sums
+  __shared__ float part_m[NW][16], part_l[NW][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const int64_t item = (int64_t)blockIdx.x * MX_WAVES + w;
-  if (item >= a.items) return;                                   // no barriers below
-  const int split = (int)(item % a.splits);
-  const int64_t tile_at = item / a.splits;
+  const int split = (int)(blockIdx.x % a.splits);
+  const int64_t tile_at = blockIdx.x / a.splits;
   const int tile = (int)(tile_at % a.tiles);
   const int64_t kvrow = tile_at / a.tiles;
   const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
@@ -109,6 +118,16 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) 
   int least = live ? seen : 0x7FFFFFFF;                          // tokens below it need no mask
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
+
+  // the wave's entries, 64 at a time: lane i holds number i of the block, `next` the block after
+  const int32_t* row = a.table + kvrow * a.W;
+  auto entry_id = [&](int k) {
+    const int e = e0 + wave_entry<NW>(w, k);
+    const int id = e < e1 ? row[e] : -1;
+    return id < 0 || id >= a.NP ? -1 : id;
+  };
+  int ids = entry_id(lane), next = e0 + 64 * NW < e1 ? entry_id(64 + lane) : -1;
+  auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
 
   // queries: scaled by a power of two to a largest element in [2^14, 2^15)
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
@@ -153,18 +172,9 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) 
 #pragma unroll
   for (int mb = 0; mb < D / 16; ++mb) acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
   float m = M_NONE, l = 0.f;
-  const int32_t* row = a.table + kvrow * a.W;
 
-  for (int e = e0; e < e1; e += 2) {
-    int id[2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      id[p] = e + p < e1 ? row[e + p] : -1;
-      if (id[p] < 0 || id[p] >= a.NP) id[p] = -1;
-    }
-    MxPair<D> x;
-    load_pair<D>(x, a, id, c, g);
-
+  // one step: the pair `x` of entries e, e + 1
+  auto step = [&](const MxPair<D>& x, int e) {
     f4 s[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -188,8 +198,8 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) 
           if ((t >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
       }
       // tokens that a row does not see
-      if ((e + p + 1) * PS > least || id[p] < 0) {
-        const int lim = id[p] < 0 ? 0 : seen - (e + p) * PS;
+      if ((e + p + 1) * PS > least || x.id[p] < 0) {
+        const int lim = x.id[p] < 0 ? 0 : seen - (e + p) * PS;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (4 * g + q >= lim) s[p][q] = -__builtin_inff();
@@ -208,11 +218,12 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) 
       m = mn;
     }
     h8 pb, pl;
+    const float base = m - P_SHIFT;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float v = __builtin_amdgcn_exp2f(s[p][q] - m + P_SHIFT);
+        const float v = __builtin_amdgcn_exp2f(s[p][q] - base);
         l += v;
         pb[4 * p + q] = (_Float16)v;
         if constexpr (QF32) pl[4 * p + q] = (_Float16)(v - (float)pb[4 * p + q]);
@@ -232,83 +243,126 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx_rows_kernel(const MxAttn a) 
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     typedef __attribute__((address_space(3))) s4v lds_s4;
-    const char* base = reinterpret_cast<const char*>(&vt[w][0]);
+    const char* from = reinterpret_cast<const char*>(&vt[w][0]);
 #pragma unroll
     for (int mb = 0; mb < D / 16; ++mb) {
       s4v t[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const int at = p * (PS * D / 8) + v_chunk<D>(4 * g + (c >> 2), 2 * mb + ((c & 3) >> 1));
-        t[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + at * 16 + (c & 1) * 8));
+        t[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + at * 16 + (c & 1) * 8));
       }
       const h8 va = __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
       acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[mb], 0, 0, 0);
       if constexpr (QF32) acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[mb], 0, 0, 0);
     }
+  };
+
+  // the next pair's loads are under way while a pair is worked on
+  MxPair<D> x, y;
+  int at = e0 + 2 * w, k = 0, block = 0;                         // the pair's first entry, its number in the block
+  if (at < e1) load_pair<D>(x, a, page(0), page(1), c, g);
+  while (at < e1) {
+    const int to = at + 2 * NW;
+    if (to < e1) load_pair<D>(y, a, page(k + 2), page(k + 3), c, g);
+    step(x, at);
+    x = y;
+    at = to;
+    k += 2;
+    if (k == 64) {
+      k = 0;
+      block += 64;
+      ids = next;
+      next = at + 64 * NW < e1 ? entry_id(block + 64 + lane) : -1;
+    }
   }
 
+  // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
   l = xsum16_32(l);
-  if (!active) return;
-  if (a.splits > 1) {
-    const int64_t slot = (tile_at * a.splits + split) * 16 + c;
-    if (g == 0) { a.ws_m[slot] = m; a.ws_l[slot] = l; }
+  __syncthreads();
+  if (g == 0) { part_m[w][c] = m; part_l[w][c] = l; }
+  f4* sums = reinterpret_cast<f4*>(&vt[w][0]);
 #pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb) *reinterpret_cast<f4*>(a.ws_acc + slot * D + 16 * mb + 4 * g) = acc[mb];
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;                   // NaN stays
-  const int64_t at = b * a.osb + i * a.ost + head * a.osh + 4 * g;
+  for (int mb = 0; mb < D / 16; ++mb) sums[c * (D / 4) + ((4 * mb + g) ^ c)] = acc[mb];
+  __syncthreads();
+  const int rows = a.L * a.G - tile * 16 < 16 ? a.L * a.G - tile * 16 : 16;
+  for (int k2 = threadIdx.x; k2 < rows * (D / 4); k2 += 64 * NW) {
+    const int cr = k2 / (D / 4), u = k2 - cr * (D / 4);
+    float M = part_m[0][cr], L = 0.f;
 #pragma unroll
-  for (int mb = 0; mb < D / 16; ++mb) {
-    float o[4];
+    for (int v = 1; v < NW; ++v) M = fmaxf(M, part_m[v][cr]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = live ? acc[mb][q] * inv : 0.f;
-    store_out4(a, at + 16 * mb, o);
+    for (int v = 0; v < NW; ++v) {
+      const float wgt = __builtin_amdgcn_exp2f(part_m[v][cr] - M);
+      L += wgt * part_l[v][cr];
+      o += reinterpret_cast<const f4*>(&vt[v][0])[cr * (D / 4) + (u ^ cr)] * wgt;
+    }
+    if (a.splits > 1) {
+      const int64_t slot = (int64_t)blockIdx.x * 16 + cr;
+      if (u == 0) { a.ws_m[slot] = M; a.ws_l[slot] = L; }
+      *reinterpret_cast<f4*>(a.ws_acc + slot * D + 4 * u) = o;
+    } else {
+      const int rr = tile * 16 + cr, ir = rr / a.G;
+      const float inv = L == 0.f ? 0.f : 1.0f / L;               // NaN stays
+      float out[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) out[q] = ir < n.queries ? o[q] * inv : 0.f;
+      store_out4(a, b * a.osb + ir * a.ost + (hk * a.G + rr - ir * a.G) * a.osh + 4 * u, out);
+    }
   }
 }
 
-// The splits of one query row: a wave, D / 64 channels a lane.
+// The splits of one query row: a workgroup, whose threads take 4 channels of every PARTS-th split.
 template <int D>
-__global__ __launch_bounds__(64 * MX_WAVES) void mx_merge_kernel(const MxAttn a) {
-  constexpr int PER = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * MX_WAVES + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
+  constexpr int UNITS = D / 4, PARTS = 256 / UNITS;
+  __shared__ f4 sum[PARTS][UNITS];
+  __shared__ float sum_l[PARTS], top[4];
   const int rows = a.L * a.G;
-  if (at >= (int64_t)a.B * a.Hkv * rows) return;
-  const int r = (int)(at % rows);
-  const int64_t kvrow = at / rows;
+  const int r = (int)(blockIdx.x % rows);
+  const int64_t kvrow = blockIdx.x / rows;
   const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
   const int tile = r / 16, i = r / a.G, head = hk * a.G + (r - i * a.G);
   const MxRows n = mx_rows(a, kvrow, b);
   const bool live = i < n.queries;
-  const int entries = mx_entries(a, n, tile * 16, 16);
-  const int parts = live ? (entries + a.chunk - 1) / a.chunk : 0;
+  const int parts = live ? (mx_entries(a, n, tile * 16, 16) + a.chunk - 1) / a.chunk : 0;
   const int64_t first = (kvrow * a.tiles + tile) * a.splits * 16 + (r & 15);
-  float M = M_NONE, L = 0.f, o[PER];
+  float M = M_NONE;
+  for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) o[j] = 0.f;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
-  for (int s = 0; s < parts; ++s) {
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  const int u = threadIdx.x % UNITS, part = threadIdx.x / UNITS;
+  float L = 0.f;
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = part; s < parts; s += PARTS) {
     const int64_t slot = first + (int64_t)s * 16;
     const float wgt = __builtin_amdgcn_exp2f(a.ws_m[slot] - M);
     L += wgt * a.ws_l[slot];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) o[j] += wgt * a.ws_acc[slot * D + PER * lane + j];
+    o += *reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u) * wgt;
   }
+  sum[part][u] = o;
+  if (u == 0) sum_l[part] = L;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int p = 1; p < PARTS; ++p) { o += sum[p][u]; L += sum_l[p]; }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
-  const int64_t to = b * a.osb + i * a.ost + head * a.osh + PER * lane;
+  float out[4];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const float v = o[j] * inv;
-    if (a.out_dtype == IAK_DTYPE_F32) reinterpret_cast<float*>(a.out)[to + j] = v;
-    else if (a.out_dtype == IAK_DTYPE_F16) reinterpret_cast<_Float16*>(a.out)[to + j] = (_Float16)v;
-    else reinterpret_cast<__bf16*>(a.out)[to + j] = (__bf16)v;
-  }
+  for (int q = 0; q < 4; ++q) out[q] = o[q] * inv;
+  store_out4(a, b * a.osb + i * a.ost + head * a.osh + 4 * u, out);
 }
 
 template <int D, bool QF32> void launch_rows(const MxAttn& a, hipStream_t stream) {
-  hipLaunchKernelGGL((mx_rows_kernel<D, QF32>), dim3((uint32_t)((a.items + MX_WAVES - 1) / MX_WAVES)), dim3(64 * MX_WAVES),
-                     0, stream, a);
+  const dim3 grid((uint32_t)a.items);
+  constexpr int MANY = D == 128 ? 8 : 16;
+  if (a.waves > 4) hipLaunchKernelGGL((mx_rows_kernel<D, QF32, MANY>), grid, dim3(64 * MANY), 0, stream, a);
+  else hipLaunchKernelGGL((mx_rows_kernel<D, QF32, 4>), grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -318,10 +372,9 @@ hipError_t launch_mx_attention(const MxAttn& a, hipStream_t stream) {
   if (a.D == 128) f32 ? launch_rows<128, true>(a, stream) : launch_rows<128, false>(a, stream);
   else f32 ? launch_rows<64, true>(a, stream) : launch_rows<64, false>(a, stream);
   if (a.splits > 1) {
-    const int64_t waves = (int64_t)a.B * a.Hkv * a.L * a.G;
-    const dim3 grid((uint32_t)((waves + MX_WAVES - 1) / MX_WAVES));
-    if (a.D == 128) hipLaunchKernelGGL(mx_merge_kernel<128>, grid, dim3(64 * MX_WAVES), 0, stream, a);
-    else hipLaunchKernelGGL(mx_merge_kernel<64>, grid, dim3(64 * MX_WAVES), 0, stream, a);
+    const dim3 grid((uint32_t)((int64_t)a.B * a.Hkv * a.L * a.G));
+    if (a.D == 128) hipLaunchKernelGGL(mx_merge_kernel<128>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(mx_merge_kernel<64>, grid, dim3(256), 0, stream, a);
   }
   return hipGetLastError();
 }

@@ -18,9 +18,10 @@ struct MxAttn {
   int B, L, Hq, Hkv, G, D, W;
   int64_t NP;
   int tiles;      // tiles of 16 query rows (query token * G + head of the group) per KV row
-  int splits;     // parts of `chunk` table entries (even, when there are several) per tile
+  int splits;     // parts of `chunk` table entries per tile
   int chunk;
-  int64_t items;  // B * Hkv * tiles * splits
+  int waves;      // 4 per workgroup, or more (16): as many as the kernel has
+  int64_t items;  // B * Hkv * tiles * splits workgroups
 
   const void* q; int q_dtype; int q_vec; int64_t qsb, qst, qsh;          // *_vec: rows lie on 16 bytes
   void* out; int out_dtype; int out_vec; int64_t osb, ost, osh;
