@@ -65,6 +65,36 @@ struct MxPlan {
   size_t ws_m, ws_l, ws_acc, total;
 };
 
+// Up to this many tiles, a tile that is not split is a workgroup's of more than four waves: one a CU.
+constexpr double FEW_TILES = 256;
+
+// Splits of each of `tiles` rows of W table entries: the least of a cost in microseconds that was
+// fitted to measurements (17 shapes of 8 to 800 rows by 16 to 2,048 entries, within a fifth).
+// The card holds R workgroups at a time; a round of them takes START and the entries' time; a
+// round that is not full runs faster, at most twice; a second kernel merges the splits.
+//   256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 190 us, 4 228, 6 195, 8 203
+//   512 rows x 125: 1 split 31 us, 2 42, 4 44;   64 rows x 128: 1 split 18 us, 4 14.6, 8 13.8, 16 17
+int64_t rows_splits(double tiles, int W, int D) {
+  const double R = D == 128 ? 768 : 1024, START = 3, ENTRY = D == 128 ? 0.3 : 0.2, MERGE = 6;
+  const int64_t most = (W + 15) / 16;
+  int64_t best = 1;
+  double least = 0;
+  auto consider = [&](int64_t s) {
+    if (s < 1) s = 1;
+    if (s > most) s = most;
+    const bool wide = s == 1 && tiles <= FEW_TILES;               // workgroups of 8 or 16 waves
+    const double many = wide ? (D == 128 ? 2 : 4) : 1;
+    const double rounds = tiles * s / (wide ? FEW_TILES : R), full = std::floor(rounds), rest = rounds - full;
+    const double cost = (full + (rest > 0 ? 0.5 + 0.5 * rest : 0)) * (START + ENTRY * W / (s * many)) + (s > 1 ? MERGE : 0);
+    if (least == 0 || cost < least) { least = cost; best = s; }
+  };
+  consider(1);
+  if (tiles >= 4 * R || most <= 1) return best;
+  for (int64_t s = 2; s < most && s < 256; s *= 2) consider(s);
+  for (int rounds = 1; rounds <= 4; ++rounds) consider((int64_t)(rounds * R / tiles));
+  return best;
+}
+
 iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   if (!a) return fail(IAK_EINVAL, "args is NULL");
   iak_status st = validate_mx_cache(a->batch, a->q_len, a->num_kv_heads, a->head_dim, a->page_size, a->table_width, a->num_pages);
@@ -91,15 +121,12 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
   if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
   const int W = a->table_width > 0 ? a->table_width : 1;
-  // about 2,048 workgroups of four waves (two for each place on the card), of at least 32
-  // entries each; a row of few entries is one workgroup's, of sixteen waves when the grid is small
-  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(2048.0 / tiles);
-  if (splits > (W + 31) / 32) splits = (W + 31) / 32;
-  if (splits < 1) splits = 1;
+  int64_t splits = a->splits > 0 ? a->splits : rows_splits(tiles, W, a->head_dim);
+  if (splits > (W + 1) / 2) splits = (W + 1) / 2;
   while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
-  p->waves = p->splits == 1 && tiles < 512 && W > 8 ? 16 : 4;
+  p->waves = p->splits == 1 && tiles <= FEW_TILES ? 16 : 4;
   p->items = (int64_t)tiles * p->splits;
   if (p->splits > 1) {
     const size_t slots = (size_t)p->items * 16;

@@ -28,9 +28,6 @@ namespace iak {
 
 namespace {
 
-#ifndef MXOCC
-#define MXOCC 3
-#endif
 constexpr float P_SHIFT = 6.0f;          // weights <= 2^(6 + RESCALE_SLACK) = 2^14
 constexpr float M_NONE = -3.402823466e38f;
 
@@ -61,11 +58,11 @@ __device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0
     const uint8_t* kc = a.k_codes + page * (PS * D / 2);
     const uint8_t* vc = a.v_codes + page * (PS * D / 2);
     if constexpr (D == 128) {
-      const u4 k = *reinterpret_cast<const u4*>(kc + code), v = *reinterpret_cast<const u4*>(vc + code);
+      const u4 k = ld_nt(reinterpret_cast<const u4*>(kc + code)), v = ld_nt(reinterpret_cast<const u4*>(vc + code));
 #pragma unroll
       for (int i = 0; i < 4; ++i) { r.k[p][i] = k[i]; r.v[p][i] = v[i]; }
     } else {
-      const u2 k = *reinterpret_cast<const u2*>(kc + code), v = *reinterpret_cast<const u2*>(vc + code);
+      const u2 k = ld_nt(reinterpret_cast<const u2*>(kc + code)), v = ld_nt(reinterpret_cast<const u2*>(vc + code));
 #pragma unroll
       for (int i = 0; i < 2; ++i) { r.k[p][i] = k[i]; r.v[p][i] = v[i]; }
     }
@@ -97,7 +94,7 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
 template <int NW> __device__ __forceinline__ int wave_entry(int w, int i) { return 2 * (w + NW * (i >> 1)) + (i & 1); }
 
 template <int D, bool QF32, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows_kernel(const MxAttn a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_kernel(const MxAttn a) {
   __shared__ u4 vt[NW][2 * PS * D / 8];                          // V rows; at the end the waves' sums
   __shared__ float part_m[NW][16], part_l[NW][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -119,14 +116,15 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
 
-  // the wave's entries, 64 at a time: lane i holds number i of the block, `next` the block after
+  // the wave's entries, 64 at a time: lane i holds number i of the block, in
+  // `next` of the block after it
   const int32_t* row = a.table + kvrow * a.W;
   auto entry_id = [&](int k) {
     const int e = e0 + wave_entry<NW>(w, k);
     const int id = e < e1 ? row[e] : -1;
     return id < 0 || id >= a.NP ? -1 : id;
   };
-  int ids = entry_id(lane), next = e0 + 64 * NW < e1 ? entry_id(64 + lane) : -1;
+  int ids = entry_id(lane), next = entry_id(64 + lane);
   auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
 
   // queries: scaled by a power of two to a largest element in [2^14, 2^15)
@@ -173,33 +171,60 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows
   for (int mb = 0; mb < D / 16; ++mb) acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
   float m = M_NONE, l = 0.f;
 
-  // one step: the pair `x` of entries e, e + 1
-  auto step = [&](const MxPair<D>& x, int e) {
-    f4 s[2];
+  // one step: the pair `x` of entries e, e + 1; then `x` is the pair of pages to0, to1
+  auto step = [&](MxPair<D>& x, int e, int to0, int to1) {
+    f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const float ks[2] = {mx_scale(x.ks[0]), mx_scale(x.ks[1])}, vs[2] = {mx_scale(x.vs[0]), mx_scale(x.vs[1])};
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      s[p] = f4{0.f, 0.f, 0.f, 0.f};
-      const float ks = mx_scale(x.ks[p]);
+    for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
+      for (int p = 0; p < 2; ++p) {
         uint32_t o[4];
-        mx8_to_f16(x.k[p][j], ks, o);
+        mx8_to_f16(x.k[p][j], ks[p], o);
         const h8 ka = make_h8(o[0], o[1], o[2], o[3]);
         s[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[j], s[p], 0, 0, 0);
         if constexpr (QF32) s[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[j], s[p], 0, 0, 0);
       }
-      s[p] *= mult;
-      // tokens with a NaN block (rare): their scores are NaN
-      const uint64_t bad = __builtin_amdgcn_ballot_w64(x.ks[p] == MX_SCALE_NAN || x.vs[p] == MX_SCALE_NAN);
-      if (bad) {
-        const uint32_t t = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48));
+
+    // V: rows of this lane's token into LDS, while the scores are under way
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        uint32_t o[4];
+        mx8_to_f16(x.v[p][j], vs[p], o);
+        vt[w][p * (PS * D / 8) + v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+
+    // what is left to do with the pair: which tokens are NaN (rare), which pages are none
+    uint32_t most = x.ks[0] > x.ks[1] ? x.ks[0] : x.ks[1], vmost = x.vs[0] > x.vs[1] ? x.vs[0] : x.vs[1];
+    most = most > vmost ? most : vmost;
+    uint32_t nan_tokens[2] = {0u, 0u};
+    if (__builtin_amdgcn_ballot_w64(most == MX_SCALE_NAN)) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(x.ks[p] == MX_SCALE_NAN || x.vs[p] == MX_SCALE_NAN);
+        nan_tokens[p] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
+      }
+    }
+    const int id[2] = {x.id[0], x.id[1]};
+    load_pair<D>(x, a, to0, to1, c, g);                          // under way during the rest of the step
+
+#pragma unroll
+    for (int p = 0; p < 2; ++p) s[p] *= mult;
+    if (nan_tokens[0] | nan_tokens[1]) {                         // their scores are NaN
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if ((t >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
-      }
-      // tokens that a row does not see
-      if ((e + p + 1) * PS > least || x.id[p] < 0) {
-        const int lim = x.id[p] < 0 ? 0 : seen - (e + p) * PS;
+          if ((nan_tokens[p] >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
+    }
+    if ((e + 2) * PS > least || (id[0] | id[1]) < 0) {           // tokens that a row does not see
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int lim = id[p] < 0 ? 0 : seen - (e + p) * PS;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (4 * g + q >= lim) s[p][q] = -__builtin_inff();
@@ -229,19 +254,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows
         if constexpr (QF32) pl[4 * p + q] = (_Float16)(v - (float)pb[4 * p + q]);
       }
 
-    // V: rows of this lane's token into LDS, four tokens of a channel back
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const float vs = mx_scale(x.vs[p]);
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        uint32_t o[4];
-        mx8_to_f16(x.v[p][j], vs, o);
-        vt[w][p * (PS * D / 8) + v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // V back: four tokens of a channel in each lane
     typedef __attribute__((address_space(3))) s4v lds_s4;
     const char* from = reinterpret_cast<const char*>(&vt[w][0]);
 #pragma unroll
@@ -258,22 +271,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? MXOCC : 2) void mx_rows
     }
   };
 
-  // the next pair's loads are under way while a pair is worked on
-  MxPair<D> x, y;
-  int at = e0 + 2 * w, k = 0, block = 0;                         // the pair's first entry, its number in the block
-  if (at < e1) load_pair<D>(x, a, page(0), page(1), c, g);
-  while (at < e1) {
-    const int to = at + 2 * NW;
-    if (to < e1) load_pair<D>(y, a, page(k + 2), page(k + 3), c, g);
-    step(x, at);
-    x = y;
-    at = to;
+  // Twelve waves a CU are what hides the loads: a ring of two or more pairs cost registers and was
+  // slower, as were sixteen waves of fewer registers. The bytes come at the rate that the same
+  // loads reach alone, streamed (1.14 GB in 190 us; 216 with loads that stay in the caches).
+  MxPair<D> x;
+  if (e0 + 2 * w < e1) load_pair<D>(x, a, page(0), page(1), c, g);
+  for (int at = e0 + 2 * w, k = 0, block = 0; at < e1; at += 2 * NW) {
+    step(x, at, page(k + 2), page(k + 3));                       // past the end: no page, page 0 is loaded
     k += 2;
     if (k == 64) {
       k = 0;
       block += 64;
       ids = next;
-      next = at + 64 * NW < e1 ? entry_id(block + 64 + lane) : -1;
+      next = entry_id(block + 64 + lane);
     }
   }
 
