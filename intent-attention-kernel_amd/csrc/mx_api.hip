@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 #include "iak.h"
 #include "mx_internal.h"
@@ -60,38 +61,59 @@ iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
 }
 
 struct MxPlan {
-  int G, tiles, splits, chunk, waves;
+  int G, tiles, splits, chunk, waves, chunk_rows;
   int64_t items;
   size_t ws_m, ws_l, ws_acc, total;
 };
 
-// Up to this many tiles, a tile that is not split is a workgroup's of more than four waves: one a CU.
-constexpr double FEW_TILES = 256;
+// Which kernel, and into how many splits a row's tokens go: the least of costs in microseconds
+// fitted to measurements (32 shapes of 8 to 65,536 query rows by 16 to 2,048 table entries).
+// The card holds `places` workgroups at a time. A round of them takes START and its entries'
+// time; a round that is not full runs faster, at most twice; a second kernel merges splits at
+// MERGE and the time of the partials' bytes.
+//   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 190 us, 4 228,
+//     6 195, 8 203; 512 x 125: 1 split 31, 2 42, 4 44; 64 x 128: 1 split 18, 4 14.6, 8 13.8, 16 17
+//   2,048 queries x 4 heads x 8 KV heads over 8,192 tokens: rows kernel 475, chunk kernel 293;
+//     16 x 4 x 64 over 4,000: rows 31, chunk 40 (8 splits)
+constexpr int CHUNK_ROWS = 128;
+constexpr double FEW_TILES = 256;   // up to as many unsplit tiles are workgroups of more waves: one a CU
 
-// Splits of each of `tiles` rows of W table entries: the least of a cost in microseconds that was
-// fitted to measurements (17 shapes of 8 to 800 rows by 16 to 2,048 entries, within a fifth).
-// The card holds R workgroups at a time; a round of them takes START and the entries' time; a
-// round that is not full runs faster, at most twice; a second kernel merges the splits.
-//   256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 190 us, 4 228, 6 195, 8 203
-//   512 rows x 125: 1 split 31 us, 2 42, 4 44;   64 rows x 128: 1 split 18 us, 4 14.6, 8 13.8, 16 17
-int64_t rows_splits(double tiles, int W, int D) {
-  const double R = D == 128 ? 768 : 1024, START = 3, ENTRY = D == 128 ? 0.3 : 0.2, MERGE = 6;
+struct MxChoice { bool chunk; int64_t splits; };
+
+MxChoice choose(double kvrows, int64_t rows, int W, int D, bool f32, int64_t forced) {
+  const double START = 3, MERGE = 6;
+  const bool wide_head = D == 128;
+  const double tiles = kvrows * ((rows + 15) / 16), blocks = kvrows * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS);
+  const double per_head = (rows + 15) / 16;                      // tiles that read the same pages
+  const double bytes_entry = (wide_head ? 0.30 : 0.20) / per_head;   // one entry's bytes, the card full
+  double rows_entry = wide_head ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
+  if (rows_entry < bytes_entry) rows_entry = bytes_entry;
+  const double chunk_entry = wide_head ? (f32 ? 0.92 : 0.57) : (f32 ? 0.60 : 0.48);
+  const double rows_places = wide_head ? 768 : 1024, chunk_places = wide_head || f32 ? 512 : 768;
   const int64_t most = (W + 15) / 16;
-  int64_t best = 1;
-  double least = 0;
-  auto consider = [&](int64_t s) {
-    if (s < 1) s = 1;
+  MxChoice best = {false, 1};
+  double least = -1;
+  auto consider = [&](bool chunk, int64_t s) {
     if (s > most) s = most;
-    const bool wide = s == 1 && tiles <= FEW_TILES;               // workgroups of 8 or 16 waves
-    const double many = wide ? (D == 128 ? 2 : 4) : 1;
-    const double rounds = tiles * s / (wide ? FEW_TILES : R), full = std::floor(rounds), rest = rounds - full;
-    const double cost = (full + (rest > 0 ? 0.5 + 0.5 * rest : 0)) * (START + ENTRY * W / (s * many)) + (s > 1 ? MERGE : 0);
-    if (least == 0 || cost < least) { least = cost; best = s; }
+    if (s < 1) s = 1;
+    if (forced > 0) s = forced;
+    const bool many = !chunk && s == 1 && tiles <= FEW_TILES;
+    const double work = chunk ? blocks : tiles, places = chunk ? chunk_places : many ? FEW_TILES : rows_places;
+    const double entry = (chunk ? chunk_entry : rows_entry) / (many ? (wide_head ? 2 : 4) : 1);
+    const double rounds = work * s / places, full = std::floor(rounds), rest = rounds - full;
+    double cost = (full + (rest > 0 ? 0.5 + 0.5 * rest : 0)) * (START + entry * W / s);
+    if (s > 1) cost += MERGE + kvrows * rows * s * D * 8 / 3.0e6;
+    if (least < 0 || cost < least) { least = cost; best = {chunk, s}; }
   };
-  consider(1);
-  if (tiles >= 4 * R || most <= 1) return best;
-  for (int64_t s = 2; s < most && s < 256; s *= 2) consider(s);
-  for (int rounds = 1; rounds <= 4; ++rounds) consider((int64_t)(rounds * R / tiles));
+  auto each = [&](bool chunk) {
+    const double work = chunk ? blocks : tiles, places = chunk ? chunk_places : rows_places;
+    consider(chunk, 1);
+    if (work >= 4 * places || most <= 1 || forced > 0) return;
+    for (int64_t s = 2; s < most && s < 256; s *= 2) consider(chunk, s);
+    for (int rounds = 1; rounds <= 4; ++rounds) consider(chunk, (int64_t)(rounds * places / work));
+  };
+  each(false);
+  if (rows > 16) each(true);
   return best;
 }
 
@@ -121,15 +143,19 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
   if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
   const int W = a->table_width > 0 ? a->table_width : 1;
-  int64_t splits = a->splits > 0 ? a->splits : rows_splits(tiles, W, a->head_dim);
+  MxChoice best = choose((double)a->batch * a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
+  if (const char* f = getenv("MXF")) { if (f[0]=='0') best.chunk = false; else if (f[0]=='1') best.chunk = rows > 16; }
+  p->chunk_rows = best.chunk ? CHUNK_ROWS : 0;
+  const double blocks = best.chunk ? (double)a->batch * a->num_kv_heads * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS) : tiles;
+  int64_t splits = best.splits;
   if (splits > (W + 1) / 2) splits = (W + 1) / 2;
   while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
   p->waves = p->splits == 1 && tiles <= FEW_TILES ? 16 : 4;
-  p->items = (int64_t)tiles * p->splits;
+  p->items = (int64_t)blocks * p->splits;
   if (p->splits > 1) {
-    const size_t slots = (size_t)p->items * 16;
+    const size_t slots = (size_t)tiles * p->splits * 16;
     p->ws_m = 0;
     p->ws_l = round_up(4 * slots);
     p->ws_acc = p->ws_l + round_up(4 * slots);
@@ -225,7 +251,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   iak::MxAttn k;
   k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
-  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.waves = p.waves; k.items = p.items;
+  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.waves = p.waves; k.chunk_rows = p.chunk_rows; k.items = p.items;
   k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
   k.q_vec = aligned16(a->q) && (a->q_stride_b | a->q_stride_t | a->q_stride_h) % (a->q_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
   k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;

@@ -90,6 +90,127 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
   else out4(reinterpret_cast<__bf16*>(a.out) + at, a.out_vec, x);
 }
 
+// A query row's operand: the lane's channels (D/4) g .., scaled by a power of two to a largest
+// element of the row in [2^14, 2^15), split in two for float32. Returns the factor that makes
+// base-2 scores of the products: positive, NaN for a row that is not finite. (A negative scale
+// turns the query's sign; where the factor would vanish the scores do: query 0, factor 1.)
+template <int D, bool QF32>
+__device__ __forceinline__ float load_query(const MxAttn& a, bool live, int64_t at, int g, h8 (&qhi)[D / 32],
+                                            h8 (&qlo)[QF32 ? D / 32 : 1]) {
+  float x[D / 32][8];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[s][j] = 0.f;
+  if (live) {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) mx_load_q(a, at + g * (D / 4) + 8 * s, x[s]);
+  }
+  bool fine = true;
+  float m = 0.f;
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = fabsf(x[s][j]);
+      fine = fine && v < __builtin_inff();
+      m = fmaxf(m, v);
+    }
+  m = xmax16_32(fine ? m : __builtin_inff());
+  fine = m < __builtin_inff();
+  const int e = m > 0.f ? (int)(f2u(m) >> 23) - 127 : 0;
+  const float mult = __builtin_ldexpf(fabsf(a.score_mult), e - 14);
+  const bool none = !fine || mult < 1e-30f;
+  const float sign = a.score_mult < 0.f ? -1.f : 1.f;
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = none ? 0.f : sign * __builtin_ldexpf(x[s][j], 14 - e);
+      qhi[s][j] = (_Float16)v;
+      if constexpr (QF32) qlo[s][j] = (_Float16)(v - (float)qhi[s][j]);
+    }
+  return !fine ? __builtin_nanf("") : none ? 1.f : mult;
+}
+
+// What the score results of PAGES pages (lane: row c, tokens 4g .. 4g+3 of each) become: NaN
+// where a token has a NaN block (bit per token in `nan`, rare), -inf where the row does not see
+// it; then the weights exp2(s * mult - m + P_SHIFT) in place. Moves the row's running maximum m,
+// sum l (SUM: adds the weights to it) and accumulator. The lanes of a row compare maxima only when
+// one of them is past the slack. `e`: the first page's entry number; `least`: see the kernels.
+template <int D, int PAGES, bool SUM>
+__device__ __forceinline__ void soften(f4 (&s)[PAGES], const uint32_t (&nan)[PAGES], const int (&id)[PAGES], int e, int seen,
+                                       int least, float mult, int g, float& m, f4& l, f4 (&acc)[D / 16]) {
+  uint32_t any_nan = 0u;
+  int ids = 0;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p) { any_nan |= nan[p]; ids |= id[p]; }
+  if (__builtin_expect(any_nan != 0u, 0)) {
+    asm volatile("");                                            // a branch, not selects for every call
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if ((nan[p] >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
+  }
+  if ((e + PAGES) * PS > least || ids < 0) {
+    asm volatile("");
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int lim = id[p] < 0 ? 0 : seen - (e + p) * PS;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (4 * g + q >= lim) s[p][q] = -__builtin_inff();
+    }
+  }
+  float pm = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+#pragma unroll
+  for (int p = 1; p < PAGES; ++p) pm = fmaxf(pm, fmaxf(fmaxf(s[p][0], s[p][1]), fmaxf(s[p][2], s[p][3])));
+  if (__builtin_amdgcn_ballot_w64(pm * mult > m + RESCALE_SLACK)) {
+    asm volatile("");
+    pm = xmax16_32(pm) * mult;
+    const float mn = pm > m + RESCALE_SLACK ? pm : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    l *= alpha;
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb) acc[mb] *= alpha;
+    m = mn;
+  }
+  const float base = P_SHIFT - m;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[p][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p][q], mult, base));
+      if constexpr (SUM) l[q] += s[p][q];
+    }
+}
+
+// Weights of two pages as the value product's operand, and what rounding left (float32 queries).
+__device__ __forceinline__ h8 weights(const f4 a, const f4 b) {
+  return h8{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3],
+            (_Float16)b[0], (_Float16)b[1], (_Float16)b[2], (_Float16)b[3]};
+}
+__device__ __forceinline__ h8 weights_rest(const f4 a, const f4 b, const h8 w) {
+  h8 r;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    r[q] = (_Float16)(a[q] - (float)w[q]);
+    r[4 + q] = (_Float16)(b[q] - (float)w[4 + q]);
+  }
+  return r;
+}
+
+// The value product's operand from two pages' V rows in LDS: channel 16 mb + c of tokens
+// 4g .. 4g+3 of both.
+template <int D> __device__ __forceinline__ h8 values_back(const u4* page0, const u4* page1, int mb, int c, int g) {
+  typedef __attribute__((address_space(3))) s4v lds_s4;
+  const int at = v_chunk<D>(4 * g + (c >> 2), 2 * mb + ((c & 3) >> 1)) * 16 + (c & 1) * 8;
+  const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(reinterpret_cast<const char*>(page0) + at));
+  const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(reinterpret_cast<const char*>(page1) + at));
+  return __builtin_bit_cast(h8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 // Entry i of the wave's own, of those that the workgroup's NW waves share out in pairs.
 template <int NW> __device__ __forceinline__ int wave_entry(int w, int i) { return 2 * (w + NW * (i >> 1)) + (i & 1); }
 
@@ -127,49 +248,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   int ids = entry_id(lane), next = entry_id(64 + lane);
   auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
 
-  // queries: scaled by a power of two to a largest element in [2^14, 2^15)
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
-  float mult;
-  {
-    float x[D / 32][8];
-    float m = 0.f;
-    if (live) {
-      const int64_t at = b * a.qsb + i * a.qst + head * a.qsh + g * (D / 4);
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) mx_load_q(a, at + 8 * s, x[s]);
-    } else {
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[s][j] = 0.f;
-    }
-    bool fine = true;
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = fabsf(x[s][j]);
-        fine = fine && v < __builtin_inff();
-        m = fmaxf(m, v);
-      }
-    m = xmax16_32(fine ? m : __builtin_inff());
-    fine = m < __builtin_inff();
-    const int e = m > 0.f ? (int)(f2u(m) >> 23) - 127 : 0;
-    mult = fine ? __builtin_ldexpf(a.score_mult, e - 14) : __builtin_nanf("");
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = fine ? __builtin_ldexpf(x[s][j], 14 - e) : 0.f;
-        qhi[s][j] = (_Float16)v;
-        if constexpr (QF32) qlo[s][j] = (_Float16)(v - (float)qhi[s][j]);
-      }
-  }
+  const float mult = load_query<D, QF32>(a, live, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo);
 
   f4 acc[D / 16];
 #pragma unroll
   for (int mb = 0; mb < D / 16; ++mb) acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
-  float m = M_NONE, l = 0.f;
+  float m = M_NONE;
+  f4 l = {0.f, 0.f, 0.f, 0.f};
 
   // one step: the pair `x` of entries e, e + 1; then `x` is the pair of pages to0, to1
   auto step = [&](MxPair<D>& x, int e, int to0, int to1) {
@@ -212,60 +298,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
     const int id[2] = {x.id[0], x.id[1]};
     load_pair<D>(x, a, to0, to1, c, g);                          // under way during the rest of the step
 
-#pragma unroll
-    for (int p = 0; p < 2; ++p) s[p] *= mult;
-    if (nan_tokens[0] | nan_tokens[1]) {                         // their scores are NaN
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if ((nan_tokens[p] >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
-    }
-    if ((e + 2) * PS > least || (id[0] | id[1]) < 0) {           // tokens that a row does not see
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int lim = id[p] < 0 ? 0 : seen - (e + p) * PS;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (4 * g + q >= lim) s[p][q] = -__builtin_inff();
-      }
-    }
-    float pm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    pm = xmax16_32(pm);
-    const bool grow = pm > m + RESCALE_SLACK;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float mn = grow ? pm : m;
-      const float alpha = __builtin_amdgcn_exp2f(m - mn);
-      l *= alpha;
-#pragma unroll
-      for (int mb = 0; mb < D / 16; ++mb) acc[mb] *= alpha;
-      m = mn;
-    }
-    h8 pb, pl;
-    const float base = m - P_SHIFT;
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float v = __builtin_amdgcn_exp2f(s[p][q] - base);
-        l += v;
-        pb[4 * p + q] = (_Float16)v;
-        if constexpr (QF32) pl[4 * p + q] = (_Float16)(v - (float)pb[4 * p + q]);
-      }
-
-    // V back: four tokens of a channel in each lane
-    typedef __attribute__((address_space(3))) s4v lds_s4;
-    const char* from = reinterpret_cast<const char*>(&vt[w][0]);
+    soften<D, 2, true>(s, nan_tokens, id, e, seen, least, mult, g, m, l, acc);
+    const h8 pb = weights(s[0], s[1]);
+    h8 pl;
+    if constexpr (QF32) pl = weights_rest(s[0], s[1], pb);
 #pragma unroll
     for (int mb = 0; mb < D / 16; ++mb) {
-      s4v t[2];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int at = p * (PS * D / 8) + v_chunk<D>(4 * g + (c >> 2), 2 * mb + ((c & 3) >> 1));
-        t[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + at * 16 + (c & 1) * 8));
-      }
-      const h8 va = __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      const h8 va = values_back<D>(&vt[w][0], &vt[w][PS * D / 8], mb, c, g);
       acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[mb], 0, 0, 0);
       if constexpr (QF32) acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[mb], 0, 0, 0);
     }
@@ -288,9 +327,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   }
 
   // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
-  l = xsum16_32(l);
+  const float sum = xsum16_32((l[0] + l[1]) + (l[2] + l[3]));
   __syncthreads();
-  if (g == 0) { part_m[w][c] = m; part_l[w][c] = l; }
+  if (g == 0) { part_m[w][c] = m; part_l[w][c] = sum; }
   f4* sums = reinterpret_cast<f4*>(&vt[w][0]);
 #pragma unroll
   for (int mb = 0; mb < D / 16; ++mb) sums[c * (D / 4) + ((4 * mb + g) ^ c)] = acc[mb];
@@ -323,29 +362,227 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   }
 }
 
-// The splits of one query row: a workgroup, whose threads take 4 channels of every PARTS-th split.
-template <int D>
+// Tiles of 64 RT query rows: prompt chunks. The four waves take 16 RT rows each and walk the
+// same tokens, 64 (four pages) a step; each wave converts one page of K and V of the next step,
+// which all read from LDS (two buffers, one barrier a step): per row, the vector instructions are
+// what bounds it, so each code is converted once per workgroup, and the sum of the weights is a
+// product with ones on the matrix cores. The rest is the rows kernel's.
+template <int D, bool QF32, int RT>
+__global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
+  __shared__ u4 kt[2][4][PS * D / 8], vt[2][4][PS * D / 8];
+  __shared__ u4 nan_in[2];
+  constexpr int BM = 64 * RT;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  const int wide = (a.L * a.G + BM - 1) / BM;                    // tiles of BM rows
+  const int split = (int)(blockIdx.x % a.splits);
+  const int64_t tile_at = blockIdx.x / a.splits;
+  const int64_t kvrow = tile_at / wide;
+  const int tile = wide - 1 - (int)(tile_at % wide);             // those that see most first
+  const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
+  const MxRows n = mx_rows(a, kvrow, b);
+  const int entries = mx_entries(a, n, tile * BM, BM);
+  const int e0 = split * a.chunk, e1 = e0 + a.chunk < entries ? e0 + a.chunk : entries;
+  if (split > 0 && e0 >= e1) return;                             // uniform; the merge does not look at it
+
+  const int rows = a.L * a.G;
+  int seen[RT], least[RT];
+  h8 qhi[RT][D / 32], qlo[RT][QF32 ? D / 32 : 1];
+  float mult[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
+    const bool live = r < rows && i < n.queries;
+    seen[t] = live ? mx_seen(a, n, i) : 0;
+    least[t] = live ? seen[t] : 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least[t], o, 64); least[t] = x < least[t] ? x : least[t]; }
+    mult[t] = load_query<D, QF32>(a, live, b * a.qsb + i * a.qst + head * a.qsh, g, qhi[t], qlo[t]);
+  }
+
+  // entries 64 at a time: lane i holds entry i of the block, in `next` of the block after it
+  const int32_t* row = a.table + kvrow * a.W;
+  auto entry_id = [&](int k) {
+    const int e = e0 + k;
+    const int id = e < e1 ? row[e] : -1;
+    return id < 0 || id >= a.NP ? -1 : id;
+  };
+  int ids = entry_id(lane), next = entry_id(64 + lane);
+  auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
+
+  // this wave's page of a step: loaded a step ahead, converted into LDS during the step before
+  uint32_t kr[D / 32], ks, vr[D / 32], vs;
+  auto load_page = [&](int id) {
+    const int64_t p = id < 0 ? 0 : id;
+    const uint32_t code = c * (D / 2) + g * (D / 8), sc = c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK;
+    const uint8_t *kc = a.k_codes + p * (PS * D / 2) + code, *vc = a.v_codes + p * (PS * D / 2) + code;
+    if constexpr (D == 128) {
+      const u4 k = *reinterpret_cast<const u4*>(kc), v = *reinterpret_cast<const u4*>(vc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { kr[i] = k[i]; vr[i] = v[i]; }
+    } else {
+      const u2 k = *reinterpret_cast<const u2*>(kc), v = *reinterpret_cast<const u2*>(vc);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { kr[i] = k[i]; vr[i] = v[i]; }
+    }
+    ks = (a.k_scales + p * (PS * D / MX_BLOCK))[sc];
+    vs = (a.v_scales + p * (PS * D / MX_BLOCK))[sc];
+  };
+  auto convert = [&](int buf) {
+    const float sk = mx_scale(ks), sv = mx_scale(vs);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      uint32_t o[4];
+      mx8_to_f16(kr[j], sk, o);
+      kt[buf][w][v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
+      mx8_to_f16(vr[j], sv, o);
+      vt[buf][w][v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
+    }
+    const uint64_t bad = __builtin_amdgcn_ballot_w64((ks > vs ? ks : vs) == MX_SCALE_NAN);
+    if (lane == 0)
+      reinterpret_cast<uint32_t*>(&nan_in[buf])[w] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
+  };
+
+  f4 acc[RT][D / 16], l[RT];
+  float m[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m[t] = M_NONE;
+    l[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+  int k = 0, block = 0;                                          // number of entry e in the block
+  auto step = [&](int buf, int e) {
+    f4 s[RT][4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t][p] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const h8 ka = __builtin_bit_cast(h8, kt[buf][p][v_chunk<D>(c, g * (D / 32) + j)]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[t][j], s[t][p], 0, 0, 0);
+          if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[t][j], s[t][p], 0, 0, 0);
+        }
+      }
+    }
+    const u4 bad = nan_in[buf];
+    const int id[4] = {page(k), page(k + 1), page(k + 2), page(k + 3)};
+    convert(buf ^ 1);
+    load_page(page(k + 8 + w));
+    uint32_t nan_tokens[4] = {0u, 0u, 0u, 0u};
+    if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1] | bad[2] | bad[3])) {
+      asm volatile("");
+#pragma unroll
+      for (int p = 0; p < 4; ++p) nan_tokens[p] = __builtin_amdgcn_readfirstlane(bad[p]);
+    }
+    h8 pb[RT][2], pl[RT][QF32 ? 2 : 1];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      soften<D, 4, false>(s[t], nan_tokens, id, e, seen[t], least[t], mult[t], g, m[t], l[t], acc[t]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pb[t][h] = weights(s[t][2 * h], s[t][2 * h + 1]);
+        if constexpr (QF32) pl[t][h] = weights_rest(s[t][2 * h], s[t][2 * h + 1], pb[t][h]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[t][h], l[t], 0, 0, 0);
+        if constexpr (QF32) l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t][h], l[t], 0, 0, 0);
+      }
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) {
+        const h8 va = values_back<D>(vt[buf][2 * h], vt[buf][2 * h + 1], mb, c, g);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[t][h], acc[t][mb], 0, 0, 0);
+          if constexpr (QF32) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[t][h], acc[t][mb], 0, 0, 0);
+        }
+      }
+    }
+    k += 4;
+    if (k == 64) {
+      k = 0;
+      block += 64;
+      ids = next;
+      next = entry_id(block + 64 + lane);
+    }
+    __syncthreads();                                             // this buffer is free, the other one is whole
+  };
+  if (e0 < e1) {
+    load_page(page(w));
+    convert(0);
+    load_page(page(4 + w));
+    __syncthreads();
+    for (int e = e0; e < e1; e += 8) {
+      step(0, e);
+      if (e + 4 < e1) step(1, e + 4);
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
+    const float sum = l[t][0];
+    if (r >= rows) continue;
+    if (a.splits > 1) {
+      const int64_t slot = ((kvrow * a.tiles + (r >> 4)) * a.splits + split) * 16 + c;
+      if (g == 0) { a.ws_m[slot] = m[t]; a.ws_l[slot] = sum; }
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) *reinterpret_cast<f4*>(a.ws_acc + slot * D + 16 * mb + 4 * g) = acc[t][mb];
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;           // NaN stays
+      const int64_t at = b * a.osb + i * a.ost + head * a.osh + 4 * g;
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) {
+        float o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = i < n.queries ? acc[t][mb][q] * inv : 0.f;
+        store_out4(a, at + 16 * mb, o);
+      }
+    }
+  }
+}
+
+// The splits of 256 / (D / 4 PARTS) query rows a workgroup: a thread takes 4 channels of every
+// PARTS-th split of its row. PARTS > 1, where a row has many splits, is one row a workgroup.
+template <int D, int PARTS>
 __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
-  constexpr int UNITS = D / 4, PARTS = 256 / UNITS;
+  constexpr int UNITS = D / 4, ROWS = 256 / (UNITS * PARTS);
+  static_assert(PARTS == 1 || ROWS == 1, "one row, or one part");
   __shared__ f4 sum[PARTS][UNITS];
   __shared__ float sum_l[PARTS], top[4];
   const int rows = a.L * a.G;
-  const int r = (int)(blockIdx.x % rows);
-  const int64_t kvrow = blockIdx.x / rows;
-  const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
+  const int u = threadIdx.x % UNITS, part = PARTS > 1 ? threadIdx.x / UNITS : 0;
+  const int64_t at = (int64_t)blockIdx.x * ROWS + (PARTS > 1 ? 0 : threadIdx.x / UNITS);
+  const bool there = at < (int64_t)a.B * a.Hkv * rows;           // always, where there are barriers
+  const int64_t kvrow = there ? at / rows : 0;
+  const int r = there ? (int)(at - kvrow * rows) : 0;
+  const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow - (int64_t)b * a.Hkv);
   const int tile = r / 16, i = r / a.G, head = hk * a.G + (r - i * a.G);
   const MxRows n = mx_rows(a, kvrow, b);
   const bool live = i < n.queries;
-  const int parts = live ? (mx_entries(a, n, tile * 16, 16) + a.chunk - 1) / a.chunk : 0;
+  const int parts = live && there ? (mx_entries(a, n, tile * 16, 16) + a.chunk - 1) / a.chunk : 0;
   const int64_t first = (kvrow * a.tiles + tile) * a.splits * 16 + (r & 15);
   float M = M_NONE;
-  for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
+  if constexpr (PARTS > 1) {
+    for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  const int u = threadIdx.x % UNITS, part = threadIdx.x / UNITS;
+    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  } else {
+    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
+  }
   float L = 0.f;
   f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -353,14 +590,17 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
     const int64_t slot = first + (int64_t)s * 16;
     const float wgt = __builtin_amdgcn_exp2f(a.ws_m[slot] - M);
     L += wgt * a.ws_l[slot];
-    o += *reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u) * wgt;
+    o += ld_nt(reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u)) * wgt;
   }
-  sum[part][u] = o;
-  if (u == 0) sum_l[part] = L;
-  __syncthreads();
-  if (part != 0) return;
+  if constexpr (PARTS > 1) {
+    sum[part][u] = o;
+    if (u == 0) sum_l[part] = L;
+    __syncthreads();
+    if (part != 0) return;
 #pragma unroll
-  for (int p = 1; p < PARTS; ++p) { o += sum[p][u]; L += sum_l[p]; }
+    for (int p = 1; p < PARTS; ++p) { o += sum[p][u]; L += sum_l[p]; }
+  }
+  if (!there) return;
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   float out[4];
 #pragma unroll
@@ -368,8 +608,21 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
   store_out4(a, b * a.osb + i * a.ost + head * a.osh + 4 * u, out);
 }
 
+// Rows whose splits a thread walks alone, eight at most; more are shared by a workgroup.
+template <int D> void launch_mx_merge(const MxAttn& a, hipStream_t stream) {
+  constexpr int UNITS = D / 4;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.L * a.G;
+  if (a.splits <= 8) {
+    const int per = 256 / UNITS;
+    hipLaunchKernelGGL((mx_merge_kernel<D, 1>), dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((mx_merge_kernel<D, 256 / UNITS>), dim3((uint32_t)rows), dim3(256), 0, stream, a);
+  }
+}
+
 template <int D, bool QF32> void launch_rows(const MxAttn& a, hipStream_t stream) {
   const dim3 grid((uint32_t)a.items);
+  if (a.chunk_rows) { hipLaunchKernelGGL((mx_chunk_kernel<D, QF32, 2>), grid, dim3(256), 0, stream, a); return; }
   constexpr int MANY = D == 128 ? 8 : 16;
   if (a.waves > 4) hipLaunchKernelGGL((mx_rows_kernel<D, QF32, MANY>), grid, dim3(64 * MANY), 0, stream, a);
   else hipLaunchKernelGGL((mx_rows_kernel<D, QF32, 4>), grid, dim3(256), 0, stream, a);
@@ -382,9 +635,8 @@ hipError_t launch_mx_attention(const MxAttn& a, hipStream_t stream) {
   if (a.D == 128) f32 ? launch_rows<128, true>(a, stream) : launch_rows<128, false>(a, stream);
   else f32 ? launch_rows<64, true>(a, stream) : launch_rows<64, false>(a, stream);
   if (a.splits > 1) {
-    const dim3 grid((uint32_t)((int64_t)a.B * a.Hkv * a.L * a.G));
-    if (a.D == 128) hipLaunchKernelGGL(mx_merge_kernel<128>, grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(mx_merge_kernel<64>, grid, dim3(256), 0, stream, a);
+    if (a.D == 128) launch_mx_merge<128>(a, stream);
+    else launch_mx_merge<64>(a, stream);
   }
   return hipGetLastError();
 }

@@ -21,7 +21,8 @@ struct MxAttn {
   int splits;     // parts of `chunk` table entries per tile
   int chunk;
   int waves;      // 4 per workgroup, or more (16): as many as the kernel has
-  int64_t items;  // B * Hkv * tiles * splits workgroups
+  int chunk_rows; // 64 or 128: the chunk kernel with tiles of that many rows; 0: the rows kernel
+  int64_t items;  // workgroups: B * Hkv * splits * tiles (of 16 or of chunk_rows rows)
 
   const void* q; int q_dtype; int q_vec; int64_t qsb, qst, qsh;          // *_vec: rows lie on 16 bytes
   void* out; int out_dtype; int out_vec; int64_t osb, ost, osh;
