@@ -47,8 +47,9 @@ iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
   if (st != IAK_OK) return st;
   if (a->dtype < 0 || a->dtype > 2) return fail(IAK_EINVAL, "bad dtype %d", a->dtype);
   if (a->batch == 0 || a->count == 0) return IAK_OK;
-  // one thread per 8 channels, fewer than 2^32 of them in a launch
-  if ((double)a->batch * a->count * a->num_kv_heads * (a->head_dim / 8) > 4.0e9)
+  // a thread per 8 channels: numbers below 2^31 in a sequence, below 2^32 in a launch
+  const double threads = ((double)a->count + 15) * a->num_kv_heads * (a->head_dim / 8) + 256;
+  if (threads > 2.0e9 || threads * (a->batch < 32768 ? a->batch : 32768) > 4.0e9)
     return fail(IAK_EINVAL, "too many tokens for one call (%d x %d x %d heads)", a->batch, a->count, a->num_kv_heads);
   if (!a->k || !a->v) return fail(IAK_EINVAL, "k/v is NULL");
   if (!a->page_table && a->table_width > 0) return fail(IAK_EINVAL, "page_table is NULL");
@@ -253,9 +254,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   k.W = a->table_width; k.NP = a->num_pages;
   k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.waves = p.waves; k.chunk_rows = p.chunk_rows; k.items = p.items;
   k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
-  k.q_vec = aligned16(a->q) && (a->q_stride_b | a->q_stride_t | a->q_stride_h) % (a->q_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
   k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;
-  k.out_vec = aligned16(a->out) && (a->out_stride_b | a->out_stride_t | a->out_stride_h) % (a->out_dtype == IAK_DTYPE_F32 ? 4 : 8) == 0;
   k.table = a->page_table; k.valid = a->valid_tokens; k.q_lens = a->q_lens;
   k.k_codes = reinterpret_cast<const uint8_t*>(a->k_codes); k.k_scales = reinterpret_cast<const uint8_t*>(a->k_scales);
   k.v_codes = reinterpret_cast<const uint8_t*>(a->v_codes); k.v_scales = reinterpret_cast<const uint8_t*>(a->v_scales);

@@ -44,24 +44,17 @@ __device__ __forceinline__ int mx_entries(const MxAttn& a, const MxRows& n, int 
   return (mx_seen(a, n, last / a.G) + 15) / 16;
 }
 
-template <typename T> __device__ __forceinline__ void mx_load8(const T* p, bool vec, float (&x)[8]) {
-  if (vec) {
-    T t[8];
-    *reinterpret_cast<u4*>(t) = *reinterpret_cast<const u4*>(p);
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<u4*>(t + 4) = *reinterpret_cast<const u4*>(p + 4);
+// N query values at element offset `at`, wherever they lie: 16-byte loads, all under way at once.
+template <typename T, int N> __device__ __forceinline__ void mx_load(const T* p, float (&x)[N]) {
+  T t[N];
+  __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)p[j];
-  }
+  for (int j = 0; j < N; ++j) x[j] = (float)t[j];
 }
-
-// Eight query values at element offset `at`.
-__device__ __forceinline__ void mx_load_q(const MxAttn& a, int64_t at, float (&x)[8]) {
-  if (a.q_dtype == IAK_DTYPE_F32) mx_load8(reinterpret_cast<const float*>(a.q) + at, a.q_vec, x);
-  else if (a.q_dtype == IAK_DTYPE_F16) mx_load8(reinterpret_cast<const _Float16*>(a.q) + at, a.q_vec, x);
-  else mx_load8(reinterpret_cast<const __bf16*>(a.q) + at, a.q_vec, x);
+template <int N> __device__ __forceinline__ void mx_load_q(const MxAttn& a, int64_t at, float (&x)[N]) {
+  if (a.q_dtype == IAK_DTYPE_F32) mx_load(reinterpret_cast<const float*>(a.q) + at, x);
+  else if (a.q_dtype == IAK_DTYPE_F16) mx_load(reinterpret_cast<const _Float16*>(a.q) + at, x);
+  else mx_load(reinterpret_cast<const __bf16*>(a.q) + at, x);
 }
 
 }  // namespace iak

@@ -71,23 +71,16 @@ __device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void out4(T* p, bool vec, const float (&x)[4]) {
+template <typename T> __device__ __forceinline__ void out4(T* p, const float (&x)[4]) {
   T t[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) t[j] = (T)x[j];
-  if (vec) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<u4*>(p) = *reinterpret_cast<const u4*>(t);
-    else *reinterpret_cast<u2*>(p) = *reinterpret_cast<const u2*>(t);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = t[j];
-  }
+  __builtin_memcpy(p, t, sizeof(t));                             // one store, wherever the row lies
 }
 __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const float (&x)[4]) {
-  if (a.out_dtype == IAK_DTYPE_F32) out4(reinterpret_cast<float*>(a.out) + at, a.out_vec, x);
-  else if (a.out_dtype == IAK_DTYPE_F16) out4(reinterpret_cast<_Float16*>(a.out) + at, a.out_vec, x);
-  else out4(reinterpret_cast<__bf16*>(a.out) + at, a.out_vec, x);
+  if (a.out_dtype == IAK_DTYPE_F32) out4(reinterpret_cast<float*>(a.out) + at, x);
+  else if (a.out_dtype == IAK_DTYPE_F16) out4(reinterpret_cast<_Float16*>(a.out) + at, x);
+  else out4(reinterpret_cast<__bf16*>(a.out) + at, x);
 }
 
 // A query row's operand: the lane's channels (D/4) g .., scaled by a power of two to a largest
@@ -95,27 +88,19 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
 // base-2 scores of the products: positive, NaN for a row that is not finite. (A negative scale
 // turns the query's sign; where the factor would vanish the scores do: query 0, factor 1.)
 template <int D, bool QF32>
-__device__ __forceinline__ float load_query(const MxAttn& a, bool live, int64_t at, int g, h8 (&qhi)[D / 32],
+__device__ __forceinline__ float load_query(const MxAttn& a, bool there, int64_t at, int g, h8 (&qhi)[D / 32],
                                             h8 (&qlo)[QF32 ? D / 32 : 1]) {
-  float x[D / 32][8];
+  float x[D / 4];
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s)
+  for (int j = 0; j < D / 4; ++j) x[j] = 0.f;
+  if (there) mx_load_q(a, at + g * (D / 4), x);
+  float m = 0.f, nan = 0.f;                                      // nan: NaN if any value is infinite or NaN, else 0
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[s][j] = 0.f;
-  if (live) {
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) mx_load_q(a, at + g * (D / 4) + 8 * s, x[s]);
+  for (int j = 0; j < D / 4; ++j) {
+    m = fmaxf(m, fabsf(x[j]));
+    nan = __builtin_fmaf(x[j], 0.f, nan);
   }
-  bool fine = true;
-  float m = 0.f;
-#pragma unroll
-  for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = fabsf(x[s][j]);
-      fine = fine && v < __builtin_inff();
-      m = fmaxf(m, v);
-    }
+  bool fine = nan == 0.f;
   m = xmax16_32(fine ? m : __builtin_inff());
   fine = m < __builtin_inff();
   const int e = m > 0.f ? (int)(f2u(m) >> 23) - 127 : 0;
@@ -126,7 +111,7 @@ __device__ __forceinline__ float load_query(const MxAttn& a, bool live, int64_t 
   for (int s = 0; s < D / 32; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = none ? 0.f : sign * __builtin_ldexpf(x[s][j], 14 - e);
+      const float v = none ? 0.f : sign * __builtin_ldexpf(x[8 * s + j], 14 - e);
       qhi[s][j] = (_Float16)v;
       if constexpr (QF32) qlo[s][j] = (_Float16)(v - (float)qhi[s][j]);
     }
@@ -249,7 +234,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
 
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
-  const float mult = load_query<D, QF32>(a, live, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo);
+  const float mult = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo);
 
   f4 acc[D / 16];
 #pragma unroll
@@ -392,12 +377,12 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
-    const bool live = r < rows && i < n.queries;
+    const bool active = r < rows, live = active && i < n.queries;
     seen[t] = live ? mx_seen(a, n, i) : 0;
     least[t] = live ? seen[t] : 0x7FFFFFFF;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least[t], o, 64); least[t] = x < least[t] ? x : least[t]; }
-    mult[t] = load_query<D, QF32>(a, live, b * a.qsb + i * a.qst + head * a.qsh, g, qhi[t], qlo[t]);
+    mult[t] = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi[t], qlo[t]);
   }
 
   // entries 64 at a time: lane i holds entry i of the block, in `next` of the block after it

@@ -7,7 +7,9 @@
 // x / 2^e is exact, so a code is rounded once, by the conversion instruction.
 //
 // A thread takes 8 channels of K and the same 8 of V: 16-byte loads, one dword of codes
-// stored, and four neighbouring lanes agree on the block's maximum over lane swaps.
+// stored, and four neighbouring lanes agree on the block's maximum over lane swaps. What
+// bounds it is the bytes. Long calls give a workgroup 16 tokens of one head, whose codes are
+// one run of memory wherever a page has room; calls of few tokens give it all heads of one.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,35 +24,24 @@ namespace {
 
 constexpr int MX_THREADS = 256;
 
-// Eight values as floats; `vec`: one or two 16-byte loads, else element by element.
-template <typename T> __device__ __forceinline__ void load8f(const T* p, bool vec, float (&x)[8]) {
-  if (vec) {
-    T t[8];
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<u4*>(t) = *reinterpret_cast<const u4*>(p);
-      *reinterpret_cast<u4*>(t + 4) = *reinterpret_cast<const u4*>(p + 4);
-    } else {
-      *reinterpret_cast<u4*>(t) = *reinterpret_cast<const u4*>(p);
-    }
+// Eight values as floats, wherever they lie: one or two 16-byte loads, which the hardware takes
+// at any address of the type.
+template <typename T> __device__ __forceinline__ void load8f(const T* p, float (&x)[8]) {
+  T t[8];
+  __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)p[j];
-  }
+  for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
 }
 
 // The codes (8 per lane, one dword) and the scale byte of the block that lanes 4n .. 4n+3 hold.
 __device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint32_t& byte) {
   float m = 0.f;
-  bool fine = true;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = fabsf(x[j]);
-    fine = fine && a < __builtin_inff();          // false for NaN too
-    m = fmaxf(m, a);
-  }
-  m = fine ? m : __builtin_inff();
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+  float nan = 0.f;                                // NaN if any value is infinite or NaN, else 0
+#pragma unroll
+  for (int j = 0; j < 8; ++j) nan = __builtin_fmaf(x[j], 0.f, nan);
+  m = nan == 0.f ? m : __builtin_inff();
   m = fmaxf(m, __shfl_xor(m, 1, 64));
   m = fmaxf(m, __shfl_xor(m, 2, 64));
   if (m == __builtin_inff()) { byte = MX_SCALE_NAN; return 0u; }
@@ -66,18 +57,11 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint32_t& byte) {
   return o;
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   T t[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) t[j] = (T)x[j];
-  if (vec) {
-    *reinterpret_cast<u4*>(p) = *reinterpret_cast<const u4*>(t);
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<u4*>(p + 4) = *reinterpret_cast<const u4*>(t + 4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = t[j];
-  }
+  __builtin_memcpy(p, t, sizeof(t));
 }
 
 // Eight values of a code dword and its scale byte.
@@ -92,17 +76,20 @@ __device__ __forceinline__ void values8(uint32_t codes, uint32_t byte, float (&x
   }
 }
 
-struct TokenAt { int b, i, h, c; bool in; };   // channel chunk c of 8
+struct TokenAt { int i, h, c; bool in; };   // token, head, chunk c of 8 channels
 
-__device__ __forceinline__ TokenAt token_at(const iak_mx_tokens_args& a) {
-  const int chunks = a.head_dim / 8;
-  int64_t n = (int64_t)blockIdx.x * MX_THREADS + threadIdx.x;
+// Thread number -> (token / group, head, token % group, chunk); group is 16 or 1, see token_group().
+__device__ __forceinline__ TokenAt token_at(const iak_mx_tokens_args& a, int group) {
+  const uint32_t chunk_bits = a.head_dim == 128 ? 4 : 3, group_bits = group == 16 ? 4 : 0;
+  const uint32_t n = blockIdx.x * (uint32_t)MX_THREADS + threadIdx.x;
+  const uint32_t row = n >> (chunk_bits + group_bits);
+  const uint32_t tokens = row / (uint32_t)a.num_kv_heads;
   TokenAt t;
-  t.c = (int)(n % chunks); n /= chunks;
-  t.h = (int)(n % a.num_kv_heads); n /= a.num_kv_heads;
-  t.i = (int)(n % a.count); n /= a.count;
-  t.b = (int)(n < a.batch ? n : a.batch - 1);
-  t.in = n < a.batch;
+  t.c = (int)(n & ((1u << chunk_bits) - 1));
+  t.h = (int)(row - tokens * (uint32_t)a.num_kv_heads);
+  const uint32_t i = (tokens << group_bits) + ((n >> chunk_bits) & (uint32_t)(group - 1));
+  t.in = i < (uint32_t)a.count;
+  t.i = t.in ? (int)i : 0;
   return t;
 }
 
@@ -119,48 +106,48 @@ __device__ __forceinline__ int row_tokens(const iak_mx_tokens_args& a, int64_t r
 }
 
 template <typename T>
-__global__ __launch_bounds__(MX_THREADS) void mx_append_kernel(const iak_mx_tokens_args a, bool vec) {
-  const TokenAt t = token_at(a);
-  const int n = new_tokens(a, t.b);
-  const int64_t row = (int64_t)t.b * a.num_kv_heads + t.h;
-  const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
-  float k[8], v[8];
-  load8f(reinterpret_cast<const T*>(a.k) + t.b * a.k_stride_b + t.i * a.k_stride_t + t.h * a.k_stride_h + 8 * t.c, vec, k);
-  load8f(reinterpret_cast<const T*>(a.v) + t.b * a.v_stride_b + t.i * a.v_stride_t + t.h * a.v_stride_h + 8 * t.c, vec, v);
-  uint32_t kb, vb;
-  const uint32_t kc = quantise8(k, kb), vc = quantise8(v, vb);   // whole waves: the lanes of a block agree on its maximum
-  if (!t.in || t.i >= n || !at.there) return;
-  const int64_t code = at.token * (a.head_dim / 8) + t.c;
-  reinterpret_cast<uint32_t*>(a.k_codes)[code] = kc;
-  reinterpret_cast<uint32_t*>(a.v_codes)[code] = vc;
-  if ((t.c & 3) == 0) {
-    reinterpret_cast<uint8_t*>(a.k_scales)[code >> 2] = (uint8_t)kb;
-    reinterpret_cast<uint8_t*>(a.v_scales)[code >> 2] = (uint8_t)vb;
+__global__ __launch_bounds__(MX_THREADS) void mx_append_kernel(const iak_mx_tokens_args a, int group) {
+  const TokenAt t = token_at(a, group);
+  for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    const int n = new_tokens(a, b);
+    if (!t.in || t.i >= n) continue;
+    // the values come while the token's place is looked up; the four lanes of a block are one
+    // token's and go together
+    float k[8], v[8];
+    load8f(reinterpret_cast<const T*>(a.k) + b * a.k_stride_b + t.i * a.k_stride_t + t.h * a.k_stride_h + 8 * t.c, k);
+    load8f(reinterpret_cast<const T*>(a.v) + b * a.v_stride_b + t.i * a.v_stride_t + t.h * a.v_stride_h + 8 * t.c, v);
+    const int64_t row = (int64_t)b * a.num_kv_heads + t.h;
+    const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
+    if (!at.there) continue;
+    uint32_t kb, vb;
+    const uint32_t kc = quantise8(k, kb), vc = quantise8(v, vb);
+    const int64_t code = at.token * (a.head_dim / 8) + t.c;
+    reinterpret_cast<uint32_t*>(a.k_codes)[code] = kc;
+    reinterpret_cast<uint32_t*>(a.v_codes)[code] = vc;
+    if ((t.c & 3) == 0) {
+      reinterpret_cast<uint8_t*>(a.k_scales)[code >> 2] = (uint8_t)kb;
+      reinterpret_cast<uint8_t*>(a.v_scales)[code >> 2] = (uint8_t)vb;
+    }
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(MX_THREADS) void mx_read_kernel(const iak_mx_tokens_args a, bool vec) {
-  const TokenAt t = token_at(a);
+__global__ __launch_bounds__(MX_THREADS) void mx_read_kernel(const iak_mx_tokens_args a, int group) {
+  const TokenAt t = token_at(a, group);
   if (!t.in) return;
-  const int n = new_tokens(a, t.b);
-  const int64_t row = (int64_t)t.b * a.num_kv_heads + t.h;
-  const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
-  float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (t.i < n && at.there) {
-    const int64_t code = at.token * (a.head_dim / 8) + t.c;
-    values8(reinterpret_cast<const uint32_t*>(a.k_codes)[code], reinterpret_cast<const uint8_t*>(a.k_scales)[code >> 2], k);
-    values8(reinterpret_cast<const uint32_t*>(a.v_codes)[code], reinterpret_cast<const uint8_t*>(a.v_scales)[code >> 2], v);
+  for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    const int n = new_tokens(a, b);
+    const int64_t row = (int64_t)b * a.num_kv_heads + t.h;
+    const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
+    float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (t.i < n && at.there) {
+      const int64_t code = at.token * (a.head_dim / 8) + t.c;
+      values8(reinterpret_cast<const uint32_t*>(a.k_codes)[code], reinterpret_cast<const uint8_t*>(a.k_scales)[code >> 2], k);
+      values8(reinterpret_cast<const uint32_t*>(a.v_codes)[code], reinterpret_cast<const uint8_t*>(a.v_scales)[code >> 2], v);
+    }
+    store8(reinterpret_cast<T*>(a.k) + b * a.k_stride_b + t.i * a.k_stride_t + t.h * a.k_stride_h + 8 * t.c, k);
+    store8(reinterpret_cast<T*>(a.v) + b * a.v_stride_b + t.i * a.v_stride_t + t.h * a.v_stride_h + 8 * t.c, v);
   }
-  store8(reinterpret_cast<T*>(a.k) + t.b * a.k_stride_b + t.i * a.k_stride_t + t.h * a.k_stride_h + 8 * t.c, vec, k);
-  store8(reinterpret_cast<T*>(a.v) + t.b * a.v_stride_b + t.i * a.v_stride_t + t.h * a.v_stride_h + 8 * t.c, vec, v);
-}
-
-// whether K and V may be read and written as 16-byte vectors
-bool vectors(const iak_mx_tokens_args& a) {
-  const int per = a.dtype == IAK_DTYPE_F32 ? 4 : 8;
-  const int64_t strides = a.k_stride_b | a.k_stride_t | a.k_stride_h | a.v_stride_b | a.v_stride_t | a.v_stride_h;
-  return strides % per == 0 && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15u) == 0;
 }
 
 template <typename F> hipError_t by_dtype(int dtype, F&& f) {
@@ -170,24 +157,26 @@ template <typename F> hipError_t by_dtype(int dtype, F&& f) {
   return hipGetLastError();
 }
 
-int64_t token_blocks(const iak_mx_tokens_args& a) {
-  const int64_t n = (int64_t)a.batch * a.count * a.num_kv_heads * (a.head_dim / 8);
-  return (n + MX_THREADS - 1) / MX_THREADS;
+// Tokens of one head that neighbouring threads take: 16, or 1 where that would leave most idle.
+int token_group(const iak_mx_tokens_args& a) { return a.count >= 16 ? 16 : 1; }
+
+dim3 token_grid(const iak_mx_tokens_args& a) {
+  const int64_t group = token_group(a);
+  const int64_t n = (a.count + group - 1) / group * group * a.num_kv_heads * (a.head_dim / 8);
+  return dim3((uint32_t)((n + MX_THREADS - 1) / MX_THREADS), (uint32_t)(a.batch < 32768 ? a.batch : 32768));
 }
 
 }  // namespace
 
 hipError_t launch_mx_append(const iak_mx_tokens_args& a, hipStream_t stream) {
-  const bool vec = vectors(a);
   return by_dtype(a.dtype, [&](auto t) {
-    hipLaunchKernelGGL((mx_append_kernel<decltype(t)>), dim3((uint32_t)token_blocks(a)), dim3(MX_THREADS), 0, stream, a, vec);
+    hipLaunchKernelGGL((mx_append_kernel<decltype(t)>), token_grid(a), dim3(MX_THREADS), 0, stream, a, token_group(a));
   });
 }
 
 hipError_t launch_mx_read(const iak_mx_tokens_args& a, hipStream_t stream) {
-  const bool vec = vectors(a);
   return by_dtype(a.dtype, [&](auto t) {
-    hipLaunchKernelGGL((mx_read_kernel<decltype(t)>), dim3((uint32_t)token_blocks(a)), dim3(MX_THREADS), 0, stream, a, vec);
+    hipLaunchKernelGGL((mx_read_kernel<decltype(t)>), token_grid(a), dim3(MX_THREADS), 0, stream, a, token_group(a));
   });
 }
 

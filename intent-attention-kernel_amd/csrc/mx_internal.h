@@ -24,8 +24,8 @@ struct MxAttn {
   int chunk_rows; // 64 or 128: the chunk kernel with tiles of that many rows; 0: the rows kernel
   int64_t items;  // workgroups: B * Hkv * splits * tiles (of 16 or of chunk_rows rows)
 
-  const void* q; int q_dtype; int q_vec; int64_t qsb, qst, qsh;          // *_vec: rows lie on 16 bytes
-  void* out; int out_dtype; int out_vec; int64_t osb, ost, osh;
+  const void* q; int q_dtype; int64_t qsb, qst, qsh;
+  void* out; int out_dtype; int64_t osb, ost, osh;
   const int32_t* table;
   const int32_t* valid;
   const int32_t* q_lens;   // may be null

@@ -29,8 +29,8 @@ pages are read on the stream the call is made on.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, fields
-from typing import Dict, Optional, Tuple
+from dataclasses import dataclass
+from typing import Callable, Dict, Optional, Tuple
 
 import torch
 
@@ -59,42 +59,51 @@ class MxFp4Pools:
         return cls(*(torch.zeros(s, dtype=torch.uint8, device=device) for s in (codes, scales, codes, scales)))
 
     def tensors(self) -> Dict[str, torch.Tensor]:
-        return {f.name: getattr(self, f.name) for f in fields(self)}
+        return {"k_codes": self.k_codes, "k_scales": self.k_scales, "v_codes": self.v_codes, "v_scales": self.v_scales}
+
+
+def _device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The one ROCm device of all tensors (None: absent), or require_device's errors."""
+    first = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != first or first < 0):
+            return require_device(*(x for x in tensors if x is not None), what=what)
+    N.load()
+    return tensors[0].device
 
 
 def _check_cache(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor,
                  q_lens: Optional[torch.Tensor], B: int, D: int) -> Tuple[int, int, int]:
     """(Hkv, W, NP) of the pools and the metadata, or ValueError."""
-    if page_table.dim() != 3 or page_table.shape[0] != B or page_table.dtype != torch.int32:
+    if page_table.dim() != 3 or page_table.shape[0] != B or page_table.dtype is not torch.int32:
         raise ValueError(f"page_table must be int32 [{B}, Hkv, W], got {page_table.dtype} {tuple(page_table.shape)}")
-    Hkv, W = page_table.shape[1], page_table.shape[2]
-    if valid_tokens.shape != (B, Hkv) or valid_tokens.dtype != torch.int32:
+    _, Hkv, W = page_table.shape
+    if valid_tokens.shape != (B, Hkv) or valid_tokens.dtype is not torch.int32:
         raise ValueError(f"valid_tokens must be int32 [{B}, {Hkv}], got {valid_tokens.dtype} "
                          f"{tuple(valid_tokens.shape)}")
-    if q_lens is not None and (q_lens.shape != (B,) or q_lens.dtype != torch.int32):
+    if q_lens is not None and (q_lens.shape != (B,) or q_lens.dtype is not torch.int32):
         raise ValueError(f"q_lens must be int32 [{B}], got {q_lens.dtype} {tuple(q_lens.shape)}")
     if D not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {D}")
     NP = pools.k_codes.shape[0] if pools.k_codes.dim() else -1
-    for name, t in pools.tensors().items():
-        _check_pool(name, t, NP, (PAGE_SIZE, D // 2 if name.endswith("codes") else D // BLOCK), (torch.uint8,))
+    codes, scales = (NP, PAGE_SIZE, D // 2), (NP, PAGE_SIZE, D // BLOCK)
+    for t, shape in ((pools.k_codes, codes), (pools.k_scales, scales), (pools.v_codes, codes), (pools.v_scales, scales)):
+        if t.shape != shape or t.dtype is not torch.uint8 or not t.is_contiguous():
+            for name, x in pools.tensors().items():
+                _check_pool(name, x, NP, (codes if name.endswith("codes") else scales)[1:], (torch.uint8,))
     return Hkv, W, NP
 
 
-def _on(device: torch.device):
-    """A guard that makes ``device`` current, where it is not."""
-    return torch.cuda.device(device) if device.index not in (None, torch.cuda.current_device()) else _HERE
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
+def _launch(device: torch.device, call: Callable, *args) -> None:
+    """``call(*args)`` with ``device`` current, as launches on its streams need."""
+    if device.index is None or device.index == _current_device():
+        call(*args)
+    else:
+        with torch.cuda.device(device):
+            call(*args)
 
 
 def _tokens_args(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor,
@@ -106,14 +115,12 @@ def _tokens_args(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, page_table
         raise ValueError(f"page_table has {heads} KV heads, k has {Hkv}")
     page_table, valid_tokens = page_table.contiguous(), valid_tokens.contiguous()
     q_lens = None if q_lens is None else q_lens.contiguous()
-    a = N.MxTokensArgs()
-    a.batch, a.count, a.num_kv_heads, a.head_dim, a.page_size, a.table_width, a.num_pages = B, L, Hkv, D, PAGE_SIZE, W, NP
-    a.k, (a.k_stride_b, a.k_stride_t, a.k_stride_h, _) = k.data_ptr(), k.stride()
-    a.v, (a.v_stride_b, a.v_stride_t, a.v_stride_h, _) = v.data_ptr(), v.stride()
-    a.dtype = _DT[k.dtype]
-    a.page_table, a.valid_tokens, a.q_lens = page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens)
-    a.k_codes, a.k_scales = pools.k_codes.data_ptr(), pools.k_scales.data_ptr()
-    a.v_codes, a.v_scales = pools.v_codes.data_ptr(), pools.v_scales.data_ptr()
+    kb, kt, kh, _ = k.stride()
+    vb, vt, vh, _ = v.stride()
+    a = N.MxTokensArgs(B, L, Hkv, D, PAGE_SIZE, W, NP, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, _DT[k.dtype],
+                       page_table.data_ptr(), valid_tokens.data_ptr(), None if q_lens is None else q_lens.data_ptr(),
+                       pools.k_codes.data_ptr(), pools.k_scales.data_ptr(), pools.v_codes.data_ptr(),
+                       pools.v_scales.data_ptr())
     return a, (page_table, valid_tokens, q_lens)
 
 
@@ -129,13 +136,14 @@ def append_mxfp4_tokens(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, pag
         raise ValueError(f"k and v must have one shape [B, L, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype not in _DT or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be float16, bfloat16 or float32, got {k.dtype} and {v.dtype}")
-    extra = () if q_lens is None else (q_lens,)
-    dev = require_device(k, v, page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit token cache")
-    k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
+    dev = _device("4-bit token cache", k, v, page_table, valid_tokens, q_lens, pools.k_codes, pools.k_scales, pools.v_codes,
+                  pools.v_scales)
+    if k.stride(-1) != 1 or v.stride(-1) != 1:
+        k, v = k.contiguous(), v.contiguous()
     a, keep = _tokens_args(k, v, pools, page_table, valid_tokens, q_lens)
-    with _on(dev):
-        N.mx_append_tokens(a, current_stream_handle(dev))
-    torch.autograd.graph.increment_version(tuple(pools.tensors().values()))   # written through raw pointers
+    _launch(dev, N.mx_append_tokens, a, current_stream_handle(dev))
+    # written through raw pointers
+    torch.autograd.graph.increment_version((pools.k_codes, pools.k_scales, pools.v_codes, pools.v_scales))
 
 
 def read_mxfp4_tokens(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor, count: int, *,
@@ -148,16 +156,15 @@ def read_mxfp4_tokens(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens:
         raise ValueError(f"dtype must be float16, bfloat16 or float32, got {dtype}")
     if count < 0:
         raise ValueError(f"count must not be negative, got {count}")
-    extra = () if q_lens is None else (q_lens,)
-    dev = require_device(page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit token cache")
+    dev = _device("4-bit token cache", page_table, valid_tokens, q_lens, pools.k_codes, pools.k_scales, pools.v_codes,
+                  pools.v_scales)
     if page_table.dim() != 3 or pools.k_codes.dim() != 3:
         raise ValueError(f"page_table must be [B, Hkv, W] and codes [NP, {PAGE_SIZE}, D/2], got "
                          f"{tuple(page_table.shape)} and {tuple(pools.k_codes.shape)}")
     shape = (page_table.shape[0], int(count), page_table.shape[1], 2 * pools.k_codes.shape[2])
-    k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     a, keep = _tokens_args(k, v, pools, page_table, valid_tokens, q_lens)
-    with _on(dev):
-        N.mx_read_tokens(a, current_stream_handle(dev))
+    _launch(dev, N.mx_read_tokens, a, current_stream_handle(dev))
     return k, v
 
 
@@ -180,8 +187,7 @@ class MxFp4Plan:
     def run(self, stream: Optional[int] = None) -> None:
         """Launch on ``stream`` (default: torch's current stream)."""
         s = current_stream_handle(self.device) if stream is None else stream
-        with _on(self.device):
-            N.mx_attention(self.args, s, self._ws_ptr, self.workspace_bytes)
+        _launch(self.device, N.mx_attention, self.args, s, self._ws_ptr, self.workspace_bytes)
 
 
 def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor, *,
@@ -191,8 +197,8 @@ def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor
     """Check the arguments of ``mxfp4_paged_attention`` once, for repeated runs over the same
     tensors. The plan reads the tensors in place: page_table, valid_tokens and q_lens must be
     contiguous, q (and ``out``) have a unit last stride."""
-    extra = tuple(t for t in (q_lens, out) if t is not None)
-    dev = require_device(q, page_table, valid_tokens, *extra, *pools.tensors().values(), what="4-bit cache attention")
+    dev = _device("4-bit cache attention", q, page_table, valid_tokens, q_lens, out, pools.k_codes, pools.k_scales,
+                  pools.v_codes, pools.v_scales)
     if q.dim() not in (3, 4):
         raise ValueError(f"q must have shape [B, Hq, D] or [B, L, Hq, D], got {tuple(q.shape)}")
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
@@ -214,16 +220,13 @@ def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor
     if out.dtype not in _DT or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out dtype {out.dtype} is not {out_dtype or 'float16 / bfloat16 / float32'}")
     o4 = out.unsqueeze(1) if out.dim() == 3 else out
-    a = N.MxAttentionArgs()
-    a.batch, a.q_len, a.num_q_heads, a.num_kv_heads, a.head_dim = B, L, Hq, Hkv, D
-    a.page_size, a.table_width, a.num_pages = PAGE_SIZE, W, NP
-    a.q, a.q_dtype, (a.q_stride_b, a.q_stride_t, a.q_stride_h, _) = q.data_ptr(), _DT[q.dtype], q4.stride()
-    a.out, a.out_dtype, (a.out_stride_b, a.out_stride_t, a.out_stride_h, _) = out.data_ptr(), _DT[out.dtype], o4.stride()
-    a.page_table, a.valid_tokens, a.q_lens = page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens)
-    a.k_codes, a.k_scales = pools.k_codes.data_ptr(), pools.k_scales.data_ptr()
-    a.v_codes, a.v_scales = pools.v_codes.data_ptr(), pools.v_scales.data_ptr()
-    a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    a.causal, a.splits = int(bool(causal)), int(splits)
+    qb, qt, qh, _ = q4.stride()
+    ob, ot, oh, _ = o4.stride()
+    a = N.MxAttentionArgs(B, L, Hq, Hkv, D, PAGE_SIZE, W, NP, q.data_ptr(), _DT[q.dtype], qb, qt, qh, out.data_ptr(),
+                          _DT[out.dtype], ob, ot, oh, page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens),
+                          pools.k_codes.data_ptr(), pools.k_scales.data_ptr(), pools.v_codes.data_ptr(),
+                          pools.v_scales.data_ptr(), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
+                          int(bool(causal)), int(splits))
     return MxFp4Plan(a, dev, out, keep=(q, page_table, valid_tokens, q_lens, *pools.tensors().values()))
 
 

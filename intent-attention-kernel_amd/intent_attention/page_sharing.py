@@ -30,9 +30,9 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .decode_core import PAGE_SIZE, PagePools, current_stream_handle, require_device
+from .decode_core import PAGE_SIZE, PagePools, current_stream_handle
 from .mla_core import LatentPools
-from .mxfp4 import MxFp4Pools, _on
+from .mxfp4 import MxFp4Pools, _device, _launch
 
 Pools = Union[PagePools, LatentPools, MxFp4Pools, torch.Tensor, Sequence[torch.Tensor]]
 Indices = Union[torch.Tensor, Sequence[int]]
@@ -42,18 +42,11 @@ def _pool_tensors(pools: Optional[Pools]) -> List[torch.Tensor]:
     """The tensors of the pools, each once (K and V may be one pool)."""
     if pools is None:
         return []
-    if isinstance(pools, torch.Tensor):
-        ts: Iterable[torch.Tensor] = (pools,)
-    elif isinstance(pools, (PagePools, LatentPools, MxFp4Pools)):
-        ts = pools.tensors().values()
+    if isinstance(pools, (PagePools, LatentPools, MxFp4Pools)):
+        ts: Iterable = (t for t in vars(pools).values() if isinstance(t, torch.Tensor))
     else:
-        ts = pools
-    seen, out = set(), []
-    for t in ts:
-        if (t.data_ptr(), t.numel() * t.element_size()) not in seen:
-            seen.add((t.data_ptr(), t.numel() * t.element_size()))
-            out.append(t)
-    return out
+        ts = (pools,) if isinstance(pools, torch.Tensor) else pools
+    return list({(t.data_ptr(), t.numel() * t.element_size()): t for t in ts}.values())
 
 
 def _fill_arrays(a, tensors: List[torch.Tensor], NP: int) -> None:
@@ -61,20 +54,20 @@ def _fill_arrays(a, tensors: List[torch.Tensor], NP: int) -> None:
         raise ValueError(f"at most {N.MAX_PAGE_ARRAYS} pool tensors, got {len(tensors)}")
     n = 0
     for t in tensors:
-        if not t.is_contiguous() or t.dim() == 0 or NP == 0 or t.numel() % NP or t.shape[0] % NP:
-            if NP == 0 and t.numel() == 0:
-                continue
+        size = t.numel()
+        if NP == 0 and size == 0:
+            continue
+        if NP == 0 or t.dim() == 0 or size % NP or t.shape[0] % NP or not t.is_contiguous():
             raise ValueError(f"every pool tensor must be contiguous with a row for each of {NP} pages, "
                              f"got {tuple(t.shape)}")
-        row = t.numel() // NP * t.element_size()
-        if row:
-            a.arrays[n].base, a.arrays[n].row_bytes = t.data_ptr(), row
+        if size:
+            a.arrays[n] = (t.data_ptr(), size // NP * t.element_size())
             n += 1
     a.num_arrays = n
 
 
 def _check_state(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor) -> Tuple[int, int, int, int]:
-    if page_table.dim() != 3 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+    if page_table.dim() != 3 or page_table.dtype is not torch.int32 or not page_table.is_contiguous():
         raise ValueError(f"page_table must be contiguous int32 [B, R, W], got {page_table.dtype} "
                          f"{tuple(page_table.shape)}")
     B, R, W = page_table.shape
@@ -91,7 +84,7 @@ def _check_state(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: tor
 def _indices(name: str, x: Indices, device: torch.device, count: Optional[int] = None) -> torch.Tensor:
     """int32 [n] on the device; a list of ints is uploaded."""
     if isinstance(x, torch.Tensor):
-        if x.dim() != 1 or x.dtype != torch.int32:
+        if x.dim() != 1 or x.dtype is not torch.int32:
             raise ValueError(f"{name} must be int32 [n], got {x.dtype} {tuple(x.shape)}")
         if x.device != device:
             raise ValueError(f"{name} must be on {device}, got {x.device}")
@@ -109,14 +102,13 @@ def _indices(name: str, x: Indices, device: torch.device, count: Optional[int] =
 def _sequences(what: str, page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
                pools: Optional[Pools] = None):
     tensors = _pool_tensors(pools)
-    dev = require_device(page_table, valid_tokens, refs, *tensors, what=what)
+    dev = _device(what, page_table, valid_tokens, refs, *tensors)
     B, R, W, NP = _check_state(page_table, valid_tokens, refs)
     seqs = _indices("seqs", seqs, dev)
-    a = N.SequencesArgs()
-    a.num_seqs, a.rows_per_seq, a.table_width, a.page_size, a.num_pages = B, R, W, PAGE_SIZE, NP
-    a.page_table, a.valid_tokens, a.refs = page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr()
-    a.count, a.seqs = seqs.shape[0], seqs.data_ptr()
-    _fill_arrays(a, tensors, NP)
+    a = N.SequencesArgs(B, R, W, PAGE_SIZE, NP, page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr(),
+                        seqs.shape[0], seqs.data_ptr())
+    if tensors:
+        _fill_arrays(a, tensors, NP)
     return a, dev, seqs, tensors
 
 
@@ -132,8 +124,7 @@ def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor]) -> t
     a.missing = missing.data_ptr()
     size = N.sequences_workspace(a)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        launch(a, current_stream_handle(dev), ws.data_ptr(), size)
+    _launch(dev, launch, a, current_stream_handle(dev), ws.data_ptr(), size)
     return missing
 
 
@@ -170,8 +161,7 @@ def free_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: t
     become -1 and the lengths 0. Indices outside the table are left out, one listed twice is
     freed once."""
     a, dev, seqs, _ = _sequences("page sharing", page_table, valid_tokens, refs, seqs)
-    with _on(dev):
-        N.free_sequences(a, current_stream_handle(dev))
+    _launch(dev, N.free_sequences, a, current_stream_handle(dev))
     _written(page_table, valid_tokens, refs)
 
 
@@ -184,18 +174,15 @@ def compact_pages(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: to
     pages' old rows keep their bytes, so what was queued with the old table still finds them
     until their ids are handed out again."""
     tensors = _pool_tensors(pools)
-    dev = require_device(page_table, valid_tokens, refs, *tensors, what="page compaction")
+    dev = _device("page compaction", page_table, valid_tokens, refs, *tensors)
     B, R, W, NP = _check_state(page_table, valid_tokens, refs)
     table, new_refs, page_map = torch.empty_like(page_table), torch.empty_like(refs), torch.empty_like(refs)
-    a = N.CompactPagesArgs()
-    a.num_rows, a.table_width, a.page_size, a.num_pages = B * R, W, PAGE_SIZE, NP
-    a.page_table, a.valid_tokens, a.refs = page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr()
-    a.out_table, a.out_refs, a.page_map = table.data_ptr(), new_refs.data_ptr(), page_map.data_ptr()
+    a = N.CompactPagesArgs(B * R, W, PAGE_SIZE, NP, page_table.data_ptr(), valid_tokens.data_ptr(), refs.data_ptr(),
+                           table.data_ptr(), new_refs.data_ptr(), page_map.data_ptr())
     _fill_arrays(a, tensors, NP)
     size = N.compact_pages_workspace(a)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        N.compact_pages(a, current_stream_handle(dev), ws.data_ptr(), size)
+    _launch(dev, N.compact_pages, a, current_stream_handle(dev), ws.data_ptr(), size)
     if tensors:
         _written(*tensors)
     return table, new_refs, page_map
@@ -208,13 +195,12 @@ def copy_pages(pools: Pools, src: Indices, dst: Indices, *, num_pages: Optional[
     tensors = _pool_tensors(pools)
     if not tensors:
         raise ValueError("no pool tensor given")
-    dev = require_device(*tensors, what="page copy")
+    dev = _device("page copy", *tensors)
     NP = tensors[0].shape[0] if num_pages is None else int(num_pages)
     src = _indices("src", src, dev)
     dst = _indices("dst", dst, dev, src.shape[0])
     a = N.CopyPagesArgs()
     a.num_pages, a.count, a.src, a.dst = NP, src.shape[0], src.data_ptr(), dst.data_ptr()
     _fill_arrays(a, tensors, NP)
-    with _on(dev):
-        N.copy_pages(a, current_stream_handle(dev))
+    _launch(dev, N.copy_pages, a, current_stream_handle(dev))
     _written(*tensors)
