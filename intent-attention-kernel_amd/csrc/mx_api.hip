@@ -5,7 +5,6 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <cstdlib>
 
 #include "iak.h"
 #include "mx_internal.h"
@@ -68,29 +67,29 @@ struct MxPlan {
 };
 
 // Which kernel, and into how many splits a row's tokens go: the least of costs in microseconds
-// fitted to measurements (32 shapes of 8 to 65,536 query rows by 16 to 2,048 table entries).
-// The card holds `places` workgroups at a time. A round of them takes START and its entries'
-// time; a round that is not full runs faster, at most twice; a second kernel merges splits at
-// MERGE and the time of the partials' bytes.
+// fitted to measurements (40 shapes of 8 to 65,536 query rows by 16 to 2,048 table entries).
+// A CU holds two to four workgroups at a time. A round of as many takes START and its entries'
+// time, one of fewer runs faster; a second kernel merges splits at MERGE and the time of the
+// partials' bytes.
 //   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 190 us, 4 228,
 //     6 195, 8 203; 512 x 125: 1 split 31, 2 42, 4 44; 64 x 128: 1 split 18, 4 14.6, 8 13.8, 16 17
 //   2,048 queries x 4 heads x 8 KV heads over 8,192 tokens: rows kernel 475, chunk kernel 293;
-//     16 x 4 x 64 over 4,000: rows 31, chunk 40 (8 splits)
+//     512 x 4 x 8: rows 140, chunk 96 (4 splits); 16 x 4 x 64 over 4,000: rows 30, chunk 40
 constexpr int CHUNK_ROWS = 128;
-constexpr double FEW_TILES = 256;   // up to as many unsplit tiles are workgroups of more waves: one a CU
+constexpr double CUS = 256;         // and up to as many unsplit tiles are workgroups of more waves
 
 struct MxChoice { bool chunk; int64_t splits; };
 
 MxChoice choose(double kvrows, int64_t rows, int W, int D, bool f32, int64_t forced) {
   const double START = 3, MERGE = 6;
-  const bool wide_head = D == 128;
-  const double tiles = kvrows * ((rows + 15) / 16), blocks = kvrows * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS);
-  const double per_head = (rows + 15) / 16;                      // tiles that read the same pages
-  const double bytes_entry = (wide_head ? 0.30 : 0.20) / per_head;   // one entry's bytes, the card full
-  double rows_entry = wide_head ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
+  const bool big = D == 128;
+  const double per_head = (double)((rows + 15) / 16);            // tiles of 16 rows that read the same pages
+  const double tiles = kvrows * per_head, blocks = kvrows * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS);
+  const double bytes_entry = (big ? 0.30 : 0.20) / per_head;     // an entry's bytes, the card full
+  double rows_entry = big ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
   if (rows_entry < bytes_entry) rows_entry = bytes_entry;
-  const double chunk_entry = wide_head ? (f32 ? 0.92 : 0.57) : (f32 ? 0.60 : 0.48);
-  const double rows_places = wide_head ? 768 : 1024, chunk_places = wide_head || f32 ? 512 : 768;
+  const double chunk_entry = big ? (f32 ? 0.92 : 0.57) : (f32 ? 0.60 : 0.48);
+  const int rows_places = big ? 3 : 4, chunk_places = big || f32 ? 2 : 3;   // workgroups a CU
   const int64_t most = (W + 15) / 16;
   MxChoice best = {false, 1};
   double least = -1;
@@ -98,23 +97,24 @@ MxChoice choose(double kvrows, int64_t rows, int W, int D, bool f32, int64_t for
     if (s > most) s = most;
     if (s < 1) s = 1;
     if (forced > 0) s = forced;
-    const bool many = !chunk && s == 1 && tiles <= FEW_TILES;
-    const double work = chunk ? blocks : tiles, places = chunk ? chunk_places : many ? FEW_TILES : rows_places;
-    const double entry = (chunk ? chunk_entry : rows_entry) / (many ? (wide_head ? 2 : 4) : 1);
-    const double rounds = work * s / places, full = std::floor(rounds), rest = rounds - full;
-    double cost = (full + (rest > 0 ? 0.5 + 0.5 * rest : 0)) * (START + entry * W / s);
-    if (s > 1) cost += MERGE + kvrows * rows * s * D * 8 / 3.0e6;
+    const bool many = !chunk && s == 1 && tiles <= CUS;
+    const double each = std::ceil((chunk ? blocks : tiles) * s / CUS);      // workgroups of the busiest CU
+    const int places = chunk ? chunk_places : many ? 1 : rows_places;
+    const double full = std::floor(each / places), rest = each - full * places;
+    const double entry = (chunk ? chunk_entry : rows_entry) / (many ? (big ? 3 : 5) : 1);
+    double cost = (full + (rest > 0 ? 0.42 + 0.58 * rest / places : 0)) * (START + entry * W / s);
+    if (s > 1) cost += MERGE + kvrows * rows * s * D * 8 / 4.0e6;
     if (least < 0 || cost < least) { least = cost; best = {chunk, s}; }
   };
-  auto each = [&](bool chunk) {
-    const double work = chunk ? blocks : tiles, places = chunk ? chunk_places : rows_places;
+  auto each_split = [&](bool chunk) {
+    const double work = chunk ? blocks : tiles, places = CUS * (chunk ? chunk_places : rows_places);
     consider(chunk, 1);
     if (work >= 4 * places || most <= 1 || forced > 0) return;
     for (int64_t s = 2; s < most && s < 256; s *= 2) consider(chunk, s);
     for (int rounds = 1; rounds <= 4; ++rounds) consider(chunk, (int64_t)(rounds * places / work));
   };
-  each(false);
-  if (rows > 16) each(true);
+  each_split(false);
+  if (rows > 16) each_split(true);
   return best;
 }
 
@@ -138,6 +138,7 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   if (a->num_pages > 0 && (!a->k_codes || !a->k_scales || !a->v_codes || !a->v_scales))
     return fail(IAK_EINVAL, "a code or scale pool is NULL");
   if (!aligned16(a->k_codes) || !aligned16(a->v_codes)) return fail(IAK_EINVAL, "code pools must be 16-byte aligned");
+  if (!aligned4(a->k_scales) || !aligned4(a->v_scales)) return fail(IAK_EINVAL, "scale pools must be 4-byte aligned");
   const int64_t rows = (int64_t)a->q_len * p->G;
   if (rows > 0x3FFFFFFF) return fail(IAK_EINVAL, "q_len %d x %d heads per KV head is too long", a->q_len, p->G);
   p->tiles = (int)((rows + 15) / 16);
@@ -145,7 +146,6 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
   const int W = a->table_width > 0 ? a->table_width : 1;
   MxChoice best = choose((double)a->batch * a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
-  if (const char* f = getenv("MXF")) { if (f[0]=='0') best.chunk = false; else if (f[0]=='1') best.chunk = rows > 16; }
   p->chunk_rows = best.chunk ? CHUNK_ROWS : 0;
   const double blocks = best.chunk ? (double)a->batch * a->num_kv_heads * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS) : tiles;
   int64_t splits = best.splits;
@@ -153,7 +153,7 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
-  p->waves = p->splits == 1 && tiles <= FEW_TILES ? 16 : 4;
+  p->waves = p->splits == 1 && tiles <= CUS ? 16 : 4;
   p->items = (int64_t)blocks * p->splits;
   if (p->splits > 1) {
     const size_t slots = (size_t)tiles * p->splits * 16;

@@ -43,9 +43,18 @@ template <int D> __device__ __forceinline__ int v_chunk(int t, int ch) {
 
 template <int D> struct MxPair {   // two pages as a lane loads them
   uint32_t k[2][D / 32], v[2][D / 32];
-  uint32_t ks[2], vs[2];
+  uint32_t ks[2], vs[2];           // four scale bytes, the lane's own among them (own_scale)
   int id[2];                       // wave-uniform; -1: no page
 };
+
+// A lane's scale bytes come as the aligned four they are among: a byte loaded alone is zero-
+// extended where the loop turns, and that waits for loads that the next round is meant to await.
+template <int D> __device__ __forceinline__ uint32_t scale_word(const uint8_t* page_scales, int c, int g) {
+  return reinterpret_cast<const uint32_t*>(page_scales)[(c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK) >> 2];
+}
+template <int D> __device__ __forceinline__ uint32_t own_scale(uint32_t word, int c, int g) {
+  return __builtin_amdgcn_ubfe(word, 8 * ((c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK) & 3), 8);
+}
 
 template <int D>
 __device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0, int id1, int c, int g) {
@@ -54,7 +63,7 @@ __device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const int64_t page = r.id[p] < 0 ? 0 : r.id[p];
-    const uint32_t code = c * (D / 2) + g * (D / 8), sc = c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK;
+    const uint32_t code = c * (D / 2) + g * (D / 8);
     const uint8_t* kc = a.k_codes + page * (PS * D / 2);
     const uint8_t* vc = a.v_codes + page * (PS * D / 2);
     if constexpr (D == 128) {
@@ -66,8 +75,8 @@ __device__ __forceinline__ void load_pair(MxPair<D>& r, const MxAttn& a, int id0
 #pragma unroll
       for (int i = 0; i < 2; ++i) { r.k[p][i] = k[i]; r.v[p][i] = v[i]; }
     }
-    r.ks[p] = (a.k_scales + page * (PS * D / MX_BLOCK))[sc];
-    r.vs[p] = (a.v_scales + page * (PS * D / MX_BLOCK))[sc];
+    r.ks[p] = scale_word<D>(a.k_scales + page * (PS * D / MX_BLOCK), c, g);
+    r.vs[p] = scale_word<D>(a.v_scales + page * (PS * D / MX_BLOCK), c, g);
   }
 }
 
@@ -227,11 +236,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   const int32_t* row = a.table + kvrow * a.W;
   auto entry_id = [&](int k) {
     const int e = e0 + wave_entry<NW>(w, k);
-    const int id = e < e1 ? row[e] : -1;
-    return id < 0 || id >= a.NP ? -1 : id;
+    return e < e1 ? row[e] : -1;
   };
   int ids = entry_id(lane), next = entry_id(64 + lane);
-  auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
+  const uint32_t pages = (uint32_t)a.NP;
+  auto page = [&](int k) {
+    const int id = k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64);
+    return (uint32_t)id < pages ? id : -1;
+  };
 
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
   const float mult = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo);
@@ -245,7 +257,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   // one step: the pair `x` of entries e, e + 1; then `x` is the pair of pages to0, to1
   auto step = [&](MxPair<D>& x, int e, int to0, int to1) {
     f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    const float ks[2] = {mx_scale(x.ks[0]), mx_scale(x.ks[1])}, vs[2] = {mx_scale(x.vs[0]), mx_scale(x.vs[1])};
+    const uint32_t kb[2] = {own_scale<D>(x.ks[0], c, g), own_scale<D>(x.ks[1], c, g)};
+    const uint32_t vb[2] = {own_scale<D>(x.vs[0], c, g), own_scale<D>(x.vs[1], c, g)};
+    const float ks[2] = {mx_scale(kb[0]), mx_scale(kb[1])}, vs[2] = {mx_scale(vb[0]), mx_scale(vb[1])};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -270,13 +284,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 
     // what is left to do with the pair: which tokens are NaN (rare), which pages are none
-    uint32_t most = x.ks[0] > x.ks[1] ? x.ks[0] : x.ks[1], vmost = x.vs[0] > x.vs[1] ? x.vs[0] : x.vs[1];
+    uint32_t most = kb[0] > kb[1] ? kb[0] : kb[1], vmost = vb[0] > vb[1] ? vb[0] : vb[1];
     most = most > vmost ? most : vmost;
     uint32_t nan_tokens[2] = {0u, 0u};
     if (__builtin_amdgcn_ballot_w64(most == MX_SCALE_NAN)) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint64_t bad = __builtin_amdgcn_ballot_w64(x.ks[p] == MX_SCALE_NAN || x.vs[p] == MX_SCALE_NAN);
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(kb[p] == MX_SCALE_NAN || vb[p] == MX_SCALE_NAN);
         nan_tokens[p] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
       }
     }
@@ -389,17 +403,20 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
   const int32_t* row = a.table + kvrow * a.W;
   auto entry_id = [&](int k) {
     const int e = e0 + k;
-    const int id = e < e1 ? row[e] : -1;
-    return id < 0 || id >= a.NP ? -1 : id;
+    return e < e1 ? row[e] : -1;
   };
   int ids = entry_id(lane), next = entry_id(64 + lane);
-  auto page = [&](int k) { return k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64); };
+  const uint32_t pages = (uint32_t)a.NP;
+  auto page = [&](int k) {
+    const int id = k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64);
+    return (uint32_t)id < pages ? id : -1;
+  };
 
   // this wave's page of a step: loaded a step ahead, converted into LDS during the step before
   uint32_t kr[D / 32], ks, vr[D / 32], vs;
   auto load_page = [&](int id) {
     const int64_t p = id < 0 ? 0 : id;
-    const uint32_t code = c * (D / 2) + g * (D / 8), sc = c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK;
+    const uint32_t code = c * (D / 2) + g * (D / 8);
     const uint8_t *kc = a.k_codes + p * (PS * D / 2) + code, *vc = a.v_codes + p * (PS * D / 2) + code;
     if constexpr (D == 128) {
       const u4 k = *reinterpret_cast<const u4*>(kc), v = *reinterpret_cast<const u4*>(vc);
@@ -410,11 +427,12 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) { kr[i] = k[i]; vr[i] = v[i]; }
     }
-    ks = (a.k_scales + p * (PS * D / MX_BLOCK))[sc];
-    vs = (a.v_scales + p * (PS * D / MX_BLOCK))[sc];
+    ks = scale_word<D>(a.k_scales + p * (PS * D / MX_BLOCK), c, g);
+    vs = scale_word<D>(a.v_scales + p * (PS * D / MX_BLOCK), c, g);
   };
   auto convert = [&](int buf) {
-    const float sk = mx_scale(ks), sv = mx_scale(vs);
+    const uint32_t kb = own_scale<D>(ks, c, g), vb = own_scale<D>(vs, c, g);
+    const float sk = mx_scale(kb), sv = mx_scale(vb);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       uint32_t o[4];
@@ -423,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
       mx8_to_f16(vr[j], sv, o);
       vt[buf][w][v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
     }
-    const uint64_t bad = __builtin_amdgcn_ballot_w64((ks > vs ? ks : vs) == MX_SCALE_NAN);
+    const uint64_t bad = __builtin_amdgcn_ballot_w64((kb > vb ? kb : vb) == MX_SCALE_NAN);
     if (lane == 0)
       reinterpret_cast<uint32_t*>(&nan_in[buf])[w] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
   };
@@ -443,11 +461,13 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
   auto step = [&](int buf, int e) {
     f4 s[RT][4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) s[t][p] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int p = 0; p < 4; ++p) s[t][p] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
         const h8 ka = __builtin_bit_cast(h8, kt[buf][p][v_chunk<D>(c, g * (D / 32) + j)]);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -455,7 +475,6 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
           if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[t][j], s[t][p], 0, 0, 0);
         }
       }
-    }
     const u4 bad = nan_in[buf];
     const int id[4] = {page(k), page(k + 1), page(k + 2), page(k + 3)};
     convert(buf ^ 1);
