@@ -127,57 +127,71 @@ __device__ __forceinline__ float load_query(const MxAttn& a, bool there, int64_t
   return !fine ? __builtin_nanf("") : none ? 1.f : mult;
 }
 
-// What the score results of PAGES pages (lane: row c, tokens 4g .. 4g+3 of each) become: NaN
-// where a token has a NaN block (bit per token in `nan`, rare), -inf where the row does not see
-// it; then the weights exp2(s * mult - m + P_SHIFT) in place. Moves the row's running maximum m,
-// sum l (SUM: adds the weights to it) and accumulator. The lanes of a row compare maxima only when
-// one of them is past the slack. `e`: the first page's entry number; `least`: see the kernels.
-template <int D, int PAGES, bool SUM>
-__device__ __forceinline__ void soften(f4 (&s)[PAGES], const uint32_t (&nan)[PAGES], const int (&id)[PAGES], int e, int seen,
-                                       int least, float mult, int g, float& m, f4& l, f4 (&acc)[D / 16]) {
+// The softmax of PAGES pages' score results (lane: row c of T tiles, tokens 4g .. 4g+3 of each
+// page), in three parts, each of which leaves the straight line at one rarely taken branch:
+//   hide    scores become NaN where a token has a NaN block (bit per token in `nan`) and -inf
+//           where the row does not see it; `e`: the first page's entry, `least`: tokens that
+//           every row of the wave sees
+//   raise   moves a row's running maximum m, with its sum l and accumulator, where a score
+//           exceeds it by more than the slack: the lanes of a row compare theirs only then
+//   soften  scores become the weights exp2(s * mult - m + P_SHIFT)
+template <int PAGES, int T>
+__device__ __forceinline__ void hide(f4 (&s)[T][PAGES], const uint32_t (&nan)[PAGES], const int (&id)[PAGES], int e,
+                                     const int (&seen)[T], int least, int g) {
   uint32_t any_nan = 0u;
   int ids = 0;
 #pragma unroll
   for (int p = 0; p < PAGES; ++p) { any_nan |= nan[p]; ids |= id[p]; }
-  if (__builtin_expect(any_nan != 0u, 0)) {
+  if (any_nan != 0u || ids < 0 || (e + PAGES) * PS > least) {
     asm volatile("");                                            // a branch, not selects for every call
 #pragma unroll
-    for (int p = 0; p < PAGES; ++p)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if ((nan[p] >> (4 * g + q)) & 1u) s[p][q] = __builtin_nanf("");
+      for (int p = 0; p < PAGES; ++p) {
+        const int lim = id[p] < 0 ? 0 : seen[t] - (e + p) * PS;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if ((nan[p] >> (4 * g + q)) & 1u) s[t][p][q] = __builtin_nanf("");
+          if (4 * g + q >= lim) s[t][p][q] = -__builtin_inff();
+        }
+      }
   }
-  if ((e + PAGES) * PS > least || ids < 0) {
+}
+
+template <int D, int PAGES, int T>
+__device__ __forceinline__ void raise(const f4 (&s)[T][PAGES], const float (&mult)[T], float (&m)[T], f4 (&l)[T],
+                                      f4 (&acc)[T][D / 16]) {
+  float top[T];
+  bool over = false;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    top[t] = fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3]));
+#pragma unroll
+    for (int p = 1; p < PAGES; ++p)
+      top[t] = fmaxf(top[t], fmaxf(fmaxf(s[t][p][0], s[t][p][1]), fmaxf(s[t][p][2], s[t][p][3])));
+    over = over || top[t] * mult[t] > m[t] + RESCALE_SLACK;
+  }
+  if (__builtin_amdgcn_ballot_w64(over)) {
     asm volatile("");
 #pragma unroll
-    for (int p = 0; p < PAGES; ++p) {
-      const int lim = id[p] < 0 ? 0 : seen - (e + p) * PS;
+    for (int t = 0; t < T; ++t) {
+      const float pm = xmax16_32(top[t]) * mult[t];
+      const float mn = pm > m[t] + RESCALE_SLACK ? pm : m[t];
+      const float alpha = __builtin_amdgcn_exp2f(m[t] - mn);
+      l[t] *= alpha;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (4 * g + q >= lim) s[p][q] = -__builtin_inff();
+      for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] *= alpha;
+      m[t] = mn;
     }
   }
-  float pm = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-#pragma unroll
-  for (int p = 1; p < PAGES; ++p) pm = fmaxf(pm, fmaxf(fmaxf(s[p][0], s[p][1]), fmaxf(s[p][2], s[p][3])));
-  if (__builtin_amdgcn_ballot_w64(pm * mult > m + RESCALE_SLACK)) {
-    asm volatile("");
-    pm = xmax16_32(pm) * mult;
-    const float mn = pm > m + RESCALE_SLACK ? pm : m;
-    const float alpha = __builtin_amdgcn_exp2f(m - mn);
-    l *= alpha;
-#pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb) acc[mb] *= alpha;
-    m = mn;
-  }
+}
+
+template <int PAGES> __device__ __forceinline__ void soften(f4 (&s)[PAGES], float mult, float m) {
   const float base = P_SHIFT - m;
 #pragma unroll
   for (int p = 0; p < PAGES; ++p)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s[p][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p][q], mult, base));
-      if constexpr (SUM) l[q] += s[p][q];
-    }
+    for (int q = 0; q < 4; ++q) s[p][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p][q], mult, base));
 }
 
 // Weights of two pages as the value product's operand, and what rounding left (float32 queries).
@@ -226,8 +240,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
 
   const int r = tile * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
   const bool active = r < a.L * a.G, live = active && i < n.queries;
-  const int seen = live ? mx_seen(a, n, i) : 0;
-  int least = live ? seen : 0x7FFFFFFF;                          // tokens below it need no mask
+  const int seen[1] = {live ? mx_seen(a, n, i) : 0};
+  int least = live ? seen[0] : 0x7FFFFFFF;                       // tokens below it need no mask
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
 
@@ -241,22 +255,22 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   int ids = entry_id(lane), next = entry_id(64 + lane);
   const uint32_t pages = (uint32_t)a.NP;
   auto page = [&](int k) {
-    const int id = k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64);
+    const int here = __builtin_amdgcn_readlane(ids, k & 63), after = __builtin_amdgcn_readlane(next, k & 63);
+    const int id = k < 64 ? here : after;
     return (uint32_t)id < pages ? id : -1;
   };
 
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
-  const float mult = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo);
+  const float mult[1] = {load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo)};
 
-  f4 acc[D / 16];
+  f4 acc[1][D / 16], l[1] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-  for (int mb = 0; mb < D / 16; ++mb) acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
-  float m = M_NONE;
-  f4 l = {0.f, 0.f, 0.f, 0.f};
+  for (int mb = 0; mb < D / 16; ++mb) acc[0][mb] = f4{0.f, 0.f, 0.f, 0.f};
+  float m[1] = {M_NONE};
 
   // one step: the pair `x` of entries e, e + 1; then `x` is the pair of pages to0, to1
   auto step = [&](MxPair<D>& x, int e, int to0, int to1) {
-    f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    f4 s[1][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
     const uint32_t kb[2] = {own_scale<D>(x.ks[0], c, g), own_scale<D>(x.ks[1], c, g)};
     const uint32_t vb[2] = {own_scale<D>(x.vs[0], c, g), own_scale<D>(x.vs[1], c, g)};
     const float ks[2] = {mx_scale(kb[0]), mx_scale(kb[1])}, vs[2] = {mx_scale(vb[0]), mx_scale(vb[1])};
@@ -267,8 +281,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
         uint32_t o[4];
         mx8_to_f16(x.k[p][j], ks[p], o);
         const h8 ka = make_h8(o[0], o[1], o[2], o[3]);
-        s[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[j], s[p], 0, 0, 0);
-        if constexpr (QF32) s[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[j], s[p], 0, 0, 0);
+        s[0][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[j], s[0][p], 0, 0, 0);
+        if constexpr (QF32) s[0][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[j], s[0][p], 0, 0, 0);
       }
 
     // V: rows of this lane's token into LDS, while the scores are under way
@@ -297,15 +311,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
     const int id[2] = {x.id[0], x.id[1]};
     load_pair<D>(x, a, to0, to1, c, g);                          // under way during the rest of the step
 
-    soften<D, 2, true>(s, nan_tokens, id, e, seen, least, mult, g, m, l, acc);
-    const h8 pb = weights(s[0], s[1]);
+    hide<2, 1>(s, nan_tokens, id, e, seen, least, g);
+    raise<D, 2, 1>(s, mult, m, l, acc);
+    soften<2>(s[0], mult[0], m[0]);
+    l[0] += s[0][0] + s[0][1];
+    const h8 pb = weights(s[0][0], s[0][1]);
     h8 pl;
-    if constexpr (QF32) pl = weights_rest(s[0], s[1], pb);
+    if constexpr (QF32) pl = weights_rest(s[0][0], s[0][1], pb);
 #pragma unroll
     for (int mb = 0; mb < D / 16; ++mb) {
       const h8 va = values_back<D>(&vt[w][0], &vt[w][PS * D / 8], mb, c, g);
-      acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[mb], 0, 0, 0);
-      if constexpr (QF32) acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[mb], 0, 0, 0);
+      acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[0][mb], 0, 0, 0);
+      if constexpr (QF32) acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[0][mb], 0, 0, 0);
     }
   };
 
@@ -326,12 +343,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   }
 
   // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
-  const float sum = xsum16_32((l[0] + l[1]) + (l[2] + l[3]));
+  const float sum = xsum16_32((l[0][0] + l[0][1]) + (l[0][2] + l[0][3]));
   __syncthreads();
-  if (g == 0) { part_m[w][c] = m; part_l[w][c] = sum; }
+  if (g == 0) { part_m[w][c] = m[0]; part_l[w][c] = sum; }
   f4* sums = reinterpret_cast<f4*>(&vt[w][0]);
 #pragma unroll
-  for (int mb = 0; mb < D / 16; ++mb) sums[c * (D / 4) + ((4 * mb + g) ^ c)] = acc[mb];
+  for (int mb = 0; mb < D / 16; ++mb) sums[c * (D / 4) + ((4 * mb + g) ^ c)] = acc[0][mb];
   __syncthreads();
   const int rows = a.L * a.G - tile * 16 < 16 ? a.L * a.G - tile * 16 : 16;
   for (int k2 = threadIdx.x; k2 < rows * (D / 4); k2 += 64 * NW) {
@@ -385,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
   if (split > 0 && e0 >= e1) return;                             // uniform; the merge does not look at it
 
   const int rows = a.L * a.G;
-  int seen[RT], least[RT];
+  int seen[RT], least = 0x7FFFFFFF;
   h8 qhi[RT][D / 32], qlo[RT][QF32 ? D / 32 : 1];
   float mult[RT];
 #pragma unroll
@@ -393,11 +410,11 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
     const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
     const bool active = r < rows, live = active && i < n.queries;
     seen[t] = live ? mx_seen(a, n, i) : 0;
-    least[t] = live ? seen[t] : 0x7FFFFFFF;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least[t], o, 64); least[t] = x < least[t] ? x : least[t]; }
+    least = live && seen[t] < least ? seen[t] : least;
     mult[t] = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi[t], qlo[t]);
   }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
 
   // entries 64 at a time: lane i holds entry i of the block, in `next` of the block after it
   const int32_t* row = a.table + kvrow * a.W;
@@ -408,7 +425,8 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
   int ids = entry_id(lane), next = entry_id(64 + lane);
   const uint32_t pages = (uint32_t)a.NP;
   auto page = [&](int k) {
-    const int id = k < 64 ? __builtin_amdgcn_readlane(ids, k) : __builtin_amdgcn_readlane(next, k - 64);
+    const int here = __builtin_amdgcn_readlane(ids, k & 63), after = __builtin_amdgcn_readlane(next, k & 63);
+    const int id = k < 64 ? here : after;
     return (uint32_t)id < pages ? id : -1;
   };
 
@@ -442,8 +460,7 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
       vt[buf][w][v_chunk<D>(c, g * (D / 32) + j)] = u4{o[0], o[1], o[2], o[3]};
     }
     const uint64_t bad = __builtin_amdgcn_ballot_w64((kb > vb ? kb : vb) == MX_SCALE_NAN);
-    if (lane == 0)
-      reinterpret_cast<uint32_t*>(&nan_in[buf])[w] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
+    reinterpret_cast<uint32_t*>(&nan_in[buf])[w] = (uint32_t)(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xFFFFu;
   };
 
   f4 acc[RT][D / 16], l[RT];
@@ -479,16 +496,15 @@ __global__ __launch_bounds__(256, 2) void mx_chunk_kernel(const MxAttn a) {
     const int id[4] = {page(k), page(k + 1), page(k + 2), page(k + 3)};
     convert(buf ^ 1);
     load_page(page(k + 8 + w));
-    uint32_t nan_tokens[4] = {0u, 0u, 0u, 0u};
-    if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1] | bad[2] | bad[3])) {
-      asm volatile("");
+    uint32_t nan_tokens[4];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) nan_tokens[p] = __builtin_amdgcn_readfirstlane(bad[p]);
-    }
+    for (int p = 0; p < 4; ++p) nan_tokens[p] = __builtin_amdgcn_readfirstlane(bad[p]);
+    hide<4, RT>(s, nan_tokens, id, e, seen, least, g);
+    raise<D, 4, RT>(s, mult, m, l, acc);
     h8 pb[RT][2], pl[RT][QF32 ? 2 : 1];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      soften<D, 4, false>(s[t], nan_tokens, id, e, seen[t], least[t], mult[t], g, m[t], l[t], acc[t]);
+      soften<4>(s[t], mult[t], m[t]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         pb[t][h] = weights(s[t][2 * h], s[t][2 * h + 1]);
