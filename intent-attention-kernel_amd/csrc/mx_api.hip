@@ -67,54 +67,54 @@ struct MxPlan {
 };
 
 // Which kernel, and into how many splits a row's tokens go: the least of costs in microseconds
-// fitted to measurements (40 shapes of 8 to 65,536 query rows by 16 to 2,048 table entries).
-// A CU holds two to four workgroups at a time. A round of as many takes START and its entries'
-// time, one of fewer runs faster; a second kernel merges splits at MERGE and the time of the
-// partials' bytes.
-//   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 190 us, 4 228,
-//     6 195, 8 203; 512 x 125: 1 split 31, 2 42, 4 44; 64 x 128: 1 split 18, 4 14.6, 8 13.8, 16 17
-//   2,048 queries x 4 heads x 8 KV heads over 8,192 tokens: rows kernel 475, chunk kernel 293;
-//     512 x 4 x 8: rows 140, chunk 96 (4 splits); 16 x 4 x 64 over 4,000: rows 30, chunk 40
-constexpr int CHUNK_ROWS = 128;
+// fitted to measurements (60 shapes of 8 to 131,072 query rows by 16 to 2,048 table entries).
+// A CU holds one to four workgroups at a time. A round of as many takes START and its entries'
+// time, one of fewer runs faster; where sequences differ, rounds before the last are not full. A
+// second kernel merges splits at MERGE and the time of the partials' bytes.
+//   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 182 us, 4 228,
+//     6 195, 8 203; 512 x 125: 1 split 25, 2 29, 4 31; 64 x 128: 1 split 18, 4 14.6, 8 13.8, 16 17
+//   rows kernel | chunk kernel, tiles of 128 rows | of 256, in us (best splits), head_dim 128:
+//     1 x 2,048 queries x 32 heads x 8 KV heads over 8,192 tokens: 412 | 266 (1) | 261 (1)
+//     1 x 512 x 32 x 8 over 8,192: 126 (2) | 92 (4) | 85 (4);  8 x 16 x 32 x 8 over 4,000: 24 | 35 (8)
+//     16 x 512 x 32 x 8 over 512: 168 | 80 (1) | 91 (1);  2 x 4,096 x 16 x 2 over 4,096: 272 | 169 | 155
+//     8 x 300 x 8 x 2 over 1,000: 26 | 33 (1) | 36 (3)
 constexpr double CUS = 256;         // and up to as many unsplit tiles are workgroups of more waves
 
-struct MxChoice { bool chunk; int64_t splits; };
+struct MxChoice { int chunk_rows; int64_t splits; };             // chunk_rows 0: the rows kernel
 
-MxChoice choose(double kvrows, int64_t rows, int W, int D, bool f32, int64_t forced) {
-  const double START = 3, MERGE = 6;
+MxChoice choose(int B, int Hkv, int64_t rows, int W, int D, bool f32, int64_t forced) {
   const bool big = D == 128;
-  const double per_head = (double)((rows + 15) / 16);            // tiles of 16 rows that read the same pages
-  const double tiles = kvrows * per_head, blocks = kvrows * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS);
-  const double bytes_entry = (big ? 0.30 : 0.20) / per_head;     // an entry's bytes, the card full
-  double rows_entry = big ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
-  if (rows_entry < bytes_entry) rows_entry = bytes_entry;
-  const double chunk_entry = big ? (f32 ? 0.92 : 0.57) : (f32 ? 0.60 : 0.48);
-  const int rows_places = big ? 3 : 4, chunk_places = big || f32 ? 2 : 3;   // workgroups a CU
+  const double MERGE = 6, kvrows = (double)B * Hkv;
   const int64_t most = (W + 15) / 16;
-  MxChoice best = {false, 1};
+  MxChoice best = {0, 1};
   double least = -1;
-  auto consider = [&](bool chunk, int64_t s) {
-    if (s > most) s = most;
-    if (s < 1) s = 1;
-    if (forced > 0) s = forced;
-    const bool many = !chunk && s == 1 && tiles <= CUS;
-    const double each = std::ceil((chunk ? blocks : tiles) * s / CUS);      // workgroups of the busiest CU
-    const int places = chunk ? chunk_places : many ? 1 : rows_places;
-    const double full = std::floor(each / places), rest = each - full * places;
-    const double entry = (chunk ? chunk_entry : rows_entry) / (many ? (big ? 3 : 5) : 1);
-    double cost = (full + (rest > 0 ? 0.42 + 0.58 * rest / places : 0)) * (START + entry * W / s);
-    if (s > 1) cost += MERGE + kvrows * rows * s * D * 8 / 4.0e6;
-    if (least < 0 || cost < least) { least = cost; best = {chunk, s}; }
+  // tiles of `chunk` rows (0: the rows kernel's 16), of which a CU holds `places`
+  auto each_split = [&](int chunk, int places, double start, double entry, double fill) {
+    const double work = kvrows * (double)((rows + (chunk ? chunk : 16) - 1) / (chunk ? chunk : 16));
+    auto consider = [&](int64_t s) {
+      if (s > most) s = most;
+      if (s < 1) s = 1;
+      if (forced > 0) s = forced;
+      const bool many = chunk == 0 && s == 1 && work <= CUS;     // one workgroup of more waves a CU
+      const int room = many ? 1 : places;
+      const double each = std::ceil(work * s / CUS);             // workgroups of the busiest CU
+      const double before = std::ceil(each / room) - 1, last = each - before * room;
+      double cost = (before * fill + (last == room ? 1 : 0.42 + 0.58 * last / room)) *
+                    (start + entry / (many ? (big ? 3 : 5) : 1) * W / s);
+      if (s > 1) cost += MERGE + kvrows * rows * ((double)s * D * 8 / 5.5e6 + (s > 8 ? 1e-3 : 0));   // past 8: a workgroup a row
+      if (least < 0 || cost < least) { least = cost; best = {chunk, s}; }
+    };
+    consider(1);
+    if (work >= 4 * CUS * places || most <= 1 || forced > 0) return;
+    for (int64_t s = 2; s < most && s < 256; s *= 2) consider(s);
+    for (int rounds = 1; rounds <= 4; ++rounds) consider((int64_t)(rounds * CUS * places / work));
   };
-  auto each_split = [&](bool chunk) {
-    const double work = chunk ? blocks : tiles, places = CUS * (chunk ? chunk_places : rows_places);
-    consider(chunk, 1);
-    if (work >= 4 * places || most <= 1 || forced > 0) return;
-    for (int64_t s = 2; s < most && s < 256; s *= 2) consider(chunk, s);
-    for (int rounds = 1; rounds <= 4; ++rounds) consider(chunk, (int64_t)(rounds * places / work));
-  };
-  each_split(false);
-  if (rows > 16) each_split(true);
+  const double bytes_entry = (big ? 0.30 : 0.20) / (double)((rows + 15) / 16);   // an entry's bytes, shared by its tiles
+  const double rows_entry = big ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
+  const double fill = B > 1 ? 0.75 : 1;
+  each_split(0, big ? 3 : 4, 3, rows_entry < bytes_entry ? bytes_entry : rows_entry, 1);
+  if (rows > 16) each_split(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50), fill);
+  if (rows > 128) each_split(256, 1, big ? 7 : 5, big ? (f32 ? 0.88 : 0.50) : (f32 ? 0.57 : 0.345), fill);
   return best;
 }
 
@@ -145,9 +145,10 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
   if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
   const int W = a->table_width > 0 ? a->table_width : 1;
-  MxChoice best = choose((double)a->batch * a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
-  p->chunk_rows = best.chunk ? CHUNK_ROWS : 0;
-  const double blocks = best.chunk ? (double)a->batch * a->num_kv_heads * ((rows + CHUNK_ROWS - 1) / CHUNK_ROWS) : tiles;
+  MxChoice best = choose(a->batch, a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
+  p->chunk_rows = best.chunk_rows;
+  const double blocks =
+      best.chunk_rows ? (double)a->batch * a->num_kv_heads * ((rows + best.chunk_rows - 1) / best.chunk_rows) : tiles;
   int64_t splits = best.splits;
   if (splits > (W + 1) / 2) splits = (W + 1) / 2;
   while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;

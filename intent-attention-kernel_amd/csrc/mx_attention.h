@@ -1,6 +1,6 @@
-// Arguments of the 4-bit cache's attention kernels, and what each of them works out of the
-// lengths on the device: how many tokens a query row sees, and how many table entries a tile
-// of rows has to walk.
+// What the 4-bit cache's attention kernels share: how many tokens a query row sees and how
+// many table entries a tile of rows has to walk, out of the lengths on the device; a row's
+// query operand; the parts of the softmax; V's way through LDS.
 #ifndef IAK_MX_ATTENTION_H
 #define IAK_MX_ATTENTION_H
 
@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "iak_device.h"
+#include "mx_format.h"
 #include "mx_internal.h"
 
 namespace iak {
@@ -44,6 +45,22 @@ __device__ __forceinline__ int mx_entries(const MxAttn& a, const MxRows& n, int 
   return (mx_seen(a, n, last / a.G) + 15) / 16;
 }
 
+// Which KV row, tile of rows and split a workgroup takes. The KV rows turn fastest, so that the
+// workgroups that read the same pages meet in one XCD's L2 where the number of KV rows is a
+// multiple of 8, and every XCD has its share of each split and tile where lengths differ; those
+// that see most start first. (With the splits fastest, 4 x 1,024 queries over 1,024 tokens took
+// 85 us and take 58; 5 ragged sequences of 509 queries over 4,000 took 74 and take 59.)
+struct MxPart { uint32_t kvrow; int tile, split; };
+
+__device__ __forceinline__ MxPart mx_part(const MxAttn& a, int tiles) {
+  const uint32_t kvrows = (uint32_t)a.B * a.Hkv, rest = blockIdx.x / kvrows;
+  MxPart p;
+  p.kvrow = blockIdx.x - rest * kvrows;
+  p.split = (int)(rest / tiles);
+  p.tile = tiles - 1 - (int)(rest - (uint32_t)p.split * tiles);
+  return p;
+}
+
 // N query values at element offset `at`, wherever they lie: 16-byte loads, all under way at once.
 template <typename T, int N> __device__ __forceinline__ void mx_load(const T* p, float (&x)[N]) {
   T t[N];
@@ -55,6 +72,167 @@ template <int N> __device__ __forceinline__ void mx_load_q(const MxAttn& a, int6
   if (a.q_dtype == IAK_DTYPE_F32) mx_load(reinterpret_cast<const float*>(a.q) + at, x);
   else if (a.q_dtype == IAK_DTYPE_F16) mx_load(reinterpret_cast<const _Float16*>(a.q) + at, x);
   else mx_load(reinterpret_cast<const __bf16*>(a.q) + at, x);
+}
+
+constexpr float P_SHIFT = 6.0f;          // weights <= 2^(6 + RESCALE_SLACK) = 2^14
+constexpr float M_NONE = -3.402823466e38f;
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+// 16-byte chunk of V row `t` (of a page) that holds logical chunk `ch`: rows are 2 D bytes, and
+// the exclusive or lets both the row-wise writes (one chunk of 16 rows, four chunks apart) and
+// the transposed reads (two chunks of 16 rows) touch every LDS bank equally.
+template <int D> __device__ __forceinline__ int v_chunk(int t, int ch) {
+  if constexpr (D == 128) return t * 16 + (ch ^ (((t & 7) << 1) | (t >> 3)));
+  else return t * 8 + (ch ^ ((((t >> 1) & 3) << 1) | (t >> 3)));
+}
+
+// A lane's scale bytes come as the aligned four they are among: a byte loaded alone is zero-
+// extended where the loop turns, and that waits for loads that the next round is meant to await.
+template <int D> __device__ __forceinline__ uint32_t scale_word(const uint8_t* page_scales, int c, int g) {
+  return reinterpret_cast<const uint32_t*>(page_scales)[(c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK) >> 2];
+}
+template <int D> __device__ __forceinline__ uint32_t own_scale(uint32_t word, int c, int g) {
+  return __builtin_amdgcn_ubfe(word, 8 * ((c * (D / MX_BLOCK) + g * (D / 4) / MX_BLOCK) & 3), 8);
+}
+
+template <typename T> __device__ __forceinline__ void out4(T* p, const float (&x)[4]) {
+  T t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = (T)x[j];
+  __builtin_memcpy(p, t, sizeof(t));                             // one store, wherever the row lies
+}
+__device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const float (&x)[4]) {
+  if (a.out_dtype == IAK_DTYPE_F32) out4(reinterpret_cast<float*>(a.out) + at, x);
+  else if (a.out_dtype == IAK_DTYPE_F16) out4(reinterpret_cast<_Float16*>(a.out) + at, x);
+  else out4(reinterpret_cast<__bf16*>(a.out) + at, x);
+}
+
+// A query row's operand: the lane's channels (D/4) g .., scaled by a power of two to a largest
+// element of the row in [2^14, 2^15), split in two for float32. Returns the factor that makes
+// base-2 scores of the products: positive, NaN for a row that is not finite. (A negative scale
+// turns the query's sign; where the factor would vanish the scores do: query 0, factor 1.)
+template <int D, bool QF32>
+__device__ __forceinline__ float load_query(const MxAttn& a, bool there, int64_t at, int g, h8 (&qhi)[D / 32],
+                                            h8 (&qlo)[QF32 ? D / 32 : 1]) {
+  float x[D / 4];
+#pragma unroll
+  for (int j = 0; j < D / 4; ++j) x[j] = 0.f;
+  if (there) mx_load_q(a, at + g * (D / 4), x);
+  float m = 0.f, nan = 0.f;                                      // nan: NaN if any value is infinite or NaN, else 0
+#pragma unroll
+  for (int j = 0; j < D / 4; ++j) {
+    m = fmaxf(m, fabsf(x[j]));
+    nan = __builtin_fmaf(x[j], 0.f, nan);
+  }
+  bool fine = nan == 0.f;
+  m = xmax16_32(fine ? m : __builtin_inff());
+  fine = m < __builtin_inff();
+  const int e = m > 0.f ? (int)(f2u(m) >> 23) - 127 : 0;
+  const float mult = __builtin_ldexpf(fabsf(a.score_mult), e - 14);
+  const bool none = !fine || mult < 1e-30f;
+  const float sign = a.score_mult < 0.f ? -1.f : 1.f;
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = none ? 0.f : sign * __builtin_ldexpf(x[8 * s + j], 14 - e);
+      qhi[s][j] = (_Float16)v;
+      if constexpr (QF32) qlo[s][j] = (_Float16)(v - (float)qhi[s][j]);
+    }
+  return !fine ? __builtin_nanf("") : none ? 1.f : mult;
+}
+
+// The softmax of PAGES pages' score results (lane: row c of T tiles, tokens 4g .. 4g+3 of each
+// page), in three parts, each of which leaves the straight line at one rarely taken branch:
+//   hide    scores become NaN where a token has a NaN block (bit per token in `nan`) and -inf
+//           where the row does not see it; `e`: the first page's entry, `least`: tokens that
+//           every row of the wave sees
+//   raise   moves a row's running maximum m, with its sum l and accumulator, where a score
+//           exceeds it by more than the slack: the lanes of a row compare theirs only then
+//   soften  scores become the weights exp2(s * mult - m + P_SHIFT)
+template <int PAGES, int T>
+__device__ __forceinline__ void hide(f4 (&s)[T][PAGES], const uint32_t (&nan)[PAGES], const int (&id)[PAGES], int e,
+                                     const int (&seen)[T], int least, int g) {
+  uint32_t any_nan = 0u;
+  int ids = 0;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p) { any_nan |= nan[p]; ids |= id[p]; }
+  if (any_nan != 0u || ids < 0 || (e + PAGES) * PS > least) {
+    asm volatile("");                                            // a branch, not selects for every call
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p) {
+        const int lim = id[p] < 0 ? 0 : seen[t] - (e + p) * PS;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if ((nan[p] >> (4 * g + q)) & 1u) s[t][p][q] = __builtin_nanf("");
+          if (4 * g + q >= lim) s[t][p][q] = -__builtin_inff();
+        }
+      }
+  }
+}
+
+template <int D, int PAGES, int T>
+__device__ __forceinline__ void raise(const f4 (&s)[T][PAGES], const float (&mult)[T], float (&m)[T], f4 (&l)[T],
+                                      f4 (&acc)[T][D / 16]) {
+  float top[T];
+  bool over = false;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    top[t] = fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3]));
+#pragma unroll
+    for (int p = 1; p < PAGES; ++p)
+      top[t] = fmaxf(top[t], fmaxf(fmaxf(s[t][p][0], s[t][p][1]), fmaxf(s[t][p][2], s[t][p][3])));
+    over = over || top[t] * mult[t] > m[t] + RESCALE_SLACK;
+  }
+  if (__builtin_amdgcn_ballot_w64(over)) {
+    asm volatile("");
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float pm = xmax16_32(top[t]) * mult[t];
+      const float mn = pm > m[t] + RESCALE_SLACK ? pm : m[t];
+      const float alpha = __builtin_amdgcn_exp2f(m[t] - mn);
+      l[t] *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] *= alpha;
+      m[t] = mn;
+    }
+  }
+}
+
+template <int PAGES> __device__ __forceinline__ void soften(f4 (&s)[PAGES], float mult, float m) {
+  const float base = P_SHIFT - m;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s[p][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p][q], mult, base));
+}
+
+// Weights of two pages as the value product's operand, and what rounding left (float32 queries).
+__device__ __forceinline__ h8 weights(const f4 a, const f4 b) {
+  return h8{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3],
+            (_Float16)b[0], (_Float16)b[1], (_Float16)b[2], (_Float16)b[3]};
+}
+__device__ __forceinline__ h8 weights_rest(const f4 a, const f4 b, const h8 w) {
+  h8 r;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    r[q] = (_Float16)(a[q] - (float)w[q]);
+    r[4 + q] = (_Float16)(b[q] - (float)w[4 + q]);
+  }
+  return r;
+}
+
+// The value product's operand from two pages' V rows in LDS: channel 16 mb + c of tokens
+// 4g .. 4g+3 of both.
+template <int D> __device__ __forceinline__ h8 values_back(const u4* page0, const u4* page1, int mb, int c, int g) {
+  typedef __attribute__((address_space(3))) s4v lds_s4;
+  const int at = v_chunk<D>(4 * g + (c >> 2), 2 * mb + ((c & 3) >> 1)) * 16 + (c & 1) * 8;
+  const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(reinterpret_cast<const char*>(page0) + at));
+  const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(reinterpret_cast<const char*>(page1) + at));
+  return __builtin_bit_cast(h8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 }  // namespace iak

@@ -21,7 +21,7 @@ struct MxAttn {
   int splits;     // parts of `chunk` table entries per tile
   int chunk;
   int waves;      // 4 per workgroup, or more (16): as many as the kernel has
-  int chunk_rows; // 64 or 128: the chunk kernel with tiles of that many rows; 0: the rows kernel
+  int chunk_rows; // 128 or 256: the chunk kernel with tiles of that many rows; 0: the rows kernel
   int64_t items;  // workgroups: B * Hkv * splits * tiles (of 16 or of chunk_rows rows)
 
   const void* q; int q_dtype; int64_t qsb, qst, qsh;
@@ -41,6 +41,7 @@ struct MxAttn {
 hipError_t launch_mx_append(const iak_mx_tokens_args& a, hipStream_t stream);
 hipError_t launch_mx_read(const iak_mx_tokens_args& a, hipStream_t stream);
 hipError_t launch_mx_attention(const MxAttn& a, hipStream_t stream);
+void launch_mx_chunk(const MxAttn& a, hipStream_t stream);
 
 hipError_t launch_copy_pages(const iak_copy_pages_args& a, hipStream_t stream);
 size_t sequences_workspace(const iak_sequences_args& a);
