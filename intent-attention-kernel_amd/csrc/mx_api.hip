@@ -78,6 +78,7 @@ struct MxPlan {
 //     1 x 512 x 32 x 8 over 8,192: 126 (2) | 92 (4) | 85 (4);  8 x 16 x 32 x 8 over 4,000: 24 | 35 (8)
 //     16 x 512 x 32 x 8 over 512: 168 | 80 (1) | 91 (1);  2 x 4,096 x 16 x 2 over 4,096: 272 | 169 | 155
 //     8 x 300 x 8 x 2 over 1,000: 26 | 33 (1) | 36 (3)
+//     the first with float32 queries: 537 | 443 (1) | 453 (1)
 constexpr double CUS = 256;         // and up to as many unsplit tiles are workgroups of more waves
 
 struct MxChoice { int chunk_rows; int64_t splits; };             // chunk_rows 0: the rows kernel
@@ -114,7 +115,7 @@ MxChoice choose(int B, int Hkv, int64_t rows, int W, int D, bool f32, int64_t fo
   const double fill = B > 1 ? 0.75 : 1;
   each_split(0, big ? 3 : 4, 3, rows_entry < bytes_entry ? bytes_entry : rows_entry, 1);
   if (rows > 16) each_split(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50), fill);
-  if (rows > 128) each_split(256, 1, big ? 7 : 5, big ? (f32 ? 0.88 : 0.50) : (f32 ? 0.57 : 0.345), fill);
+  if (rows > 128 && !f32) each_split(256, 1, big ? 7 : 5, big ? 0.50 : 0.345, fill);
   return best;
 }
 

@@ -2,7 +2,7 @@
 // for gfx950. The mathematics, the lanes' parts and the softmax are the rows kernel's
 // (mx_attention.hip); what differs is who reads the cache.
 //
-// A workgroup takes 32 rows a wave: 256 rows in eight waves, or 128 in four. All walk the same
+// A workgroup takes 32 rows a wave: 256 rows in eight waves (16-bit queries), or 128 in four. All walk the same
 // tokens, 64 (four pages) a step. Each wave converts its share of the next step's pages (one
 // page of K or of V in eight waves, of both in four) into LDS, from where all read them: two
 // buffers, one barrier a step. The sum of the weights is a product with ones on the matrix cores.
@@ -224,8 +224,10 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
 
 template <int D, bool QF32> void launch_chunk(const MxAttn& a, hipStream_t stream) {
   const dim3 grid((uint32_t)a.items);
-  if (a.chunk_rows == 256) hipLaunchKernelGGL((mx_chunk_kernel<D, QF32, 8>), grid, dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((mx_chunk_kernel<D, QF32, 4>), grid, dim3(256), 0, stream, a);
+  if constexpr (!QF32) {
+    if (a.chunk_rows == 256) { hipLaunchKernelGGL((mx_chunk_kernel<D, false, 8>), grid, dim3(512), 0, stream, a); return; }
+  }
+  hipLaunchKernelGGL((mx_chunk_kernel<D, QF32, 4>), grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace

@@ -21,7 +21,7 @@ struct MxAttn {
   int splits;     // parts of `chunk` table entries per tile
   int chunk;
   int waves;      // 4 per workgroup, or more (16): as many as the kernel has
-  int chunk_rows; // 128 or 256: the chunk kernel with tiles of that many rows; 0: the rows kernel
+  int chunk_rows; // 128 or 256 (16-bit queries): the chunk kernel with tiles of that many rows; 0: the rows kernel
   int64_t items;  // workgroups: B * Hkv * splits * tiles (of 16 or of chunk_rows rows)
 
   const void* q; int q_dtype; int64_t qsb, qst, qsh;

@@ -57,10 +57,10 @@ def row_values(codes, scales, row, tokens, num_pages):
     return out, there
 
 
-def attention(q, pools, table, valid, q_lens=None, causal=True, sm_scale=None):
+def attention(q, pools, table, valid, q_lens=None, causal=True, sm_scale=None, queries=None):
     """(out, sum of p |v|, score bound) in float64: q [B, L, Hq, D]; the second and third are
     what error bounds are made of: per output the weighted sum of |v|, per query the largest
-    sm_scale * sum |q| |k|."""
+    sm_scale * sum |q| |k|. `queries`: the query tokens to work out, all if None."""
     B, L, Hq, D = q.shape
     Hkv, W = table.shape[1:]
     G, NP = Hq // Hkv, pools["k_codes"].shape[0]
@@ -74,7 +74,7 @@ def attention(q, pools, table, valid, q_lens=None, causal=True, sm_scale=None):
             v, _ = row_values(pools["v_codes"], pools["v_scales"], table[b, h], T, NP)
             nan = there & (np.isnan(k).any(-1) | np.isnan(v).any(-1))
             k, v = np.nan_to_num(k, nan=0.0), np.nan_to_num(v, nan=0.0)
-            for i in range(n):
+            for i in range(n) if queries is None else [i for i in queries if i < n]:
                 seen = there & (np.arange(T) < (T - n + i + 1 if causal else T))
                 for x in range(h * G, (h + 1) * G):
                     if not seen.any():

@@ -48,7 +48,7 @@ def _bound(mass, reach, out, T, D, q_dtype, out_dtype, vmax):
     return rel * mass + T * 2.0 ** -31 * vmax + HALF[out_dtype] * np.abs(out) + 2.0 ** -25
 
 
-def _check(q, dtype, host, pools, table, valid, q_lens=None, causal=True, out_dtype=None, got=None, **kw):
+def _check(q, dtype, host, pools, table, valid, q_lens=None, causal=True, out_dtype=None, got=None, queries=None, **kw):
     import torch
     import intent_attention as ia
     tq = q if isinstance(q, torch.Tensor) else _t(q).to(getattr(torch, dtype))
@@ -57,12 +57,16 @@ def _check(q, dtype, host, pools, table, valid, q_lens=None, causal=True, out_dt
         got = ia.mxfp4_paged_attention(tq, pools, _t(table), _t(valid), q_lens=None if q_lens is None else _t(q_lens),
                                        causal=causal, out_dtype=None if out_dtype is None else getattr(torch, out_dtype), **kw)
     h4 = hq[:, None] if hq.ndim == 3 else hq
-    want, mass, reach = O.attention(h4, host, table, valid, q_lens, causal, kw.get("sm_scale"))
+    want, mass, reach = O.attention(h4, host, table, valid, q_lens, causal, kw.get("sm_scale"), queries)
     g = got.double().cpu().numpy().reshape(want.shape)
     assert got.shape == tq.shape and got.dtype == getattr(torch, out_dtype or dtype)
+    if queries is not None:
+        want, mass, reach, g = want[:, queries], mass[:, queries], reach[:, queries], g[:, queries]
     assert np.array_equal(np.isnan(g), np.isnan(want)), "NaN in other places"
     T = int(max(1, np.clip(valid, 0, table.shape[2] * 16).max())) if valid.size else 1
-    vmax = 6 * 2.0 ** min(13, int(host["v_scales"][host["v_scales"] < 255].astype(int).max()) - 127) if host["v_scales"].size else 0
+    values = [O.row_values(host["v_codes"], host["v_scales"], table[b, h], int(np.clip(valid[b, h], 0, table.shape[2] * 16)),
+                           host["v_codes"].shape[0])[0] for b, h in np.ndindex(*valid.shape)]
+    vmax = max((float(np.nan_to_num(np.abs(x), nan=0.0).max()) for x in values if x.size), default=0.0)
     tol = _bound(mass, reach, np.nan_to_num(want), T, h4.shape[-1], dtype, out_dtype or dtype, vmax)
     worst = float((np.abs(np.nan_to_num(g) - np.nan_to_num(want)) / tol).max()) if g.size else 0.0
     assert worst <= 1.0
@@ -328,6 +332,95 @@ def test_attention_query_values(L, dtype):
         q[:, :, 6] *= 2.0 ** -100
     tq = torch.from_numpy(q).to(getattr(torch, dtype)).to(_dev())
     _check(tq, dtype, host, pools, table, valid)
+
+
+# Sizes that the kernel for many query rows takes, in each of its forms: tiles of 128 rows and, for
+# 16-bit queries, of 256; the whole row or splits of it.
+PROMPTS = [
+    # B, L, Hq, Hkv, D, W, dtype, causal, splits
+    (1, 203, 4, 2, 64, 13, "float16", True, 16),
+    (2, 140, 8, 2, 128, 14, "bfloat16", True, 16),
+    (2, 140, 4, 1, 128, 15, "float32", False, 16),
+    (2, 140, 8, 2, 64, 10, "float32", True, 16),
+    (1, 2050, 16, 2, 64, 20, "bfloat16", False, 0),
+    (1, 2050, 16, 2, 128, 20, "float16", False, 0),
+    (1, 2050, 16, 2, 64, 20, "float32", False, 0),
+    (1, 1500, 12, 3, 128, 10, "float32", False, 1),
+    (2, 1100, 16, 2, 64, 70, "float16", True, 0),
+    (2, 1100, 16, 2, 128, 70, "bfloat16", True, 0),
+    (1, 1500, 4, 1, 64, 200, "bfloat16", True, 6),
+    (1, 1500, 4, 1, 128, 300, "float16", True, 6),
+]
+
+
+@pytest.mark.parametrize("B,L,Hq,Hkv,D,W,dtype,causal,splits", PROMPTS)
+def test_attention_of_prompts(B, L, Hq, Hkv, D, W, dtype, causal, splits):
+    """Prompts with all that may be in them at once: ragged lengths, pages that are none, NaN
+    blocks seen by some queries and by none, any bytes past the last token, queries of all sizes and
+    infinite ones, q and out as parts of wider tensors."""
+    import torch
+    import intent_attention as ia
+    rng = np.random.default_rng(L + D + W)
+    NP, T = B * Hkv * W + 7, W * 16
+    host, _ = _pools(rng, NP, D)
+    table = _table(rng, B, Hkv, W, NP)
+    valid = np.full((B, Hkv), T - 5, np.int32)
+    valid[-1, -1] = T - 42
+    for n in ("k_scales", "v_scales"):
+        for b in range(B):
+            for h in range(Hkv):
+                for t in range(valid[b, h], T):
+                    host[n][table[b, h, t // 16], t % 16] = rng.choice([0, 255, 254, 141, 103])
+    host["k_scales"][table[0, 0, (T - 9) // 16], (T - 9) % 16, 1] = 255       # seen by the last of causal queries
+    host["v_scales"][table[-1, -1, (T - 45) // 16], (T - 45) % 16, 0] = 255
+    table[0, -1, [1, W // 2, W - 1]] = [-1, NP, 2 ** 31 - 1]
+    pools = ia.MxFp4Pools(**{n: _t(x) for n, x in host.items()})
+    q = (2 * rng.standard_normal((B, L, Hq, D))).astype(np.float32)
+    q[:, L // 2] *= 2.0 ** -12
+    q[:, L // 2 + 1, :, 1:] = 0
+    q[:, L // 2 + 1] *= 2.0 ** 10
+    q[0, L - 2, 0, 3], q[-1, 1, -1, 0] = np.inf, np.nan
+    wide = torch.full((B, Hq, L, D + 3), 3.0, device=_dev()).to(getattr(torch, dtype))
+    wide[..., 2:D + 2] = _t(q).transpose(1, 2).to(wide.dtype)
+    tq = wide[..., 2:D + 2].transpose(1, 2)
+    buf = torch.full((B, L, Hq, D + 5), 7.0, device=_dev()).to(getattr(torch, dtype))
+    lens = np.array([L, max(0, L - 77)][:B], np.int32)
+    ia.mxfp4_paged_attention(tq, pools, _t(table), _t(valid), q_lens=_t(lens), causal=causal, out=buf[..., 1:D + 1],
+                             splits=splits)
+    queries = sorted({0, 1, 7, L // 3, L // 2, L // 2 + 1, L - 79, L - 78, L - 77, L - 5, L - 4, L - 3, L - 2, L - 1}
+                     | {int(i) for i in rng.integers(0, L, 20)})
+    got = _check(tq, dtype, host, pools, table, valid, lens, causal, got=buf[..., 1:D + 1], queries=queries)
+    assert (buf[..., 0] == 7).all() and (buf[..., D + 1:] == 7).all()
+    assert (got[-1, lens[-1]:] == 0).all()
+
+
+def test_attention_of_prompts_replays():
+    """A captured prompt, replayed with other data and lengths between eager work: the eager results, bit for bit."""
+    import torch
+    import intent_attention as ia
+    rng = np.random.default_rng(12)
+    for B, L, Hq, Hkv, D, W, splits in ((2, 140, 8, 2, 128, 14, 16), (2, 1100, 16, 2, 64, 70, 0)):
+        _, pools = _pools(rng, B * Hkv * W, D)
+        table, valid = _t(_table(rng, B, Hkv, W, B * Hkv * W)), _t(np.full((B, Hkv), W * 16, np.int32))
+        q = torch.randn((B, L, Hq, D), device=_dev()).half()
+        plan = ia.make_mxfp4_plan(q, pools, table, valid, splits=splits)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            plan.run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.run()
+        for it in range(4):
+            q.copy_(torch.randn_like(q))
+            valid.fill_(W * 16 - 31 * it)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = plan.out.clone()
+            want = ia.mxfp4_paged_attention(q, pools, table, valid, splits=splits)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), it
 
 
 def test_attention_sharp_and_growing_scores():
