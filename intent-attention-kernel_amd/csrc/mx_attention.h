@@ -109,9 +109,10 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
 }
 
 // A query row's operand: the lane's channels (D/4) g .., scaled by a power of two to a largest
-// element of the row in [2^14, 2^15), split in two for float32. Returns the factor that makes
-// base-2 scores of the products: positive, NaN for a row that is not finite. (A negative scale
-// turns the query's sign; where the factor would vanish the scores do: query 0, factor 1.)
+// element of the row in [2^14, 2^15), split in two for float32. Returns the positive factor that
+// makes base-2 scores of the products. (A negative scale turns the query's sign; where the factor
+// would vanish the scores do: query 0, factor 1. A row that is not finite is NaN, factor 1: NaN
+// scores for the tokens that it sees, and none if it sees none.)
 template <int D, bool QF32>
 __device__ __forceinline__ float load_query(const MxAttn& a, bool there, int64_t at, int g, h8 (&qhi)[D / 32],
                                             h8 (&qlo)[QF32 ? D / 32 : 1]) {
@@ -136,11 +137,11 @@ __device__ __forceinline__ float load_query(const MxAttn& a, bool there, int64_t
   for (int s = 0; s < D / 32; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = none ? 0.f : sign * __builtin_ldexpf(x[8 * s + j], 14 - e);
+      const float v = !fine ? __builtin_nanf("") : none ? 0.f : sign * __builtin_ldexpf(x[8 * s + j], 14 - e);
       qhi[s][j] = (_Float16)v;
       if constexpr (QF32) qlo[s][j] = (_Float16)(v - (float)qhi[s][j]);
     }
-  return !fine ? __builtin_nanf("") : none ? 1.f : mult;
+  return none ? 1.f : mult;
 }
 
 // The softmax of PAGES pages' score results (lane: row c of T tiles, tokens 4g .. 4g+3 of each

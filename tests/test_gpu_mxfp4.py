@@ -334,6 +334,22 @@ def test_attention_query_values(L, dtype):
     _check(tq, dtype, host, pools, table, valid)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_attention_of_queries_that_are_not_finite_and_see_nothing(dtype):
+    """Infinite and NaN queries: zeros where a query sees no token, among queries that see some."""
+    rng = np.random.default_rng(5)
+    B, L, Hq, Hkv, D, W, NP = 2, 6, 4, 1, 64, 14, 40
+    host, pools = _pools(rng, NP, D)
+    table = _table(rng, B, Hkv, W, NP)
+    table[1, 0, 0] = -1
+    valid = np.array([[3], [19]], np.int32)           # the first three queries before the row's start; on no page
+    q = rng.standard_normal((B, L, Hq, D)).astype(np.float32)
+    q[:, 1, 0, 3], q[:, 2, 1, 0], q[:, 4, 2, 5] = np.nan, np.inf, np.nan
+    for splits in (1, 3):
+        got = _check(q, dtype, host, pools, table, valid, splits=splits)
+        assert (got[0, :3] == 0).all() and bool(got[0, 4, 2].isnan().all())
+
+
 # Sizes that the kernel for many query rows takes, in each of its forms: tiles of 128 rows and, for
 # 16-bit queries, of 256; the whole row or splits of it.
 PROMPTS = [
