@@ -36,7 +36,7 @@ iak_status validate_mx_cache(int batch, int count, int kv_heads, int head_dim, i
   if (head_dim != 64 && head_dim != 128) return fail(IAK_ENOTSUP, "head_dim %d is not supported (64 or 128)", head_dim);
   if (page_size != 16) return fail(IAK_ENOTSUP, "page_size %d is not supported (16)", page_size);
   if (num_pages > 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)num_pages);
-  if (width > 0x7FFFFFF) return fail(IAK_EINVAL, "table_width %d: a row's tokens exceed int32", width);
+  if (width > 0x7FFFFF0) return fail(IAK_EINVAL, "table_width %d: a row's tokens exceed int32", width);
   return IAK_OK;
 }
 
@@ -59,6 +59,8 @@ iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
     return fail(IAK_EINVAL, "code pools must be 4-byte aligned");
   return IAK_OK;
 }
+
+constexpr float LOG2_E = 1.44269504088896340736f;
 
 struct MxPlan {
   int G, tiles, splits, chunk, waves, chunk_rows;
@@ -127,7 +129,7 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
     return fail(IAK_EINVAL, "num_q_heads %d is not a multiple of num_kv_heads %d", a->num_q_heads, a->num_kv_heads);
   if (a->q_dtype < 0 || a->q_dtype > 2 || a->out_dtype < 0 || a->out_dtype > 2)
     return fail(IAK_EINVAL, "bad q/out dtype (%d, %d)", a->q_dtype, a->out_dtype);
-  if (!std::isfinite(a->sm_scale)) return fail(IAK_EINVAL, "sm_scale is not finite");
+  if (!std::isfinite(a->sm_scale * LOG2_E)) return fail(IAK_EINVAL, "sm_scale is not finite, in base 2 too");
   if (a->causal != 0 && a->causal != 1) return fail(IAK_EINVAL, "causal must be 0 or 1, got %d", a->causal);
   if (a->splits < 0) return fail(IAK_EINVAL, "splits %d is negative", a->splits);
   *p = MxPlan{};
@@ -214,6 +216,14 @@ iak_status validate_compact(const iak_compact_pages_args* a) {
   if (a->num_pages > 0 && (!a->refs || !a->out_refs || !a->page_map)) return fail(IAK_EINVAL, "refs, out_refs or page_map is NULL");
   if ((int64_t)a->num_rows * a->table_width > 0 && (!a->page_table || !a->out_table || !a->valid_tokens))
     return fail(IAK_EINVAL, "page_table, out_table or valid_tokens is NULL");
+  const void* in[3] = {a->page_table, a->valid_tokens, a->refs};
+  const void* out[3] = {a->out_table, a->out_refs, a->page_map};
+  for (int k = 0; k < 3; ++k) {
+    if (!aligned4(in[k]) || !aligned4(out[k])) return fail(IAK_EINVAL, "int32 arrays must be 4-byte aligned");
+    for (int j = 0; j < 3; ++j)
+      if (out[k] && (out[k] == in[j] || (j != k && out[k] == out[j])))
+        return fail(IAK_EINVAL, "an output of a compaction is another of its arrays");
+  }
   return validate_arrays(a->num_arrays, a->arrays, a->num_pages);
 }
 
@@ -260,7 +270,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   k.table = a->page_table; k.valid = a->valid_tokens; k.q_lens = a->q_lens;
   k.k_codes = reinterpret_cast<const uint8_t*>(a->k_codes); k.k_scales = reinterpret_cast<const uint8_t*>(a->k_scales);
   k.v_codes = reinterpret_cast<const uint8_t*>(a->v_codes); k.v_scales = reinterpret_cast<const uint8_t*>(a->v_scales);
-  k.score_mult = a->sm_scale * 1.44269504088896340736f;
+  k.score_mult = a->sm_scale * LOG2_E;
   k.causal = a->causal;
   char* ws = reinterpret_cast<char*>(workspace);
   k.ws_m = reinterpret_cast<float*>(ws + p.ws_m);

@@ -452,7 +452,7 @@ hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace
   c.hole = take(np / 2 + 1);
   c.mover = take(np / 2 + 1);
   const int64_t moves = a.num_pages / 2 + 1;
-  c.move_groups = a.num_arrays > 0 ? (int)(moves < 4096 ? moves : 4096) : 0;
+  c.move_groups = a.num_arrays > 0 && a.num_pages > 0 ? (int)(moves < 4096 ? moves : 4096) : 0;
   const int64_t items = a.num_pages > (int64_t)a.num_rows * a.table_width ? a.num_pages : (int64_t)a.num_rows * a.table_width;
   const int64_t rest = (items + POOL_THREADS - 1) / POOL_THREADS;
   if (a.num_pages > 0) {

@@ -165,6 +165,20 @@ def test_compaction(B, R, W, NP):
         s.check()                                  # the arguments stay, the moved rows are copied
 
 
+def test_compaction_of_no_pages():
+    """No page in the pools, arrays named all the same: entries as they are, nothing copied."""
+    import torch
+    from intent_attention import _native as N
+    table, valid = _t([[5, -1, 2]]), _t([20])
+    out, pool = torch.zeros_like(table), torch.full((64,), 9, dtype=torch.uint8, device=_dev())
+    ws = torch.full((4096,), 255, dtype=torch.uint8, device=_dev())
+    a = N.CompactPagesArgs(1, 3, 16, 0, table.data_ptr(), valid.data_ptr(), None, out.data_ptr())
+    a.num_arrays = 1
+    a.arrays[0] = (pool.data_ptr(), 16)
+    N.compact_pages(a, torch.cuda.current_stream().cuda_stream, ws.data_ptr(), N.compact_pages_workspace(a))
+    assert out.tolist() == table.tolist() and bool((pool == 9).all())
+
+
 def test_compaction_without_pools_and_copy_pages():
     import torch
     import intent_attention as ia

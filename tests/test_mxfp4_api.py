@@ -124,6 +124,37 @@ def test_page_refusals():
         N.compact_pages_workspace(p)
 
 
+def test_compaction_refusals():
+    def args():
+        p = N.CompactPagesArgs()
+        p.num_rows, p.table_width, p.page_size, p.num_pages = 2, 3, 16, 10
+        p.page_table, p.valid_tokens, p.refs, p.out_table, p.out_refs, p.page_map = 256, 512, 768, 1024, 1280, 1536
+        return p
+    assert N.compact_pages_workspace(args()) > 0
+    for field, value, text in (("page_size", 0, "size"), ("num_pages", 1 << 31, "size"), ("out_table", 256, "another"),
+                               ("out_refs", 768, "another"), ("page_map", 1280, "another"), ("refs", 0, "NULL"),
+                               ("page_map", 1538, "aligned"), ("valid_tokens", 514, "aligned"), ("num_arrays", -1, "num_arrays")):
+        a = args()
+        setattr(a, field, value)
+        with pytest.raises(ValueError, match=text):
+            N.compact_pages_workspace(a)
+    need = N.compact_pages_workspace(args())
+    for ws, size in ((0, need), (256, need - 1), (260, need)):
+        with pytest.raises(ValueError, match="workspace"):
+            N.compact_pages(args(), 0, ws, size)
+
+
+def test_a_scale_that_leaves_float32_in_base_2_is_refused():
+    a = _attention_args()
+    for value, fine in ((2.3e38, True), (-2.3e38, True), (3e38, False), (-3e38, False)):
+        a.sm_scale = value
+        if fine:
+            N.mx_attention_workspace(a)
+        else:
+            with pytest.raises(ValueError, match="sm_scale"):
+                N.mx_attention_workspace(a)
+
+
 def test_host_tensors_are_refused():
     pools = ia.MxFp4Pools.empty(4, 64, "cpu")
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
