@@ -5,13 +5,18 @@
 // 1,024 pages, then a rank within them), rows by their place in the call, and rank meets
 // rank. Reference counts change by integer atomics, whose order leaves no trace.
 //
-//   grow, fork   plan_kernel   free pages per 1,024 ids; one workgroup checks the call and
-//                              sums what its rows need
-//                rank_kernel   the free ids in order, as many as are needed; the verdict
-//                apply_kernel  a workgroup per row: entries, counts, the copied last page
-//   free         free_kernel   a workgroup per row
-//   compact      plan_kernel, compact_rank_kernel (which page goes where),
-//                compact_apply_kernel (pages copied, table, counts and map written)
+//   grow, fork   seq_plan_kernel   free pages per 1,024 ids; one workgroup checks the call and
+//                                  sums what its rows need
+//                seq_rank_kernel   the free ids in order, as many as are needed; the verdict
+//                (seq_small_kernel for both, where the pages are few)
+//                seq_apply_kernel  a workgroup per row: entries, counts, the copied last page
+//   free         seq_free_kernel   a workgroup per row
+//   compact      compact_count_kernel, compact_rank_kernel (which page goes where; for few pages
+//                compact_small_kernel), compact_apply_kernel (pages copied, table, counts and
+//                map written)
+//
+// What bounds them is latency: reads that wait for each other, and the launches. Pages that
+// move are bytes at the rate of a copy: 0.67 GB of K and V rows in 130 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -27,6 +32,10 @@ namespace {
 constexpr int PAGE_GROUP = 1024;       // page ids a workgroup counts or ranks
 constexpr int POOL_THREADS = 256;
 constexpr int PLAN_THREADS = 1024;
+// Up to so many pages one workgroup plans and ranks, which saves a launch: free and fork of 6
+// sequences among 3,072 pages 27 us for 30 (19 for 22 replayed from a graph), at 18,944 23 for 22
+// replayed; a compaction of 4,266 pages 22 for 24 (14 for 18), of 17,066 24 for 24 (28 for 22).
+constexpr int64_t FEW_SEQUENCE_PAGES = 16384, FEW_COMPACT_PAGES = 8192;
 
 struct PageArrays {
   int n;
@@ -101,6 +110,19 @@ template <int WAVES> __device__ __forceinline__ void sum_groups(const int32_t* c
   scan_before<WAVES>(y, all);
 }
 
+// The ids of a thread where one workgroup of PLAN_THREADS takes all.
+struct PageRun { int begin, end; };
+__device__ __forceinline__ PageRun page_run(int64_t NP) {
+  const int per = (int)((NP + PLAN_THREADS - 1) / PLAN_THREADS), at = (int)threadIdx.x * per;
+  return PageRun{at, at + per < NP ? at + per : (int)NP};
+}
+__device__ __forceinline__ int run_free(const int32_t* refs, const PageRun& run) {
+  int n = 0;
+#pragma unroll 8
+  for (int id = run.begin; id < run.end; ++id) n += refs[id] <= 0;
+  return n;
+}
+
 // --------------------------------------------------------------------------- //
 // Grow and fork
 // --------------------------------------------------------------------------- //
@@ -147,16 +169,10 @@ __device__ __forceinline__ int count_free(const int32_t* refs, int64_t NP, int g
   return n;
 }
 
-template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
+// Is the call sound, and what does it need: by a workgroup of PLAN_THREADS. Writes `first`;
+// returns the pages needed, and in `refused` (shared) whether it is refused.
+template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, int& refused) {
   constexpr int WAVES = PLAN_THREADS / 64;
-  if ((int)blockIdx.x < a.groups) {
-    int total;
-    scan_before<WAVES>(count_free(a.refs, a.NP, blockIdx.x), total);
-    if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
-    return;
-  }
-  // the last workgroup: is the call sound, and what does it need
-  __shared__ int refused;
   if (threadIdx.x == 0) refused = 0;
   for (int k = threadIdx.x; k < a.num_seqs; k += PLAN_THREADS) a.marks[k] = 0;
   __threadfence_block();
@@ -209,10 +225,30 @@ template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_ker
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    a.head[0] = (int)(total > 0x7FFFFFFF ? 0x7FFFFFFF : total);
-    a.head[1] = refused;
+  return (int)(total > 0x7FFFFFFF ? 0x7FFFFFFF : total);
+}
+
+template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
+  if ((int)blockIdx.x < a.groups) {
+    int total;
+    scan_before<PLAN_THREADS / 64>(count_free(a.refs, a.NP, blockIdx.x), total);
+    if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
+    return;
   }
+  __shared__ int refused;
+  const int need = plan_call<KIND>(a, refused);
+  if (threadIdx.x == 0) { a.head[0] = need; a.head[1] = refused; }
+}
+
+// Plan and rank in one workgroup, for pools of few pages: a thread ranks the free pages of a run.
+template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_small_kernel(const SeqArgs a) {
+  __shared__ int refused;
+  const PageRun run = page_run(a.NP);
+  int all, rank = scan_before<PLAN_THREADS / 64>(run_free(a.refs, run), all);
+  const int need = plan_call<KIND>(a, refused);
+  if (threadIdx.x == 0) a.missing[0] = refused ? -1 : (need > all ? need - all : 0);
+  for (int id = run.begin; id < run.end && rank < need; ++id)
+    if (a.refs[id] <= 0) a.list[rank++] = id;
 }
 
 __global__ __launch_bounds__(POOL_THREADS) void seq_rank_kernel(const SeqArgs a) {
@@ -340,6 +376,29 @@ __global__ __launch_bounds__(POOL_THREADS) void compact_rank_kernel(const Compac
   }
 }
 
+// Count and rank in one workgroup, for pools of few pages.
+__global__ __launch_bounds__(PLAN_THREADS) void compact_small_kernel(const CompactArgs a) {
+  const PageRun run = page_run(a.NP);
+  int all, free_before = scan_before<PLAN_THREADS / 64>(run_free(a.refs, run), all);
+  const int L = (int)a.NP - all;
+  if (threadIdx.x == 0) {
+    a.head[0] = L;
+    if (all == 0) a.head[1] = 0;
+  }
+  for (int id = run.begin; id < run.end; ++id) {
+    const bool free_page = a.refs[id] <= 0;
+    if (id == L) a.head[1] = free_before;
+    if (free_page) {
+      if (id < L) a.hole[free_before] = id;
+      ++free_before;
+    } else if (id >= L) {
+      const int move = L - 1 - (id - free_before);
+      a.mover[move] = id;
+      a.order[id] = move;
+    }
+  }
+}
+
 __device__ __forceinline__ int moved_to(const CompactArgs& a, int id, int L) {
   return id < L ? id : a.hole[a.order[id]];
 }
@@ -394,8 +453,12 @@ SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
 
 template <int KIND> hipError_t launch_seq(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
   const SeqArgs s = seq_args(a, workspace);
-  hipLaunchKernelGGL(seq_plan_kernel<KIND>, dim3(s.groups + 1), dim3(PLAN_THREADS), 0, stream, s);
-  hipLaunchKernelGGL(seq_rank_kernel, dim3(s.groups > 0 ? s.groups : 1), dim3(POOL_THREADS), 0, stream, s);
+  if (a.num_pages <= FEW_SEQUENCE_PAGES) {
+    hipLaunchKernelGGL(seq_small_kernel<KIND>, dim3(1), dim3(PLAN_THREADS), 0, stream, s);
+  } else {
+    hipLaunchKernelGGL(seq_plan_kernel<KIND>, dim3(s.groups + 1), dim3(PLAN_THREADS), 0, stream, s);
+    hipLaunchKernelGGL(seq_rank_kernel, dim3(s.groups), dim3(POOL_THREADS), 0, stream, s);
+  }
   if (a.count > 0)
     hipLaunchKernelGGL(seq_apply_kernel<KIND>, dim3(a.count * a.rows_per_seq), dim3(POOL_THREADS), 0, stream, s);
   return hipGetLastError();
@@ -455,7 +518,9 @@ hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace
   c.move_groups = a.num_arrays > 0 && a.num_pages > 0 ? (int)(moves < 4096 ? moves : 4096) : 0;
   const int64_t items = a.num_pages > (int64_t)a.num_rows * a.table_width ? a.num_pages : (int64_t)a.num_rows * a.table_width;
   const int64_t rest = (items + POOL_THREADS - 1) / POOL_THREADS;
-  if (a.num_pages > 0) {
+  if (a.num_pages > 0 && a.num_pages <= FEW_COMPACT_PAGES) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, c);
+  } else if (a.num_pages > 0) {
     hipLaunchKernelGGL(compact_count_kernel, dim3(c.groups), dim3(POOL_THREADS), 0, stream, c);
     hipLaunchKernelGGL(compact_rank_kernel, dim3(c.groups), dim3(POOL_THREADS), 0, stream, c);
   }

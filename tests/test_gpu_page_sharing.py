@@ -62,7 +62,8 @@ class State:
             assert torch.equal(p, w)
 
 
-@pytest.mark.parametrize("B,R,W,NP", [(4, 1, 1, 9), (9, 2, 5, 100), (12, 3, 40, 2100), (70, 1, 3, 1024), (8, 5, 33, 3333)])
+@pytest.mark.parametrize("B,R,W,NP", [(4, 1, 1, 9), (9, 2, 5, 100), (12, 3, 40, 2100), (70, 1, 3, 1024), (8, 5, 33, 3333),
+                                      (12, 3, 40, 16384), (12, 3, 40, 16385), (9, 2, 30, 40000)])
 def test_grow_fork_free_follow_the_lists(B, R, W, NP):
     import intent_attention as ia
     s = State(B * 100 + W, B, R, W, NP)
@@ -95,9 +96,10 @@ def test_grow_fork_free_follow_the_lists(B, R, W, NP):
     assert done >= 4
 
 
-def test_refusals_change_nothing():
+@pytest.mark.parametrize("NP", [200, 17000])
+def test_refusals_change_nothing(NP):
     import intent_attention as ia
-    s = State(5, 8, 2, 6, 200, fill=0.5)
+    s = State(5, 8, 2, 6, NP, fill=0.5)
     two = [b for b in range(8) if b % 4 == 3]
     for b in two:
         assert s.host.valid[b] == [0, 0]
@@ -115,9 +117,14 @@ def test_refusals_change_nothing():
     s.check()
 
 
-def test_too_few_free_pages():
+@pytest.mark.parametrize("NP", [60, 17000])
+def test_too_few_free_pages(NP):
     import intent_attention as ia
-    s = State(6, 4, 1, 40, 60, fill=0.2)
+    s = State(6, 4, 1, 40, NP, fill=0.2)
+    free = [p for p in range(NP) if s.host.refs[p] == 0]
+    for p in s.rng.permutation(free)[:max(0, len(free) - 35)]:       # others hold the rest
+        s.host.refs[p] = 1
+    s.refs.copy_(_t(s.host.refs))
     short = s.host.grow([0, 3], [200, 16 * 38])
     assert short > 0
     assert ia.grow_sequences(s.table, s.valid, s.refs, [0, 3], [200, 16 * 38]).tolist() == [short]
@@ -143,7 +150,8 @@ def test_fork_of_full_empty_and_pageless_parents():
     s.check()
 
 
-@pytest.mark.parametrize("B,R,W,NP", [(1, 1, 1, 1), (4, 1, 6, 30), (12, 3, 40, 2100), (8, 5, 33, 3333), (3, 1, 5, 5000)])
+@pytest.mark.parametrize("B,R,W,NP", [(1, 1, 1, 1), (4, 1, 6, 30), (12, 3, 40, 2100), (8, 5, 33, 3333), (3, 1, 5, 5000),
+                                      (12, 3, 40, 8192), (12, 3, 40, 8193), (9, 2, 30, 20011)])
 def test_compaction(B, R, W, NP):
     import torch
     import intent_attention as ia
@@ -201,11 +209,12 @@ def test_compaction_without_pools_and_copy_pages():
         assert torch.equal(x, want[n])
 
 
-def test_page_operators_replay_in_a_graph():
+@pytest.mark.parametrize("NP", [900, 17000])
+def test_page_operators_replay_in_a_graph(NP):
     """Fork, grow, free and compact captured once, replayed on other sequences."""
     import torch
     import intent_attention as ia
-    s = State(21, 12, 2, 20, 900, fill=0.5)
+    s = State(21, 12, 2, 20, NP, fill=0.5)
     seqs, new, folks, kids, gone = _t([0]), _t([40]), _t([1]), _t([3]), _t([2])
     short = [torch.zeros(1, dtype=torch.int32, device=_dev()) for _ in range(2)]
 
