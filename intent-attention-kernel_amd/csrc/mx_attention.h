@@ -56,7 +56,7 @@ __device__ __forceinline__ MxPart mx_part(const MxAttn& a, int tiles) {
   const uint32_t kvrows = (uint32_t)a.B * a.Hkv, rest = blockIdx.x / kvrows;
   MxPart p;
   p.kvrow = blockIdx.x - rest * kvrows;
-  p.split = (int)(rest / tiles);
+  p.split = (int)(rest / (uint32_t)tiles);
   p.tile = tiles - 1 - (int)(rest - (uint32_t)p.split * tiles);
   return p;
 }

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   const MxPart part = mx_part(a, a.tiles);
   const int64_t kvrow = part.kvrow;
   const int tile = part.tile, split = part.split;
-  const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
+  const int b = (int)(part.kvrow / (uint32_t)a.Hkv), hk = (int)(part.kvrow - (uint32_t)b * a.Hkv);
   const MxRows n = mx_rows(a, kvrow, b);
   const int entries = mx_entries(a, n, tile * 16, 16);
   const int e0 = split * a.chunk, e1 = e0 + a.chunk < entries ? e0 + a.chunk : entries;

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
   const MxPart part = mx_part(a, (a.L * a.G + BM - 1) / BM);
   const int64_t kvrow = part.kvrow;
   const int tile = part.tile, split = part.split;
-  const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow % a.Hkv);
+  const int b = (int)(part.kvrow / (uint32_t)a.Hkv), hk = (int)(part.kvrow - (uint32_t)b * a.Hkv);
   const MxRows n = mx_rows(a, kvrow, b);
   const int entries = mx_entries(a, n, tile * BM, BM);
   const int e0 = split * a.chunk, e1 = e0 + a.chunk < entries ? e0 + a.chunk : entries;
