@@ -643,7 +643,7 @@ iak_status iak_fake_quant_blocks(const iak_fake_quant_blocks_args* args, void* w
  *   NaN: scale 255, codes 0.
  * It writes bytes of the addressed tokens only; tokens without a page are left out. Two
  * tokens that address one slot race. Read gives the values (exact in every dtype), and
- * zeros for tokens without a page and for i >= q_lens[b]. */
+ * zeros for tokens without a page and for i >= q_lens[b]. Code pools 4-byte aligned. */
 typedef struct {
   int32_t batch, count, num_kv_heads, head_dim, page_size, table_width;
   int64_t num_pages;
@@ -670,9 +670,11 @@ iak_status iak_mx_read_tokens(const iak_mx_tokens_args* args, void* stream);
  * matrix cores in float16 (queries scaled by a power of two per row, so that neither range
  * nor, for float16 and bfloat16 queries, bits are lost; K and V exact; weights rounded to
  * 11 bits) with float32 sums; float32 queries and their weights are split in two (22 bits).
+ * Scores, with the scale, have to be float32 numbers in base 2. Code pools are 16-byte, scale
+ * pools 4-byte aligned; q and out lie at any address of their type, and out may be q.
  * splits: parts a row's tokens are divided into (0: automatic). The parts meet in the
- * workspace (iak_mx_attention_workspace bytes, 16-byte aligned; 0: not needed); calls that
- * share one on different streams race. */
+ * workspace (iak_mx_attention_workspace bytes, 16-byte aligned, as it comes; 0: not needed);
+ * calls that share one on different streams race. */
 typedef struct {
   int32_t batch, q_len, num_q_heads, num_kv_heads, head_dim, page_size, table_width;
   int64_t num_pages;
@@ -752,8 +754,8 @@ iak_status iak_fork_sequences(const iak_sequences_args* args, void* workspace, s
 /* Compaction: with L pages in use (refs > 0), those with ids >= L move to the free ids
  * below L, the highest to the lowest: page_map [num_pages] is the new id of every page (-1:
  * free), out_refs [num_pages] the counts by new id, out_table [num_rows, table_width] the
- * table with its entries in use mapped (the others as they are). The arrays' rows are
- * copied in place; old rows keep their bytes, and page_table and refs stay as they are, so
+ * table with its entries in use mapped (-1 for one that names a free page; the others as
+ * they are). The arrays' rows are copied in place; old rows keep their bytes, and page_table and refs stay as they are, so
  * work that still reads the old table finds its pages. No output may overlap an input. */
 typedef struct {
   int32_t num_rows, table_width, page_size;

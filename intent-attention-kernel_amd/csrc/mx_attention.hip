@@ -165,8 +165,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   };
 
   // Twelve waves a CU are what hides the loads: a ring of two or more pairs cost registers and was
-  // slower, as were sixteen waves of fewer registers. The bytes come at the rate that the same
-  // loads reach alone, streamed (1.14 GB in 190 us; 216 with loads that stay in the caches).
+  // slower, as were sixteen waves of fewer registers. 256 rows of 32,768 tokens (1.14 GB) take 181 us
+  // (6.3 TB/s; 183 in three splits); loads that stay in the caches took 216 where these took 190.
+  // Short rows wait: launch, length and table, pages, LDS and store in turn are 5.5 us, and a merge
+  // kernel 4 more: 52 rows of 5,750 tokens (39 MB) take 14 + 4 us. Chunks of equal size over all
+  // rows, from the lengths on the device, were no faster (19.7, and 192 for the long rows).
   MxPair<D> x;
   if (e0 + 2 * w < e1) load_pair<D>(x, a, page(0), page(1), c, g);
   for (int at = e0 + 2 * w, k = 0, block = 0; at < e1; at += 2 * NW) {
