@@ -11,7 +11,8 @@
 // bounds it is the bytes. Long calls give a workgroup 16 tokens of one head, whose codes are
 // one run of memory wherever a page has room; calls of few tokens give it all heads of one.
 // 21,400 new tokens x 8 heads x 128 channels in 8 sequences padded to 4,001: append 29 us (111 MB,
-// 3.9 TB/s), read 33 us (111 MB and 40 MB of zeros, 4.6 TB/s); 64 new tokens: 3.4 us each.
+// 3.8 TB/s), read 24 us (the same and 43 MB of zeros, the codes from the caches); 64 new tokens:
+// 3.4 us each. Two or four tokens a thread changed nothing (50.5 us for both; 53.8).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -27,10 +28,15 @@ namespace {
 constexpr int MX_THREADS = 256;
 
 // Eight values as floats, wherever they lie: one or two 16-byte loads, which the hardware takes
-// at any address of the type.
+// at any address of the type. Values are streamed, in and out: appending and reading back 21,400
+// tokens took 63 us through the caches and takes 50.
+typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T> __device__ __forceinline__ void load8f(const T* p, float (&x)[8]) {
+  any4 w[sizeof(T) / 2];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(p) + i);
   T t[8];
-  __builtin_memcpy(t, p, sizeof(t));
+  __builtin_memcpy(t, w, sizeof(t));
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
 }
@@ -63,7 +69,10 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
   T t[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) t[j] = (T)x[j];
-  __builtin_memcpy(p, t, sizeof(t));
+  any4 w[sizeof(T) / 2];
+  __builtin_memcpy(w, t, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<any4*>(p) + i);
 }
 
 // Eight values of a code dword and its scale byte.
@@ -111,15 +120,15 @@ template <typename T>
 __global__ __launch_bounds__(MX_THREADS) void mx_append_kernel(const iak_mx_tokens_args a, int group) {
   const TokenAt t = token_at(a, group);
   for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int n = new_tokens(a, b);
+    const int64_t row = (int64_t)b * a.num_kv_heads + t.h;
+    const int tokens = row_tokens(a, row), n = new_tokens(a, b);   // loads under way together
     if (!t.in || t.i >= n) continue;
     // the values come while the token's place is looked up; the four lanes of a block are one
     // token's and go together
     float k[8], v[8];
     load8f(reinterpret_cast<const T*>(a.k) + b * a.k_stride_b + t.i * a.k_stride_t + t.h * a.k_stride_h + 8 * t.c, k);
     load8f(reinterpret_cast<const T*>(a.v) + b * a.v_stride_b + t.i * a.v_stride_t + t.h * a.v_stride_h + 8 * t.c, v);
-    const int64_t row = (int64_t)b * a.num_kv_heads + t.h;
-    const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
+    const MxSlot at = mx_slot(a.page_table + row * a.table_width, tokens - n + t.i, a.table_width, a.num_pages);
     if (!at.there) continue;
     uint32_t kb, vb;
     const uint32_t kc = quantise8(k, kb), vc = quantise8(v, vb);
@@ -138,9 +147,9 @@ __global__ __launch_bounds__(MX_THREADS) void mx_read_kernel(const iak_mx_tokens
   const TokenAt t = token_at(a, group);
   if (!t.in) return;
   for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int n = new_tokens(a, b);
     const int64_t row = (int64_t)b * a.num_kv_heads + t.h;
-    const MxSlot at = mx_slot(a.page_table + row * a.table_width, row_tokens(a, row) - n + t.i, a.table_width, a.num_pages);
+    const int tokens = row_tokens(a, row), n = new_tokens(a, b);   // loads under way together
+    const MxSlot at = mx_slot(a.page_table + row * a.table_width, tokens - n + t.i, a.table_width, a.num_pages);
     float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (t.i < n && at.there) {
       const int64_t code = at.token * (a.head_dim / 8) + t.c;
