@@ -42,8 +42,8 @@ struct PageArrays {
   iak_page_array a[IAK_MAX_PAGE_ARRAYS];
 };
 
-// Row `src` of every array to row `dst`, by the workgroup.
-__device__ __forceinline__ void copy_page(const PageArrays& p, int64_t src, int64_t dst) {
+// Row `src` of every array to row `dst`, by the workgroup. STREAM: past the caches.
+template <bool STREAM> __device__ __forceinline__ void copy_page(const PageArrays& p, int64_t src, int64_t dst) {
   for (int k = 0; k < p.n; ++k) {
     const int64_t bytes = p.a[k].row_bytes;
     char* base = reinterpret_cast<char*>(p.a[k].base);
@@ -51,8 +51,10 @@ __device__ __forceinline__ void copy_page(const PageArrays& p, int64_t src, int6
     char* to = base + dst * bytes;
     const uint64_t low = reinterpret_cast<uintptr_t>(base) | (uint64_t)bytes;
     if ((low & 15u) == 0) {
-      for (int64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x)
-        reinterpret_cast<u4*>(to)[i] = reinterpret_cast<const u4*>(from)[i];
+      for (int64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x) {
+        if constexpr (STREAM) st_nt(reinterpret_cast<u4*>(to) + i, ld_nt(reinterpret_cast<const u4*>(from) + i));
+        else reinterpret_cast<u4*>(to)[i] = reinterpret_cast<const u4*>(from)[i];
+      }
     } else if ((low & 3u) == 0) {
       for (int64_t i = threadIdx.x; i < bytes / 4; i += blockDim.x)
         reinterpret_cast<uint32_t*>(to)[i] = reinterpret_cast<const uint32_t*>(from)[i];
@@ -67,7 +69,7 @@ __global__ __launch_bounds__(POOL_THREADS) void copy_pages_kernel(const PageArra
   for (int i = blockIdx.x; i < count; i += gridDim.x) {
     const int64_t s = src[i], d = dst[i];
     if (s < 0 || s >= num_pages || d < 0 || d >= num_pages || s == d) continue;   // uniform
-    copy_page(p, s, d);
+    copy_page<false>(p, s, d);
   }
 }
 
@@ -299,7 +301,7 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
     if (own_page) {
       const int id = a.list[first];
       if (threadIdx.x == 0) { entries[n - 1] = id; a.refs[id] = 1; }
-      copy_page(a.arrays, last, id);
+      copy_page<false>(a.arrays, last, id);
     }
     if (threadIdx.x == 0) a.valid[row] = a.valid[parent];
   }
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(POOL_THREADS) void compact_apply_kernel(const Compa
   const int L = a.head[0];
   if ((int)blockIdx.x < a.move_groups) {
     const int moves = a.head[1];
-    for (int j = blockIdx.x; j < moves; j += a.move_groups) copy_page(a.arrays, a.mover[j], a.hole[j]);
+    for (int j = blockIdx.x; j < moves; j += a.move_groups) copy_page<true>(a.arrays, a.mover[j], a.hole[j]);
     return;
   }
   const int64_t step = (int64_t)(gridDim.x - a.move_groups) * POOL_THREADS;
