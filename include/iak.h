@@ -717,9 +717,10 @@ iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
  * that hold a page; a page with refs <= 0 is free. page_table [num_seqs, rows_per_seq,
  * table_width], valid_tokens [num_seqs, rows_per_seq]: entries 0 .. ceil(valid / page_size)
  * - 1 of a row are in use. All int32, on the device, changed in place.
- *   iak_free_sequences  lets go of every page of sequences seqs[0 .. count-1]: refs - 1 per
- *       entry, the entries become -1 and the lengths 0. Indices outside [0, num_seqs) are
- *       left out, one listed twice is freed once.
+ *   iak_free_sequences  lets go of the newest new_tokens[i] tokens (NULL: of all) in each row of
+ *       sequence seqs[i], of as many as there are: the lengths sink, and entries that are no
+ *       longer in use become -1, refs - 1. Indices outside [0, num_seqs) and negative numbers
+ *       are left out; a sequence listed twice loses tokens twice.
  *   iak_grow_sequences  sequence seqs[i] gets new_tokens[i] more tokens in each of its rows:
  *       entries for them come from the free pages, the lowest id first, in the order of
  *       (i, row, entry), with refs = 1.
@@ -740,7 +741,7 @@ typedef struct {
   int32_t count;
   const int32_t* seqs;
   const int32_t* parents;      /* fork */
-  const int32_t* new_tokens;   /* grow */
+  const int32_t* new_tokens;   /* grow; free: may be NULL */
   int32_t* missing;            /* grow, fork */
   int32_t num_arrays;          /* fork */
   iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];

@@ -7,14 +7,17 @@
 // page of K or of V in eight waves, of both in four) into LDS, from where all read them: two
 // buffers, one barrier a step. The sum of the weights is a product with ones on the matrix cores.
 //
-// 2,048 queries x 32 heads x 8 KV heads over 8,192 tokens, head_dim 128, float16, causal: 260 us
-// in tiles of 256, 923 TFLOP/s of the products (a matrix product of 8,192 cubed reaches 1,176);
-// 269 in tiles of 128, where 16 x 512 queries over 512 tokens take 80 and in tiles of 256 91 (two
-// workgroups a CU fill each other's waits). What bounds it are the reads of LDS, and the softmax's
-// vector instructions behind them. Tiles of 128 took 279 us before the workgroups' order was by KV
-// row; of these went, taken out on trial: the reads 69, then the conversion 13; the exponentials
-// 7, the value products 18, the score products 0. Slower were one half's products ahead of the
-// other's softmax (330), operands read ahead (340), tiles of 64 rows and wave priorities (285).
+// 2,048 queries x 32 heads x 8 KV heads over 8,192 tokens, head_dim 128, float16, causal: 256 us
+// in tiles of 256, 940 TFLOP/s of the products (a matrix product of 8,192 cubed reaches 1,176);
+// 267 in tiles of 128, where 16 x 512 queries over 512 tokens take 80 and in tiles of 256 91 (two
+// workgroups a CU fill each other's waits). The matrix cores are busy for 46 % of the time and
+// the vector instructions (softmax, conversion) for 53 %; the two overlap little. Tiles of 128 took
+// 279 us before the workgroups' order was by KV row; of these went, taken out on trial: the reads
+// of LDS 69, then the conversion 13; the exponentials 7, the value products 18, the score products
+// 0. Slower were one half's products ahead of the other's softmax (330), half the waves a barrier
+// later with their value products (268), operands read ahead (340), tiles of 64 rows and wave
+// priorities (285); with head_dim 64, where this call takes 176, four tiles of rows a wave (261)
+// and four waves a SIMD (261).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -307,19 +307,34 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
   }
 }
 
-// A workgroup per (listed sequence, row). The length is taken by one exchange, so that a
-// sequence listed twice is freed once.
+// A workgroup per (listed sequence, row). The length is lowered atomically, so that a sequence
+// listed twice loses each of its tokens once.
 __global__ __launch_bounds__(POOL_THREADS) void seq_free_kernel(const SeqArgs a) {
-  __shared__ int tokens;
+  __shared__ int tokens, left;
   const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
   const int s = a.seqs[j];
   if (s < 0 || s >= a.num_seqs) return;
   const int64_t row = (int64_t)s * a.R + h;
-  if (threadIdx.x == 0) tokens = atomicExch(&a.valid[row], 0);
+  if (threadIdx.x == 0) {
+    int old, rest = 0;
+    if (a.new_tokens) {
+      const int drop = a.new_tokens[j] < 0 ? 0 : a.new_tokens[j];
+      int seen = atomicAdd(&a.valid[row], 0);
+      do {                                                       // fails only where another workgroup's succeeds
+        old = seen;
+        rest = old > drop ? old - drop : 0;
+        seen = atomicCAS(&a.valid[row], old, rest);
+      } while (seen != old);
+    } else {
+      old = atomicExch(&a.valid[row], 0);
+    }
+    tokens = old;
+    left = rest;
+  }
   __syncthreads();
   const int n = used_entries(tokens, a.PSZ, a.W);
   int32_t* entries = a.table + row * a.W;
-  for (int e = threadIdx.x; e < n; e += POOL_THREADS) {
+  for (int e = used_entries(left, a.PSZ, a.W) + threadIdx.x; e < n; e += POOL_THREADS) {
     const int id = entries[e];
     if (id >= 0 && id < a.NP) atomicSub(&a.refs[id], 1);
     entries[e] = -1;

@@ -13,7 +13,7 @@ The state is three int32 tensors on the device, which a program keeps beside its
 * ``grow_sequences`` makes room for new tokens: pages for them, the lowest free ids first;
 * ``fork_sequences`` makes empty sequences copies of others: full pages are shared, a last
   page with room is copied, so that both may append;
-* ``free_sequences`` lets sequences go;
+* ``free_sequences`` lets sequences go, or their newest tokens;
 * ``compact_pages`` moves the pages in use to the lowest ids and returns the new table;
 * ``copy_pages`` copies pages from id to id.
 
@@ -156,11 +156,16 @@ def fork_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: t
     return missing
 
 
-def free_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices) -> None:
-    """Let go of every page of sequences ``seqs``: refs - 1 for each entry in use, the entries
-    become -1 and the lengths 0. Indices outside the table are left out, one listed twice is
-    freed once."""
+def free_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
+                   tokens: Optional[Indices] = None) -> None:
+    """Let go of sequences ``seqs``, or of the newest ``tokens[i]`` tokens of every row of
+    ``seqs[i]`` (drafts that were not taken): valid_tokens sinks, to 0 at least, entries that are
+    no longer in use become -1, refs - 1 for each. Indices outside the table and negative numbers are
+    left out, a sequence listed twice loses tokens twice."""
     a, dev, seqs, _ = _sequences("page sharing", page_table, valid_tokens, refs, seqs)
+    if tokens is not None:
+        tokens = _indices("tokens", tokens, dev, seqs.shape[0])
+        a.new_tokens = tokens.data_ptr()
     _launch(dev, N.free_sequences, a, current_stream_handle(dev))
     _written(page_table, valid_tokens, refs)
 

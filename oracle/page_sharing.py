@@ -28,16 +28,18 @@ class Pages:
     def _free(self):
         return [i for i, r in enumerate(self.refs) if r <= 0]
 
-    def free(self, seqs):
-        for s in seqs:
+    def free(self, seqs, tokens=None):
+        for k, s in enumerate(seqs):
             if not 0 <= s < len(self.table):
                 continue
             for h, row in enumerate(self.table[s]):
-                for e in range(self.used(s, h)):
+                last = self.used(s, h)
+                drop = self.valid[s][h] if tokens is None else max(0, tokens[k])
+                self.valid[s][h] = max(0, self.valid[s][h] - drop)
+                for e in range(self.used(s, h), last):
                     if self._in(row[e]):
                         self.refs[row[e]] -= 1
                     row[e] = -1
-                self.valid[s][h] = 0
 
     def _sound(self, seqs):
         return all(0 <= s < len(self.table) for s in seqs) and len(set(seqs)) == len(seqs)

@@ -173,6 +173,25 @@ def test_compaction(B, R, W, NP):
         s.check()                                  # the arguments stay, the moved rows are copied
 
 
+@pytest.mark.parametrize("B,R,W,NP", [(5, 1, 4, 40), (9, 3, 40, 1500)])
+def test_newest_tokens_let_go(B, R, W, NP):
+    """Some, none and more tokens than there are, negative numbers, a sequence twice; grown again after it."""
+    import intent_attention as ia
+    s = State(B * 7 + W, B, R, W, NP)
+    for it in range(8):
+        seqs = [int(x) for x in s.rng.integers(-1, B + 1, B)]
+        drop = [int(x) for x in s.rng.choice([0, 1, 5, 15, 16, 17, 40, -3, W * 16, 2 ** 31 - 1], B)]
+        s.host.free(seqs, drop)
+        ia.free_sequences(s.table, s.valid, s.refs, _t(seqs), _t(drop))
+        s.check()
+        one = [int(s.rng.integers(0, B))]
+        want = s.host.grow(one, [23])
+        assert ia.grow_sequences(s.table, s.valid, s.refs, one, [23]).tolist() == [want]
+        s.check()
+    with pytest.raises(ValueError, match="tokens"):
+        ia.free_sequences(s.table, s.valid, s.refs, [0, 1], [1])
+
+
 def test_compaction_of_no_pages():
     """No page in the pools, arrays named all the same: entries as they are, nothing copied."""
     import torch
@@ -310,3 +329,10 @@ def test_serving_loop(D, Hkv, G):
     assert bool((refs[:live] > 0).all())
     grow([0, 1, 4], [5, 20, 1])
     grow([0, 1, 2, 4, 5], [1, 1, 1, 1, 1])
+    grow([0, 2, 4], [18, 4, 4])                           # drafts, of which some are not taken
+    ia.free_sequences(table, valid, refs, [0, 2], [17, 2])
+    for b, n in ((0, 17), (2, 2)):
+        kept[b] = tuple(x[:-n] for x in kept[b])
+    grow([0, 2, 4], [1, 1, 1])
+    used = [-(-len(kept[b][0]) // 16) * Hkv for b in range(B)]
+    assert int(refs.sum()) == sum(used)                   # every entry counted, none more
