@@ -272,6 +272,21 @@ def test_attention_output_types_and_strides(L):
         assert (buf[..., 0] == 7).all() and (buf[..., D + 1:] == 7).all()
 
 
+@pytest.mark.parametrize("B,L,Hq,Hkv,D,W,splits", [(2, 1, 6, 2, 64, 14, 1), (2, 5, 8, 2, 128, 14, 3), (2, 140, 8, 2, 128, 14, 1),
+                                                   (2, 140, 8, 2, 128, 14, 16), (1, 2050, 16, 2, 64, 20, 1)])
+def test_attention_in_place(B, L, Hq, Hkv, D, W, splits):
+    """The output in the query's place: the same bits."""
+    import torch
+    import intent_attention as ia
+    rng = np.random.default_rng(L)
+    _, pools = _pools(rng, B * Hkv * W, D)
+    table, valid = _t(_table(rng, B, Hkv, W, B * Hkv * W)), _t(np.full((B, Hkv), W * 16 - 3, np.int32))
+    q = torch.randn((B, L, Hq, D), device=_dev()).half()
+    want = ia.mxfp4_paged_attention(q, pools, table, valid, causal=False, splits=splits)
+    got = ia.mxfp4_paged_attention(q, pools, table, valid, causal=False, splits=splits, out=q)
+    assert got is q and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("L", [1, 3, 140])
 def test_attention_invalid_pages_hold_no_tokens(L):
     rng = np.random.default_rng(L + 50)
