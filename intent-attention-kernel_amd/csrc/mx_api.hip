@@ -63,61 +63,74 @@ iak_status validate_mx_tokens(const iak_mx_tokens_args* a) {
 constexpr float LOG2_E = 1.44269504088896340736f;
 
 struct MxPlan {
-  int G, tiles, splits, chunk, waves, chunk_rows;
+  int G, tile_rows, tiles, splits, chunk, shares, waves;
   int64_t items;
-  size_t ws_m, ws_l, ws_acc, total;
+  size_t ws_m, ws_l, ws_acc, ws_parts, total;
 };
 
-// Which kernel, and into how many splits a row's tokens go: the least of costs in microseconds
-// fitted to measurements (60 shapes of 8 to 131,072 query rows by 16 to 2,048 table entries).
+// Which kernel, and into how many parts a row's tokens go: the least of costs in microseconds
+// fitted to measurements (80 shapes of 8 to 131,072 query rows by 16 to 2,048 table entries).
 // A CU holds one to four workgroups at a time. A round of as many takes START and its entries'
 // time, one of fewer runs faster; where sequences differ, rounds before the last are not full. A
-// second kernel merges splits at MERGE and the time of the partials' bytes.
-//   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 182 us, 4 228,
-//     6 195, 8 203; 512 x 125: 1 split 25, 2 29, 4 31; 64 x 128: 1 split 18, 4 14.6, 8 13.8, 16 17
+// second kernel merges the parts at MERGE and the time of their bytes. With several sequences the
+// chunk kernel's rounds can be shared out by lengths, where they are two parts a tile or more.
+//   rows kernel, 256 rows x 2,048 entries, head_dim 128: 3 splits (one full round) 183 us, 4 211,
+//     6 186, 8 190, 1 (of eight waves) 181; 512 x 125: 1 split 25, 2 29, 4 31; 64 x 128: 1 18, 4 14.6
 //   rows kernel | chunk kernel, tiles of 128 rows | of 256, in us (best splits), head_dim 128:
-//     1 x 2,048 queries x 32 heads x 8 KV heads over 8,192 tokens: 412 | 266 (1) | 261 (1)
+//     1 x 2,048 queries x 32 heads x 8 KV heads over 8,192 tokens: 412 | 266 (1) | 257 (1)
 //     1 x 512 x 32 x 8 over 8,192: 126 (2) | 92 (4) | 85 (4);  8 x 16 x 32 x 8 over 4,000: 24 | 35 (8)
 //     16 x 512 x 32 x 8 over 512: 168 | 80 (1) | 91 (1);  2 x 4,096 x 16 x 2 over 4,096: 272 | 169 | 155
 //     8 x 300 x 8 x 2 over 1,000: 26 | 33 (1) | 36 (3)
 //     the first with float32 queries: 537 | 443 (1) | 453 (1)
 constexpr double CUS = 256;         // and up to as many unsplit tiles are workgroups of more waves
 
-struct MxChoice { int chunk_rows; int64_t splits; };             // chunk_rows 0: the rows kernel
+struct MxChoice { int tile_rows; int64_t splits; int shares; };
 
 MxChoice choose(int B, int Hkv, int64_t rows, int W, int D, bool f32, int64_t forced) {
   const bool big = D == 128;
   const double MERGE = 6, kvrows = (double)B * Hkv;
   const int64_t most = (W + 15) / 16;
-  MxChoice best = {0, 1};
+  MxChoice best = {16, 1, 0};
   double least = -1;
-  // tiles of `chunk` rows (0: the rows kernel's 16), of which a CU holds `places`
-  auto each_split = [&](int chunk, int places, double start, double entry, double fill) {
-    const double work = kvrows * (double)((rows + (chunk ? chunk : 16) - 1) / (chunk ? chunk : 16));
-    auto consider = [&](int64_t s) {
+  // tiles of `tile` rows, of which a CU holds `places`
+  auto kernel = [&](int tile, int places, double start, double entry) {
+    const double work = kvrows * (double)((rows + tile - 1) / tile), round = CUS * places;
+    const double fill = tile > 16 && B > 1 ? 0.75 : 1;
+    auto keep = [&](double cost, int64_t splits, int shares) {
+      if (least < 0 || cost < least) { least = cost; best = {tile, splits, shares}; }
+    };
+    auto split = [&](int64_t s) {
       if (s > most) s = most;
       if (s < 1) s = 1;
       if (forced > 0) s = forced;
-      const bool many = chunk == 0 && s == 1 && work <= CUS;     // one workgroup of more waves a CU
+      const bool many = tile == 16 && s == 1 && work <= CUS;     // one workgroup of more waves a CU
       const int room = many ? 1 : places;
       const double each = std::ceil(work * s / CUS);             // workgroups of the busiest CU
       const double before = std::ceil(each / room) - 1, last = each - before * room;
       double cost = (before * fill + (last == room ? 1 : 0.42 + 0.58 * last / room)) *
                     (start + entry / (many ? (big ? 3 : 5) : 1) * W / s);
       if (s > 1) cost += MERGE + kvrows * rows * ((double)s * D * 8 / 5.5e6 + (s > 8 ? 1e-3 : 0));   // past 8: a workgroup a row
-      if (least < 0 || cost < least) { least = cost; best = {chunk, s}; }
+      keep(cost, s, 0);
     };
-    consider(1);
-    if (work >= 4 * CUS * places || most <= 1 || forced > 0) return;
-    for (int64_t s = 2; s < most && s < 256; s *= 2) consider(s);
-    for (int rounds = 1; rounds <= 4; ++rounds) consider((int64_t)(rounds * CUS * places / work));
+    split(1);
+    if (most <= 1 || forced > 0) return;
+    if (work < 4 * round) {
+      for (int64_t s = 2; s < most && s < 256; s *= 2) split(s);
+      for (int rounds = 1; rounds <= 4; ++rounds) split((int64_t)(rounds * round / work));
+    }
+    if (B == 1 || tile != (f32 ? 128 : 256) || work > iak::MX_SHARED_TILES || work * W > 2e9) return;
+    for (int rounds = 1; rounds <= (big ? 4 : 1); ++rounds) {
+      const double parts = rounds * round / work;                // of a tile, on average
+      if (parts < 2 || parts > most) continue;
+      keep(rounds * (start + 1) + entry * fill * W * work / round * parts / std::floor(parts) + MERGE +
+               kvrows * rows * (parts * D * 8 / 5.5e6 + (parts > 8 ? 1e-3 : 0)), 1, (int)(rounds * round));
+    }
   };
   const double bytes_entry = (big ? 0.30 : 0.20) / (double)((rows + 15) / 16);   // an entry's bytes, shared by its tiles
   const double rows_entry = big ? (f32 ? 0.205 : 0.16) : (f32 ? 0.173 : 0.14);
-  const double fill = B > 1 ? 0.75 : 1;
-  each_split(0, big ? 3 : 4, 3, rows_entry < bytes_entry ? bytes_entry : rows_entry, 1);
-  if (rows > 16) each_split(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50), fill);
-  if (rows > 128 && !f32) each_split(256, 1, big ? 7 : 5, big ? 0.50 : 0.345, fill);
+  kernel(16, big ? 3 : 4, 3, rows_entry < bytes_entry ? bytes_entry : rows_entry);
+  if (rows > 16) kernel(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50));
+  if (rows > 128 && !f32) kernel(256, 1, big ? 7 : 5, big ? 0.50 : 0.345);
   return best;
 }
 
@@ -144,27 +157,29 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   if (!aligned4(a->k_scales) || !aligned4(a->v_scales)) return fail(IAK_EINVAL, "scale pools must be 4-byte aligned");
   const int64_t rows = (int64_t)a->q_len * p->G;
   if (rows > 0x3FFFFFFF) return fail(IAK_EINVAL, "q_len %d x %d heads per KV head is too long", a->q_len, p->G);
-  p->tiles = (int)((rows + 15) / 16);
-  const double tiles = (double)a->batch * a->num_kv_heads * p->tiles;
-  if (tiles > 1.6e7) return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", tiles);
+  const double kvrows = (double)a->batch * a->num_kv_heads;
+  if (kvrows * ((rows + 15) / 16) > 1.6e7)
+    return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", kvrows * ((rows + 15) / 16));
   const int W = a->table_width > 0 ? a->table_width : 1;
-  MxChoice best = choose(a->batch, a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
-  p->chunk_rows = best.chunk_rows;
-  const double blocks =
-      best.chunk_rows ? (double)a->batch * a->num_kv_heads * ((rows + best.chunk_rows - 1) / best.chunk_rows) : tiles;
+  const MxChoice best = choose(a->batch, a->num_kv_heads, rows, W, a->head_dim, a->q_dtype == IAK_DTYPE_F32, a->splits);
+  p->tile_rows = best.tile_rows;
+  p->tiles = (int)((rows + p->tile_rows - 1) / p->tile_rows);
+  p->shares = best.shares;
+  const double tiles = kvrows * p->tiles;
   int64_t splits = best.splits;
   if (splits > (W + 1) / 2) splits = (W + 1) / 2;
-  while (splits > 1 && tiles * splits > 1.0e6) splits /= 2;
+  while (splits > 1 && tiles * splits * p->tile_rows > 1.6e7) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
   p->waves = p->splits == 1 && tiles <= CUS ? 16 : 4;
-  p->items = (int64_t)blocks * p->splits;
-  if (p->splits > 1) {
-    const size_t slots = (size_t)tiles * p->splits * 16;
+  p->items = p->shares ? p->shares : (int64_t)tiles * p->splits;
+  if (p->splits > 1 || p->shares) {
+    const size_t rows_kept = (size_t)p->items * p->tile_rows;
     p->ws_m = 0;
-    p->ws_l = round_up(4 * slots);
-    p->ws_acc = p->ws_l + round_up(4 * slots);
-    p->total = p->ws_acc + round_up(4 * slots * (size_t)a->head_dim);
+    p->ws_l = round_up(4 * rows_kept);
+    p->ws_acc = p->ws_l + round_up(4 * rows_kept);
+    p->ws_parts = p->ws_acc + round_up(4 * rows_kept * (size_t)a->head_dim);
+    p->total = p->ws_parts + (p->shares ? round_up(8 * (size_t)tiles) : 0);
   }
   return IAK_OK;
 }
@@ -264,7 +279,8 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   iak::MxAttn k;
   k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
-  k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.waves = p.waves; k.chunk_rows = p.chunk_rows; k.items = p.items;
+  k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.shares = p.shares; k.waves = p.waves;
+  k.items = p.items; k.parted = p.total > 0;
   k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
   k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;
   k.table = a->page_table; k.valid = a->valid_tokens; k.q_lens = a->q_lens;
@@ -276,6 +292,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   k.ws_m = reinterpret_cast<float*>(ws + p.ws_m);
   k.ws_l = reinterpret_cast<float*>(ws + p.ws_l);
   k.ws_acc = reinterpret_cast<float*>(ws + p.ws_acc);
+  k.ws_parts = reinterpret_cast<int2*>(ws + p.ws_parts);
   return launched(iak::launch_mx_attention(k, reinterpret_cast<hipStream_t>(stream)), "4-bit cache attention");
 }
 

@@ -45,19 +45,100 @@ __device__ __forceinline__ int mx_entries(const MxAttn& a, const MxRows& n, int 
   return (mx_seen(a, n, last / a.G) + 15) / 16;
 }
 
-// Which KV row, tile of rows and split a workgroup takes. The KV rows turn fastest, so that the
-// workgroups that read the same pages meet in one XCD's L2 where the number of KV rows is a
-// multiple of 8, and every XCD has its share of each split and tile where lengths differ; those
-// that see most start first. (With the splits fastest, 4 x 1,024 queries over 1,024 tokens took
-// 85 us and take 58; 5 ragged sequences of 509 queries over 4,000 took 74 and take 59.)
-struct MxPart { uint32_t kvrow; int tile, split; };
+// What a workgroup takes: entries e0 .. e0 + chunk - 1 of a tile of rows, part number `part` of
+// the call's; `idle`: nothing.
+struct MxPart { uint32_t kvrow; int tile, e0, chunk; uint32_t part; bool idle; };
 
-__device__ __forceinline__ MxPart mx_part(const MxAttn& a, int tiles) {
+// The KV rows turn fastest, so that the workgroups that read the same pages meet in one XCD's L2
+// where the number of KV rows is a multiple of 8, and every XCD has its share of each split and
+// tile where lengths differ; those that see most start first. (With the splits fastest, 4 x 1,024
+// queries over 1,024 tokens took 85 us and take 58.)
+__device__ __forceinline__ MxPart mx_fixed_part(const MxAttn& a) {
   const uint32_t kvrows = (uint32_t)a.B * a.Hkv, rest = blockIdx.x / kvrows;
   MxPart p;
   p.kvrow = blockIdx.x - rest * kvrows;
-  p.split = (int)(rest / (uint32_t)tiles);
-  p.tile = tiles - 1 - (int)(rest - (uint32_t)p.split * tiles);
+  const int split = (int)(rest / a.tiles);
+  p.tile = a.tiles - 1 - (int)(rest - (uint32_t)split * a.tiles);
+  p.e0 = split * a.chunk;
+  p.chunk = a.chunk;
+  p.part = (p.kvrow * a.tiles + p.tile) * a.splits + split;
+  p.idle = false;
+  return p;
+}
+
+// Sum over the wave's lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// Lengths are known on the device alone: every wave works out for itself the least chunk with
+// which all tiles' chunks are no more than a.shares, and which of them is its workgroup's. Each XCD
+// takes a run of them. `UNIT`: entries that a workgroup takes at a step.
+// 16 heads over 4 of 128: 512, 16, 16 and 16 queries over 8,000, 500, 500 and 500 tokens 63 us, and
+// 144 in fixed parts; 8 heads over one, 3 sequences of up to 1,000 queries over up to 8,000 tokens 95
+// and 132, of equal lengths 140 and 134. Decode rows lose what the working out takes: 19.7 and 18.4
+// us, 192 and 178. With head_dim 64 one round only: 5 x 509 queries over 4,000 in two 66, fixed 59.
+template <int UNIT> __device__ __forceinline__ MxPart mx_shared_part(const MxAttn& a) {
+  constexpr int MOST = MX_SHARED_TILES / 64;
+  const int lane = threadIdx.x & 63;
+  const int all = a.B * a.Hkv * a.tiles, per = (all + 63) >> 6;    // tiles, and of a lane: a run
+  int units[MOST], own = 0;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    units[j] = 0;
+    const int t = lane * per + j;
+    if (j < per && t < all) {
+      const int kvrow = t / a.tiles, tile = t - kvrow * a.tiles, b = kvrow / a.Hkv;
+      const MxRows n = mx_rows(a, kvrow, b);
+      units[j] = (mx_entries(a, n, tile * a.tile_rows, a.tile_rows) + UNIT - 1) / UNIT;
+      own += units[j];
+    }
+  }
+  const int total = __builtin_amdgcn_readlane(wave_scan(own), 63);
+  auto chunks = [&](int x, int size) { return (int)((uint32_t)(x + size - 1) / (uint32_t)size); };
+  auto count = [&](int size) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) if (j < per) n += chunks(units[j], size);
+    return n;
+  };
+  // total / shares chunks are too few and total / (shares - tiles) enough
+  int size = (total + a.shares - 1) / a.shares, enough = (total + a.shares - all - 1) / (a.shares - all);
+  size = size < 1 ? 1 : size;
+  while (size < enough) {
+    const int mid = (size + enough) >> 1;
+    if (__builtin_amdgcn_readlane(wave_scan(count(mid)), 63) <= a.shares) enough = mid;
+    else size = mid + 1;
+  }
+  const int mine = count(size), upto = wave_scan(mine), parts = __builtin_amdgcn_readlane(upto, 63);
+  const int run = (parts + 7) >> 3, part = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+  MxPart p;
+  p.idle = (int)(blockIdx.x >> 3) >= run || part >= parts;
+  if (p.idle) return p;
+  const uint64_t has = __builtin_amdgcn_ballot_w64(part < upto);
+  const int owner = __builtin_ctzll(has);                          // the first lane whose run ends behind it
+  int before = upto - mine, at = 0, first = before, n = 0;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int c = j < per ? chunks(units[j], size) : 0;
+    if (before <= part) { at = j; first = before; n = c; }
+    before += c;
+  }
+  const int t = owner * per + __builtin_amdgcn_readlane(at, owner);
+  first = __builtin_amdgcn_readlane(first, owner);
+  n = __builtin_amdgcn_readlane(n, owner);
+  p.kvrow = (uint32_t)(t / a.tiles);
+  p.tile = t - (int)p.kvrow * a.tiles;
+  p.chunk = size * UNIT;
+  p.e0 = (part - first) * p.chunk;
+  p.part = (uint32_t)part;
+  if (part == first && threadIdx.x == 0) a.ws_parts[t] = int2{first, n};
   return p;
 }
 

@@ -67,14 +67,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   __shared__ float part_m[NW][16], part_l[NW][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const MxPart part = mx_part(a, a.tiles);
+  const MxPart part = mx_fixed_part(a);
   const int64_t kvrow = part.kvrow;
-  const int tile = part.tile, split = part.split;
+  const int tile = part.tile;
   const int b = (int)(part.kvrow / (uint32_t)a.Hkv), hk = (int)(part.kvrow - (uint32_t)b * a.Hkv);
   const MxRows n = mx_rows(a, kvrow, b);
   const int entries = mx_entries(a, n, tile * 16, 16);
-  const int e0 = split * a.chunk, e1 = e0 + a.chunk < entries ? e0 + a.chunk : entries;
-  if (split > 0 && e0 >= e1) return;                             // the merge does not look at it
+  const int e0 = part.e0, e1 = e0 + part.chunk < entries ? e0 + part.chunk : entries;
+  if (e0 > 0 && e0 >= e1) return;                                // the merge does not look at it
 
   const int r = tile * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
   const bool active = r < a.L * a.G, live = active && i < n.queries;
@@ -204,8 +204,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
       L += wgt * part_l[v][cr];
       o += reinterpret_cast<const f4*>(&vt[v][0])[cr * (D / 4) + (u ^ cr)] * wgt;
     }
-    if (a.splits > 1) {
-      const int64_t slot = ((kvrow * a.tiles + tile) * a.splits + split) * 16 + cr;
+    if (a.parted) {
+      const int64_t slot = (int64_t)part.part * 16 + cr;
       if (u == 0) { a.ws_m[slot] = M; a.ws_l[slot] = L; }
       *reinterpret_cast<f4*>(a.ws_acc + slot * D + 4 * u) = o;
     } else {
@@ -219,8 +219,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   }
 }
 
-// The splits of 256 / (D / 4 PARTS) query rows a workgroup: a thread takes 4 channels of every
-// PARTS-th split of its row. PARTS > 1, where a row has many splits, is one row a workgroup.
+// The parts of 256 / (D / 4 PARTS) query rows a workgroup: a thread takes 4 channels of every
+// PARTS-th part of its row. PARTS > 1, where a row has many parts, is one row a workgroup.
 template <int D, int PARTS>
 __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
   constexpr int UNITS = D / 4, ROWS = 256 / (UNITS * PARTS);
@@ -234,27 +234,35 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
   const int64_t kvrow = there ? at / rows : 0;
   const int r = there ? (int)(at - kvrow * rows) : 0;
   const int b = (int)(kvrow / a.Hkv), hk = (int)(kvrow - (int64_t)b * a.Hkv);
-  const int tile = r / 16, i = r / a.G, head = hk * a.G + (r - i * a.G);
+  const int tile = r / a.tile_rows, i = r / a.G, head = hk * a.G + (r - i * a.G);
   const MxRows n = mx_rows(a, kvrow, b);
-  const bool live = i < n.queries;
-  const int parts = live && there ? (mx_entries(a, n, tile * 16, 16) + a.chunk - 1) / a.chunk : 0;
-  const int64_t first = (kvrow * a.tiles + tile) * a.splits * 16 + (r & 15);
+  int2 mine = {0, 0};                                            // the row's first part, and how many
+  if (there && i < n.queries) {
+    const int64_t t = kvrow * a.tiles + tile;
+    const int entries = mx_entries(a, n, tile * a.tile_rows, a.tile_rows);
+    if (!a.shares) mine = int2{(int)(t * a.splits), (entries + a.chunk - 1) / a.chunk};
+    else if (entries > 0) mine = a.ws_parts[t];
+    // lengths that change between the kernels are the caller's mistake, but no read out of bounds
+    if (a.shares && ((uint32_t)mine.x > (uint32_t)a.shares || (uint32_t)mine.y > (uint32_t)(a.shares - mine.x))) mine = int2{0, 0};
+  }
+  const int parts = mine.y;
+  const int64_t step = a.tile_rows, first = (int64_t)mine.x * step + (r & (a.tile_rows - 1));
   float M = M_NONE;
   if constexpr (PARTS > 1) {
-    for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
+    for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ws_m[first + s * step]);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = M;
     __syncthreads();
     M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   } else {
-    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + (int64_t)s * 16]);
+    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + s * step]);
   }
   float L = 0.f;
   f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = part; s < parts; s += PARTS) {
-    const int64_t slot = first + (int64_t)s * 16;
+    const int64_t slot = first + s * step;
     const float wgt = __builtin_amdgcn_exp2f(a.ws_m[slot] - M);
     L += wgt * a.ws_l[slot];
     o += ld_nt(reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u)) * wgt;
@@ -275,11 +283,13 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
   store_out4(a, b * a.osb + i * a.ost + head * a.osh + 4 * u, out);
 }
 
-// Rows whose splits a thread walks alone, eight at most; more are shared by a workgroup.
+// Rows whose parts a thread walks alone, eight at most (with shares: on average); more are shared
+// by a workgroup.
 template <int D> void launch_mx_merge(const MxAttn& a, hipStream_t stream) {
   constexpr int UNITS = D / 4;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.L * a.G;
-  if (a.splits <= 8) {
+  const int parts = a.shares ? a.shares / (a.B * a.Hkv * a.tiles) : a.splits;
+  if (parts <= 8) {
     const int per = 256 / UNITS;
     hipLaunchKernelGGL((mx_merge_kernel<D, 1>), dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, stream, a);
   } else {
@@ -298,10 +308,10 @@ template <int D, bool QF32> void launch_rows(const MxAttn& a, hipStream_t stream
 
 hipError_t launch_mx_attention(const MxAttn& a, hipStream_t stream) {
   const bool f32 = a.q_dtype == IAK_DTYPE_F32;
-  if (a.chunk_rows) launch_mx_chunk(a, stream);
+  if (a.tile_rows > 16) launch_mx_chunk(a, stream);
   else if (a.D == 128) f32 ? launch_rows<128, true>(a, stream) : launch_rows<128, false>(a, stream);
   else f32 ? launch_rows<64, true>(a, stream) : launch_rows<64, false>(a, stream);
-  if (a.splits > 1) {
+  if (a.parted) {
     if (a.D == 128) launch_mx_merge<128>(a, stream);
     else launch_mx_merge<64>(a, stream);
   }

@@ -39,14 +39,15 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
   __shared__ u4 nan_in[2][2];                                    // a word a page: its tokens with a NaN block
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const MxPart part = mx_part(a, (a.L * a.G + BM - 1) / BM);
+  const MxPart part = a.shares ? mx_shared_part<4>(a) : mx_fixed_part(a);
+  if (part.idle) return;                                         // uniform, as below
   const int64_t kvrow = part.kvrow;
-  const int tile = part.tile, split = part.split;
+  const int tile = part.tile;
   const int b = (int)(part.kvrow / (uint32_t)a.Hkv), hk = (int)(part.kvrow - (uint32_t)b * a.Hkv);
   const MxRows n = mx_rows(a, kvrow, b);
   const int entries = mx_entries(a, n, tile * BM, BM);
-  const int e0 = split * a.chunk, e1 = e0 + a.chunk < entries ? e0 + a.chunk : entries;
-  if (split > 0 && e0 >= e1) return;                             // uniform; the merge does not look at it
+  const int e0 = part.e0, e1 = e0 + part.chunk < entries ? e0 + part.chunk : entries;
+  if (e0 > 0 && e0 >= e1) return;                                // the merge does not look at it
 
   const int rows = a.L * a.G;
   int seen[RT], least = 0x7FFFFFFF;
@@ -206,8 +207,8 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
     const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
     const float sum = l[t][0];
     if (r >= rows) continue;
-    if (a.splits > 1) {
-      const int64_t slot = ((kvrow * a.tiles + (r >> 4)) * a.splits + split) * 16 + c;
+    if (a.parted) {
+      const int64_t slot = (int64_t)part.part * BM + (w * RT + t) * 16 + c;
       if (g == 0) { a.ws_m[slot] = m[t]; a.ws_l[slot] = sum; }
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) *reinterpret_cast<f4*>(a.ws_acc + slot * D + 16 * mb + 4 * g) = acc[t][mb];
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
 template <int D, bool QF32> void launch_chunk(const MxAttn& a, hipStream_t stream) {
   const dim3 grid((uint32_t)a.items);
   if constexpr (!QF32) {
-    if (a.chunk_rows == 256) { hipLaunchKernelGGL((mx_chunk_kernel<D, false, 8>), grid, dim3(512), 0, stream, a); return; }
+    if (a.tile_rows == 256) { hipLaunchKernelGGL((mx_chunk_kernel<D, false, 8>), grid, dim3(512), 0, stream, a); return; }
   }
   hipLaunchKernelGGL((mx_chunk_kernel<D, QF32, 4>), grid, dim3(256), 0, stream, a);
 }

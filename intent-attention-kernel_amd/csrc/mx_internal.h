@@ -13,16 +13,20 @@ namespace iak {
 // Sets the calling thread's iak_last_error() text and returns `st`.
 iak_status report(iak_status st, const char* text);
 
+constexpr int MX_SHARED_TILES = 512;   // most tiles that are shared out
+
 // Kernel-side arguments of the 4-bit cache's attention (built from iak_mx_attention_args).
 struct MxAttn {
   int B, L, Hq, Hkv, G, D, W;
   int64_t NP;
-  int tiles;      // tiles of 16 query rows (query token * G + head of the group) per KV row
+  int tile_rows;  // query rows (query token * G + head of the group) of a workgroup: 16: the rows
+                  // kernel; 128 or 256 (16-bit queries): the chunk kernel
+  int tiles;      // such tiles per KV row
   int splits;     // parts of `chunk` table entries per tile
   int chunk;
-  int waves;      // 4 per workgroup, or more (16): as many as the kernel has
-  int chunk_rows; // 128 or 256 (16-bit queries): the chunk kernel with tiles of that many rows; 0: the rows kernel
-  int64_t items;  // workgroups: B * Hkv * splits * tiles (of 16 or of chunk_rows rows)
+  int shares;     // 0, or so many workgroups share out the tiles' entries evenly (mx_shared_part)
+  int waves;      // rows kernel: 4 per workgroup, or more (16): as many as it has
+  int64_t items;  // workgroups
 
   const void* q; int q_dtype; int64_t qsb, qst, qsh;
   void* out; int out_dtype; int64_t osb, ost, osh;
@@ -33,9 +37,11 @@ struct MxAttn {
   float score_mult;        // sm_scale * log2(e)
   int causal;
 
-  float* ws_m;             // [B, Hkv, tiles, splits, 16]
-  float* ws_l;
-  float* ws_acc;           // [B, Hkv, tiles, splits, 16, D]
+  bool parted;             // the tiles' parts meet in the workspace
+  float* ws_m;             // [parts, tile_rows]: tile t's part s is t * splits + s, or with shares
+  float* ws_l;             //   ws_parts[t].x + s of ws_parts[t].y
+  float* ws_acc;           // [parts, tile_rows, D]
+  int2* ws_parts;          // [B, Hkv, tiles], with shares
 };
 
 hipError_t launch_mx_append(const iak_mx_tokens_args& a, hipStream_t stream);

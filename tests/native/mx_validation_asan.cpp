@@ -70,11 +70,12 @@ void attention(int n) {
     a.sm_scale = 0.1f;
     const iak_status st = iak_mx_attention_workspace(&a, &bytes);
     count(st);
-    // per split, of two table entries at least, a maximum, a sum and head_dim values for each of
-    // the rows, in tiles of 16
-    const double slots = 16.0 * a.batch * a.num_kv_heads * ((a.q_len * (a.num_q_heads / a.num_kv_heads) + 15) / 16);
-    const double one = slots * 4 * (2 + a.head_dim);
-    if (st != IAK_OK || (bytes != 0 && (bytes < 2 * one || bytes > (a.table_width / 2 + 1) * one + 1024)) || (a.splits == 1 && bytes != 0)) {
+    // per part of two table entries at least a maximum, a sum and head_dim values for each of the
+    // rows, in tiles of 16 to 256; more parts than tiles
+    const int rows = a.q_len * (a.num_q_heads / a.num_kv_heads);
+    const double value = 4.0 * (2 + a.head_dim) * a.batch * a.num_kv_heads;
+    const double least = value * 16 * ((rows + 15) / 16), most = value * 256 * ((rows + 255) / 256) * (a.table_width / 2 + 1);
+    if (st != IAK_OK || (bytes != 0 && (bytes < least || bytes > most + 8192)) || (a.splits == 1 && bytes != 0)) {
       std::printf("mx-asan: workspace of %zu bytes for a well-formed call (B=%d L=%d Hq=%d Hkv=%d W=%d splits=%d)\n", bytes,
                   a.batch, a.q_len, a.num_q_heads, a.num_kv_heads, a.table_width, a.splits);
       std::exit(1);

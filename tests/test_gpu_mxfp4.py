@@ -425,12 +425,51 @@ def test_attention_of_prompts(B, L, Hq, Hkv, D, W, dtype, causal, splits):
     assert (got[-1, lens[-1]:] == 0).all()
 
 
+# Several prompts whose tiles of rows are shared out over the card by their lengths.
+SHARED = [
+    # L, Hq, Hkv, D, W, valid tokens (a sequence each), q_lens, dtype, causal
+    (700, 8, 2, 128, 200, [3190, 700, 33], None, "float16", True),
+    (700, 8, 2, 128, 200, [3190, 1, 40], [700, 0, 33], "bfloat16", True),
+    (700, 8, 2, 64, 250, [5, 3999, 2000], [3, 650, 699], "float16", True),
+    (700, 8, 2, 64, 250, [4000, 0, 0], [1, 0, 700], "bfloat16", False),
+    (700, 8, 2, 128, 200, [100, 3200, 1600], [100, 555, 700], "float32", True),
+    (700, 8, 2, 64, 250, [4000, 4000, 16], [700, 700, 1], "float32", True),
+    (700, 8, 2, 128, 200, [0, 0, 0], None, "float16", True),
+    (509, 16, 4, 128, 250, [4000, 1500, 2000, 20, 3999], [509, 400, 509, 10, 1], "float16", True),      # two rounds
+    (129, 24, 1, 64, 400, [6400, 300, 17, 0, 6000, 1], [129, 128, 1, 5, 60, 0], "float16", True),
+]
+
+
+@pytest.mark.parametrize("L,Hq,Hkv,D,W,tokens,q_lens,dtype,causal", SHARED)
+def test_attention_of_unequal_prompts(L, Hq, Hkv, D, W, tokens, q_lens, dtype, causal):
+    import intent_attention as ia
+    rng = np.random.default_rng(L + W + D)
+    B = len(tokens)
+    NP = B * Hkv * W + 3
+    host, pools = _pools(rng, NP, D)
+    table = _table(rng, B, Hkv, W, NP)
+    table[0, 0, W // 3] = -1
+    valid = np.array(tokens, np.int32)[:, None].repeat(Hkv, 1)
+    valid[:, -1] = np.maximum(0, valid[:, -1] - 21)                        # heads differ too
+    q = (2 * rng.standard_normal((B, L, Hq, D))).astype(np.float32)
+    q[0, 0, 0, 0] = np.nan
+    lens = None if q_lens is None else np.array(q_lens, np.int32)
+    queries = sorted({0, 1, L // 2, L - 2, L - 1} | {n + k for n in (q_lens or []) for k in (-1, 0) if 0 <= n + k < L}
+                     | {int(i) for i in rng.integers(0, L, 8)})
+    tq = _t(q).to(getattr(__import__("torch"), dtype))
+    plan = ia.make_mxfp4_plan(tq, pools, _t(table), _t(valid), causal=causal)
+    tiles = B * Hkv * -(-L * Hq // Hkv // (128 if dtype == "float32" else 256))
+    rows = 65536 * (2 if tiles > 132 else 1)                               # of the rounds that are shared out
+    assert plan.workspace_bytes == 2 * 4 * rows + 4 * rows * D + -(-8 * tiles // 256) * 256, "not the shared form"
+    _check(tq, dtype, host, pools, table, valid, lens, causal, queries=queries)
+
+
 def test_attention_of_prompts_replays():
     """A captured prompt, replayed with other data and lengths between eager work: the eager results, bit for bit."""
     import torch
     import intent_attention as ia
     rng = np.random.default_rng(12)
-    for B, L, Hq, Hkv, D, W, splits in ((2, 140, 8, 2, 128, 14, 16), (2, 1100, 16, 2, 64, 70, 0)):
+    for B, L, Hq, Hkv, D, W, splits in ((2, 140, 8, 2, 128, 14, 16), (2, 1100, 16, 2, 64, 70, 0), (3, 700, 8, 2, 128, 200, 0)):
         _, pools = _pools(rng, B * Hkv * W, D)
         table, valid = _t(_table(rng, B, Hkv, W, B * Hkv * W)), _t(np.full((B, Hkv), W * 16, np.int32))
         q = torch.randn((B, L, Hq, D), device=_dev()).half()
