@@ -131,6 +131,14 @@ MxChoice choose(int B, int Hkv, int64_t rows, int W, int D, bool f32, int64_t fo
   kernel(16, big ? 3 : 4, 3, rows_entry < bytes_entry ? bytes_entry : rows_entry);
   if (rows > 16) kernel(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50));
   if (rows > 128 && !f32) kernel(256, 1, big ? 7 : 5, big ? 0.50 : 0.345);
+  // Long rows of several sequences (parts above 2,048 tokens), at most a third of a round: shared out
+  // too, whatever the cost says, for it knows the longest row alone. 32 sequences x 8 KV heads of up to
+  // 32,768 tokens, head_dim 128: equal 192 us for 182 (eight waves a tile, unsplit), a third to all of it
+  // 136 for 158, one long among short ones 28 for 141; 64 of up to 16,384, more than a third: 222 for
+  // 200, 161 for 154.
+  const double work = kvrows * (double)((rows + 15) / 16), round = CUS * (big ? 3 : 4);
+  if (best.tile_rows == 16 && B > 1 && forced == 0 && W / best.splits > 128 && 3 * work <= round && work * W < 2e9)
+    best = {16, 1, (int)round};
   return best;
 }
 
@@ -171,7 +179,7 @@ iak_status validate_mx_attention(const iak_mx_attention_args* a, MxPlan* p) {
   while (splits > 1 && tiles * splits * p->tile_rows > 1.6e7) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
-  p->waves = p->splits == 1 && tiles <= CUS ? 16 : 4;
+  p->waves = p->splits == 1 && !p->shares && tiles <= CUS ? 16 : 4;
   p->items = p->shares ? p->shares : (int64_t)tiles * p->splits;
   if (p->splits > 1 || p->shares) {
     const size_t rows_kept = (size_t)p->items * p->tile_rows;

@@ -78,26 +78,32 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 
 // Lengths are known on the device alone: every wave works out for itself the least chunk with
-// which all tiles' chunks are no more than a.shares, and which of them is its workgroup's. Each XCD
-// takes a run of them. `UNIT`: entries that a workgroup takes at a step.
+// which all tiles' chunks are no more than a.shares, and which of them is its workgroup's; RUNS:
+// each XCD takes a run of them. `UNIT`: entries that a workgroup takes at a step.
 // 16 heads over 4 of 128: 512, 16, 16 and 16 queries over 8,000, 500, 500 and 500 tokens 63 us, and
 // 144 in fixed parts; 8 heads over one, 3 sequences of up to 1,000 queries over up to 8,000 tokens 95
-// and 132, of equal lengths 140 and 134. Decode rows lose what the working out takes: 19.7 and 18.4
-// us, 192 and 178. With head_dim 64 one round only: 5 x 509 queries over 4,000 in two 66, fixed 59.
-template <int UNIT> __device__ __forceinline__ MxPart mx_shared_part(const MxAttn& a) {
+// and 132, of equal lengths 140 and 134. With head_dim 64 one round
+// only: 5 x 509 queries over 4,000 in two 66, fixed 59. Short decode rows lose what the working out
+// takes (13 of up to 8,191 tokens: 19.7 us and 18.4).
+template <int UNIT, bool RUNS> __device__ __forceinline__ MxPart mx_shared_part(const MxAttn& a) {
   constexpr int MOST = MX_SHARED_TILES / 64;
   const int lane = threadIdx.x & 63;
   const int all = a.B * a.Hkv * a.tiles, per = (all + 63) >> 6;    // tiles, and of a lane: a run
   int units[MOST], own = 0;
+  uint32_t kv = (uint32_t)(lane * per) / (uint32_t)a.tiles, b = kv / (uint32_t)a.Hkv;   // of the lane's tile, counted up from here
+  int tile = lane * per - (int)kv * a.tiles, hk = (int)(kv - b * (uint32_t)a.Hkv);
 #pragma unroll
   for (int j = 0; j < MOST; ++j) {
     units[j] = 0;
-    const int t = lane * per + j;
-    if (j < per && t < all) {
-      const int kvrow = t / a.tiles, tile = t - kvrow * a.tiles, b = kvrow / a.Hkv;
-      const MxRows n = mx_rows(a, kvrow, b);
+    if (j < per && lane * per + j < all) {
+      const MxRows n = mx_rows(a, kv, (int)b);
       units[j] = (mx_entries(a, n, tile * a.tile_rows, a.tile_rows) + UNIT - 1) / UNIT;
       own += units[j];
+      if (++tile == a.tiles) {
+        tile = 0;
+        ++kv;
+        if (++hk == a.Hkv) { hk = 0; ++b; }
+      }
     }
   }
   const int total = __builtin_amdgcn_readlane(wave_scan(own), 63);
@@ -111,15 +117,21 @@ template <int UNIT> __device__ __forceinline__ MxPart mx_shared_part(const MxAtt
   // total / shares chunks are too few and total / (shares - tiles) enough
   int size = (total + a.shares - 1) / a.shares, enough = (total + a.shares - all - 1) / (a.shares - all);
   size = size < 1 ? 1 : size;
-  while (size < enough) {
-    const int mid = (size + enough) >> 1;
-    if (__builtin_amdgcn_readlane(wave_scan(count(mid)), 63) <= a.shares) enough = mid;
-    else size = mid + 1;
+  int mine = count(size), upto = wave_scan(mine), parts = __builtin_amdgcn_readlane(upto, 63);
+  if (parts > a.shares) {                                          // rows of one length are done here
+    ++size;
+    while (size < enough) {
+      const int mid = (size + enough) >> 1;
+      if (__builtin_amdgcn_readlane(wave_scan(count(mid)), 63) <= a.shares) enough = mid;
+      else size = mid + 1;
+    }
+    mine = count(size);
+    upto = wave_scan(mine);
+    parts = __builtin_amdgcn_readlane(upto, 63);
   }
-  const int mine = count(size), upto = wave_scan(mine), parts = __builtin_amdgcn_readlane(upto, 63);
-  const int run = (parts + 7) >> 3, part = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+  const int run = (parts + 7) >> 3, part = RUNS ? (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
   MxPart p;
-  p.idle = (int)(blockIdx.x >> 3) >= run || part >= parts;
+  p.idle = (RUNS && (int)(blockIdx.x >> 3) >= run) || part >= parts;
   if (p.idle) return p;
   const uint64_t has = __builtin_amdgcn_ballot_w64(part < upto);
   const int owner = __builtin_ctzll(has);                          // the first lane whose run ends behind it

@@ -67,7 +67,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   __shared__ float part_m[NW][16], part_l[NW][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const MxPart part = mx_fixed_part(a);
+  const MxPart part = NW == 4 && a.shares ? mx_shared_part<2 * NW, false>(a) : mx_fixed_part(a);
+  if (part.idle) return;                                         // uniform, as below
   const int64_t kvrow = part.kvrow;
   const int tile = part.tile;
   const int b = (int)(part.kvrow / (uint32_t)a.Hkv), hk = (int)(part.kvrow - (uint32_t)b * a.Hkv);
@@ -165,11 +166,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && !QF32 ? 3 : 2) void mx_rows_ker
   };
 
   // Twelve waves a CU are what hides the loads: a ring of two or more pairs cost registers and was
-  // slower, as were sixteen waves of fewer registers. 256 rows of 32,768 tokens (1.14 GB) take 181 us
-  // (6.3 TB/s; 183 in three splits); loads that stay in the caches took 216 where these took 190.
-  // Short rows wait: launch, length and table, pages, LDS and store in turn are 5.5 us, and a merge
-  // kernel 4 more: 52 rows of 5,750 tokens (39 MB) take 14 + 4 us. Chunks of equal size over all
-  // rows, from the lengths on the device, were no faster (19.7, and 192 for the long rows).
+  // slower, as were sixteen waves of fewer registers. 256 rows of 32,768 tokens (1.14 GB) take 188 us
+  // in three parts each (6.1 TB/s; 192 shared out, 182 unsplit in eight waves a tile); loads that stay
+  // in the caches took 216 where these took 190. Short rows wait: launch, length and table, pages, LDS
+  // and store in turn are 5.5 us, and a merge kernel 4 more: 52 rows of 5,750 tokens (39 MB) take 14 + 4
+  // us. Loads that wait for no other issued first (table, query, length) changed nothing.
   MxPair<D> x;
   if (e0 + 2 * w < e1) load_pair<D>(x, a, page(0), page(1), c, g);
   for (int at = e0 + 2 * w, k = 0, block = 0; at < e1; at += 2 * NW) {
@@ -256,6 +257,7 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
     __syncthreads();
     M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   } else {
+#pragma unroll 8
     for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + s * step]);
   }
   float L = 0.f;
@@ -283,13 +285,13 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
   store_out4(a, b * a.osb + i * a.ost + head * a.osh + 4 * u, out);
 }
 
-// Rows whose parts a thread walks alone, eight at most (with shares: on average); more are shared
-// by a workgroup.
+// Rows whose parts a thread walks alone, eight at most; more are shared by a workgroup. With shares,
+// where a few rows may have most parts: below 4,096 rows by a workgroup (8 rows of 32,768 tokens among
+// 248 of 819: 29 us and 45; 4 x 256 queries x 16 heads, one sequence of 16,000 tokens: 69 and 50).
 template <int D> void launch_mx_merge(const MxAttn& a, hipStream_t stream) {
   constexpr int UNITS = D / 4;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.L * a.G;
-  const int parts = a.shares ? a.shares / (a.B * a.Hkv * a.tiles) : a.splits;
-  if (parts <= 8) {
+  if (a.shares ? rows >= 4096 : a.splits <= 8) {
     const int per = 256 / UNITS;
     hipLaunchKernelGGL((mx_merge_kernel<D, 1>), dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, stream, a);
   } else {

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mx_chunk_kernel(const MxAttn a) {
   __shared__ u4 nan_in[2][2];                                    // a word a page: its tokens with a NaN block
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const MxPart part = a.shares ? mx_shared_part<4>(a) : mx_fixed_part(a);
+  const MxPart part = a.shares ? mx_shared_part<4, true>(a) : mx_fixed_part(a);
   if (part.idle) return;                                         // uniform, as below
   const int64_t kvrow = part.kvrow;
   const int tile = part.tile;

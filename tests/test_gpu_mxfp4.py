@@ -464,6 +464,31 @@ def test_attention_of_unequal_prompts(L, Hq, Hkv, D, W, tokens, q_lens, dtype, c
     _check(tq, dtype, host, pools, table, valid, lens, causal, queries=queries)
 
 
+@pytest.mark.parametrize("B,L,G,Hkv,D,W,dtype", [(32, 1, 4, 2, 128, 2048, "float16"), (48, 3, 5, 2, 64, 2500, "bfloat16"),
+                                                 (64, 1, 8, 1, 128, 2048, "float32"), (85, 2, 2, 1, 64, 2048, "float32")])
+def test_attention_of_one_long_row_among_short_ones(B, L, G, Hkv, D, W, dtype):
+    """Decode rows that are shared out by their lengths: one fills its table, some are empty."""
+    import torch
+    import intent_attention as ia
+    rng = np.random.default_rng(B)
+    NP, round_ = 600, 768 if D == 128 else 1024
+    host, pools = _pools(rng, NP, D)
+    table = rng.integers(0, NP, (B, Hkv, W)).astype(np.int32)              # pages many times over
+    table[1, 0, 1000] = NP
+    valid = rng.integers(0, 90, (B, Hkv)).astype(np.int32)
+    valid[1, 0], valid[2], valid[3] = W * 16 - 7, 0, 1
+    q = (2 * rng.standard_normal((B, L, G * Hkv, D))).astype(np.float32)
+    q[5, 0, 0, 3] = np.inf
+    lens = None if L == 1 else rng.integers(0, L + 1, B).astype(np.int32)
+    if L > 1:
+        lens[1] = L
+    tq = _t(q).to(getattr(torch, dtype))
+    plan = ia.make_mxfp4_plan(tq, pools, _t(table), _t(valid))
+    rows, tiles = round_ * 16, B * Hkv * -(-L * G // 16)
+    assert plan.workspace_bytes == 2 * 4 * rows + 4 * rows * D + -(-8 * tiles // 256) * 256, "not the shared form"
+    _check(tq, dtype, host, pools, table, valid, lens)
+
+
 def test_attention_of_prompts_replays():
     """A captured prompt, replayed with other data and lengths between eager work: the eager results, bit for bit."""
     import torch
