@@ -25,6 +25,7 @@ that has tokens or is itself a parent).
 """
 from __future__ import annotations
 
+import struct
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -38,12 +39,15 @@ Pools = Union[PagePools, LatentPools, MxFp4Pools, torch.Tensor, Sequence[torch.T
 Indices = Union[torch.Tensor, Sequence[int]]
 
 
+_entry = struct.Struct("Pq")           # iak_page_array
+
+
 def _pool_tensors(pools: Optional[Pools]) -> List[torch.Tensor]:
     """The tensors of the pools, each once (K and V may be one pool)."""
     if pools is None:
         return []
     if isinstance(pools, (PagePools, LatentPools, MxFp4Pools)):
-        ts: Iterable = (t for t in vars(pools).values() if isinstance(t, torch.Tensor))
+        ts: Iterable = [t for t in vars(pools).values() if isinstance(t, torch.Tensor)]
     else:
         ts = (pools,) if isinstance(pools, torch.Tensor) else pools
     return list({(t.data_ptr(), t.numel() * t.element_size()): t for t in ts}.values())
@@ -52,7 +56,7 @@ def _pool_tensors(pools: Optional[Pools]) -> List[torch.Tensor]:
 def _fill_arrays(a, tensors: List[torch.Tensor], NP: int) -> None:
     if len(tensors) > N.MAX_PAGE_ARRAYS:
         raise ValueError(f"at most {N.MAX_PAGE_ARRAYS} pool tensors, got {len(tensors)}")
-    n = 0
+    n, offset = 0, type(a).arrays.offset
     for t in tensors:
         size = t.numel()
         if NP == 0 and size == 0:
@@ -61,7 +65,7 @@ def _fill_arrays(a, tensors: List[torch.Tensor], NP: int) -> None:
             raise ValueError(f"every pool tensor must be contiguous with a row for each of {NP} pages, "
                              f"got {tuple(t.shape)}")
         if size:
-            a.arrays[n] = (t.data_ptr(), size // NP * t.element_size())
+            _entry.pack_into(a, offset + n * _entry.size, t.data_ptr(), size // NP * t.element_size())
             n += 1
     a.num_arrays = n
 
