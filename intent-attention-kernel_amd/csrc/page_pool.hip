@@ -5,11 +5,10 @@
 // 1,024 pages, then a rank within them), rows by their place in the call, and rank meets
 // rank. Reference counts change by integer atomics, whose order leaves no trace.
 //
-//   grow, fork   seq_plan_kernel   free pages per 1,024 ids; one workgroup checks the call and
-//                                  sums what its rows need
-//                seq_rank_kernel   the free ids in order, as many as are needed; the verdict
-//                (seq_small_kernel for both, where the pages are few)
-//                seq_apply_kernel  a workgroup per row: entries, counts, the copied last page
+//   grow, fork   seq_plan_kernel   a bit a page: free, and their number per 1,024 ids; one
+//                                  workgroup checks the call and sums what its rows need
+//                seq_apply_kernel  a workgroup per row: the verdict, the row's free pages out of the
+//                                  bits, entries, counts, the copied last page
 //   free         seq_free_kernel   a workgroup per row
 //   compact      compact_count_kernel, compact_rank_kernel (which page goes where; for few pages
 //                compact_small_kernel), compact_apply_kernel (pages copied, table, counts and
@@ -32,10 +31,12 @@ namespace {
 constexpr int PAGE_GROUP = 1024;       // page ids a workgroup counts or ranks
 constexpr int POOL_THREADS = 256;
 constexpr int PLAN_THREADS = 1024;
-// Up to so many pages one workgroup plans and ranks, which saves a launch: free and fork of 6
-// sequences among 3,072 pages 27 us for 30 (19 for 22 replayed from a graph), at 18,944 23 for 22
-// replayed; a compaction of 4,266 pages 22 for 24 (14 for 18), of 17,066 24 for 24 (28 for 22).
-constexpr int64_t FEW_SEQUENCE_PAGES = 16384, FEW_COMPACT_PAGES = 8192;
+// Up to so many pages one workgroup counts and ranks for a compaction, which saves a launch: of 4,266
+// pages 22 us for 24 (14 for 18 replayed from a graph), of 17,066 24 for 24 (28 for 22).
+constexpr int64_t FEW_COMPACT_PAGES = 8192;
+// Pages of larger pools are moved past the caches: 1.4 GB of them 139 us for 150; of 175 MB, which the
+// caches hold, 33 us for 26.
+constexpr double STREAM_BYTES = 512.0 * 1024 * 1024;
 
 struct PageArrays {
   int n;
@@ -143,7 +144,7 @@ struct SeqArgs {
   int32_t* group_free;                 // [groups] free pages
   int32_t* marks;                      // [num_seqs] 1: listed in seqs
   int32_t* first;                      // [count * R] pages of the rows before
-  int32_t* list;                       // [NP] free ids in order
+  uint64_t* free_bits;                 // [groups, 16] bit i of word j: page 64 j + i of the group is free
   PageArrays arrays;
 };
 
@@ -231,9 +232,14 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
 }
 
 template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
+  static_assert(PLAN_THREADS == PAGE_GROUP, "a thread a page");
   if ((int)blockIdx.x < a.groups) {
+    const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + threadIdx.x;
+    const bool free_page = id < a.NP && a.refs[id] <= 0;
+    const uint64_t bits = __builtin_amdgcn_ballot_w64(free_page);
+    if ((threadIdx.x & 63) == 0) a.free_bits[id >> 6] = bits;
     int total;
-    scan_before<PLAN_THREADS / 64>(count_free(a.refs, a.NP, blockIdx.x), total);
+    scan_before<PLAN_THREADS / 64>(free_page, total);
     if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
     return;
   }
@@ -242,52 +248,60 @@ template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_ker
   if (threadIdx.x == 0) { a.head[0] = need; a.head[1] = refused; }
 }
 
-// Plan and rank in one workgroup, for pools of few pages: a thread ranks the free pages of a run.
-template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_small_kernel(const SeqArgs a) {
-  __shared__ int refused;
-  const PageRun run = page_run(a.NP);
-  int all, rank = scan_before<PLAN_THREADS / 64>(run_free(a.refs, run), all);
-  const int need = plan_call<KIND>(a, refused);
-  if (threadIdx.x == 0) a.missing[0] = refused ? -1 : (need > all ? need - all : 0);
-  for (int id = run.begin; id < run.end && rank < need; ++id)
-    if (a.refs[id] <= 0) a.list[rank++] = id;
-}
-
-__global__ __launch_bounds__(POOL_THREADS) void seq_rank_kernel(const SeqArgs a) {
-  constexpr int WAVES = POOL_THREADS / 64;
-  int before, all;
-  sum_groups<WAVES>(a.group_free, blockIdx.x, a.groups, before, all);
-  const int need = a.head[0];
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.missing[0] = a.head[1] ? -1 : (need > all ? need - all : 0);
-  if (before >= need) return;                                    // uniform
-  for (int k0 = 0; k0 < PAGE_GROUP; k0 += POOL_THREADS) {
-    const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + k0 + threadIdx.x;
-    const bool free_page = id < a.NP && a.refs[id] <= 0;
-    int total;
-    const int rank = before + scan_before<WAVES>(free_page, total);
-    if (free_page) a.list[rank] = (int)id;
-    before += total;
+// The free pages numbered first .. first + n - 1 in order of id, of which there are so many:
+// take(number - first, id). By the workgroup, a word of 64 pages a thread at a time; `before`,
+// `own`: free pages before and of the thread's run of `per` groups.
+template <typename F>
+__device__ __forceinline__ void take_pages(const SeqArgs& a, int per, int before, int own, int first, int n, F&& take) {
+  __shared__ int start_group, start_before;
+  if (before <= first && first < before + own) {                 // one thread
+    int g = (int)threadIdx.x * per;
+    for (int in = a.group_free[g]; before + in <= first; in = a.group_free[g]) { before += in; ++g; }
+    start_group = g;
+    start_before = before;
+  }
+  __syncthreads();
+  const int64_t words = (int64_t)a.groups * (PAGE_GROUP / 64);
+  int64_t at = (int64_t)start_group * (PAGE_GROUP / 64);
+  int base = start_before;
+  for (; base < first + n && at < words; at += POOL_THREADS) {   // uniform
+    const int64_t word = at + threadIdx.x;
+    uint64_t bits = word < words ? a.free_bits[word] : 0;
+    int total, number = base + scan_before<POOL_THREADS / 64>(__builtin_popcountll(bits), total);
+    for (; bits != 0 && number < first + n; bits &= bits - 1, ++number)
+      if (number >= first) take(number - first, (int)(word * 64 + __builtin_ctzll(bits)));
+    base += total;
   }
 }
 
 template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_kernel(const SeqArgs a) {
-  if (a.missing[0] != 0) return;
+  // loads that wait for no other first; what they name is looked at where the verdict is that it is sound
   const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
-  const int64_t row = (int64_t)a.seqs[j] * a.R + h;
+  const bool listed = a.count > 0;
+  const int need = a.head[0], refused = a.head[1], seq = listed ? a.seqs[j] : 0, first = listed ? a.first[k] : 0;
+  const int other = listed ? (KIND == SEQ_GROW ? a.new_tokens : a.parents)[j] : 0;
+  const int per = (a.groups + POOL_THREADS - 1) / POOL_THREADS;
+  int own = 0, all;
+  for (int i = 0, g = (int)threadIdx.x * per; i < per && g < a.groups; ++i, ++g) own += a.group_free[g];
+  const int before = scan_before<POOL_THREADS / 64>(own, all);
+  const int verdict = refused ? -1 : (need > all ? need - all : 0);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.missing[0] = verdict;
+  if (verdict != 0 || !listed) return;
+  const int64_t row = (int64_t)seq * a.R + h;
   int32_t* entries = a.table + row * a.W;
-  const int first = a.first[k];
   if constexpr (KIND == SEQ_GROW) {
-    const int old = a.valid[row] < 0 ? 0 : a.valid[row], tokens = old + a.new_tokens[j];
+    const int old = a.valid[row] < 0 ? 0 : a.valid[row], tokens = old + other;
     const int have = used_entries(old, a.PSZ, a.W), want = used_entries(tokens, a.PSZ, a.W);
-    for (int e = have + threadIdx.x; e < want; e += POOL_THREADS) {
-      const int id = a.list[first + e - have];
-      entries[e] = id;
-      a.refs[id] = 1;
-    }
+    if (want > have)
+      take_pages(a, per, before, own, first, want - have, [&](int e, int id) {
+        entries[have + e] = id;
+        a.refs[id] = 1;
+      });
     __syncthreads();                                             // every thread has read the old length
     if (threadIdx.x == 0) a.valid[row] = tokens;
   } else {
-    const int64_t parent = (int64_t)a.parents[j] * a.R + h;
+    __shared__ int fresh;
+    const int64_t parent = (int64_t)other * a.R + h;
     const int32_t* from = a.table + parent * a.W;
     int n;
     int64_t last;
@@ -299,9 +313,10 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
       if (id >= 0 && id < a.NP) atomicAdd(&a.refs[id], 1);
     }
     if (own_page) {
-      const int id = a.list[first];
-      if (threadIdx.x == 0) { entries[n - 1] = id; a.refs[id] = 1; }
-      copy_page<false>(a.arrays, last, id);
+      take_pages(a, per, before, own, first, 1, [&](int, int id) { fresh = id; });
+      __syncthreads();
+      if (threadIdx.x == 0) { entries[n - 1] = fresh; a.refs[fresh] = 1; }
+      copy_page<false>(a.arrays, last, fresh);
     }
     if (threadIdx.x == 0) a.valid[row] = a.valid[parent];
   }
@@ -357,6 +372,7 @@ struct CompactArgs {
   int32_t* hole;         // [NP / 2 + 1] where move j goes
   int32_t* mover;        // [NP / 2 + 1] what move j moves
   int move_groups;       // workgroups that copy pages
+  bool stream;           // past the caches
   PageArrays arrays;
 };
 
@@ -424,7 +440,10 @@ __global__ __launch_bounds__(POOL_THREADS) void compact_apply_kernel(const Compa
   const int L = a.head[0];
   if ((int)blockIdx.x < a.move_groups) {
     const int moves = a.head[1];
-    for (int j = blockIdx.x; j < moves; j += a.move_groups) copy_page<true>(a.arrays, a.mover[j], a.hole[j]);
+    for (int j = blockIdx.x; j < moves; j += a.move_groups) {
+      if (a.stream) copy_page<true>(a.arrays, a.mover[j], a.hole[j]);
+      else copy_page<false>(a.arrays, a.mover[j], a.hole[j]);
+    }
     return;
   }
   const int64_t step = (int64_t)(gridDim.x - a.move_groups) * POOL_THREADS;
@@ -463,21 +482,16 @@ SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
     s.group_free = take((size_t)s.groups);
     s.marks = take((size_t)s.num_seqs);
     s.first = take((size_t)a.count * a.rows_per_seq);
-    s.list = take((size_t)a.num_pages);
+    s.free_bits = reinterpret_cast<uint64_t*>(take((size_t)s.groups * (PAGE_GROUP / 32)));
   }
   return s;
 }
 
 template <int KIND> hipError_t launch_seq(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
   const SeqArgs s = seq_args(a, workspace);
-  if (a.num_pages <= FEW_SEQUENCE_PAGES) {
-    hipLaunchKernelGGL(seq_small_kernel<KIND>, dim3(1), dim3(PLAN_THREADS), 0, stream, s);
-  } else {
-    hipLaunchKernelGGL(seq_plan_kernel<KIND>, dim3(s.groups + 1), dim3(PLAN_THREADS), 0, stream, s);
-    hipLaunchKernelGGL(seq_rank_kernel, dim3(s.groups), dim3(POOL_THREADS), 0, stream, s);
-  }
-  if (a.count > 0)
-    hipLaunchKernelGGL(seq_apply_kernel<KIND>, dim3(a.count * a.rows_per_seq), dim3(POOL_THREADS), 0, stream, s);
+  const int rows = a.count * a.rows_per_seq;
+  hipLaunchKernelGGL(seq_plan_kernel<KIND>, dim3(s.groups + 1), dim3(PLAN_THREADS), 0, stream, s);
+  hipLaunchKernelGGL(seq_apply_kernel<KIND>, dim3(rows > 0 ? rows : 1), dim3(POOL_THREADS), 0, stream, s);
   return hipGetLastError();
 }
 
@@ -495,7 +509,7 @@ hipError_t launch_copy_pages(const iak_copy_pages_args& a, hipStream_t stream) {
 size_t sequences_workspace(const iak_sequences_args& a) {
   const size_t groups = (size_t)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
   return up256(8) + up256(4 * groups) + up256(4 * (size_t)a.num_seqs) + up256(4 * (size_t)a.count * a.rows_per_seq) +
-         up256(4 * (size_t)a.num_pages);
+         up256(groups * (PAGE_GROUP / 8));
 }
 
 hipError_t launch_free_sequences(const iak_sequences_args& a, hipStream_t stream) {
@@ -522,7 +536,12 @@ hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace
   c.out_table = a.out_table; c.out_refs = a.out_refs; c.page_map = a.page_map;
   c.groups = (int)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
   c.arrays.n = a.num_arrays;
-  for (int k = 0; k < a.num_arrays; ++k) c.arrays.a[k] = a.arrays[k];
+  int64_t pool = 0;
+  for (int k = 0; k < a.num_arrays; ++k) {
+    c.arrays.a[k] = a.arrays[k];
+    pool += a.arrays[k].row_bytes;
+  }
+  c.stream = (double)pool * a.num_pages > STREAM_BYTES;
   const size_t np = (size_t)a.num_pages;
   char* p = reinterpret_cast<char*>(workspace);
   auto take = [&](size_t ints) { int32_t* r = reinterpret_cast<int32_t*>(p); p += up256(4 * ints); return r; };
