@@ -257,17 +257,34 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const MxAttn a) {
     __syncthreads();
     M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   } else {
-#pragma unroll 8
-    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ws_m[first + s * step]);
+    for (int s0 = 0; s0 < parts; s0 += 8) {                      // loads of a batch all under way at once
+      float top8[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top8[k] = s0 + k < parts ? a.ws_m[first + (s0 + k) * step] : M_NONE;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) M = fmaxf(M, top8[k]);
+    }
   }
   float L = 0.f;
   f4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = part; s < parts; s += PARTS) {
-    const int64_t slot = first + s * step;
-    const float wgt = __builtin_amdgcn_exp2f(a.ws_m[slot] - M);
-    L += wgt * a.ws_l[slot];
-    o += ld_nt(reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u)) * wgt;
+  for (int s0 = part; s0 < parts; s0 += 4 * PARTS) {
+    float m4[4], l4[4];
+    f4 o4[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + k * PARTS;
+      const int64_t slot = first + (s < parts ? s : part) * step;
+      m4[k] = s < parts ? a.ws_m[slot] : -__builtin_inff();
+      l4[k] = a.ws_l[slot];
+      o4[k] = ld_nt(reinterpret_cast<const f4*>(a.ws_acc + slot * D + 4 * u));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (s0 + k * PARTS >= parts) break;
+      const float wgt = __builtin_amdgcn_exp2f(m4[k] - M);
+      L += wgt * l4[k];
+      o += o4[k] * wgt;
+    }
   }
   if constexpr (PARTS > 1) {
     sum[part][u] = o;
