@@ -74,7 +74,7 @@
 extern "C" {
 #endif
 
-#define IAK_ABI_VERSION 11
+#define IAK_ABI_VERSION 12
 
 /* Grid size from which merge_in_kernel = 2 merges inside the decode kernel; it
  * also does so on grids of at most IAK_MERGE_IN_KERNEL_SMALL_WORKGROUPS workgroups
@@ -723,7 +723,10 @@ iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
  *       are left out; a sequence listed twice loses tokens twice.
  *   iak_grow_sequences  sequence seqs[i] gets new_tokens[i] more tokens in each of its rows:
  *       entries for them come from the free pages, the lowest id first, in the order of
- *       (i, row, entry), with refs = 1.
+ *       (i, row, entry), with refs = 1. granted [num_seqs] (may be NULL; no other array of the
+ *       call) is written whole: new_tokens[i] of sequence seqs[i] if the call was done, 0 of
+ *       every other and of all if it was not. As the q_lens of what follows on the stream it
+ *       keeps tokens that got no room from being appended over older ones.
  *   iak_fork_sequences  sequence seqs[i], which has no tokens, becomes a copy of parents[i]:
  *       it shares the parent's pages (refs + 1), except that a last page which is not full
  *       is copied (every array) into a free page, chosen in the order of (i, row).
@@ -745,6 +748,7 @@ typedef struct {
   int32_t* missing;            /* grow, fork */
   int32_t num_arrays;          /* fork */
   iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
+  int32_t* granted;            /* grow; may be NULL */
 } iak_sequences_args;
 
 iak_status iak_sequences_workspace(const iak_sequences_args* args, size_t* bytes);

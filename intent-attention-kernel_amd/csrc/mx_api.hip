@@ -231,6 +231,23 @@ iak_status validate_planned(const iak_sequences_args* a, const char* null, const
   return IAK_OK;
 }
 
+// grow: `granted` is cleared before the other arrays are read, so it must be none of them
+iak_status validate_granted(const iak_sequences_args* a) {
+  if (!a->granted) return IAK_OK;
+  if (!aligned4(a->granted)) return fail(IAK_EINVAL, "granted must be 4-byte aligned");
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(a->granted), end = begin + 4 * (uintptr_t)a->num_seqs;
+  const uint64_t rows = (uint64_t)a->num_seqs * a->rows_per_seq, count = (uint64_t)a->count;
+  const struct { const int32_t* p; uint64_t n; const char* name; } others[] = {
+      {a->page_table, rows * a->table_width, "page_table"}, {a->valid_tokens, rows, "valid_tokens"},
+      {a->refs, (uint64_t)a->num_pages, "refs"}, {a->seqs, count, "seqs"}, {a->new_tokens, count, "new_tokens"},
+      {a->missing, 1, "missing"}};
+  for (const auto& o : others) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(o.p);
+    if (at < end && begin < at + 4 * o.n) return fail(IAK_EINVAL, "granted overlaps %s", o.name);
+  }
+  return IAK_OK;
+}
+
 iak_status validate_compact(const iak_compact_pages_args* a) {
   if (!a) return fail(IAK_EINVAL, "args is NULL");
   if (a->num_rows < 0 || a->table_width < 0 || a->page_size <= 0 || a->num_pages < 0 || a->num_pages > 0x7FFFFFFFLL)
@@ -333,6 +350,7 @@ iak_status iak_free_sequences(const iak_sequences_args* a, void* stream) {
 iak_status iak_grow_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   iak_status st = validate_sequences(a);
   if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->new_tokens ? "new_tokens" : nullptr, workspace, workspace_bytes);
+  if (st == IAK_OK) st = validate_granted(a);
   if (st != IAK_OK) return st;
   return launched(iak::launch_grow_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "grow sequences");
 }

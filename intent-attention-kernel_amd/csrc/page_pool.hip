@@ -139,6 +139,7 @@ struct SeqArgs {
   int count;
   const int32_t* seqs; const int32_t* parents; const int32_t* new_tokens;
   int32_t* missing;
+  int32_t* granted;                    // [num_seqs] tokens that the call makes room for, or null (grow)
   int groups;                          // ceil(NP / PAGE_GROUP)
   int32_t* head;                       // [0] pages needed, [1] the call is refused
   int32_t* group_free;                 // [groups] free pages
@@ -177,7 +178,10 @@ __device__ __forceinline__ int count_free(const int32_t* refs, int64_t NP, int g
 template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, int& refused) {
   constexpr int WAVES = PLAN_THREADS / 64;
   if (threadIdx.x == 0) refused = 0;
-  for (int k = threadIdx.x; k < a.num_seqs; k += PLAN_THREADS) a.marks[k] = 0;
+  for (int k = threadIdx.x; k < a.num_seqs; k += PLAN_THREADS) {
+    a.marks[k] = 0;
+    if (KIND == SEQ_GROW && a.granted) a.granted[k] = 0;
+  }
   __threadfence_block();
   __syncthreads();
   bool bad = false;
@@ -298,7 +302,10 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
         a.refs[id] = 1;
       });
     __syncthreads();                                             // every thread has read the old length
-    if (threadIdx.x == 0) a.valid[row] = tokens;
+    if (threadIdx.x == 0) {
+      a.valid[row] = tokens;
+      if (a.granted && h == 0) a.granted[seq] = other;
+    }
   } else {
     __shared__ int fresh;
     const int64_t parent = (int64_t)other * a.R + h;
@@ -472,6 +479,7 @@ SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
   s.num_seqs = a.num_seqs; s.R = a.rows_per_seq; s.W = a.table_width; s.PSZ = a.page_size; s.NP = a.num_pages;
   s.table = a.page_table; s.valid = a.valid_tokens; s.refs = a.refs;
   s.count = a.count; s.seqs = a.seqs; s.parents = a.parents; s.new_tokens = a.new_tokens; s.missing = a.missing;
+  s.granted = a.granted;
   s.groups = (int)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
   s.arrays.n = a.num_arrays;
   for (int k = 0; k < a.num_arrays; ++k) s.arrays.a[k] = a.arrays[k];

@@ -14,7 +14,7 @@ from typing import Optional
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # IAK_LIBRARY selects another build of the same ABI (e.g. a tuning variant)
 LIB_PATH = os.environ.get("IAK_LIBRARY") or os.path.join(_HERE, "libiak.so")
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 IAK_OK, IAK_EINVAL, IAK_ENOTSUP, IAK_EHIP = 0, 1, 2, 3
 
@@ -247,7 +247,7 @@ class SequencesArgs(ctypes.Structure):
         ("num_pages", c_i64),
         ("page_table", c_void_p), ("valid_tokens", c_void_p), ("refs", c_void_p),
         ("count", c_i32), ("seqs", c_void_p), ("parents", c_void_p), ("new_tokens", c_void_p), ("missing", c_void_p),
-        ("num_arrays", c_i32), ("arrays", PageArray * MAX_PAGE_ARRAYS),
+        ("num_arrays", c_i32), ("arrays", PageArray * MAX_PAGE_ARRAYS), ("granted", c_void_p),
     ]
 
 

@@ -21,7 +21,10 @@ Nothing waits for the device. Which page goes where is a function of the argumen
 ``grow_sequences`` and ``fork_sequences`` do all of a call or nothing of it, and return an
 int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
 of range or listed twice, a negative count, a row longer than its table, a forked sequence
-that has tokens or is itself a parent).
+that has tokens or is itself a parent). What is queued behind a call that was not done runs
+all the same: ``grow_sequences(..., granted=lens)`` leaves in ``lens`` how many tokens each
+sequence got room for, 0 then, and ``append_mxfp4_tokens(..., q_lens=lens)`` writes no more.
+Without it read the answer before tokens are appended, for they would land on older ones.
 """
 from __future__ import annotations
 
@@ -133,15 +136,24 @@ def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor]) -> t
 
 
 def grow_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
-                   new_tokens: Indices, *, missing: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   new_tokens: Indices, *, granted: Optional[torch.Tensor] = None,
+                   missing: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Room for ``new_tokens[i]`` more tokens in every row of sequence ``seqs[i]``: the table
     entries they need get free pages (the lowest ids first, in the order of i, row, entry),
-    refs 1, and valid_tokens grows. All or nothing; returns ``missing`` (module docstring)."""
+    refs 1, and valid_tokens grows. All or nothing; returns ``missing`` (module docstring).
+    ``granted`` (int32 [B]) is written whole: ``new_tokens[i]`` at ``seqs[i]``, 0 at every other
+    sequence, and 0 at all of them if nothing was done: the ``q_lens`` of the append and the
+    attention behind it."""
     a, dev, seqs, _ = _sequences("page allocation", page_table, valid_tokens, refs, seqs)
     new_tokens = _indices("new_tokens", new_tokens, dev, seqs.shape[0])
     a.new_tokens = new_tokens.data_ptr()
+    if granted is not None:
+        B = page_table.shape[0]
+        if granted.shape != (B,) or granted.dtype != torch.int32 or granted.device != dev or not granted.is_contiguous():
+            raise ValueError(f"granted must be contiguous int32 [{B}] on {dev}, got {granted.dtype} {tuple(granted.shape)}")
+        a.granted = granted.data_ptr()
     missing = _planned(N.grow_sequences, a, dev, missing)
-    _written(page_table, valid_tokens, refs, missing)
+    _written(page_table, valid_tokens, refs, missing, *(() if granted is None else (granted,)))
     return missing
 
 
