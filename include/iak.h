@@ -723,7 +723,11 @@ iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
  *       are left out; a sequence listed twice loses tokens twice.
  *   iak_grow_sequences  sequence seqs[i] gets new_tokens[i] more tokens in each of its rows:
  *       entries for them come from the free pages, the lowest id first, in the order of
- *       (i, row, entry), with refs = 1. granted [num_seqs] (may be NULL; no other array of the
+ *       (i, row, entry), with refs = 1. A row that gets tokens and whose last page has room
+ *       but refs > 1 (sequences forked and then cut back share such pages) is given a page of
+ *       its own in that entry, a copy (every array), and lets go of the other, so that what is
+ *       appended reaches no other owner; without arrays such a call is refused.
+ *       granted [num_seqs] (may be NULL; no other array of the
  *       call) is written whole: new_tokens[i] of sequence seqs[i] if the call was done, 0 of
  *       every other and of all if it was not. As the q_lens of what follows on the stream it
  *       keeps tokens that got no room from being appended over older ones.
@@ -732,8 +736,8 @@ iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
  *       is copied (every array) into a free page, chosen in the order of (i, row).
  * Grow and fork do all of it or nothing and say which in missing[0]: 0 done; n > 0: n more
  * free pages would be needed; -1: an index outside [0, num_seqs) or listed twice among
- * seqs, a negative new_tokens, a row longer than its table, a forked sequence with tokens, or
- * one that is also a parent. Results do not depend on timing. Workspace:
+ * seqs, a negative new_tokens, a row that would be longer than its table, a shared last page
+ * and no arrays, a forked sequence with tokens, or one that is also a parent. Results do not depend on timing. Workspace:
  * iak_sequences_workspace bytes, 16-byte aligned (free needs none). */
 typedef struct {
   int32_t num_seqs, rows_per_seq, table_width, page_size;
@@ -746,7 +750,7 @@ typedef struct {
   const int32_t* parents;      /* fork */
   const int32_t* new_tokens;   /* grow; free: may be NULL */
   int32_t* missing;            /* grow, fork */
-  int32_t num_arrays;          /* fork */
+  int32_t num_arrays;          /* grow, fork */
   iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
   int32_t* granted;            /* grow; may be NULL */
 } iak_sequences_args;

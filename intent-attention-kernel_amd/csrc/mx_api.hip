@@ -351,6 +351,7 @@ iak_status iak_grow_sequences(const iak_sequences_args* a, void* workspace, size
   iak_status st = validate_sequences(a);
   if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->new_tokens ? "new_tokens" : nullptr, workspace, workspace_bytes);
   if (st == IAK_OK) st = validate_granted(a);
+  if (st == IAK_OK) st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
   if (st != IAK_OK) return st;
   return launched(iak::launch_grow_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "grow sequences");
 }

@@ -8,7 +8,8 @@
 //   grow, fork   seq_plan_kernel   a bit a page: free, and their number per 1,024 ids; one
 //                                  workgroup checks the call and sums what its rows need
 //                seq_apply_kernel  a workgroup per row: the verdict, the row's free pages out of the
-//                                  bits, entries, counts, the copied last page
+//                                  bits, entries, counts, the copied last page (a fork's where it
+//                                  has room, a growing row's where others hold it too)
 //   free         seq_free_kernel   a workgroup per row
 //   compact      compact_count_kernel, compact_rank_kernel (which page goes where; for few pages
 //                compact_small_kernel), compact_apply_kernel (pages copied, table, counts and
@@ -164,6 +165,13 @@ __device__ __forceinline__ bool ragged_last(const SeqArgs& a, int64_t parent_row
   return page >= 0 && page < a.NP;
 }
 
+// Whether a growing row of `tokens` gets its last page anew: it has room, and others hold it too.
+__device__ __forceinline__ bool shared_last(const SeqArgs& a, int64_t row, int tokens) {
+  if (tokens <= 0 || tokens % a.PSZ == 0) return false;
+  const int64_t page = a.table[row * a.W + used_entries(tokens, a.PSZ, a.W) - 1];
+  return page >= 0 && page < a.NP && a.refs[page] > 1;
+}
+
 __device__ __forceinline__ int count_free(const int32_t* refs, int64_t NP, int group) {
   int n = 0;
   for (int k = threadIdx.x; k < PAGE_GROUP; k += blockDim.x) {
@@ -218,7 +226,13 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
           const int old = a.valid[(int64_t)a.seqs[j] * a.R + h];
           const int64_t tokens = (int64_t)(old < 0 ? 0 : old) + a.new_tokens[j];
           if (tokens > (int64_t)a.W * a.PSZ) refused = 1;
-          else need = used_entries((int)tokens, a.PSZ, a.W) - used_entries(old, a.PSZ, a.W);
+          else {
+            need = used_entries((int)tokens, a.PSZ, a.W) - used_entries(old, a.PSZ, a.W);
+            if (a.new_tokens[j] > 0 && shared_last(a, (int64_t)a.seqs[j] * a.R + h, old)) {
+              ++need;
+              if (a.arrays.n == 0) refused = 1;
+            }
+          }
         } else {
           int n;
           int64_t page;
@@ -283,6 +297,7 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
   const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
   const bool listed = a.count > 0;
   const int need = a.head[0], refused = a.head[1], seq = listed ? a.seqs[j] : 0, first = listed ? a.first[k] : 0;
+  const int after = k + 1 < (int)gridDim.x ? a.first[k + 1] : need;   // where the row's pages end
   const int other = listed ? (KIND == SEQ_GROW ? a.new_tokens : a.parents)[j] : 0;
   const int per = (a.groups + POOL_THREADS - 1) / POOL_THREADS;
   int own = 0, all;
@@ -295,13 +310,21 @@ template <int KIND> __global__ __launch_bounds__(POOL_THREADS) void seq_apply_ke
   int32_t* entries = a.table + row * a.W;
   if constexpr (KIND == SEQ_GROW) {
     const int old = a.valid[row] < 0 ? 0 : a.valid[row], tokens = old + other;
-    const int have = used_entries(old, a.PSZ, a.W), want = used_entries(tokens, a.PSZ, a.W);
-    if (want > have)
-      take_pages(a, per, before, own, first, want - have, [&](int e, int id) {
-        entries[have + e] = id;
+    const int have = used_entries(old, a.PSZ, a.W), want = used_entries(tokens, a.PSZ, a.W), n = after - first;
+    __shared__ int fresh;
+    const bool anew = n > want - have;                           // shared_last() when planned: counts sink here
+    const int last = anew ? entries[have - 1] : 0;
+    if (n > 0)
+      take_pages(a, per, before, own, first, n, [&](int e, int id) {
+        entries[have - anew + e] = id;
         a.refs[id] = 1;
+        if (anew && e == 0) fresh = id;
       });
     __syncthreads();                                             // every thread has read the old length
+    if (anew) {
+      if (threadIdx.x == 0) atomicSub(&a.refs[last], 1);
+      copy_page<false>(a.arrays, last, fresh);
+    }
     if (threadIdx.x == 0) {
       a.valid[row] = tokens;
       if (a.granted && h == 0) a.granted[seq] = other;

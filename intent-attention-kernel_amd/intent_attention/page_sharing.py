@@ -10,7 +10,8 @@ The state is three int32 tensors on the device, which a program keeps beside its
   valid_tokens  [B, R]     the tokens of each row; its first ceil(valid / 16) entries are in use
   refs          [NP]       how many table entries (and other owners) hold a page; 0: free
 
-* ``grow_sequences`` makes room for new tokens: pages for them, the lowest free ids first;
+* ``grow_sequences`` makes room for new tokens: pages for them, the lowest free ids first,
+  and a copy of a row's last page where it has room but others hold it too;
 * ``fork_sequences`` makes empty sequences copies of others: full pages are shared, a last
   page with room is copied, so that both may append;
 * ``free_sequences`` lets sequences go, or their newest tokens;
@@ -20,8 +21,8 @@ The state is three int32 tensors on the device, which a program keeps beside its
 Nothing waits for the device. Which page goes where is a function of the arguments alone.
 ``grow_sequences`` and ``fork_sequences`` do all of a call or nothing of it, and return an
 int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
-of range or listed twice, a negative count, a row longer than its table, a forked sequence
-that has tokens or is itself a parent). What is queued behind a call that was not done runs
+of range or listed twice, a negative count, a row that would be longer than its table, a
+last page to be copied and no pools, a forked sequence that has tokens or is itself a parent). What is queued behind a call that was not done runs
 all the same: ``grow_sequences(..., granted=lens)`` leaves in ``lens`` how many tokens each
 sequence got room for, 0 then, and ``append_mxfp4_tokens(..., q_lens=lens)`` writes no more.
 Without it read the answer before tokens are appended, for they would land on older ones.
@@ -136,15 +137,19 @@ def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor]) -> t
 
 
 def grow_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
-                   new_tokens: Indices, *, granted: Optional[torch.Tensor] = None,
+                   new_tokens: Indices, pools: Optional[Pools] = None, *, granted: Optional[torch.Tensor] = None,
                    missing: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Room for ``new_tokens[i]`` more tokens in every row of sequence ``seqs[i]``: the table
     entries they need get free pages (the lowest ids first, in the order of i, row, entry),
     refs 1, and valid_tokens grows. All or nothing; returns ``missing`` (module docstring).
+    A row whose last page has room but refs above 1 (sequences that were forked and then cut back
+    to inside a page they share) gets a page of its own for it, copied in every tensor of
+    ``pools``, and lets go of the shared one; without ``pools`` such a call is refused (-1): what is
+    appended reaches no other owner.
     ``granted`` (int32 [B]) is written whole: ``new_tokens[i]`` at ``seqs[i]``, 0 at every other
     sequence, and 0 at all of them if nothing was done: the ``q_lens`` of the append and the
     attention behind it."""
-    a, dev, seqs, _ = _sequences("page allocation", page_table, valid_tokens, refs, seqs)
+    a, dev, seqs, tensors = _sequences("page allocation", page_table, valid_tokens, refs, seqs, pools)
     new_tokens = _indices("new_tokens", new_tokens, dev, seqs.shape[0])
     a.new_tokens = new_tokens.data_ptr()
     if granted is not None:
@@ -153,7 +158,7 @@ def grow_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: t
             raise ValueError(f"granted must be contiguous int32 [{B}] on {dev}, got {granted.dtype} {tuple(granted.shape)}")
         a.granted = granted.data_ptr()
     missing = _planned(N.grow_sequences, a, dev, missing)
-    _written(page_table, valid_tokens, refs, missing, *(() if granted is None else (granted,)))
+    _written(page_table, valid_tokens, refs, missing, *(() if granted is None else (granted,)), *tensors)
     return missing
 
 

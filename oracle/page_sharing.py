@@ -44,25 +44,37 @@ class Pages:
     def _sound(self, seqs):
         return all(0 <= s < len(self.table) for s in seqs) and len(set(seqs)) == len(seqs)
 
-    def grow(self, seqs, new):
+    def grow(self, seqs, new, pools=False):
+        """``pools``: there are arrays to copy a last page in that others hold too."""
         if not self._sound(seqs) or any(n < 0 for n in new):
             return -1
-        needs = []
+        needs, shared = [], []
         for s, n in zip(seqs, new):
             for h in range(len(self.table[s])):
                 old = max(0, self.valid[s][h])
                 if old + n > self.width * PS:
                     return -1
-                needs.append((s, h, -(-old // PS), -(-(old + n) // PS), old + n))
+                last = self.table[s][h][old // PS] if n > 0 and old % PS else -1
+                anew = self._in(last) and self.refs[last] > 1
+                if anew and not pools:
+                    return -1
+                needs.append((s, h, -(-old // PS) - anew, -(-(old + n) // PS), old + n))
+                if anew:
+                    shared.append((s, h, old // PS))
         free = self._free()
         need = sum(b - a for _, _, a, b, _ in needs)
         if need > len(free):
             return need - len(free)
         it = iter(free)
+        lost = {(s, h): self.table[s][h][e] for s, h, e in shared}
+        for page in lost.values():
+            self.refs[page] -= 1
         for s, h, a, b, tokens in needs:
             for e in range(a, b):
                 self.table[s][h][e] = page = next(it)
                 self.refs[page] = 1
+            if (s, h) in lost:
+                self.copied.append((lost[s, h], self.table[s][h][a]))
             self.valid[s][h] = tokens
         return 0
 

@@ -162,3 +162,132 @@ def test_granted_is_checked():
             call()
     assert ia.grow_sequences(*s.state(), [], [], granted=lens).item() == 0
     assert lens.tolist() == [0, 0, 0] and int(s.refs.sum()) == 0
+
+
+def test_a_row_cut_back_into_a_shared_page_grows_apart():
+    """Fork at a page's end, let tokens go into the shared page, grow and append: the sibling's tokens
+    stay, the kept ones of the row come along; without pools the call is refused."""
+    import torch
+    import intent_attention as ia
+    for cut, first, then in ((4, [1], [4]), (1, [0, 1], [3, 20]), (15, [1, 0], [1, 1]), (20, [1], [40])):
+        s = Loop(3, 2, 6, 30, cut)
+        assert s.step([0], [48])[0] == 0
+        assert ia.fork_sequences(*s.state(), [0], [1], s.pools).item() == 0
+        ia.free_sequences(*s.state(), [1], [cut])
+        s.kept[1] = s.kept[0][:, :48 - cut]
+        if len(first) == 2:                                # both owners cut back, both grown in one call
+            ia.free_sequences(*s.state(), [0], [cut])
+            s.kept[0] = s.kept[1]
+        s.check()
+        before = [t.clone() for t in (*s.state(), *s.pools.tensors().values())]
+        assert s.step(first, then)[0] == -1                # no pools to copy in
+        for t, b in zip((*s.state(), *s.pools.tensors().values()), before):
+            assert torch.equal(t, b)
+        assert s.step(first, [0] * len(first))[0] == 0     # no tokens, nothing to copy
+        assert s.step(first, then, pools=s.pools)[0] == 0
+        s.check()
+        used = sum(2 * -(-x.shape[1] // 16) for x in s.kept if x is not None)
+        assert int(s.refs.sum()) == used
+        rows = s.table.flatten(0, 1).tolist()
+        for page in range(30):                             # every entry counted where it is
+            assert s.refs[page].item() == sum(r.count(page) for r in rows)
+
+
+def test_copies_of_shared_pages_come_too_few():
+    """A copy needs a free page like any other: one too few, nothing done; then the sibling leaves."""
+    import torch
+    import intent_attention as ia
+    s = Loop(2, 1, 4, 3)
+    assert s.step([0], [48])[0] == 0
+    assert ia.fork_sequences(*s.state(), [0], [1], s.pools).item() == 0
+    ia.free_sequences(*s.state(), [1], [5])
+    s.kept[1] = s.kept[0][:, :43]
+    before = [t.clone() for t in (*s.state(), *s.pools.tensors().values())]
+    assert s.step([1], [2], pools=s.pools)[0] == 1
+    for t, b in zip((*s.state(), *s.pools.tensors().values()), before):
+        assert torch.equal(t, b)
+    ia.free_sequences(*s.state(), [0])
+    s.kept[0] = None
+    assert s.step([1], [2])[0] == 0                        # the page is its own now: no pools needed
+    s.check()
+
+
+@pytest.mark.parametrize("B,R,W,NP", [(6, 1, 3, 30), (9, 3, 20, 1500), (40, 8, 9, 6000), (9, 2, 30, 40000)])
+def test_growing_rows_with_shared_last_pages_follow_the_lists(B, R, W, NP):
+    """Entries that any rows share, some counted by others, some no pages: grown with arrays and without."""
+    from tests.test_gpu_page_sharing import State
+    import intent_attention as ia
+    s = State(B + W, B, R, W, NP, fill=0.7)
+    rng = np.random.default_rng(B)
+    done = copies = 0
+    for it in range(10):
+        for _ in range(B):                                 # rows that share what lies at the same entry
+            b, c, h, g = (int(rng.integers(0, n)) for n in (B, B, R, R))
+            n = min(s.host.used(b, h), s.host.used(c, g))
+            if n:
+                s.host.table[b][h][n - 1] = s.host.table[c][g][n - 1] if rng.random() < 0.8 else int(rng.choice([-1, NP]))
+        counts = [0] * NP
+        for b in range(B):
+            for h in range(R):
+                for e in range(s.host.used(b, h)):
+                    if 0 <= s.host.table[b][h][e] < NP:
+                        counts[s.host.table[b][h][e]] += 1
+        for p in rng.choice(NP, 3, replace=False):
+            counts[p] += 1
+        s.host.refs = counts
+        s.table.copy_(_t(s.host.table))
+        s.refs.copy_(_t(counts))
+        seqs = [int(x) for x in rng.permutation(B)[:max(1, B // 2)]]
+        new = [int(x) for x in rng.integers(0, 25, len(seqs))]
+        pools = it % 4 != 3
+        want = s.host.grow(seqs, new, pools)
+        copies += len(s.host.copied)
+        got = ia.grow_sequences(s.table, s.valid, s.refs, _t(seqs), _t(new), s.pools if pools else None)
+        assert got.item() == want
+        done += want == 0
+        s.check()
+        drop = [int(x) for x in rng.integers(0, 30, B)]
+        s.host.free(list(range(B)), drop)
+        ia.free_sequences(s.table, s.valid, s.refs, list(range(B)), drop)
+        s.check()
+    assert done >= 3 and copies >= 3
+
+
+def test_copies_of_shared_pages_replay():
+    """Captured once: rows that share their last page, that do not, and a call that is refused."""
+    import torch
+    import intent_attention as ia
+    from tests.test_gpu_page_sharing import State
+    s = State(3, 6, 2, 12, 300, fill=0.5)
+    seqs, new, short = _t([0, 1]), _t([5, 5]), torch.zeros(1, dtype=torch.int32, device=_dev())
+    lens = torch.zeros(6, dtype=torch.int32, device=_dev())
+    keep = [x.clone() for x in (s.table, s.valid, s.refs, *s.pools)]
+
+    def step():
+        ia.grow_sequences(s.table, s.valid, s.refs, seqs, new, s.pools, granted=lens, missing=short)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for x, k in zip((s.table, s.valid, s.refs, *s.pools), keep):
+        x.copy_(k)
+    for a, n, shared in (([0, 1], [5, 6], True), ([2, 4], [1, 30], False), ([5, 5], [1, 1], True), ([1, 5], [9, 2], True)):
+        if shared:
+            for b in a:
+                for h in range(2):
+                    if s.host.valid[b][h] % 16:
+                        s.host.refs[s.host.table[b][h][s.host.valid[b][h] // 16]] += 1
+        s.refs.copy_(_t(s.host.refs))
+        seqs.copy_(_t(a))
+        new.copy_(_t(n))
+        want = s.host.grow(a, n, True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert short.item() == want
+        assert lens.tolist() == [dict(zip(a, n)).get(b, 0) if want == 0 else 0 for b in range(6)]
+        s.check()
