@@ -16,7 +16,10 @@ serving loop appends each new token as it comes, at 4.25 bits a value.
 All of them take the same page table [B, Hkv, W] and ``valid_tokens`` [B, Hkv], the tokens
 each row holds INCLUDING the newest ones: append first, then attend. With ``q_lens`` [B]
 sequence b has q_lens[b] new tokens, the first of the batch's L; the rest is padding (not
-written by append, zero from read and attention).
+written by append, zero from read and attention). A length below 0 counts as 0, one past the
+table as the table's 16 W tokens, in all of them: the newest tokens of such a row are the
+table's last slots, and an append writes over what they hold. ``grow_sequences`` lets no row
+become longer than its table; a program that counts lengths itself must not either.
 
 The values: per block of 32 channels e = clamp(floor(log2 max|x|) - 2, -23, 13) and codes
 rounded to the nearest even of x / 2^e, at most 6 in magnitude (the OCP microscaling
@@ -128,8 +131,8 @@ def append_mxfp4_tokens(k: torch.Tensor, v: torch.Tensor, pools: MxFp4Pools, pag
                         valid_tokens: torch.Tensor, *, q_lens: Optional[torch.Tensor] = None) -> None:
     """Quantise the newest tokens' ``k``, ``v`` [B, L, Hkv, D] (float16, bfloat16 or float32,
     one dtype, any strides) into the pools: token i < q_lens[b] (default L) of sequence b is
-    number valid_tokens[b, h] - q_lens[b] + i of row (b, h). Tokens before 0, past the table
-    or on a page id outside the pools are left out; nothing else of the pools is written.
+    number min(valid_tokens[b, h], 16 W) - q_lens[b] + i of row (b, h). Tokens before 0 or on a
+    page id outside the pools are left out; nothing else of the pools is written.
     Rows that share a page (``fork_sequences`` shares full pages only) must not both append
     to it."""
     if k.dim() != 4 or k.shape != v.shape:
