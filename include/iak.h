@@ -669,9 +669,13 @@ iak_status iak_mx_read_tokens(const iak_mx_tokens_args* args, void* stream);
  *   i >= q_lens[b].
  * A token with a NaN block makes every query that sees it NaN, as does a query that is
  * not finite itself; tokens that a query does not see never reach it. Products run on the
- * matrix cores in float16 (queries scaled by a power of two per row, so that neither range
- * nor, for float16 and bfloat16 queries, bits are lost; K and V exact; weights rounded to
- * 11 bits) with float32 sums; float32 queries and their weights are split in two (22 bits).
+ * matrix cores in float16 with float32 sums; K and V are exact there. A query row is scaled by
+ * a power of two that brings its largest element to 2^14 .. 2^15: float16 and bfloat16
+ * elements are exact down to 2^-28 of the row's largest, smaller ones off by at most 2^-39 of
+ * it; float32 elements are split in two, off by at most 2^-22 of themselves or 2^-39 of the
+ * largest. (A score is so off by up to |sm_scale| 2^-39 max|q| sum|k|, which counts only where
+ * the query's largest channels meet keys that are smaller by as much.) Weights are rounded to
+ * 11 bits, those of float32 queries split in two (22 bits).
  * Scores, with the scale, have to be float32 numbers in base 2. Code pools are 16-byte, scale
  * pools 4-byte aligned; q and out lie at any address of their type, and out may be q.
  * splits: parts a row's tokens are divided into (0: automatic). The parts meet in the

@@ -202,7 +202,10 @@ __device__ __forceinline__ void store_out4(const MxAttn& a, int64_t at, const fl
 }
 
 // A query row's operand: the lane's channels (D/4) g .., scaled by a power of two to a largest
-// element of the row in [2^14, 2^15), split in two for float32. Returns the positive factor that
+// element of the row in [2^14, 2^15), split in two for float32. What float16 cannot hold below
+// that is rounded to its smallest step, 2^-24: off by 2^-25, 2^-39 of the row's largest, and not
+// at all for 16-bit elements of 2^-28 of it or more. A scale per 32 channels would lose nothing,
+// but would have to go into K's (2^-24 to 49,152 already), which float16 cannot hold either. Returns the positive factor that
 // makes base-2 scores of the products. (A negative scale turns the query's sign; where the factor
 // would vanish the scores do: query 0, factor 1. A row that is not finite is NaN, factor 1: NaN
 // scores for the tokens that it sees, and none if it sees none.)

@@ -243,7 +243,8 @@ def mxfp4_paged_attention(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.
     Query i < q_lens[b] (default L) of head h reads row (b, h // (Hq // Hkv)) of the table and
     sees its tokens up to its own, number valid_tokens - q_lens[b] + i, or with
     ``causal=False`` all valid_tokens: out = softmax(sm_scale q . k) v, sm_scale = 1 / sqrt(D)
-    by default; zeros where a query sees nothing and for i >= q_lens[b]. ``splits``: parts
+    by default; zeros where a query sees nothing and for i >= q_lens[b]. Elements of a query row
+    below 2^-28 of its largest are rounded, off by at most 2^-39 of that. ``splits``: parts
     the rows' tokens are divided into (0: automatic). Returns ``out``, shaped as q."""
     page_table, valid_tokens = page_table.contiguous(), valid_tokens.contiguous()
     q_lens = None if q_lens is None else q_lens.contiguous()
