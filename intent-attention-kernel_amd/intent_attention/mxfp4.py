@@ -244,8 +244,11 @@ def mxfp4_paged_attention(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.
     sees its tokens up to its own, number valid_tokens - q_lens[b] + i, or with
     ``causal=False`` all valid_tokens: out = softmax(sm_scale q . k) v, sm_scale = 1 / sqrt(D)
     by default; zeros where a query sees nothing and for i >= q_lens[b]. Elements of a query row
-    below 2^-28 of its largest are rounded, off by at most 2^-39 of that. ``splits``: parts
-    the rows' tokens are divided into (0: automatic). Returns ``out``, shaped as q."""
+    below 2^-28 of its largest are rounded, off by at most 2^-39 of that. The softmax weights of
+    float16 and bfloat16 queries are rounded to 11 bits for the product with v (a float16 output's
+    own precision; with ``out_dtype=torch.float32`` it shows: 2^-11 of sum p |v| at most), those
+    of float32 queries to 22. ``splits``: parts the rows' tokens are divided into (0: automatic).
+    Returns ``out``, shaped as q."""
     page_table, valid_tokens = page_table.contiguous(), valid_tokens.contiguous()
     q_lens = None if q_lens is None else q_lens.contiguous()
     if q.dim() and q.stride(-1) != 1:

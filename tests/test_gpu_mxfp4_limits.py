@@ -114,3 +114,25 @@ def test_elements_of_every_size_count_to_the_stated_step(L):
             # out = tanh(score), its slope at most 1; weights of 11 bits (22), exponentials, sums
             tol = 0.5 * off + 0.5 * 16 * 2.0 ** -24 + (2.0 ** -22 if dtype == "float32" else 2.0 ** -11) + 2.0 ** -20
             assert float((got.double().cpu() - np.tanh(0.5)).abs().max()) <= tol, (dtype, p)
+
+
+@pytest.mark.parametrize("L", [1, 140])
+def test_weights_of_16_bit_queries_keep_11_bits(L):
+    """In a wider output the weights' rounding shows: 2^-11 of sum p |v|, no more."""
+    import torch
+    import intent_attention as ia
+    rng = np.random.default_rng(L + 4)
+    B, Hq, Hkv, D, W, NP = 1, 8, 2, 64, 14, 30
+    host, pools = _pools(rng, NP, D)
+    table, valid = _table(rng, B, Hkv, W, NP), np.full((B, Hkv), 16 * W, np.int32)
+    T, vmax = 16 * W, 6 * 2.0 ** 0                                   # scale bytes up to 127
+    q = torch.from_numpy(rng.standard_normal((B, L, Hq, D)).astype(np.float32)).to(_dev())
+    queries = sorted({0, L // 2, L - 1})
+    for dtype, weight in ((torch.float16, 2.0 ** -11), (torch.bfloat16, 2.0 ** -11), (torch.float32, 2.0 ** -22)):
+        got = ia.mxfp4_paged_attention(q.to(dtype), pools, _t(table), _t(valid), out_dtype=torch.float32).double().cpu().numpy()
+        hq = q.to(dtype).double().cpu().numpy()
+        want, mass, reach = O.attention(hq, host, table, valid, queries=queries)
+        score = (((D + 6) * 2.0 ** -24 + 2.0 ** -22) * reach + _score_error(hq, host, table, valid, 1 / np.sqrt(D)))[..., None]
+        rel = 2 * np.expm1(2 * score) + weight + 2.0 ** -22 + 2 * (T + 8) * 2.0 ** -24
+        tol = rel * mass + T * 2.0 ** -31 * vmax + HALF["float32"] * np.abs(want)
+        assert float((np.abs(got - want)[:, queries] / tol[:, queries]).max()) <= 1.0, dtype
