@@ -207,7 +207,7 @@ iak_status validate_sequences(const iak_sequences_args* a) {
   if (a->num_seqs < 0 || a->rows_per_seq <= 0 || a->table_width < 0 || a->page_size <= 0 || a->num_pages < 0 || a->count < 0)
     return fail(IAK_EINVAL, "bad size (num_seqs=%d, rows_per_seq=%d, table_width=%d, page_size=%d, num_pages=%lld, count=%d)",
                 a->num_seqs, a->rows_per_seq, a->table_width, a->page_size, (long long)a->num_pages, a->count);
-  if (a->num_pages > 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)a->num_pages);
+  if (a->num_pages >= 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)a->num_pages);
   if ((double)a->table_width * a->page_size > 2147483647.0)
     return fail(IAK_EINVAL, "table_width %d x page_size %d: a row's tokens exceed int32", a->table_width, a->page_size);
   // one workgroup of 256 threads per listed row

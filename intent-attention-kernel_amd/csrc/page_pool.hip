@@ -79,20 +79,21 @@ __global__ __launch_bounds__(POOL_THREADS) void copy_pages_kernel(const PageArra
 // Sums over a workgroup. Every thread of it calls them.
 // --------------------------------------------------------------------------- //
 
-// Sum of `x` over the threads before this one; `total`: over all. WAVES waves.
-template <int WAVES> __device__ __forceinline__ int scan_before(int x, int& total) {
-  __shared__ int wave_sum[WAVES];
+// Sum of `x` over the threads before this one; `total`: over all. WAVES waves; T: int, or where
+// the sum may pass 32 bits int64_t.
+template <int WAVES, typename T> __device__ __forceinline__ T scan_before(T x, T& total) {
+  __shared__ T wave_sum[WAVES];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int s = x;
+  T s = x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(s, o, 64);
+    const T y = __shfl_up(s, o, 64);
     if (lane >= o) s += y;
   }
   __syncthreads();                      // the last call's sums have been read
   if (lane == 63) wave_sum[w] = s;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
 #pragma unroll
   for (int k = 0; k < WAVES; ++k) {
@@ -219,7 +220,7 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
     }
     for (int k0 = 0; k0 < rows; k0 += PLAN_THREADS) {
       const int k = k0 + threadIdx.x;
-      int need = 0;
+      int64_t need = 0;                                          // 1,024 rows' sum may pass 2^31
       if (k < rows) {
         const int j = k / a.R, h = k - j * a.R;
         if constexpr (KIND == SEQ_GROW) {
@@ -239,8 +240,8 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
           need = ragged_last(a, (int64_t)a.parents[j] * a.R + h, n, page);
         }
       }
-      int all;
-      const int before = scan_before<WAVES>(need, all);
+      int64_t all;
+      const int64_t before = scan_before<WAVES>(need, all);
       if (k < rows) a.first[k] = (int)(total + before > 0x7FFFFFFF ? 0x7FFFFFFF : total + before);
       total += all;
     }
@@ -257,7 +258,7 @@ template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_ker
     const uint64_t bits = __builtin_amdgcn_ballot_w64(free_page);
     if ((threadIdx.x & 63) == 0) a.free_bits[id >> 6] = bits;
     int total;
-    scan_before<PLAN_THREADS / 64>(free_page, total);
+    scan_before<PLAN_THREADS / 64>((int)free_page, total);
     if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
     return;
   }
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(POOL_THREADS) void compact_rank_kernel(const Compac
     const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + k0 + threadIdx.x;
     const bool in = id < a.NP, free_page = in && a.refs[id] <= 0;
     int total;
-    const int free_before = before + scan_before<WAVES>(free_page, total);
+    const int free_before = before + scan_before<WAVES>((int)free_page, total);
     before += total;
     if (in && id == L) a.head[1] = free_before;
     if (free_page && id < L) a.hole[free_before] = (int)id;

@@ -291,3 +291,19 @@ def test_copies_of_shared_pages_replay():
         assert short.item() == want
         assert lens.tolist() == [dict(zip(a, n)).get(b, 0) if want == 0 else 0 for b in range(6)]
         s.check()
+
+
+def test_needs_that_pass_32_bits_are_counted():
+    """1,024 rows of 2^21 entries each: 2^31 pages, more than there are; nothing is done."""
+    import torch
+    import intent_attention as ia
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GiB of device memory")
+    W, NP = 1 << 21, 1000
+    table = torch.empty((1, 1024, W), dtype=torch.int32, device=_dev())    # not looked at
+    table[0, :, 0] = 5
+    valid, refs = torch.zeros((1, 1024), dtype=torch.int32, device=_dev()), torch.zeros(NP, dtype=torch.int32, device=_dev())
+    lens = _t([7])
+    for new, answer in ((16 * W, 2 ** 31 - 1 - NP), (16 * (W - 1), 1024 * (W - 1) - NP)):
+        assert ia.grow_sequences(table, valid, refs, [0], [new], granted=lens).item() == answer
+        assert lens.item() == 0 and not bool(valid.any()) and not bool(refs.any()) and bool((table[0, :, 0] == 5).all())
