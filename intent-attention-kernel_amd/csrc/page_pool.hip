@@ -505,11 +505,12 @@ SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
   s.count = a.count; s.seqs = a.seqs; s.parents = a.parents; s.new_tokens = a.new_tokens; s.missing = a.missing;
   s.granted = a.granted;
   s.groups = (int)((a.num_pages + PAGE_GROUP - 1) / PAGE_GROUP);
-  s.arrays.n = a.num_arrays;
-  for (int k = 0; k < a.num_arrays; ++k) s.arrays.a[k] = a.arrays[k];
+  s.arrays.n = 0;
   char* p = reinterpret_cast<char*>(workspace);
   auto take = [&](size_t ints) { int32_t* r = reinterpret_cast<int32_t*>(p); p += up256(4 * ints); return r; };
-  if (p) {
+  if (p) {                             // grow and fork, whose arrays are checked; a free's are nobody's
+    s.arrays.n = a.num_arrays;
+    for (int k = 0; k < a.num_arrays; ++k) s.arrays.a[k] = a.arrays[k];
     s.head = take(2);
     s.group_free = take((size_t)s.groups);
     s.marks = take((size_t)s.num_seqs);

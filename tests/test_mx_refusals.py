@@ -1,7 +1,13 @@
 """Further refusals of the 4-bit token cache's and the page operators' entry points, without a GPU."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 from intent_attention import _native as N
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _seqs():
@@ -18,5 +24,31 @@ def _seqs():
 def test_granted_is_none_of_the_other_arrays(at, text):
     a = _seqs()
     a.granted = at
+    with pytest.raises(ValueError, match=text):
+        N.grow_sequences(a, 0, 1 << 20, N.sequences_workspace(a))
+
+
+def test_free_does_not_read_the_arrays():
+    """A free whose num_arrays nobody set: the arrays are grow's and fork's. In a process that sees no
+    device, so that nothing is launched: an error, and no crash."""
+    code = ("import sys; sys.path.insert(0, 'intent-attention-kernel_amd')\n"
+            "from intent_attention import _native as N\n"
+            "a = N.SequencesArgs()\n"
+            "a.num_seqs, a.rows_per_seq, a.table_width, a.page_size, a.num_pages, a.count = 4, 2, 9, 16, 50, 2\n"
+            "a.page_table = a.valid_tokens = a.refs = a.seqs = 4096\n"
+            "for n in (25, -1, 1 << 30):\n"
+            "    a.num_arrays = n\n"
+            "    try: N.free_sequences(a, 0)\n"
+            "    except RuntimeError as e: print('launch', e)\n")
+    env = dict(os.environ, HIP_VISIBLE_DEVICES="-1", ROCR_VISIBLE_DEVICES="-1")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env, cwd=ROOT)
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+    assert r.stdout.count("launch") == 3, r.stdout
+
+
+@pytest.mark.parametrize("n,text", [(-1, "num_arrays"), (25, "num_arrays"), (1, "row_bytes")])
+def test_grow_checks_its_arrays(n, text):
+    a = _seqs()
+    a.num_arrays, a.arrays[0].base = n, 65536
     with pytest.raises(ValueError, match=text):
         N.grow_sequences(a, 0, 1 << 20, N.sequences_workspace(a))
