@@ -18,7 +18,8 @@ The state is three int32 tensors on the device, which a program keeps beside its
 * ``compact_pages`` moves the pages in use to the lowest ids and returns the new table;
 * ``copy_pages`` copies pages from id to id.
 
-Nothing waits for the device. Which page goes where is a function of the arguments alone.
+Nothing waits for the device; indices and counts may be lists, except in a graph under capture.
+Which page goes where is a function of the arguments alone.
 ``grow_sequences`` and ``fork_sequences`` do all of a call or nothing of it, and return an
 int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
 of range or listed twice, a negative count, a row that would be longer than its table, a
@@ -35,7 +36,7 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .decode_core import PAGE_SIZE, PagePools, current_stream_handle
+from .decode_core import PAGE_SIZE, PagePools, current_stream_handle, uploads_pinned
 from .mla_core import LatentPools
 from .mxfp4 import MxFp4Pools, _device, _launch
 
@@ -90,7 +91,8 @@ def _check_state(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: tor
 
 
 def _indices(name: str, x: Indices, device: torch.device, count: Optional[int] = None) -> torch.Tensor:
-    """int32 [n] on the device; a list of ints is uploaded."""
+    """int32 [n] on the device; a list of ints is uploaded, from pinned memory: a pageable copy waits
+    for what the stream has queued."""
     if isinstance(x, torch.Tensor):
         if x.dim() != 1 or x.dtype is not torch.int32:
             raise ValueError(f"{name} must be int32 [n], got {x.dtype} {tuple(x.shape)}")
@@ -101,7 +103,10 @@ def _indices(name: str, x: Indices, device: torch.device, count: Optional[int] =
         vals = [int(v) for v in x]
         if any(not -2 ** 31 <= v < 2 ** 31 for v in vals):
             raise ValueError(f"{name} must be int32 values")
-        x = torch.tensor(vals, dtype=torch.int32, device=device)
+        pinned = uploads_pinned(device)
+        if device.type == "cuda" and not pinned:
+            raise ValueError(f"{name} must be a device tensor in a graph under capture: a replay cannot read a list again")
+        x = torch.tensor(vals, dtype=torch.int32, device="cpu", pin_memory=pinned).to(device, non_blocking=pinned)
     if count is not None and x.shape[0] != count:
         raise ValueError(f"{name} must have {count} entries, got {x.shape[0]}")
     return x

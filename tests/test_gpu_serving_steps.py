@@ -307,3 +307,50 @@ def test_needs_that_pass_32_bits_are_counted():
     for new, answer in ((16 * W, 2 ** 31 - 1 - NP), (16 * (W - 1), 1024 * (W - 1) - NP)):
         assert ia.grow_sequences(table, valid, refs, [0], [new], granted=lens).item() == answer
         assert lens.item() == 0 and not bool(valid.any()) and not bool(refs.any()) and bool((table[0, :, 0] == 5).all())
+
+
+def test_calls_with_lists_do_not_wait():
+    """Each call returns while 0.1 s of work queued before it still runs, and does what it should."""
+    import torch
+    import intent_attention as ia
+    s = Loop(4, 2, 5, 30)
+    x = torch.zeros((8192, 8192), dtype=torch.float16, device=_dev())
+    y = torch.empty_like(x)
+
+    def busy():
+        for _ in range(100):
+            torch.mm(x, x, out=y)
+        e = torch.cuda.Event()
+        e.record()
+        return e
+
+    for warm in (True, False):
+        calls = (lambda: ia.grow_sequences(*s.state(), [0, 2], [20, 3]),
+                 lambda: ia.fork_sequences(*s.state(), [0], [1], s.pools),
+                 lambda: ia.free_sequences(*s.state(), [0, 2], [1, 3]),
+                 lambda: ia.copy_pages(s.pools, [1], [29]),
+                 lambda: ia.free_sequences(*s.state(), [0, 1]))
+        for i, call in enumerate(calls):
+            done = None if warm else busy()
+            call()
+            assert warm or not done.query(), i
+            torch.cuda.synchronize()
+        assert int(s.refs.sum()) == 0 and not bool(s.valid.any())
+
+
+def test_lists_are_refused_under_capture():
+    """A replay could not read them again."""
+    import torch
+    import intent_attention as ia
+    s = Loop(4, 2, 5, 30)
+    seqs, new = _t([0, 2]), _t([20, 3])
+    ia.grow_sequences(*s.state(), seqs, new)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.zeros(1, device=_dev())
+        with pytest.raises(ValueError, match="capture"):
+            ia.grow_sequences(*s.state(), [0, 2], [20, 3])
+        with pytest.raises(ValueError, match="capture"):
+            ia.grow_sequences(*s.state(), seqs, [20, 3])
+    torch.cuda.synchronize()
+    assert s.valid.tolist() == [[20, 20], [0, 0], [3, 3], [0, 0]]
