@@ -191,6 +191,7 @@ class MxFp4Plan:
         """Launch on ``stream`` (default: torch's current stream)."""
         s = current_stream_handle(self.device) if stream is None else stream
         _launch(self.device, N.mx_attention, self.args, s, self._ws_ptr, self.workspace_bytes)
+        torch.autograd.graph.increment_version(self.out)        # written through a raw pointer
 
 
 def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor, *,
@@ -256,6 +257,4 @@ def mxfp4_paged_attention(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.
     plan = make_mxfp4_plan(q, pools, page_table, valid_tokens, q_lens=q_lens, causal=causal, sm_scale=sm_scale, out=out,
                            out_dtype=out_dtype, splits=splits)
     plan.run()
-    if out is not None:
-        torch.autograd.graph.increment_version(out)
     return plan.out

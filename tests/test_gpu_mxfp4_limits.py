@@ -136,3 +136,29 @@ def test_weights_of_16_bit_queries_keep_11_bits(L):
         rel = 2 * np.expm1(2 * score) + weight + 2.0 ** -22 + 2 * (T + 8) * 2.0 ** -24
         tol = rel * mass + T * 2.0 ** -31 * vmax + HALF["float32"] * np.abs(want)
         assert float((np.abs(got - want)[:, queries] / tol[:, queries]).max()) <= 1.0, dtype
+
+
+def test_a_plans_run_marks_its_output():
+    """torch's version counter of `out` moves with every run, the plan's own and a caller's, in place too."""
+    import torch
+    import intent_attention as ia
+    pools = ia.MxFp4Pools.empty(4, 64, _dev())
+    table, valid = _t(np.zeros((1, 2, 2), np.int32)), _t(np.full((1, 2), 20, np.int32))
+    q = torch.randn((1, 4, 64), device=_dev()).half()
+    for out in (None, torch.empty_like(q), q):
+        plan = ia.make_mxfp4_plan(q, pools, table, valid, out=out)
+        for _ in range(2):
+            before = plan.out._version
+            plan.run()
+            assert plan.out._version == before + 1
+        if out is not None:
+            before = out._version
+            ia.mxfp4_paged_attention(q, pools, table, valid, out=out)
+            assert out._version == before + 1
+    x = q.clone().requires_grad_()
+    y = (x * 1).sin()                                                # sin keeps its input for its gradient
+    with torch.no_grad():
+        kept = y.grad_fn._saved_self
+        ia.make_mxfp4_plan(kept, pools, table, valid, out=kept).run()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
