@@ -75,12 +75,20 @@ def _device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
     return tensors[0].device
 
 
+def _check_int32(**sizes: int) -> None:
+    """ValueError for sizes that the int32 fields of an argument block would wrap."""
+    for name, n in sizes.items():
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise ValueError(f"{name} {n} does not fit int32")
+
+
 def _check_cache(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens: torch.Tensor,
                  q_lens: Optional[torch.Tensor], B: int, D: int) -> Tuple[int, int, int]:
     """(Hkv, W, NP) of the pools and the metadata, or ValueError."""
     if page_table.dim() != 3 or page_table.shape[0] != B or page_table.dtype is not torch.int32:
         raise ValueError(f"page_table must be int32 [{B}, Hkv, W], got {page_table.dtype} {tuple(page_table.shape)}")
     _, Hkv, W = page_table.shape
+    _check_int32(table_width=W * PAGE_SIZE, rows=B * Hkv)
     if valid_tokens.shape != (B, Hkv) or valid_tokens.dtype is not torch.int32:
         raise ValueError(f"valid_tokens must be int32 [{B}, {Hkv}], got {valid_tokens.dtype} "
                          f"{tuple(valid_tokens.shape)}")
@@ -159,6 +167,7 @@ def read_mxfp4_tokens(pools: MxFp4Pools, page_table: torch.Tensor, valid_tokens:
         raise ValueError(f"dtype must be float16, bfloat16 or float32, got {dtype}")
     if count < 0:
         raise ValueError(f"count must not be negative, got {count}")
+    _check_int32(count=count)
     dev = _device("4-bit token cache", page_table, valid_tokens, q_lens, pools.k_codes, pools.k_scales, pools.v_codes,
                   pools.v_scales)
     if page_table.dim() != 3 or pools.k_codes.dim() != 3:
@@ -217,6 +226,7 @@ def make_mxfp4_plan(q: torch.Tensor, pools: MxFp4Pools, page_table: torch.Tensor
             raise ValueError(f"{name} must be contiguous")
     if q.stride(-1) != 1:
         raise ValueError("q must have a unit last stride")
+    _check_int32(splits=splits, q_len=L)
     if out is None:
         out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
     elif out.shape != q.shape or out.stride(-1) != 1:

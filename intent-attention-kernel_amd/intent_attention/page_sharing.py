@@ -38,7 +38,7 @@ import torch
 from . import _native as N
 from .decode_core import PAGE_SIZE, PagePools, current_stream_handle, uploads_pinned
 from .mla_core import LatentPools
-from .mxfp4 import MxFp4Pools, _device, _launch
+from .mxfp4 import MxFp4Pools, _check_int32, _device, _launch
 
 Pools = Union[PagePools, LatentPools, MxFp4Pools, torch.Tensor, Sequence[torch.Tensor]]
 Indices = Union[torch.Tensor, Sequence[int]]
@@ -87,6 +87,7 @@ def _check_state(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: tor
         raise ValueError(f"refs must be contiguous int32 [num_pages], got {refs.dtype} {tuple(refs.shape)}")
     if R == 0:
         raise ValueError("page_table has no rows per sequence")
+    _check_int32(table_width=W * PAGE_SIZE, rows=B * R)
     return B, R, W, refs.shape[0]
 
 

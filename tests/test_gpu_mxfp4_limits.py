@@ -162,3 +162,16 @@ def test_a_plans_run_marks_its_output():
         ia.make_mxfp4_plan(kept, pools, table, valid, out=kept).run()
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_numbers_that_an_int32_would_wrap():
+    import torch
+    import intent_attention as ia
+    pools = ia.MxFp4Pools.empty(4, 64, _dev())
+    table, valid = _t(np.zeros((1, 2, 2), np.int32)), _t(np.full((1, 2), 20, np.int32))
+    q = torch.randn((1, 4, 64), device=_dev()).half()
+    for splits in (2 ** 32, 2 ** 32 + 1, 2 ** 31, -2 ** 32):
+        with pytest.raises(ValueError, match="splits"):
+            ia.mxfp4_paged_attention(q, pools, table, valid, splits=splits)
+    with pytest.raises(ValueError, match="count"):
+        ia.read_mxfp4_tokens(pools, table[:0], valid[:0], 2 ** 32)

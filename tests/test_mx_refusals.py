@@ -4,8 +4,11 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
+import intent_attention as ia
 from intent_attention import _native as N
+from intent_attention import mxfp4, page_sharing
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -52,3 +55,16 @@ def test_grow_checks_its_arrays(n, text):
     a.num_arrays, a.arrays[0].base = n, 65536
     with pytest.raises(ValueError, match=text):
         N.grow_sequences(a, 0, 1 << 20, N.sequences_workspace(a))
+
+
+def test_sizes_that_an_int32_would_wrap():
+    """Tables of 2^32 entries and more, which a 32-bit field would make narrow ones."""
+    meta = lambda *s: torch.empty(s, dtype=torch.int32, device="meta")  # noqa: E731
+    pools = ia.MxFp4Pools.empty(4, 64, "cpu")
+    for B, H, W in ((1, 1, 2 ** 32), (1, 2, 2 ** 32 + 5), (1, 1, 2 ** 27), (2 ** 17, 2 ** 15, 1)):
+        with pytest.raises(ValueError, match="int32"):
+            mxfp4._check_cache(pools, meta(B, H, W), meta(B, H), None, B, 64)
+        with pytest.raises(ValueError, match="int32"):
+            page_sharing._check_state(meta(B, H, W), meta(B, H), meta(4))
+    assert mxfp4._check_cache(pools, meta(1, 1, 2 ** 27 - 1), meta(1, 1), None, 1, 64) == (1, 2 ** 27 - 1, 4)
+    assert page_sharing._check_state(meta(1, 1, 2 ** 27 - 1), meta(1, 1), meta(4)) == (1, 1, 2 ** 27 - 1, 4)
