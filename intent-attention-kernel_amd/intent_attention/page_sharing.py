@@ -3,7 +3,9 @@
 ``iak_compact_pages``, ``iak_copy_pages``, include/iak.h).
 
 The state is three int32 tensors on the device, which a program keeps beside its pools
-(``PagePools``, ``LatentPools``, ``MxFp4Pools``, or any tensors with a row per page):
+(``PagePools``, ``LatentPools``, ``MxFp4Pools``, or any tensors with a row per page; with
+``PagePools`` the decode's ``page_tags`` are such a tensor and go along in a list,
+``[*pools.tensors().values(), page_tags]``):
 
   page_table    [B, R, W]  the pages of row (b, r): R = KV heads for K/V pools; a latent
                            table [B, W] is passed as [B, 1, W]

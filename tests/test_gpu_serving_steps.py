@@ -354,3 +354,43 @@ def test_lists_are_refused_under_capture():
             ia.grow_sequences(*s.state(), seqs, [20, 3])
     torch.cuda.synchronize()
     assert s.valid.tolist() == [[20, 20], [0, 0], [3, 3], [0, 0]]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_pools_of_several_precisions_move_with_their_tags(D):
+    """The decode over pages that were compacted, forked and grown apart with their scales and tags:
+    the same bits as before, for the children as for their parents."""
+    import torch
+    import intent_attention as ia
+    from tests._pools import random_case, to_device_pools
+    B, Hkv, W, NP = 4, 2, 9, 120
+    q, host, _, _, tags = random_case(D, B, 8, Hkv, D, NP, W, {"FP16": .3, "FP8": .2, "INT8": .2, "INT4": .2, "INT4_RESIDUAL": .1})
+    rng = np.random.default_rng(D)
+    pools, tags, q = to_device_pools(host, _dev()), _t(tags), torch.from_numpy(q).to(_dev())
+    lens = [130, 0, 75, 0]
+    table, refs, pages = np.full((B, Hkv, W), -1), np.zeros(NP, int), iter(rng.permutation(NP))
+    for b, h in np.ndindex(B, Hkv):
+        for e in range(-(-lens[b] // 16)):
+            table[b, h, e] = next(pages)
+            refs[table[b, h, e]] = 1
+    table, refs, valid = _t(table), _t(refs), _t([[n] * Hkv for n in lens])
+    every = [*pools.tensors().values(), tags]
+
+    def decode():
+        counts = (valid + 15) // 16
+        return ia.paged_decode(q, pools, table, counts.int(), tags, valid_tokens=valid)
+
+    q[1], q[3] = q[0], q[2]
+    before = decode()
+    table, refs, page_map = ia.compact_pages(table, valid, refs, every)
+    assert int(refs[:int((refs > 0).sum())].min()) > 0
+    assert torch.equal(decode(), before)
+    assert ia.fork_sequences(table, valid, refs, [0, 2], [1, 3], every).item() == 0
+    out = decode()
+    assert torch.equal(out[[0, 2]], before[[0, 2]]) and torch.equal(out[[1, 3]], before[[0, 2]])
+    ia.free_sequences(table, valid, refs, [1, 3], [20, 20])            # to inside pages that are shared
+    cut = decode()
+    assert ia.grow_sequences(table, valid, refs, [1, 3], [1, 1], every).item() == 0
+    valid -= _t([[0], [1], [0], [1]])                                  # no token written: look at the copies alone
+    assert torch.equal(decode(), cut)
+    assert not torch.equal(table[1, :, 6], table[0, :, 6])             # 110 tokens: the seventh page is its own
