@@ -132,7 +132,7 @@ MxChoice choose(int B, int Hkv, int64_t rows, int W, int D, bool f32, int64_t fo
   if (rows > 16) kernel(128, big || f32 ? 2 : 3, 4, big ? (f32 ? 0.88 : 0.57) : (f32 ? 0.55 : 0.50));
   if (rows > 128 && !f32) kernel(256, 1, big ? 7 : 5, big ? 0.50 : 0.345);
   // Long rows of several sequences (parts above 2,048 tokens), at most a third of a round: shared out
-  // too, whatever the cost says, for it knows the longest row alone. 32 sequences x 8 KV heads of up to
+  // too, whatever the cost says, for it knows the table's width alone. 32 sequences x 8 KV heads of up to
   // 32,768 tokens, head_dim 128: equal 192 us for 182 (eight waves a tile, unsplit), a third to all of it
   // 136 for 158, one long among short ones 28 for 141; 64 of up to 16,384, more than a third: 222 for
   // 200, 161 for 154.
@@ -302,7 +302,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   if (p.total > 0 && (!workspace || workspace_bytes < p.total || !aligned16(workspace)))
     return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", p.total, workspace_bytes, workspace);
   iak::MxAttn k;
-  k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
+  k.B = a->batch; k.L = a->q_len; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
   k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.shares = p.shares; k.waves = p.waves;
   k.items = p.items; k.parted = p.total > 0;

@@ -10,8 +10,8 @@
 // stored, and four neighbouring lanes agree on the block's maximum over lane swaps. What
 // bounds it is the bytes. Long calls give a workgroup 16 tokens of one head, whose codes are
 // one run of memory wherever a page has room; calls of few tokens give it all heads of one.
-// 21,400 new tokens x 8 heads x 128 channels in 8 sequences padded to 4,001: append 29 us (111 MB,
-// 3.8 TB/s), read 24 us (the same and 43 MB of zeros, the codes from the caches); 64 new tokens:
+// 21,400 new tokens x 8 heads x 128 channels in 8 sequences padded to 4,001: append 27 us (111 MB,
+// 4.1 TB/s), read 23 us (the same and 43 MB of zeros, the codes from the caches); 64 new tokens:
 // 3.4 us each. Two or four tokens a thread changed nothing (50.5 us for both; 53.8).
 
 #include <hip/hip_runtime.h>
