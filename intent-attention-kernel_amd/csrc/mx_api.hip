@@ -302,7 +302,7 @@ iak_status iak_mx_attention(const iak_mx_attention_args* a, void* workspace, siz
   if (p.total > 0 && (!workspace || workspace_bytes < p.total || !aligned16(workspace)))
     return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", p.total, workspace_bytes, workspace);
   iak::MxAttn k;
-  k.B = a->batch; k.L = a->q_len; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
+  k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
   k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.shares = p.shares; k.waves = p.waves;
   k.items = p.items; k.parted = p.total > 0;
