@@ -16,8 +16,8 @@
 //                map written)
 //
 // What bounds them is latency: reads that wait for each other, and the launches. That a growing
-// row's last page may be shared costs two of them (entry, count): 1.1 us of 11 replayed, 64 x 8
-// rows of one new token grown and freed. Pages that
+// row's last page may be shared costs two of them (entry, count): 64 x 8 rows
+// of one new token grown and freed take 12.3 us replayed, without them 10.9. Pages that
 // move are bytes at the rate of a copy: 0.67 GB of K and V rows in 130 us.
 
 #include <hip/hip_runtime.h>
@@ -242,8 +242,14 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
           need = ragged_last(a, (int64_t)a.parents[j] * a.R + h, n, page);
         }
       }
-      int64_t all;
-      const int64_t before = scan_before<WAVES>(need, all);
+      int64_t all, before;
+      if (a.W <= 0x7FFFFFFF / PLAN_THREADS) {                    // 32 bits hold it: 4.6 us for 4.9
+        int all32;
+        before = scan_before<WAVES>((int)need, all32);
+        all = all32;
+      } else {
+        before = scan_before<WAVES>(need, all);
+      }
       if (k < rows) a.first[k] = (int)(total + before > 0x7FFFFFFF ? 0x7FFFFFFF : total + before);
       total += all;
     }
