@@ -631,10 +631,10 @@ iak_status iak_fake_quant_blocks(const iak_fake_quant_blocks_args* args, void* w
  * order; valid_tokens [batch, num_kv_heads] counts its tokens, clamped to 0 ..
  * 16 * table_width: a longer row is a full one to every call, so that its newest tokens are
  * the table's last slots (an append writes them over what is there; iak_grow_sequences
- * lets no row become longer than its table). The newest n tokens of a sequence are its last: with q_lens [batch]
- * (NULL: count for all; clamped to 0 .. count) token i < q_lens[b] is number
- * valid_tokens[b, h] - q_lens[b] + i of row (b, h). Page ids outside [0, num_pages) hold
- * no tokens.
+ * lets no row become longer than its table). The newest n tokens of a sequence are its last:
+ * with q_lens [batch] (NULL: count for all; clamped to 0 .. count) token i < q_lens[b] is
+ * number valid_tokens[b, h] - q_lens[b] + i of row (b, h). Page ids outside [0, num_pages)
+ * hold no tokens.
  */
 
 /* Write (append) or read the newest tokens: k, v [batch, count, num_kv_heads, head_dim]

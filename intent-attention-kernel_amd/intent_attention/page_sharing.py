@@ -29,6 +29,7 @@ last page to be copied and no pools, a forked sequence that has tokens or is its
 all the same: ``grow_sequences(..., granted=lens)`` leaves in ``lens`` how many tokens each
 sequence got room for, 0 then, and ``append_mxfp4_tokens(..., q_lens=lens)`` writes no more.
 Without it read the answer before tokens are appended, for they would land on older ones.
+A fork that was not done leaves its children empty: read its answer before they grow.
 """
 from __future__ import annotations
 
