@@ -62,6 +62,7 @@
  *   iak_fork_sequences,          kv_memory_manager.py:145-231; these keep page tables, lengths and reference
  *   iak_free_sequences,          counts on the device)
  *   iak_compact_pages, iak_copy_pages, iak_sequences_workspace, iak_compact_pages_workspace
+ *   iak_beam_select             (no counterpart: the choice of a beam search's continuations)
  *   iak_status_string           (no counterpart: the reference raises ValueError/RuntimeError in Python)
  */
 #ifndef IAK_H
@@ -74,7 +75,7 @@
 extern "C" {
 #endif
 
-#define IAK_ABI_VERSION 12
+#define IAK_ABI_VERSION 13
 
 /* Grid size from which merge_in_kernel = 2 merges inside the decode kernel; it
  * also does so on grids of at most IAK_MERGE_IN_KERNEL_SMALL_WORKGROUPS workgroups
@@ -787,6 +788,37 @@ typedef struct {
 
 iak_status iak_compact_pages_workspace(const iak_compact_pages_args* args, size_t* bytes);
 iak_status iak_compact_pages(const iak_compact_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A beam search's choice: of the continuations of each request's beams the `count` best.
+ * Candidate (k, v) of request b is beam k continued with token v:
+ *   scores[b, k] + logits[b, k, v] - log(sum_u exp(logits[b, k, u]))
+ * logits [batch, beams, vocab] (dtype IAK_DTYPE_*, element strides, unit vocabulary stride);
+ * scores [batch, beams] float32, the beams' sums of log-probabilities. finished [batch, beams]
+ * bytes (may be NULL): a beam whose byte is not 0 goes on as it is: its one candidate is
+ * end_token with scores[b, k], the other tokens' are -inf. A beam whose score is not finite,
+ * or that is not finished and has a logit that is NaN or +inf or none above -inf, is out of the search:
+ * all its candidates are -inf. Written, best first:
+ *   out_scores [batch, count] float32, out_tokens [batch, count] int32, and
+ *   out_parents [batch, count] int32: the beam's row b * beams + k.
+ * Equal candidates come in the order of k * vocab + v, those of -inf too. Candidates are compared
+ * in 64 bits, with the beams' normalisers off by about 1e-9 (they decide between different beams;
+ * those of one beam come in the order of their logits) and rounded to float32 at the end.
+ * 1 <= count <= 64, count <= beams * vocab < 2^31, beams <= 256. Workspace:
+ * iak_beam_select_workspace bytes, 16-byte aligned, as it comes; calls that share one on different
+ * streams race. */
+typedef struct {
+  int32_t batch, beams, vocab, count;
+  const void* logits; int32_t dtype; int64_t stride_b, stride_k;
+  const float* scores;
+  const uint8_t* finished;
+  int32_t end_token;
+  float* out_scores;
+  int32_t* out_parents;
+  int32_t* out_tokens;
+} iak_beam_select_args;
+
+iak_status iak_beam_select_workspace(const iak_beam_select_args* args, size_t* bytes);
+iak_status iak_beam_select(const iak_beam_select_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

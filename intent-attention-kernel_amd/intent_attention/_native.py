@@ -14,7 +14,7 @@ from typing import Optional
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # IAK_LIBRARY selects another build of the same ABI (e.g. a tuning variant)
 LIB_PATH = os.environ.get("IAK_LIBRARY") or os.path.join(_HERE, "libiak.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 IAK_OK, IAK_EINVAL, IAK_ENOTSUP, IAK_EHIP = 0, 1, 2, 3
 
@@ -262,6 +262,17 @@ class CompactPagesArgs(ctypes.Structure):
     ]
 
 
+class BeamSelectArgs(ctypes.Structure):
+    """Mirror of ``iak_beam_select_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("beams", c_i32), ("vocab", c_i32), ("count", c_i32),
+        ("logits", c_void_p), ("dtype", c_i32), ("stride_b", c_i64), ("stride_k", c_i64),
+        ("scores", c_void_p), ("finished", c_void_p), ("end_token", c_i32),
+        ("out_scores", c_void_p), ("out_parents", c_void_p), ("out_tokens", c_void_p),
+    ]
+
+
 EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_paged_decode_workspace", "iak_paged_decode",
             "iak_mla_decode_workspace", "iak_mla_decode", "iak_quantize_pages",
@@ -274,7 +285,8 @@ EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_timing_event_elapsed", "iak_timing_event_destroy",
             "iak_mx_append_tokens", "iak_mx_read_tokens", "iak_mx_attention_workspace", "iak_mx_attention",
             "iak_copy_pages", "iak_sequences_workspace", "iak_free_sequences", "iak_grow_sequences",
-            "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages")
+            "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages",
+            "iak_beam_select_workspace", "iak_beam_select")
 NOALLOC_SCRATCH_BYTES = 16 << 20   # IAK_NOALLOC_SCRATCH_BYTES
 
 _lib: Optional[ctypes.CDLL] = None
@@ -370,7 +382,9 @@ def load() -> ctypes.CDLL:
                        ("iak_grow_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_fork_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_compact_pages_workspace", (CompactPagesArgs, size_p)),
-                       ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p))):
+                       ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_beam_select_workspace", (BeamSelectArgs, size_p)),
+                       ("iak_beam_select", (BeamSelectArgs, c_void_p, ctypes.c_size_t, c_void_p))):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(args[0]), *args[1:]]
@@ -592,3 +606,13 @@ def compact_pages_workspace(args: CompactPagesArgs) -> int:
 
 def compact_pages(args: CompactPagesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
     check(load().iak_compact_pages(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))
+
+
+def beam_select_workspace(args: BeamSelectArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_beam_select_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def beam_select(args: BeamSelectArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
+    check(load().iak_beam_select(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))
