@@ -62,6 +62,8 @@
  *   iak_fork_sequences,          kv_memory_manager.py:145-231; these keep page tables, lengths and reference
  *   iak_free_sequences,          counts on the device)
  *   iak_compact_pages, iak_copy_pages, iak_sequences_workspace, iak_compact_pages_workspace
+ *   iak_reorder_sequences, iak_reorder_sequences_workspace
+ *                               (no counterpart: the beams' page tables in the order of that choice)
  *   iak_beam_select             (no counterpart: the choice of a beam search's continuations)
  *   iak_status_string           (no counterpart: the reference raises ValueError/RuntimeError in Python)
  */
@@ -766,6 +768,18 @@ iak_status iak_sequences_workspace(const iak_sequences_args* args, size_t* bytes
 iak_status iak_free_sequences(const iak_sequences_args* args, void* stream);
 iak_status iak_grow_sequences(const iak_sequences_args* args, void* workspace, size_t workspace_bytes, void* stream);
 iak_status iak_fork_sequences(const iak_sequences_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequence seqs[i] becomes a copy of what parents[i] was before the call, all at once: parents may
+ * be listed as seqs themselves, and any number of times (seqs[i] = parents[i]: it stays as it is). Rows
+ * share the parent's pages (refs + 1) and let go of their own (refs - 1; entries no longer in use
+ * become -1). A last page that is not full stays with one owner: the parent if it stays itself or is not among
+ * seqs, else its first child in the call; the others get copies of it (every array) in free pages, the lowest ids
+ * first, in the order of (i, row): pages that were free before the call. All of it or nothing:
+ * missing[0] is 0 done; n > 0: n more free pages would be needed; -1: an index outside
+ * [0, num_seqs) or listed twice among seqs. seqs, parents and missing are none of the arrays that
+ * are changed. Workspace: iak_reorder_sequences_workspace bytes, 16-byte aligned. */
+iak_status iak_reorder_sequences_workspace(const iak_sequences_args* args, size_t* bytes);
+iak_status iak_reorder_sequences(const iak_sequences_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Compaction: with L pages in use (refs > 0), those with ids >= L move to the free ids
  * below L, the highest to the lowest: page_map [num_pages] is the new id of every page (-1:

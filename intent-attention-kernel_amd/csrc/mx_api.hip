@@ -221,11 +221,10 @@ iak_status validate_sequences(const iak_sequences_args* a) {
   return IAK_OK;
 }
 
-// grow and fork: `null`: the name of an argument they need and did not get
-iak_status validate_planned(const iak_sequences_args* a, const char* null, const void* workspace, size_t workspace_bytes) {
+// grow, fork and reorder: `null`: the name of an argument they need and did not get
+iak_status validate_planned(const iak_sequences_args* a, const char* null, size_t need, const void* workspace, size_t workspace_bytes) {
   if (null) return fail(IAK_EINVAL, "%s is NULL", null);
   if (!a->missing) return fail(IAK_EINVAL, "missing is NULL");
-  const size_t need = iak::sequences_workspace(*a);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(IAK_EINVAL, "workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", need, workspace_bytes, workspace);
   return IAK_OK;
@@ -349,7 +348,7 @@ iak_status iak_free_sequences(const iak_sequences_args* a, void* stream) {
 
 iak_status iak_grow_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   iak_status st = validate_sequences(a);
-  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->new_tokens ? "new_tokens" : nullptr, workspace, workspace_bytes);
+  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->new_tokens ? "new_tokens" : nullptr, iak::sequences_workspace(*a), workspace, workspace_bytes);
   if (st == IAK_OK) st = validate_granted(a);
   if (st == IAK_OK) st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
   if (st != IAK_OK) return st;
@@ -358,10 +357,27 @@ iak_status iak_grow_sequences(const iak_sequences_args* a, void* workspace, size
 
 iak_status iak_fork_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   iak_status st = validate_sequences(a);
-  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->parents ? "parents" : nullptr, workspace, workspace_bytes);
+  if (st == IAK_OK) st = validate_planned(a, a && a->count > 0 && !a->parents ? "parents" : nullptr, iak::sequences_workspace(*a), workspace, workspace_bytes);
   if (st == IAK_OK) st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
   if (st != IAK_OK) return st;
   return launched(iak::launch_fork_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "fork sequences");
+}
+
+iak_status iak_reorder_sequences_workspace(const iak_sequences_args* a, size_t* bytes) {
+  if (!bytes) return fail(IAK_EINVAL, "bytes is NULL");
+  iak_status st = validate_sequences(a);
+  if (st != IAK_OK) return st;
+  *bytes = iak::reorder_workspace(*a);
+  return IAK_OK;
+}
+
+iak_status iak_reorder_sequences(const iak_sequences_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  iak_status st = validate_sequences(a);
+  if (st == IAK_OK)
+    st = validate_planned(a, a->count > 0 && !a->parents ? "parents" : nullptr, iak::reorder_workspace(*a), workspace, workspace_bytes);
+  if (st == IAK_OK) st = validate_arrays(a->num_arrays, a->arrays, a->num_pages);
+  if (st != IAK_OK) return st;
+  return launched(iak::launch_reorder_sequences(*a, workspace, reinterpret_cast<hipStream_t>(stream)), "reorder sequences");
 }
 
 iak_status iak_compact_pages_workspace(const iak_compact_pages_args* a, size_t* bytes) {

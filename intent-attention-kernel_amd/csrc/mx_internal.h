@@ -55,6 +55,8 @@ size_t sequences_workspace(const iak_sequences_args& a);
 hipError_t launch_free_sequences(const iak_sequences_args& a, hipStream_t stream);
 hipError_t launch_grow_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream);
 hipError_t launch_fork_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream);
+size_t reorder_workspace(const iak_sequences_args& a);
+hipError_t launch_reorder_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream);
 size_t compact_workspace(const iak_compact_pages_args& a);
 hipError_t launch_compact_pages(const iak_compact_pages_args& a, void* workspace, hipStream_t stream);
 

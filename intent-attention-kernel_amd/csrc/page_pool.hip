@@ -11,6 +11,10 @@
 //                                  bits, entries, counts, the copied last page (a fork's where it
 //                                  has room, a growing row's where others hold it too)
 //   free         seq_free_kernel   a workgroup per row
+//   reorder      reorder_plan_kernel   as seq_plan_kernel, and a workgroup per row that puts the parent's
+//                                      entries aside: rows become each other's copies at once
+//                reorder_apply_kernel  a workgroup per row: counts and entries where they differ (rows
+//                                      that share a beginning leave it alone), the last page
 //   compact      compact_count_kernel, compact_rank_kernel (which page goes where; for few pages
 //                compact_small_kernel), compact_apply_kernel (pages copied, table, counts and
 //                map written)
@@ -258,16 +262,21 @@ template <int KIND> __device__ __forceinline__ int plan_call(const SeqArgs& a, i
   return (int)(total > 0x7FFFFFFF ? 0x7FFFFFFF : total);
 }
 
-template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
+// The free pages of group blockIdx.x: a bit each, and their number.
+__device__ __forceinline__ void mark_free(const SeqArgs& a) {
   static_assert(PLAN_THREADS == PAGE_GROUP, "a thread a page");
+  const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + threadIdx.x;
+  const bool free_page = id < a.NP && a.refs[id] <= 0;
+  const uint64_t bits = __builtin_amdgcn_ballot_w64(free_page);
+  if ((threadIdx.x & 63) == 0) a.free_bits[id >> 6] = bits;
+  int total;
+  scan_before<PLAN_THREADS / 64>((int)free_page, total);
+  if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
+}
+
+template <int KIND> __global__ __launch_bounds__(PLAN_THREADS) void seq_plan_kernel(const SeqArgs a) {
   if ((int)blockIdx.x < a.groups) {
-    const int64_t id = (int64_t)blockIdx.x * PAGE_GROUP + threadIdx.x;
-    const bool free_page = id < a.NP && a.refs[id] <= 0;
-    const uint64_t bits = __builtin_amdgcn_ballot_w64(free_page);
-    if ((threadIdx.x & 63) == 0) a.free_bits[id >> 6] = bits;
-    int total;
-    scan_before<PLAN_THREADS / 64>((int)free_page, total);
-    if (threadIdx.x == 0) a.group_free[blockIdx.x] = total;
+    mark_free(a);
     return;
   }
   __shared__ int refused;
@@ -504,6 +513,118 @@ __global__ __launch_bounds__(POOL_THREADS) void compact_apply_kernel(const Compa
   }
 }
 
+// --------------------------------------------------------------------------- //
+// Reorder
+// --------------------------------------------------------------------------- //
+
+struct ReorderArgs : SeqArgs {
+  int32_t* heir;                       // [num_seqs] who has a sequence's last page afterwards: -1 itself, or number in the call
+  int32_t* stage;                      // [count * R, W] the parents' entries in use
+  int32_t* lengths;                    // [count * R] and their lengths
+};
+
+// Whether row (j, h) of the call gets a page of its own: it becomes another's copy, whose last page is
+// not full and goes to someone else.
+__device__ __forceinline__ bool reorder_copies(const ReorderArgs& a, int j, int h, int& n, int64_t& page) {
+  const int p = a.parents[j];
+  return p != a.seqs[j] && ragged_last(a, (int64_t)p * a.R + h, n, page) && a.heir[p] != j;
+}
+
+__device__ __forceinline__ int plan_reorder(const ReorderArgs& a, int& refused) {
+  constexpr int WAVES = PLAN_THREADS / 64;
+  if (threadIdx.x == 0) refused = 0;
+  for (int k = threadIdx.x; k < a.num_seqs; k += PLAN_THREADS) { a.marks[k] = 0; a.heir[k] = -1; }
+  __threadfence_block();
+  __syncthreads();
+  bool bad = false;
+  for (int k = threadIdx.x; k < a.count; k += PLAN_THREADS) {
+    const int s = a.seqs[k], p = a.parents[k];
+    if (p < 0 || p >= a.num_seqs) bad = true;
+    if (s < 0 || s >= a.num_seqs) { bad = true; continue; }
+    if (atomicAdd(&a.marks[s], 1) != 0) bad = true;
+    a.heir[s] = 0x7FFFFFFF;            // its own row goes to another
+  }
+  if (bad) refused = 1;
+  __threadfence_block();
+  __syncthreads();
+  if (refused) return 0;               // uniform
+  for (int k = threadIdx.x; k < a.count; k += PLAN_THREADS) {
+    const int s = a.seqs[k], p = a.parents[k];
+    atomicMin(&a.heir[p], s == p ? -1 : k);
+  }
+  __threadfence_block();
+  __syncthreads();
+  int64_t total = 0;
+  const int rows = a.count * a.R;
+  for (int k0 = 0; k0 < rows; k0 += PLAN_THREADS) {
+    const int k = k0 + threadIdx.x;
+    int need = 0, all, n;
+    int64_t page;
+    if (k < rows) { const int j = k / a.R; need = reorder_copies(a, j, k - j * a.R, n, page); }
+    const int before = scan_before<WAVES>(need, all);
+    if (k < rows) a.first[k] = (int)total + before;
+    total += all;
+  }
+  return (int)total;                   // a page a row: below 2^24
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void reorder_plan_kernel(const ReorderArgs a) {
+  if ((int)blockIdx.x < a.groups) {
+    mark_free(a);
+    return;
+  }
+  if ((int)blockIdx.x == a.groups) {
+    __shared__ int refused;
+    const int need = plan_reorder(a, refused);
+    if (threadIdx.x == 0) { a.head[0] = need; a.head[1] = refused; }
+    return;
+  }
+  // a wave a row
+  const int k = ((int)blockIdx.x - a.groups - 1) * (PLAN_THREADS / 64) + (int)(threadIdx.x >> 6);
+  if (k >= a.count * a.R) return;
+  const int j = k / a.R, p = a.parents[j];
+  if (p < 0 || p >= a.num_seqs || p == a.seqs[j]) return;
+  const int64_t parent = (int64_t)p * a.R + (k - j * a.R);
+  const int tokens = a.valid[parent], n = used_entries(tokens, a.PSZ, a.W), lane = threadIdx.x & 63;
+  const int32_t* from = a.table + parent * a.W;
+  int32_t* to = a.stage + (int64_t)k * a.W;
+  for (int e = lane; e < n; e += 64) to[e] = from[e];
+  if (lane == 0) a.lengths[k] = tokens;
+}
+
+__global__ __launch_bounds__(POOL_THREADS) void reorder_apply_kernel(const ReorderArgs a) {
+  const int k = blockIdx.x, j = k / a.R, h = k - j * a.R;
+  const bool listed = a.count > 0;
+  const int need = a.head[0], refused = a.head[1], seq = listed ? a.seqs[j] : 0, first = listed ? a.first[k] : 0;
+  const int after = k + 1 < (int)gridDim.x ? a.first[k + 1] : need, parent = listed ? a.parents[j] : 0;
+  const int per = (a.groups + POOL_THREADS - 1) / POOL_THREADS;
+  int own = 0, all;
+  for (int i = 0, g = (int)threadIdx.x * per; i < per && g < a.groups; ++i, ++g) own += a.group_free[g];
+  const int before = scan_before<POOL_THREADS / 64>(own, all);
+  const int verdict = refused ? -1 : (need > all ? need - all : 0);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.missing[0] = verdict;
+  if (verdict != 0 || !listed || seq == parent) return;
+  const int64_t row = (int64_t)seq * a.R + h;
+  int32_t* entries = a.table + row * a.W;
+  const int32_t* to = a.stage + (int64_t)k * a.W;
+  const int was = used_entries(a.valid[row], a.PSZ, a.W), tokens = a.lengths[k], n = used_entries(tokens, a.PSZ, a.W);
+  const bool copies = after > first;
+  __shared__ int fresh;
+  if (copies) take_pages(a, per, before, own, first, 1, [&](int, int id) { fresh = id; });
+  __syncthreads();                     // every thread has read the old length
+  for (int e = threadIdx.x; e < was || e < n; e += POOL_THREADS) {
+    const bool anew = copies && e == n - 1;
+    const int old = e < was ? entries[e] : -1, id = anew ? fresh : e < n ? to[e] : -1;
+    if (e < was && e < n && old == id) continue;
+    if (old >= 0 && old < a.NP && e < was) atomicSub(&a.refs[old], 1);
+    if (anew) a.refs[id] = 1;
+    else if (id >= 0 && id < a.NP) atomicAdd(&a.refs[id], 1);
+    entries[e] = id;
+  }
+  if (copies) copy_page<false>(a.arrays, to[n - 1], fresh);
+  if (threadIdx.x == 0) a.valid[row] = tokens;
+}
+
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 SeqArgs seq_args(const iak_sequences_args& a, void* workspace) {
@@ -563,6 +684,27 @@ hipError_t launch_grow_sequences(const iak_sequences_args& a, void* workspace, h
 }
 hipError_t launch_fork_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
   return launch_seq<SEQ_FORK>(a, workspace, stream);
+}
+
+// What a reorder keeps behind the rest.
+size_t reorder_workspace(const iak_sequences_args& a) {
+  const size_t rows = (size_t)a.count * a.rows_per_seq;
+  return sequences_workspace(a) + up256(4 * (size_t)a.num_seqs) + up256(4 * rows * a.table_width) + up256(4 * rows);
+}
+hipError_t launch_reorder_sequences(const iak_sequences_args& a, void* workspace, hipStream_t stream) {
+  ReorderArgs r;
+  static_cast<SeqArgs&>(r) = seq_args(a, workspace);
+  const int rows = a.count * a.rows_per_seq;
+  char* p = reinterpret_cast<char*>(workspace) + sequences_workspace(a);
+  r.heir = reinterpret_cast<int32_t*>(p);
+  p += up256(4 * (size_t)a.num_seqs);
+  r.stage = reinterpret_cast<int32_t*>(p);
+  p += up256(4 * (size_t)rows * a.table_width);
+  r.lengths = reinterpret_cast<int32_t*>(p);
+  constexpr int ROWS = PLAN_THREADS / 64;
+  hipLaunchKernelGGL(reorder_plan_kernel, dim3(r.groups + 1 + (rows + ROWS - 1) / ROWS), dim3(PLAN_THREADS), 0, stream, r);
+  hipLaunchKernelGGL(reorder_apply_kernel, dim3(rows > 0 ? rows : 1), dim3(POOL_THREADS), 0, stream, r);
+  return hipGetLastError();
 }
 
 size_t compact_workspace(const iak_compact_pages_args& a) {

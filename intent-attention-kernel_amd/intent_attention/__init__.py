@@ -54,7 +54,14 @@ from .mxfp4 import (
     mxfp4_paged_attention,
     read_mxfp4_tokens,
 )
-from .page_sharing import compact_pages, copy_pages, fork_sequences, free_sequences, grow_sequences
+from .page_sharing import (
+    compact_pages,
+    copy_pages,
+    fork_sequences,
+    free_sequences,
+    grow_sequences,
+    reorder_sequences,
+)
 from .beam_search import beam_select
 from .kv_memory_manager import KVMemoryManager, PageFormatPolicy, PageState, PageStorageFormat
 from .prefetch import BlockPrefetcher, get_prefetch_stream, get_prefetcher, launch_prefetch_pages, reset_prefetcher
@@ -86,7 +93,7 @@ __all__ = [
     "build_page_tables", "routing_to_kernel_tensors",
     "MxFp4Plan", "MxFp4Pools", "append_mxfp4_tokens", "make_mxfp4_plan", "mxfp4_paged_attention", "read_mxfp4_tokens",
     "beam_select",
-    "compact_pages", "copy_pages", "fork_sequences", "free_sequences", "grow_sequences",
+    "compact_pages", "copy_pages", "fork_sequences", "free_sequences", "grow_sequences", "reorder_sequences",
     "KVMemoryManager", "PageFormatPolicy", "PageState", "PageStorageFormat",
     "BlockPrefetcher", "get_prefetch_stream", "get_prefetcher", "launch_prefetch_pages", "reset_prefetcher",
     "AdaptiveFormatKernelConfig", "AdaptivePageFormat", "adaptive_format_decode_attention_reference_dispatch",

@@ -286,7 +286,7 @@ EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_mx_append_tokens", "iak_mx_read_tokens", "iak_mx_attention_workspace", "iak_mx_attention",
             "iak_copy_pages", "iak_sequences_workspace", "iak_free_sequences", "iak_grow_sequences",
             "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages",
-            "iak_beam_select_workspace", "iak_beam_select")
+            "iak_beam_select_workspace", "iak_beam_select", "iak_reorder_sequences_workspace", "iak_reorder_sequences")
 NOALLOC_SCRATCH_BYTES = 16 << 20   # IAK_NOALLOC_SCRATCH_BYTES
 
 _lib: Optional[ctypes.CDLL] = None
@@ -383,6 +383,8 @@ def load() -> ctypes.CDLL:
                        ("iak_fork_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_compact_pages_workspace", (CompactPagesArgs, size_p)),
                        ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_reorder_sequences_workspace", (SequencesArgs, size_p)),
+                       ("iak_reorder_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_beam_select_workspace", (BeamSelectArgs, size_p)),
                        ("iak_beam_select", (BeamSelectArgs, c_void_p, ctypes.c_size_t, c_void_p))):
         fn = getattr(lib, name)
@@ -596,6 +598,16 @@ def grow_sequences(args: SequencesArgs, stream: int, workspace: int, workspace_b
 
 def fork_sequences(args: SequencesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
     check(load().iak_fork_sequences(ctypes.byref(args), workspace, workspace_bytes, stream or None))
+
+
+def reorder_sequences_workspace(args: SequencesArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_reorder_sequences_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def reorder_sequences(args: SequencesArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
+    check(load().iak_reorder_sequences(ctypes.byref(args), workspace, workspace_bytes, stream or None))
 
 
 def compact_pages_workspace(args: CompactPagesArgs) -> int:

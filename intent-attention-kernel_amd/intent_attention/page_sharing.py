@@ -1,6 +1,6 @@
 """Pages of a KV cache handed out, shared, given back and moved, on the MI355X
 (``iak_grow_sequences``, ``iak_fork_sequences``, ``iak_free_sequences``,
-``iak_compact_pages``, ``iak_copy_pages``, include/iak.h).
+``iak_reorder_sequences``, ``iak_compact_pages``, ``iak_copy_pages``, include/iak.h).
 
 The state is three int32 tensors on the device, which a program keeps beside its pools
 (``PagePools``, ``LatentPools``, ``MxFp4Pools``, or any tensors with a row per page; with
@@ -17,12 +17,14 @@ The state is three int32 tensors on the device, which a program keeps beside its
 * ``fork_sequences`` makes empty sequences copies of others: full pages are shared, a last
   page with room is copied, so that both may append;
 * ``free_sequences`` lets sequences go, or their newest tokens;
+* ``reorder_sequences`` makes sequences copies of each other, all at once: a beam search's choice
+  (``beam_select``);
 * ``compact_pages`` moves the pages in use to the lowest ids and returns the new table;
 * ``copy_pages`` copies pages from id to id.
 
 Nothing waits for the device; indices and counts may be lists, except in a graph under capture.
 Which page goes where is a function of the arguments alone.
-``grow_sequences`` and ``fork_sequences`` do all of a call or nothing of it, and return an
+``grow_sequences``, ``fork_sequences`` and ``reorder_sequences`` do all of a call or nothing of it, and return an
 int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
 of range or listed twice, a negative count, a row that would be longer than its table, a
 last page to be copied and no pools, a forked sequence that has tokens or is itself a parent). What is queued behind a call that was not done runs
@@ -133,13 +135,14 @@ def _written(*tensors: torch.Tensor) -> None:
     torch.autograd.graph.increment_version(tensors)     # written through raw pointers
 
 
-def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor]) -> torch.Tensor:
+def _planned(launch, a, dev: torch.device, missing: Optional[torch.Tensor],
+             workspace=N.sequences_workspace) -> torch.Tensor:
     if missing is None:
         missing = torch.empty(1, dtype=torch.int32, device=dev)
     elif missing.shape != (1,) or missing.dtype != torch.int32 or missing.device != dev:
         raise ValueError(f"missing must be int32 [1] on {dev}, got {missing.dtype} {tuple(missing.shape)}")
     a.missing = missing.data_ptr()
-    size = N.sequences_workspace(a)
+    size = workspace(a)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _launch(dev, launch, a, current_stream_handle(dev), ws.data_ptr(), size)
     return missing
@@ -182,6 +185,24 @@ def fork_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: t
     parents = _indices("parents", parents, dev, children.shape[0])
     a.parents = parents.data_ptr()
     missing = _planned(N.fork_sequences, a, dev, missing)
+    _written(page_table, valid_tokens, refs, missing, *tensors)
+    return missing
+
+
+def reorder_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: torch.Tensor, seqs: Indices,
+                      parents: Indices, pools: Optional[Pools] = None, *,
+                      missing: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sequence ``seqs[i]`` becomes a copy of what ``parents[i]`` was before the call, all of them at
+    once: a parent may be listed many times, and be among ``seqs`` itself (``seqs[i] == parents[i]``
+    stays as it is). Full pages are shared, and rows let go of the pages they had. A last page that
+    is not full stays with one owner, the parent if it stays itself or is not among ``seqs``, else its first
+    child in the call; the others get copies of it, in every tensor of ``pools``, in pages that were free
+    before the call (the lowest ids first, in the order of i, row). All or nothing; returns
+    ``missing`` (module docstring)."""
+    a, dev, seqs, tensors = _sequences("page sharing", page_table, valid_tokens, refs, seqs, pools)
+    parents = _indices("parents", parents, dev, seqs.shape[0])
+    a.parents = parents.data_ptr()
+    missing = _planned(N.reorder_sequences, a, dev, missing, N.reorder_sequences_workspace)
     _written(page_table, valid_tokens, refs, missing, *tensors)
     return missing
 

@@ -109,6 +109,48 @@ class Pages:
             self.valid[c][h] = self.valid[p][h]
         return 0
 
+    def reorder(self, seqs, parents):
+        if not self._sound(seqs) or not all(0 <= p < len(self.table) for p in parents):
+            return -1
+        old = [[(self.valid[b][h], self.used(b, h), list(row)) for h, row in enumerate(s)] for b, s in enumerate(self.table)]
+        heir = {}
+        for c, p in zip(seqs, parents):
+            if p not in seqs or (p, p) in zip(seqs, parents):
+                heir[p] = p
+            heir.setdefault(p, c)
+        plan = []
+        for c, p in zip(seqs, parents):
+            for h in range(len(self.table[p])):
+                tokens, n, row = old[p][h]
+                plan.append((c, p, h, c != p and heir[p] != c and n > 0 and n * PS > tokens and self._in(row[n - 1])))
+        free = self._free()
+        need = sum(x[3] for x in plan)
+        if need > len(free):
+            return need - len(free)
+        it = iter(free)
+        fresh = []
+        for c, p, h, own in plan:
+            if c == p:
+                continue
+            tokens, n, row = old[p][h]
+            was, mine = old[c][h][1:]
+            new = row[:n]
+            if own:
+                new[-1] = next(it)
+                self.copied.append((row[n - 1], new[-1]))
+                fresh.append(new[-1])
+            for page in mine[:was]:
+                if self._in(page):
+                    self.refs[page] -= 1
+            for page in row[:n - 1] if own else new:
+                if self._in(page):
+                    self.refs[page] += 1
+            self.table[c][h] = new + [-1] * (was - n) + mine[max(n, was):]
+            self.valid[c][h] = tokens
+        for page in fresh:
+            self.refs[page] = 1
+        return 0
+
     def compact(self):
         """(table, refs, page_map, moves); the state itself stays as it is."""
         live = [i for i, r in enumerate(self.refs) if r > 0]
