@@ -64,6 +64,7 @@
  *   iak_compact_pages, iak_copy_pages, iak_sequences_workspace, iak_compact_pages_workspace
  *   iak_reorder_sequences, iak_reorder_sequences_workspace
  *                               (no counterpart: the beams' page tables in the order of that choice)
+ *   iak_rotary_append           (no counterpart: keys rotated by position and stored with their values token by token)
  *   iak_beam_select             (no counterpart: the choice of a beam search's continuations)
  *   iak_status_string           (no counterpart: the reference raises ValueError/RuntimeError in Python)
  */
@@ -802,6 +803,45 @@ typedef struct {
 
 iak_status iak_compact_pages_workspace(const iak_compact_pages_args* args, size_t* bytes);
 iak_status iak_compact_pages(const iak_compact_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The newest tokens' keys, rotated by their positions, and values into their sequences' pages,
+ * and their queries rotated along. A pair of channels (x, y) of a token at position p becomes
+ *   (x cos a - y sin a, x sin a + y cos a),  a = p * inv_freq[i],
+ * pair i < rotary_dim / 2 being channels (i, i + rotary_dim / 2), or with interleaved = 1
+ * (2i, 2i + 1); channels from rotary_dim on stay as they are. inv_freq [rotary_dim / 2] float32 on the
+ * device; a is taken in 64 bits, so that far positions lose nothing.
+ *   k, v       [batch, count, num_kv_heads, head_dim], q, q_out [batch, count, num_q_heads,
+ *              head_dim] (q and q_out may both be NULL; q_out may be q), one dtype
+ *              (IAK_DTYPE_*), element strides, unit channel stride
+ *   positions  [batch, count] int32, rows position_stride_b apart; NULL: a token's number in
+ *              its row, valid_tokens - q_lens + i (a query's in the row of its KV head)
+ * page_table, valid_tokens and q_lens as for iak_mx_append_tokens: token i < q_lens[b] is number
+ * valid_tokens[b, h] - q_lens[b] + i of row (b, h); tokens before 0 or without a page are left
+ * out. Written to k_pages, v_pages, float16 [num_pages, 16, head_dim] (rotated in float32, rounded once;
+ * past float16's range: infinite), or else to the 4-bit pools k_codes .. v_scales, rounded as iak_mx_append_tokens rounds, from 64
+ * bits. With page_tags [num_pages] (float16 pages only) every page that a token goes to gets `tag`.
+ * q_out is written whole: zeros for i >= q_lens[b]. Two tokens that address one slot race.
+ * head_dim 64 or 128, page_size 16, rotary_dim a multiple of 16. Code pools 4-byte aligned. */
+typedef struct {
+  int32_t batch, count, num_q_heads, num_kv_heads, head_dim, rotary_dim, interleaved, page_size, table_width;
+  int64_t num_pages;
+  int32_t dtype;
+  const void* q; int64_t q_stride_b, q_stride_t, q_stride_h;
+  void* q_out; int64_t q_out_stride_b, q_out_stride_t, q_out_stride_h;
+  const void* k; int64_t k_stride_b, k_stride_t, k_stride_h;
+  const void* v; int64_t v_stride_b, v_stride_t, v_stride_h;
+  const float* inv_freq;
+  const int32_t* positions; int64_t position_stride_b;
+  const int32_t* page_table;
+  const int32_t* valid_tokens;
+  const int32_t* q_lens;
+  void* k_pages; void* v_pages;
+  void* k_codes; void* k_scales; void* v_codes; void* v_scales;
+  int32_t* page_tags;
+  int32_t tag;
+} iak_rotary_append_args;
+
+iak_status iak_rotary_append(const iak_rotary_append_args* args, void* stream);
 
 /* A beam search's choice: of the continuations of each request's beams the `count` best.
  * Candidate (k, v) of request b is beam k continued with token v:

@@ -262,6 +262,25 @@ class CompactPagesArgs(ctypes.Structure):
     ]
 
 
+class RotaryAppendArgs(ctypes.Structure):
+    """Mirror of ``iak_rotary_append_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("count", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("rotary_dim", c_i32), ("interleaved", c_i32), ("page_size", c_i32), ("table_width", c_i32),
+        ("num_pages", c_i64), ("dtype", c_i32),
+        ("q", c_void_p), ("q_stride_b", c_i64), ("q_stride_t", c_i64), ("q_stride_h", c_i64),
+        ("q_out", c_void_p), ("q_out_stride_b", c_i64), ("q_out_stride_t", c_i64), ("q_out_stride_h", c_i64),
+        ("k", c_void_p), ("k_stride_b", c_i64), ("k_stride_t", c_i64), ("k_stride_h", c_i64),
+        ("v", c_void_p), ("v_stride_b", c_i64), ("v_stride_t", c_i64), ("v_stride_h", c_i64),
+        ("inv_freq", c_void_p), ("positions", c_void_p), ("position_stride_b", c_i64),
+        ("page_table", c_void_p), ("valid_tokens", c_void_p), ("q_lens", c_void_p),
+        ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+        ("page_tags", c_void_p), ("tag", c_i32),
+    ]
+
+
 class BeamSelectArgs(ctypes.Structure):
     """Mirror of ``iak_beam_select_args`` (include/iak.h)."""
 
@@ -286,7 +305,8 @@ EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_mx_append_tokens", "iak_mx_read_tokens", "iak_mx_attention_workspace", "iak_mx_attention",
             "iak_copy_pages", "iak_sequences_workspace", "iak_free_sequences", "iak_grow_sequences",
             "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages",
-            "iak_beam_select_workspace", "iak_beam_select", "iak_reorder_sequences_workspace", "iak_reorder_sequences")
+            "iak_beam_select_workspace", "iak_beam_select", "iak_reorder_sequences_workspace", "iak_reorder_sequences",
+            "iak_rotary_append")
 NOALLOC_SCRATCH_BYTES = 16 << 20   # IAK_NOALLOC_SCRATCH_BYTES
 
 _lib: Optional[ctypes.CDLL] = None
@@ -385,6 +405,7 @@ def load() -> ctypes.CDLL:
                        ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_reorder_sequences_workspace", (SequencesArgs, size_p)),
                        ("iak_reorder_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_rotary_append", (RotaryAppendArgs, c_void_p)),
                        ("iak_beam_select_workspace", (BeamSelectArgs, size_p)),
                        ("iak_beam_select", (BeamSelectArgs, c_void_p, ctypes.c_size_t, c_void_p))):
         fn = getattr(lib, name)
@@ -628,3 +649,7 @@ def beam_select_workspace(args: BeamSelectArgs) -> int:
 
 def beam_select(args: BeamSelectArgs, stream: int, workspace: int, workspace_bytes: int) -> None:
     check(load().iak_beam_select(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))
+
+
+def rotary_append(args: RotaryAppendArgs, stream: int) -> None:
+    check(load().iak_rotary_append(ctypes.byref(args), stream or None))
