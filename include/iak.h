@@ -64,6 +64,9 @@
  *   iak_compact_pages, iak_copy_pages, iak_sequences_workspace, iak_compact_pages_workspace
  *   iak_reorder_sequences, iak_reorder_sequences_workspace
  *                               (no counterpart: the beams' page tables in the order of that choice)
+ *   iak_paged_chunk, iak_paged_chunk_workspace
+ *                               (no counterpart: the reference attends one query token a sequence,
+ *                               fused_selected_quant_decode.py:408-464; these several, over the same pages)
  *   iak_rotary_append           (no counterpart: keys rotated by position and stored with their values token by token)
  *   iak_beam_select             (no counterpart: the choice of a beam search's continuations)
  *   iak_status_string           (no counterpart: the reference raises ValueError/RuntimeError in Python)
@@ -803,6 +806,55 @@ typedef struct {
 
 iak_status iak_compact_pages_workspace(const iak_compact_pages_args* args, size_t* bytes);
 iak_status iak_compact_pages(const iak_compact_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of several query tokens per sequence (drafted tokens, prompt chunks) over the pages of
+ * iak_paged_decode: pools, scales, page_table, page_counts, page_tags, tag_map, map_other_tags and
+ * negative_ids as there. q, out [batch, q_len, num_q_heads, head_dim] (element strides, unit inner
+ * stride, any address of their type; out may be q).
+ * Token t of entry e of a row is its number 16 e + t; the row holds min(valid_tokens, 16 *
+ * page_counts) of them (valid_tokens [batch, num_kv_heads] may be NULL: 16 * page_counts), the
+ * queries' own the last: with q_lens [batch] (NULL: q_len for all; clamped to 0 .. q_len) query
+ * i < q_lens[b] of head h reads row (b, h / (num_q_heads / num_kv_heads)) and sees, with causal =
+ * 1, the tokens numbered below tokens - q_lens[b] + i + 1, else all:
+ *   out = softmax(sm_scale * q . k) v over those on pages that contribute (tags and ids as for the decode),
+ * 0 where there are none and for i >= q_lens[b].
+ * Tokens that a query does not see never reach it, whatever their bytes; an infinite or NaN value of one that it
+ * sees reaches its channel. A query row that is not finite is NaN if it sees a token.
+ * Products run on the matrix cores in float16 with float32 sums: K and V as exact codes, with
+ * their scales in float32 (float32 sums of log2 in the exponential), or in two parts (4-bit pages; 21 bits); query rows
+ * and weights as for iak_mx_attention. V scales of one row may differ by 2^18 without loss.
+ * splits: parts a row's tokens are divided into (0: automatic). The parts meet in the workspace
+ * (iak_paged_chunk_workspace bytes, 16-byte aligned, as it comes; 0: not needed); calls that share one
+ * on different streams race. head_dim 64 or 128, page_size 16; pools 16-byte aligned. */
+typedef struct {
+  int32_t batch, q_len, num_q_heads, num_kv_heads, head_dim, page_size, table_width;
+  int64_t num_pages;
+  const void* q; int32_t q_dtype; int64_t q_stride_b, q_stride_t, q_stride_h;
+  void* out; int32_t out_dtype; int64_t out_stride_b, out_stride_t, out_stride_h;
+  const int32_t* page_table;
+  const int32_t* page_counts;
+  const int32_t* valid_tokens;
+  const int32_t* q_lens;
+  const int32_t* page_tags;
+  uint8_t tag_map[8];
+  int32_t map_other_tags, negative_ids;
+  const void* k_fp16; const void* v_fp16;
+  const void* k_fp8; const void* v_fp8;
+  const void* k_int8; const void* v_int8;
+  const void* k_int4; const void* v_int4;
+  const void* k_int4r; const void* v_int4r;
+  const void* k_fp8_scale; const void* v_fp8_scale; int32_t fp8_scale_dtype;
+  const void* k_int8_scale; const void* v_int8_scale; int32_t int8_scale_dtype;
+  const void* k_int4_scale; const void* v_int4_scale; int32_t int4_scale_dtype;
+  int32_t int4_group;
+  const float* k_int4r_scale; const float* v_int4r_scale;
+  float sm_scale;
+  int32_t causal;
+  int32_t splits;
+} iak_paged_chunk_args;
+
+iak_status iak_paged_chunk_workspace(const iak_paged_chunk_args* args, size_t* bytes);
+iak_status iak_paged_chunk(const iak_paged_chunk_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The newest tokens' keys, rotated by their positions, and values into their sequences' pages,
  * and their queries rotated along. A pair of channels (x, y) of a token at position p becomes

@@ -1,6 +1,7 @@
-// What the 4-bit cache's attention kernels share: how many tokens a query row sees and how
-// many table entries a tile of rows has to walk, out of the lengths on the device; a row's
-// query operand; the parts of the softmax; V's way through LDS.
+// What the attention kernels over paged caches for several query rows share (the 4-bit cache's, and
+// those over pages of mixed precision, whose argument block A is an MxAttn with more): how many tokens a
+// query row sees and how many table entries a tile of rows has to walk, out of the lengths on the
+// device; a row's query operand; the parts of the softmax; V's way through LDS.
 #ifndef IAK_MX_ATTENTION_H
 #define IAK_MX_ATTENTION_H
 
@@ -16,10 +17,12 @@ namespace iak {
 // Tokens of a row and new queries of its sequence, clamped to what there is room for.
 struct MxRows { int tokens, queries, first; };   // query i sees `first + i + 1` tokens when causal
 
-__device__ __forceinline__ MxRows mx_rows(const MxAttn& a, int64_t kvrow, int b) {
+__device__ __forceinline__ int row_length(const MxAttn& a, int64_t kvrow) { return a.valid[kvrow]; }
+
+template <typename A> __device__ __forceinline__ MxRows mx_rows(const A& a, int64_t kvrow, int b) {
   MxRows n;
   const int64_t most = a.NP > 0 ? (int64_t)a.W * 16 : 0;
-  const int v = a.valid[kvrow];
+  const int v = row_length(a, kvrow);
   n.tokens = v < 0 ? 0 : (v > most ? (int)most : v);
   n.queries = a.L;
   if (a.q_lens) {
@@ -85,7 +88,7 @@ __device__ __forceinline__ int wave_scan(int x) {
 // and 132, of equal lengths 140 and 134. With head_dim 64 one round
 // only: 5 x 509 queries over 4,000 in two 66, fixed 59. Short decode rows lose what the working out
 // takes (13 of up to 8,191 tokens: 19.7 us and 18.4).
-template <int UNIT, bool RUNS> __device__ __forceinline__ MxPart mx_shared_part(const MxAttn& a) {
+template <int UNIT, bool RUNS, typename A> __device__ __forceinline__ MxPart mx_shared_part(const A& a) {
   constexpr int MOST = MX_SHARED_TILES / 64;
   const int lane = threadIdx.x & 63;
   const int all = a.B * a.Hkv * a.tiles, per = (all + 63) >> 6;    // tiles, and of a lane: a run

@@ -1,0 +1,352 @@
+// What the attention kernels for several query rows over pages of mixed precision share: a table
+// entry's page, precision and scales; a page's way from memory into LDS as float16 operands; the
+// softmax with scales.
+//
+// Every page becomes float16 tiles of codes that are exact, its scale left to 32 bits:
+//   float16          as it is
+//   INT8, FP8        the codes. K's scale multiplies the scores; V's, the weights
+//                    (2^log2 of it inside their exponential, taken out of their sum again)
+//   INT4, residual   codes times scales need up to 30 bits: two tiles, of what float16 holds of
+//                    them and what is left, both relative to a power of two of the page
+// so that a quantised page costs what its own products cost, and nothing is rounded but the
+// weights. (One tile for those, as the decode's kernel has it: products off by 2^-12 a value, 6e-4 of
+// an output where the weights' rounding costs 1.5e-4.)
+#ifndef IAK_PAGE_ATTENTION_H
+#define IAK_PAGE_ATTENTION_H
+
+#include "iak_device.h"
+#include "mx_attention.h"
+#include "step_internal.h"
+
+namespace iak {
+
+__device__ __forceinline__ int row_length(const PageAttn& a, int64_t kvrow) {
+  const int64_t c = a.counts[kvrow];
+  const int listed = c < 0 ? 0 : (c > a.W ? a.W * 16 : (int)c * 16);
+  if (!a.bounds) return listed;
+  const int v = a.bounds[kvrow];
+  return v < listed ? v : listed;
+}
+
+// --------------------------------------------------------------------------- //
+// Entries
+// --------------------------------------------------------------------------- //
+
+// A table entry as a lane looks it up: its page (-1: no tokens), native tag, what multiplies the scores
+// (km > 0) and K's codes (kf), log2 of what multiplies the weights (vl), and V's codes (vf).
+struct PageEntry { int id, tag; float km, kf, vl, vf; };
+
+// A page scale in a positive normal multiplier and what is left for the codes: its sign, or itself
+// where it is zero or not finite.
+__device__ __forceinline__ void split_scale(float s, float& mult, float& rest) {
+  const float a = fabsf(s);
+  const bool plain = a >= 1.17549435e-38f && a < __builtin_inff();
+  mult = plain ? a : 1.f;
+  rest = plain ? (s < 0.f ? -1.f : 1.f) : s;
+}
+// The power of two of a scale whose codes go as values.
+__device__ __forceinline__ float power_of(float s) { return s > 0.f && s < __builtin_inff() ? pow2f(scale_exp(s)) : 1.f; }
+
+template <int D, int KIND>
+__device__ __forceinline__ PageEntry page_entry(const PageAttn& a, const int32_t* row, int e, int end) {
+  PageEntry x = {-1, IAK_TAG_FP16, 1.f, 1.f, 0.f, 1.f};
+  if (e >= end) return x;
+  int64_t p = row[e];
+  if (a.neg_wrap && p < 0) p += a.NP;
+  if (p < 0 || p >= a.NP) return x;
+  const int t = a.tags[p], tag = (uint32_t)t < 8u ? (int)((a.tagmap >> (8 * t)) & 0xFFu) : a.other_tag;
+  if (KIND == PAGES_F16) {
+    if (tag == IAK_TAG_FP16) x.id = (int)p;
+    return x;
+  }
+  x.tag = tag;
+  if (tag == IAK_TAG_FP16) {
+    x.id = (int)p;
+  } else if (tag == IAK_TAG_INT8 || tag == IAK_TAG_FP8) {
+    x.id = (int)p;
+    const bool fp8 = tag == IAK_TAG_FP8;
+    const float k = load_scale(fp8 ? a.k_fp8_scale : a.k_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
+    float v = load_scale(fp8 ? a.v_fp8_scale : a.v_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
+    split_scale(k, x.km, x.kf);
+    split_scale(v, v, x.vf);
+    x.vl = __builtin_amdgcn_logf(v);
+  } else if (KIND == PAGES_ALL && (tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL)) {
+    x.id = (int)p;
+    float k = 0.f, v = 0.f;            // the largest scales
+    if (tag == IAK_TAG_INT4) {
+      const int groups = D / a.int4_group;                       // 1, 2 or 4
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t at = p * groups + (i < groups ? i : 0);
+        k = fmaxf(k, fabsf(load_scale(a.k_int4_scale, at, a.int4_sd)));
+        v = fmaxf(v, fabsf(load_scale(a.v_int4_scale, at, a.int4_sd)));
+      }
+    } else {
+      k = fmaxf(fabsf(a.k_int4r_scale[2 * p]), fabsf(a.k_int4r_scale[2 * p + 1]));
+      v = fmaxf(fabsf(a.v_int4r_scale[2 * p]), fabsf(a.v_int4r_scale[2 * p + 1]));
+    }
+    x.km = power_of(k);
+    v = power_of(v);
+    x.kf = 1.f / x.km;                                           // exact, as the next
+    x.vf = 1.f / v;
+    x.vl = __builtin_amdgcn_logf(v);
+  }
+  return x;
+}
+
+// One of them for the whole wave: lane `k`'s.
+__device__ __forceinline__ float lane_f(float x, int k) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(x), k)); }
+
+__device__ __forceinline__ bool wide_tag(int tag) { return tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL; }
+
+// --------------------------------------------------------------------------- //
+// A page's K or V by a wave: loaded, and put into LDS
+// --------------------------------------------------------------------------- //
+
+// Piece j of lane l is the page's bytes 1024 j + 16 l ..: whole lines. (INT4 pages of 64 channels, 512
+// bytes: 8 l ..)
+template <int D> struct PageRaw {
+  u4 x[D / 32];
+  float s0, s1;                        // INT4: its channels' scale; residual: both
+};
+
+template <typename T, bool STREAM> __device__ __forceinline__ T page_ld(const T* p) {
+  if constexpr (STREAM) return ld_nt(p);
+  else return *p;
+}
+
+template <int D, int KIND, bool STREAM>
+__device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool v, int id, int tag, int lane) {
+  if (id < 0) return;                                            // uniform, as the tag
+  const int64_t p = id;
+  if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) {
+    const u4* at = reinterpret_cast<const u4*>(v ? a.v_fp16 : a.k_fp16) + p * (PS * D / 8) + lane;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) r.x[j] = page_ld<u4, STREAM>(at + 64 * j);
+    return;
+  }
+  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
+    const uint8_t* page = reinterpret_cast<const uint8_t*>(v ? a.v_int4 : a.k_int4) + p * (PS * D / 2);
+    if constexpr (D == 128) r.x[0] = *(reinterpret_cast<const u4*>(page) + lane);
+    else {
+      const u2 x = *(reinterpret_cast<const u2*>(page) + lane);
+      r.x[0] = u4{x[0], x[1], 0u, 0u};
+    }
+    const int channel = lane % 4 * (D / 4), groups = D / a.int4_group;
+    r.s0 = load_scale(v ? a.v_int4_scale : a.k_int4_scale, p * groups + channel / a.int4_group, a.int4_sd);
+    return;
+  }
+  const void* pool = tag == IAK_TAG_INT8 ? (v ? a.v_int8 : a.k_int8) : tag == IAK_TAG_FP8 ? (v ? a.v_fp8 : a.k_fp8)
+                                                                                         : (v ? a.v_int4r : a.k_int4r);
+  const u4* at = reinterpret_cast<const u4*>(pool) + p * (PS * D / 16) + lane;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) r.x[j] = page_ld<u4, STREAM>(at + 64 * j);
+  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
+    const float* s = (v ? a.v_int4r_scale : a.k_int4r_scale) + 2 * p;
+    r.s0 = s[0];
+    r.s1 = s[1];
+  }
+}
+
+// Two values as float16 and what is left of them. The first is cut rather than rounded: the second has it.
+__device__ __forceinline__ void hi_lo(float a, float b, bool fine, uint32_t& hi, uint32_t& lo) {
+  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+  hi = bits(h);
+  lo = fine ? bits(h2{(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])}) : 0u;
+}
+
+// The pair of codes (n & 15, n >> 4 & 15), less 8 each, of byte `byte` of w, as float16: exact.
+__device__ __forceinline__ h2 nibbles(uint32_t w, int byte) {
+  const uint32_t y = __builtin_amdgcn_perm(0u, w, 0x0C000C00u | (uint32_t)byte | ((uint32_t)byte << 16));   // (b, 0, b, 0)
+  const h2 n = as_h2((y & 0x00F0000Fu) | MAGIC_I4);              // 1024 + low, 1024 + 16 high
+  return h2{n[0] - (_Float16)1032.f, (n[1] - (_Float16)1152.f) * (_Float16)0.0625f};
+}
+
+// The page into LDS as float16 rows (16-byte chunks at v_chunk); `lo`, written for wide pages alone: what is
+// left. id < 0: zeros. `rest`: kf or vf of the entry. Returns whether a value is infinite or NaN in this lane (CHECK).
+template <int D, int KIND, bool CHECK>
+__device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag, float rest, u4* hi, u4* lo, int lane) {
+  h2 sum = {0, 0};                     // NaN once anything is not finite
+  auto look = [&](const u4& x) {
+    if constexpr (CHECK) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __builtin_elementwise_fma(as_h2(x[i]), h2{0, 0}, sum);
+    }
+  };
+  if (id < 0) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) hi[64 * j + lane] = u4{0u, 0u, 0u, 0u};
+    return false;
+  }
+  if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const int f = 64 * j + lane;
+      hi[v_chunk<D>(f / (D / 8), f % (D / 8))] = r.x[j];
+      look(r.x[j]);
+    }
+  } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
+    const float s = r.s0 * rest;
+    const bool fine = fabsf(s) < __builtin_inff();
+    const int token = lane / 4, chunk = lane % 4 * (D / 32);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      u4 h, l;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const h2 n = nibbles(r.x[0][c], i);
+        uint32_t x, y;
+        hi_lo((float)n[0] * s, (float)n[1] * s, fine, x, y);
+        h[i] = x;
+        l[i] = y;
+      }
+      const int at = v_chunk<D>(token, chunk + c);
+      hi[at] = h;
+      lo[at] = l;
+      look(h);
+    }
+  } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
+    const float s0 = r.s0 * rest, s1 = r.s1 * rest;
+    const bool fine = fabsf(s0) + fabsf(s1) < __builtin_inff();
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const int f = 64 * j + lane, token = f / (D / 16), chunk = f % (D / 16) * 2;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        u4 h, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = r.x[j][2 * c + (i >> 1)];
+          const h2 m = nibbles(w, 2 * (i & 1)), n = nibbles(w, 2 * (i & 1) + 1);   // (base, residual) of two channels
+          uint32_t x, y;
+          hi_lo(__builtin_fmaf((float)m[0], s0, (float)m[1] * s1), __builtin_fmaf((float)n[0], s0, (float)n[1] * s1), fine, x, y);
+          h[i] = x;
+          l[i] = y;
+        }
+        const int at = v_chunk<D>(token, chunk + c);
+        hi[at] = h;
+        lo[at] = l;
+        look(h);
+      }
+    }
+  } else {
+    const bool fp8 = tag == IAK_TAG_FP8;
+    const h2 sign = splat2((_Float16)rest);
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const int f = 64 * j + lane, token = f / (D / 16), chunk = f % (D / 16) * 2;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[4];
+        if (fp8) {
+          fp8x4_to_f16(r.x[j][2 * c], o[0], o[1]);
+          fp8x4_to_f16(r.x[j][2 * c + 1], o[2], o[3]);
+        } else {
+          i8x4_to_f16(r.x[j][2 * c], o[0], o[1]);
+          i8x4_to_f16(r.x[j][2 * c + 1], o[2], o[3]);
+        }
+        if (rest != 1.f) {                                       // uniform, rare
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = bits(as_h2(o[i]) * sign);
+        }
+        const u4 h = u4{o[0], o[1], o[2], o[3]};
+        hi[v_chunk<D>(token, chunk + c)] = h;
+        look(h);
+      }
+    }
+  }
+  return CHECK && !((float)sum[0] + (float)sum[1] == 0.f);
+}
+
+// --------------------------------------------------------------------------- //
+// The softmax of PAGES pages whose scores and weights have multipliers (hide() is mx_attention.h's)
+// --------------------------------------------------------------------------- //
+
+template <int D, int PAGES, int T, typename L>
+__device__ __forceinline__ void raise_scaled(const f4 (&s)[T][PAGES], const float (&km)[PAGES], const float (&mult)[T], float (&m)[T],
+                                             L (&l)[T], f4 (&acc)[T][D / 16]) {
+  float top[T];
+  bool over = false;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    top[t] = -__builtin_inff();
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p)
+      top[t] = fmaxf(top[t], fmaxf(fmaxf(s[t][p][0], s[t][p][1]), fmaxf(s[t][p][2], s[t][p][3])) * fmaxf(mult[t] * km[p], 1e-37f));
+    over = over || top[t] > m[t] + RESCALE_SLACK;
+  }
+  if (__builtin_amdgcn_ballot_w64(over)) {
+    asm volatile("");
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float pm = xmax16_32(top[t]);
+      const float mn = pm > m[t] + RESCALE_SLACK ? pm : m[t];
+      const float alpha = __builtin_amdgcn_exp2f(m[t] - mn);
+      l[t] *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] *= alpha;
+      m[t] = mn;
+    }
+  }
+}
+
+// Scores become weights times V's scale 2^vl; returns their sum without it.
+template <int PAGES>
+__device__ __forceinline__ float soften_scaled(f4 (&s)[PAGES], const float (&km)[PAGES], const float (&vl)[PAGES], const float (&out)[PAGES],
+                                               float mult, float m) {
+  float sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p) {
+    const float each = fmaxf(mult * km[p], 1e-37f), base = P_SHIFT - m + vl[p];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s[p][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p][q], each, base));
+    sum = __builtin_fmaf((s[p][0] + s[p][1]) + (s[p][2] + s[p][3]), out[p], sum);
+  }
+  return sum;
+}
+
+// V's scales differ by pages: weights carry 2^(vl - E), the accumulators stand for 2^E of themselves, and E follows
+// the largest of a step's, with room below it so that it moves seldom.
+constexpr int V_ROOM = 8;
+template <int PAGES> __device__ __forceinline__ int value_power(const int (&id)[PAGES], const float (&vl)[PAGES], int E) {
+  float most = -200.f;
+#pragma unroll
+  for (int p = 0; p < PAGES; ++p) most = id[p] >= 0 && vl[p] > most ? vl[p] : most;
+  const int e = __builtin_amdgcn_readfirstlane((int)floorf(most));
+  return most < -199.f || (e <= E && e >= E - V_ROOM) ? E : e;
+}
+
+// Infinite and NaN values where a row sees them: a weight of zero would make them NaN where it does not, so the
+// products have zeros there (clean), and each is added by itself, whatever its weight. `first`: the number of the
+// pages' first token.
+__device__ __forceinline__ h8 clean(h8 x) {
+  u4 w = __builtin_bit_cast(u4, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = w[i] & 0x7C007C00u;
+    w[i] &= ((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u);
+  }
+  return __builtin_bit_cast(h8, w);
+}
+template <int D, int T>
+__device__ __forceinline__ void add_special(f4 (&acc)[T][D / 16], const u4* page, int id, int first, const int (&seen)[T], int g) {
+  if (id < 0) return;
+  for (int token = 0; token < PS; ++token) {
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb) {
+      const h4 v = *reinterpret_cast<const h4*>(reinterpret_cast<const char*>(page + v_chunk<D>(token, 2 * mb + (g >> 1))) + 8 * (g & 1));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float x = (float)v[q];
+        const bool special = !(fabsf(x) < __builtin_inff());
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+          if (special && first + token < seen[t]) acc[t][mb][q] += x;
+      }
+    }
+  }
+}
+
+}  // namespace iak
+
+#endif

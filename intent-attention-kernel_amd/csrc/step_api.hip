@@ -98,9 +98,145 @@ iak_status validate_rotary_append(const iak_rotary_append_args* a) {
   return IAK_OK;
 }
 
+constexpr float LOG2_E = 1.44269504088896340736f;
+constexpr double CUS = 256;
+size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
+
+struct ChunkPlan {
+  int G, kind, tile_rows, tiles, splits, chunk;
+  int64_t items;
+  size_t ws_m, ws_l, ws_acc, total;
+};
+
+// Which kernel, and into how many parts a row's tokens go.
+void choose_chunk(const iak_paged_chunk_args* a, int64_t rows, int W, ChunkPlan* p) {
+  const bool f32 = a->q_dtype == IAK_DTYPE_F32;
+  const double kvrows = (double)a->batch * a->num_kv_heads;
+  p->tile_rows = rows <= 64 ? 16 : (rows > 128 && !f32 ? 256 : 128);
+  p->tiles = (int)((rows + p->tile_rows - 1) / p->tile_rows);
+  const double tiles = kvrows * p->tiles, round = CUS * (p->tile_rows == 16 ? 3 : 2);
+  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(round / tiles);
+  if (splits > (W + 7) / 8 && a->splits == 0) splits = (W + 7) / 8;
+  if (splits > (W + 1) / 2) splits = (W + 1) / 2;
+  if (splits < 1) splits = 1;
+  while (splits > 1 && tiles * splits * p->tile_rows > 1.6e7) splits /= 2;
+  p->chunk = (int)((W + splits - 1) / splits);
+  p->splits = (W + p->chunk - 1) / p->chunk;
+  p->items = (int64_t)tiles * p->splits;
+}
+
+iak_status validate_paged_chunk(const iak_paged_chunk_args* a, ChunkPlan* p) {
+  if (!a) return fail(IAK_EINVAL, "args is NULL");
+  if (a->batch < 0 || a->q_len < 0 || a->num_kv_heads <= 0 || a->table_width < 0 || a->num_pages < 0)
+    return fail(IAK_EINVAL, "negative or zero size (batch=%d, q_len=%d, num_kv_heads=%d, table_width=%d, num_pages=%lld)", a->batch,
+                a->q_len, a->num_kv_heads, a->table_width, (long long)a->num_pages);
+  if (a->head_dim != 64 && a->head_dim != 128) return fail(IAK_ENOTSUP, "head_dim %d is not supported (64 or 128)", a->head_dim);
+  if (a->page_size != 16) return fail(IAK_ENOTSUP, "page_size %d is not supported (16)", a->page_size);
+  if (a->num_pages > 0x7FFFFFFFLL) return fail(IAK_EINVAL, "num_pages %lld exceeds int32 page ids", (long long)a->num_pages);
+  if (a->table_width > 0x7FFFFF0) return fail(IAK_EINVAL, "table_width %d: a row's tokens exceed int32", a->table_width);
+  if (a->num_q_heads <= 0 || a->num_q_heads % a->num_kv_heads != 0)
+    return fail(IAK_EINVAL, "num_q_heads %d is not a multiple of num_kv_heads %d", a->num_q_heads, a->num_kv_heads);
+  if (a->q_dtype < 0 || a->q_dtype > 2 || a->out_dtype < 0 || a->out_dtype > 2)
+    return fail(IAK_EINVAL, "bad q/out dtype (%d, %d)", a->q_dtype, a->out_dtype);
+  if (!std::isfinite(a->sm_scale * LOG2_E)) return fail(IAK_EINVAL, "sm_scale is not finite, in base 2 too");
+  if (a->causal != 0 && a->causal != 1) return fail(IAK_EINVAL, "causal must be 0 or 1, got %d", a->causal);
+  if (a->splits < 0) return fail(IAK_EINVAL, "splits %d is negative", a->splits);
+  *p = ChunkPlan{};
+  p->G = a->num_q_heads / a->num_kv_heads;
+  if (a->batch == 0 || a->q_len == 0) return IAK_OK;
+  if (!a->q || !a->out) return fail(IAK_EINVAL, "q/out is NULL");
+  if (!aligned(a->q, element_bytes(a->q_dtype)) || !aligned(a->out, element_bytes(a->out_dtype)))
+    return fail(IAK_EINVAL, "q or out is not aligned to its elements");
+  if (!a->page_table && a->table_width > 0) return fail(IAK_EINVAL, "page_table is NULL");
+  if (!a->page_counts) return fail(IAK_EINVAL, "page_counts is NULL");
+  if (!a->page_tags && a->num_pages > 0) return fail(IAK_EINVAL, "page_tags is NULL");
+  if (!aligned(a->page_table, 4) || !aligned(a->page_counts, 4) || !aligned(a->valid_tokens, 4) || !aligned(a->q_lens, 4) ||
+      !aligned(a->page_tags, 4))
+    return fail(IAK_EINVAL, "int32 arrays must be 4-byte aligned");
+  p->kind = iak::PAGES_F16;
+  for (int t = 0; t < 8 && a->num_pages > 0; ++t) {
+    const void *k = nullptr, *v = nullptr, *ks = nullptr, *vs = nullptr;
+    int sd = IAK_DTYPE_F32, kind = iak::PAGES_BYTE;
+    switch (a->tag_map[t]) {
+      case IAK_TAG_FP16: k = a->k_fp16; v = a->v_fp16; ks = vs = k; kind = iak::PAGES_F16; break;
+      case IAK_TAG_FP8: k = a->k_fp8; v = a->v_fp8; ks = a->k_fp8_scale; vs = a->v_fp8_scale; sd = a->fp8_scale_dtype; break;
+      case IAK_TAG_INT8: k = a->k_int8; v = a->v_int8; ks = a->k_int8_scale; vs = a->v_int8_scale; sd = a->int8_scale_dtype; break;
+      case IAK_TAG_INT4:
+        k = a->k_int4; v = a->v_int4; ks = a->k_int4_scale; vs = a->v_int4_scale; sd = a->int4_scale_dtype; kind = iak::PAGES_ALL;
+        break;
+      case IAK_TAG_INT4_RESIDUAL: k = a->k_int4r; v = a->v_int4r; ks = a->k_int4r_scale; vs = a->v_int4r_scale; kind = iak::PAGES_ALL; break;
+      default: continue;               // SKIP or unknown: contributes nothing
+    }
+    if (!k || !v || !ks || !vs) return fail(IAK_EINVAL, "tag %d maps to precision %d, whose K/V pool or scales are NULL", t, a->tag_map[t]);
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(IAK_EINVAL, "K/V pools must be 16-byte aligned");
+    if (sd != IAK_DTYPE_F16 && sd != IAK_DTYPE_F32) return fail(IAK_EINVAL, "scale dtype %d must be f16 or f32", sd);
+    if (!aligned(ks, element_bytes(sd)) || !aligned(vs, element_bytes(sd))) return fail(IAK_EINVAL, "scales are not aligned to their elements");
+    if (a->tag_map[t] == IAK_TAG_INT4 && (a->int4_group <= 0 || a->head_dim % a->int4_group || a->int4_group % (a->head_dim / 4)))
+      return fail(IAK_ENOTSUP, "int4_group %d must divide head_dim %d and be a multiple of %d", a->int4_group, a->head_dim, a->head_dim / 4);
+    if (kind > p->kind) p->kind = kind;
+  }
+  const int64_t rows = (int64_t)a->q_len * p->G;
+  if (rows > 0x3FFFFFFF) return fail(IAK_EINVAL, "q_len %d x %d heads per KV head is too long", a->q_len, p->G);
+  const double kvrows = (double)a->batch * a->num_kv_heads;
+  if (kvrows * ((rows + 15) / 16) > 1.6e7)
+    return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", kvrows * ((rows + 15) / 16));
+  choose_chunk(a, rows, a->table_width > 0 ? a->table_width : 1, p);
+  if (p->splits > 1) {
+    const size_t kept = (size_t)p->items * p->tile_rows;
+    p->ws_l = round_up(4 * kept);
+    p->ws_acc = p->ws_l + round_up(4 * kept);
+    p->total = p->ws_acc + round_up(4 * kept * (size_t)a->head_dim);
+  }
+  return IAK_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+iak_status iak_paged_chunk_workspace(const iak_paged_chunk_args* a, size_t* bytes) {
+  if (!bytes) return fail(IAK_EINVAL, "bytes is NULL");
+  ChunkPlan p;
+  iak_status st = validate_paged_chunk(a, &p);
+  if (st != IAK_OK) return st;
+  *bytes = p.total;
+  return IAK_OK;
+}
+
+iak_status iak_paged_chunk(const iak_paged_chunk_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  ChunkPlan p;
+  iak_status st = validate_paged_chunk(a, &p);
+  if (st != IAK_OK) return st;
+  if (a->batch == 0 || a->q_len == 0) return IAK_OK;
+  st = check_workspace(workspace, workspace_bytes, p.total);
+  if (st != IAK_OK) return st;
+  iak::PageAttn k{};
+  k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
+  k.W = a->table_width; k.NP = a->num_pages;
+  k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.items = p.items; k.parted = p.total > 0;
+  k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
+  k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;
+  k.table = a->page_table; k.q_lens = a->q_lens; k.counts = a->page_counts; k.bounds = a->valid_tokens;
+  k.score_mult = a->sm_scale * LOG2_E;
+  k.causal = a->causal;
+  k.kind = p.kind;
+  k.tags = a->page_tags;
+  for (int t = 0; t < 8; ++t) k.tagmap |= (uint64_t)a->tag_map[t] << (8 * t);
+  k.other_tag = a->map_other_tags ? a->tag_map[7] : IAK_TAG_SKIP;
+  k.neg_wrap = a->negative_ids;
+  k.k_fp16 = a->k_fp16; k.v_fp16 = a->v_fp16; k.k_fp8 = a->k_fp8; k.v_fp8 = a->v_fp8; k.k_int8 = a->k_int8; k.v_int8 = a->v_int8;
+  k.k_int4 = a->k_int4; k.v_int4 = a->v_int4; k.k_int4r = a->k_int4r; k.v_int4r = a->v_int4r;
+  k.k_fp8_scale = a->k_fp8_scale; k.v_fp8_scale = a->v_fp8_scale; k.fp8_sd = a->fp8_scale_dtype;
+  k.k_int8_scale = a->k_int8_scale; k.v_int8_scale = a->v_int8_scale; k.int8_sd = a->int8_scale_dtype;
+  k.k_int4_scale = a->k_int4_scale; k.v_int4_scale = a->v_int4_scale; k.int4_sd = a->int4_scale_dtype;
+  k.int4_group = a->int4_group > 0 ? a->int4_group : a->head_dim;
+  k.k_int4r_scale = a->k_int4r_scale; k.v_int4r_scale = a->v_int4r_scale;
+  char* ws = reinterpret_cast<char*>(workspace);
+  k.ws_m = reinterpret_cast<float*>(ws + p.ws_m);
+  k.ws_l = reinterpret_cast<float*>(ws + p.ws_l);
+  k.ws_acc = reinterpret_cast<float*>(ws + p.ws_acc);
+  return launched(iak::launch_page_attention(k, reinterpret_cast<hipStream_t>(stream)), "chunk attention");
+}
 
 iak_status iak_rotary_append(const iak_rotary_append_args* a, void* stream) {
   iak_status st = validate_rotary_append(a);

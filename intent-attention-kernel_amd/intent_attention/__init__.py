@@ -63,6 +63,7 @@ from .page_sharing import (
     reorder_sequences,
 )
 from .beam_search import beam_select
+from .paged_chunk import ChunkPlan, make_chunk_plan, paged_chunk_attention
 from .rotary import append_rotated_tokens
 from .kv_memory_manager import KVMemoryManager, PageFormatPolicy, PageState, PageStorageFormat
 from .prefetch import BlockPrefetcher, get_prefetch_stream, get_prefetcher, launch_prefetch_pages, reset_prefetcher
@@ -93,7 +94,7 @@ __all__ = [
     "quantize_pages", "fake_int8_pages_device",
     "build_page_tables", "routing_to_kernel_tensors",
     "MxFp4Plan", "MxFp4Pools", "append_mxfp4_tokens", "make_mxfp4_plan", "mxfp4_paged_attention", "read_mxfp4_tokens",
-    "append_rotated_tokens", "beam_select",
+    "append_rotated_tokens", "beam_select", "ChunkPlan", "make_chunk_plan", "paged_chunk_attention",
     "compact_pages", "copy_pages", "fork_sequences", "free_sequences", "grow_sequences", "reorder_sequences",
     "KVMemoryManager", "PageFormatPolicy", "PageState", "PageStorageFormat",
     "BlockPrefetcher", "get_prefetch_stream", "get_prefetcher", "launch_prefetch_pages", "reset_prefetcher",

@@ -262,6 +262,30 @@ class CompactPagesArgs(ctypes.Structure):
     ]
 
 
+class PagedChunkArgs(ctypes.Structure):
+    """Mirror of ``iak_paged_chunk_args`` (include/iak.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("q_len", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("page_size", c_i32), ("table_width", c_i32), ("num_pages", c_i64),
+        ("q", c_void_p), ("q_dtype", c_i32), ("q_stride_b", c_i64), ("q_stride_t", c_i64), ("q_stride_h", c_i64),
+        ("out", c_void_p), ("out_dtype", c_i32), ("out_stride_b", c_i64), ("out_stride_t", c_i64), ("out_stride_h", c_i64),
+        ("page_table", c_void_p), ("page_counts", c_void_p), ("valid_tokens", c_void_p), ("q_lens", c_void_p),
+        ("page_tags", c_void_p), ("tag_map", ctypes.c_uint8 * 8), ("map_other_tags", c_i32), ("negative_ids", c_i32),
+        ("k_fp16", c_void_p), ("v_fp16", c_void_p),
+        ("k_fp8", c_void_p), ("v_fp8", c_void_p),
+        ("k_int8", c_void_p), ("v_int8", c_void_p),
+        ("k_int4", c_void_p), ("v_int4", c_void_p),
+        ("k_int4r", c_void_p), ("v_int4r", c_void_p),
+        ("k_fp8_scale", c_void_p), ("v_fp8_scale", c_void_p), ("fp8_scale_dtype", c_i32),
+        ("k_int8_scale", c_void_p), ("v_int8_scale", c_void_p), ("int8_scale_dtype", c_i32),
+        ("k_int4_scale", c_void_p), ("v_int4_scale", c_void_p), ("int4_scale_dtype", c_i32),
+        ("int4_group", c_i32),
+        ("k_int4r_scale", c_void_p), ("v_int4r_scale", c_void_p),
+        ("sm_scale", c_float), ("causal", c_i32), ("splits", c_i32),
+    ]
+
+
 class RotaryAppendArgs(ctypes.Structure):
     """Mirror of ``iak_rotary_append_args`` (include/iak.h)."""
 
@@ -306,7 +330,7 @@ EXPORTED = ("iak_abi_version", "iak_status_string", "iak_last_error",
             "iak_copy_pages", "iak_sequences_workspace", "iak_free_sequences", "iak_grow_sequences",
             "iak_fork_sequences", "iak_compact_pages_workspace", "iak_compact_pages",
             "iak_beam_select_workspace", "iak_beam_select", "iak_reorder_sequences_workspace", "iak_reorder_sequences",
-            "iak_rotary_append")
+            "iak_rotary_append", "iak_paged_chunk_workspace", "iak_paged_chunk")
 NOALLOC_SCRATCH_BYTES = 16 << 20   # IAK_NOALLOC_SCRATCH_BYTES
 
 _lib: Optional[ctypes.CDLL] = None
@@ -405,6 +429,8 @@ def load() -> ctypes.CDLL:
                        ("iak_compact_pages", (CompactPagesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_reorder_sequences_workspace", (SequencesArgs, size_p)),
                        ("iak_reorder_sequences", (SequencesArgs, c_void_p, ctypes.c_size_t, c_void_p)),
+                       ("iak_paged_chunk_workspace", (PagedChunkArgs, size_p)),
+                       ("iak_paged_chunk", (PagedChunkArgs, c_void_p, ctypes.c_size_t, c_void_p)),
                        ("iak_rotary_append", (RotaryAppendArgs, c_void_p)),
                        ("iak_beam_select_workspace", (BeamSelectArgs, size_p)),
                        ("iak_beam_select", (BeamSelectArgs, c_void_p, ctypes.c_size_t, c_void_p))):
@@ -653,3 +679,13 @@ def beam_select(args: BeamSelectArgs, stream: int, workspace: int, workspace_byt
 
 def rotary_append(args: RotaryAppendArgs, stream: int) -> None:
     check(load().iak_rotary_append(ctypes.byref(args), stream or None))
+
+
+def paged_chunk_workspace(args: PagedChunkArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().iak_paged_chunk_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def paged_chunk(args: PagedChunkArgs, stream: int, workspace: int = 0, workspace_bytes: int = 0) -> None:
+    check(load().iak_paged_chunk(ctypes.byref(args), workspace or None, workspace_bytes, stream or None))

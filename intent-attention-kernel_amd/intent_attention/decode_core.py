@@ -135,6 +135,41 @@ def _scale_dtype(name: str, *ts: Optional[torch.Tensor]) -> int:
     return _DT[next(iter(dts))]
 
 
+def _check_page_pools(pools: PagePools, NP: int, D: int) -> int:
+    """ValueError for pools that are not NP pages of D channels; returns int4_group."""
+    f16, u8, i8 = (torch.float16,), (torch.uint8,), (torch.int8,)
+    _check_pool("k_fp16", pools.k_fp16, NP, (PAGE_SIZE, D), f16)
+    _check_pool("v_fp16", pools.v_fp16, NP, (PAGE_SIZE, D), f16)
+    _check_pool("k_fp8", pools.k_fp8, NP, (PAGE_SIZE, D), u8 + (torch.float8_e4m3fn,))
+    _check_pool("v_fp8", pools.v_fp8, NP, (PAGE_SIZE, D), u8 + (torch.float8_e4m3fn,))
+    _check_pool("k_int8", pools.k_int8, NP, (PAGE_SIZE, D), i8)
+    _check_pool("v_int8", pools.v_int8, NP, (PAGE_SIZE, D), i8)
+    _check_pool("k_int4", pools.k_int4, NP, (PAGE_SIZE, D // 2), u8)
+    _check_pool("v_int4", pools.v_int4, NP, (PAGE_SIZE, D // 2), u8)
+    _check_pool("k_int4r", pools.k_int4r, NP, (PAGE_SIZE, D), u8)
+    _check_pool("v_int4r", pools.v_int4r, NP, (PAGE_SIZE, D), u8)
+    sc = (torch.float16, torch.float32)
+    for n in ("k_fp8_scale", "v_fp8_scale", "k_int8_scale", "v_int8_scale"):
+        t = getattr(pools, n)
+        if t is not None and (t.dtype not in sc or t.numel() != NP):
+            raise ValueError(f"{n} must be [{NP}] float16/float32, got {tuple(t.shape)} {t.dtype}")
+    grp = int(pools.int4_group)
+    if grp <= 0 or D % grp:
+        raise ValueError(f"int4_group must be a positive divisor of head_dim {D}, got {grp}")
+    for n in ("k_int4_scale", "v_int4_scale"):
+        t = getattr(pools, n)
+        if t is not None and (t.dtype not in sc or t.numel() != NP * (D // grp)):
+            raise ValueError(f"{n} must be [{NP}, {D // grp}] float16/float32, got {tuple(t.shape)}")
+    for n in ("k_int4r_scale", "v_int4r_scale"):
+        t = getattr(pools, n)
+        if t is not None and (t.dtype != torch.float32 or t.numel() != 2 * NP):
+            raise ValueError(f"{n} must be [{NP}, 2] float32, got {tuple(t.shape)} {t.dtype}")
+    for n, t in pools.tensors().items():
+        if not t.is_contiguous():
+            raise ValueError(f"{n} must be contiguous")
+    return grp
+
+
 def paged_decode(q: torch.Tensor, pools: PagePools, page_table: torch.Tensor, page_counts: torch.Tensor,
                  page_tags: torch.Tensor, *, tag_map: Optional[Sequence[int]] = None,
                  negative_ids: bool = False, sm_scale: Optional[float] = None,
@@ -226,36 +261,7 @@ def make_plan(q: torch.Tensor, pools: PagePools, page_table: torch.Tensor, page_
         # the kernel reads q rows as 16-byte vectors: a fresh (aligned) copy
         q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
 
-    f16, u8, i8 = (torch.float16,), (torch.uint8,), (torch.int8,)
-    _check_pool("k_fp16", pools.k_fp16, NP, (PAGE_SIZE, D), f16)
-    _check_pool("v_fp16", pools.v_fp16, NP, (PAGE_SIZE, D), f16)
-    _check_pool("k_fp8", pools.k_fp8, NP, (PAGE_SIZE, D), u8 + (torch.float8_e4m3fn,))
-    _check_pool("v_fp8", pools.v_fp8, NP, (PAGE_SIZE, D), u8 + (torch.float8_e4m3fn,))
-    _check_pool("k_int8", pools.k_int8, NP, (PAGE_SIZE, D), i8)
-    _check_pool("v_int8", pools.v_int8, NP, (PAGE_SIZE, D), i8)
-    _check_pool("k_int4", pools.k_int4, NP, (PAGE_SIZE, D // 2), u8)
-    _check_pool("v_int4", pools.v_int4, NP, (PAGE_SIZE, D // 2), u8)
-    _check_pool("k_int4r", pools.k_int4r, NP, (PAGE_SIZE, D), u8)
-    _check_pool("v_int4r", pools.v_int4r, NP, (PAGE_SIZE, D), u8)
-    sc = (torch.float16, torch.float32)
-    for n in ("k_fp8_scale", "v_fp8_scale", "k_int8_scale", "v_int8_scale"):
-        t = getattr(pools, n)
-        if t is not None and (t.dtype not in sc or t.numel() != NP):
-            raise ValueError(f"{n} must be [{NP}] float16/float32, got {tuple(t.shape)} {t.dtype}")
-    grp = int(pools.int4_group)
-    if grp <= 0 or D % grp:
-        raise ValueError(f"int4_group must be a positive divisor of head_dim {D}, got {grp}")
-    for n in ("k_int4_scale", "v_int4_scale"):
-        t = getattr(pools, n)
-        if t is not None and (t.dtype not in sc or t.numel() != NP * (D // grp)):
-            raise ValueError(f"{n} must be [{NP}, {D // grp}] float16/float32, got {tuple(t.shape)}")
-    for n in ("k_int4r_scale", "v_int4r_scale"):
-        t = getattr(pools, n)
-        if t is not None and (t.dtype != torch.float32 or t.numel() != 2 * NP):
-            raise ValueError(f"{n} must be [{NP}, 2] float32, got {tuple(t.shape)} {t.dtype}")
-    for n, t in pools.tensors().items():
-        if not t.is_contiguous():
-            raise ValueError(f"{n} must be contiguous")
+    grp = _check_page_pools(pools, NP, D)
 
     if out is None:
         out = torch.empty((B, Hq, D), dtype=out_dtype or q.dtype, device=dev)
