@@ -36,6 +36,8 @@ __device__ __forceinline__ int row_length(const PageAttn& a, int64_t kvrow) {
 // (km > 0) and K's codes (kf), log2 of what multiplies the weights (vl), and V's codes (vf).
 struct PageEntry { int id, tag; float km, kf, vl, vf; };
 
+__device__ __forceinline__ bool wide_tag(int tag) { return tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL; }
+
 // A page scale in a positive normal multiplier and what is left for the codes: its sign, or itself
 // where it is zero or not finite.
 __device__ __forceinline__ void split_scale(float s, float& mult, float& rest) {
@@ -47,57 +49,72 @@ __device__ __forceinline__ void split_scale(float s, float& mult, float& rest) {
 // The power of two of a scale whose codes go as values.
 __device__ __forceinline__ float power_of(float s) { return s > 0.f && s < __builtin_inff() ? pow2f(scale_exp(s)) : 1.f; }
 
-template <int D, int KIND>
-__device__ __forceinline__ PageEntry page_entry(const PageAttn& a, const int32_t* row, int e, int end) {
-  PageEntry x = {-1, IAK_TAG_FP16, 1.f, 1.f, 0.f, 1.f};
-  if (e >= end) return x;
-  int64_t p = row[e];
+// The look-up in three steps, each of which waits for the one before: the entry, its page's tag, the
+// scales. (A step's loads can be under way while others work.)
+__device__ __forceinline__ int raw_entry(const int32_t* row, int e, int end) { return e < end ? row[e] : (int)0x80000000; }
+
+struct PageTag { int id, tag; };
+__device__ __forceinline__ int entry_page(const PageAttn& a, int raw) {   // -1: none
+  int64_t p = raw;
   if (a.neg_wrap && p < 0) p += a.NP;
-  if (p < 0 || p >= a.NP) return x;
-  const int t = a.tags[p], tag = (uint32_t)t < 8u ? (int)((a.tagmap >> (8 * t)) & 0xFFu) : a.other_tag;
-  if (KIND == PAGES_F16) {
-    if (tag == IAK_TAG_FP16) x.id = (int)p;
-    return x;
-  }
-  x.tag = tag;
-  if (tag == IAK_TAG_FP16) {
-    x.id = (int)p;
-  } else if (tag == IAK_TAG_INT8 || tag == IAK_TAG_FP8) {
-    x.id = (int)p;
-    const bool fp8 = tag == IAK_TAG_FP8;
-    const float k = load_scale(fp8 ? a.k_fp8_scale : a.k_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
-    float v = load_scale(fp8 ? a.v_fp8_scale : a.v_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
-    split_scale(k, x.km, x.kf);
-    split_scale(v, v, x.vf);
-    x.vl = __builtin_amdgcn_logf(v);
-  } else if (KIND == PAGES_ALL && (tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL)) {
-    x.id = (int)p;
-    float k = 0.f, v = 0.f;            // the largest scales
-    if (tag == IAK_TAG_INT4) {
-      const int groups = D / a.int4_group;                       // 1, 2 or 4
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t at = p * groups + (i < groups ? i : 0);
-        k = fmaxf(k, fabsf(load_scale(a.k_int4_scale, at, a.int4_sd)));
-        v = fmaxf(v, fabsf(load_scale(a.v_int4_scale, at, a.int4_sd)));
-      }
-    } else {
-      k = fmaxf(fabsf(a.k_int4r_scale[2 * p]), fabsf(a.k_int4r_scale[2 * p + 1]));
-      v = fmaxf(fabsf(a.v_int4r_scale[2 * p]), fabsf(a.v_int4r_scale[2 * p + 1]));
-    }
-    x.km = power_of(k);
-    v = power_of(v);
-    x.kf = 1.f / x.km;                                           // exact, as the next
-    x.vf = 1.f / v;
-    x.vl = __builtin_amdgcn_logf(v);
-  }
-  return x;
+  return p < 0 || p >= a.NP ? -1 : (int)p;
+}
+__device__ __forceinline__ int raw_tag(const PageAttn& a, int page) { return page < 0 ? -1 : a.tags[page]; }
+template <int KIND> __device__ __forceinline__ PageTag page_tag(const PageAttn& a, int page, int raw) {
+  const int tag = page < 0 ? (int)IAK_TAG_SKIP : (uint32_t)raw < 8u ? (int)((a.tagmap >> (8 * raw)) & 0xFFu) : a.other_tag;
+  const bool known = tag == IAK_TAG_FP16 || (KIND != PAGES_F16 && (tag == IAK_TAG_INT8 || tag == IAK_TAG_FP8)) ||
+                     (KIND == PAGES_ALL && (tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL));
+  return PageTag{known ? page : -1, known ? tag : (int)IAK_TAG_SKIP};
 }
 
-// One of them for the whole wave: lane `k`'s.
-__device__ __forceinline__ float lane_f(float x, int k) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(x), k)); }
+// A page's scales: INT8 and FP8 the ones, 4 bits the largest.
+template <int D, int KIND> __device__ __forceinline__ void page_scales(const PageAttn& a, const PageTag& x, float& k, float& v) {
+  k = v = 1.f;
+  if (KIND == PAGES_F16 || x.id < 0) return;
+  const int64_t p = x.id;
+  if (x.tag == IAK_TAG_INT8 || x.tag == IAK_TAG_FP8) {
+    const bool fp8 = x.tag == IAK_TAG_FP8;
+    k = load_scale(fp8 ? a.k_fp8_scale : a.k_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
+    v = load_scale(fp8 ? a.v_fp8_scale : a.v_int8_scale, p, fp8 ? a.fp8_sd : a.int8_sd);
+  } else if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4) {
+    const int groups = D / a.int4_group;                         // 1, 2 or 4
+    k = v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = p * groups + (i < groups ? i : 0);
+      k = fmaxf(k, fabsf(load_scale(a.k_int4_scale, at, a.int4_sd)));
+      v = fmaxf(v, fabsf(load_scale(a.v_int4_scale, at, a.int4_sd)));
+    }
+  } else if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4_RESIDUAL) {
+    k = fmaxf(fabsf(a.k_int4r_scale[2 * p]), fabsf(a.k_int4r_scale[2 * p + 1]));
+    v = fmaxf(fabsf(a.v_int4r_scale[2 * p]), fabsf(a.v_int4r_scale[2 * p + 1]));
+  }
+}
 
-__device__ __forceinline__ bool wide_tag(int tag) { return tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL; }
+template <int KIND> __device__ __forceinline__ PageEntry page_multipliers(const PageTag& x, float k, float v) {
+  PageEntry e = {x.id, x.tag, 1.f, 1.f, 0.f, 1.f};
+  if (KIND == PAGES_F16 || x.tag == IAK_TAG_FP16) return e;
+  if (wide_tag(x.tag)) {
+    e.km = power_of(k);
+    v = power_of(v);
+    e.kf = 1.f / e.km;                                           // exact, as the next
+    e.vf = 1.f / v;
+  } else {
+    split_scale(k, e.km, e.kf);
+    split_scale(v, v, e.vf);
+  }
+  e.vl = __builtin_amdgcn_logf(v);
+  return e;
+}
+
+template <int D, int KIND>
+__device__ __forceinline__ PageEntry page_entry(const PageAttn& a, const int32_t* row, int e, int end) {
+  const int page = entry_page(a, raw_entry(row, e, end));
+  const PageTag x = page_tag<KIND>(a, page, raw_tag(a, page));
+  float k, v;
+  page_scales<D, KIND>(a, x, k, v);
+  return page_multipliers<KIND>(x, k, v);
+}
 
 // --------------------------------------------------------------------------- //
 // A page's K or V by a wave: loaded, and put into LDS
@@ -115,18 +132,24 @@ template <typename T, bool STREAM> __device__ __forceinline__ T page_ld(const T*
   else return *p;
 }
 
+// (Every branch sets every field: a field that some leave alone is kept in memory by the compiler.)
 template <int D, int KIND, bool STREAM>
 __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool v, int id, int tag, int lane) {
-  if (id < 0) return;                                            // uniform, as the tag
-  const int64_t p = id;
-  if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) {
+  const int64_t p = id < 0 ? 0 : id;                             // uniform, as the tag
+  const u4 zero = {0u, 0u, 0u, 0u};
+  if (id < 0) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) r.x[j] = zero;
+    r.s0 = r.s1 = 0.f;
+  } else if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) {
     const u4* at = reinterpret_cast<const u4*>(v ? a.v_fp16 : a.k_fp16) + p * (PS * D / 8) + lane;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) r.x[j] = page_ld<u4, STREAM>(at + 64 * j);
-    return;
-  }
-  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
+    r.s0 = r.s1 = 0.f;
+  } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
     const uint8_t* page = reinterpret_cast<const uint8_t*>(v ? a.v_int4 : a.k_int4) + p * (PS * D / 2);
+#pragma unroll
+    for (int j = 1; j < D / 32; ++j) r.x[j] = zero;
     if constexpr (D == 128) r.x[0] = *(reinterpret_cast<const u4*>(page) + lane);
     else {
       const u2 x = *(reinterpret_cast<const u2*>(page) + lane);
@@ -134,17 +157,19 @@ __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool
     }
     const int channel = lane % 4 * (D / 4), groups = D / a.int4_group;
     r.s0 = load_scale(v ? a.v_int4_scale : a.k_int4_scale, p * groups + channel / a.int4_group, a.int4_sd);
-    return;
-  }
-  const void* pool = tag == IAK_TAG_INT8 ? (v ? a.v_int8 : a.k_int8) : tag == IAK_TAG_FP8 ? (v ? a.v_fp8 : a.k_fp8)
-                                                                                         : (v ? a.v_int4r : a.k_int4r);
-  const u4* at = reinterpret_cast<const u4*>(pool) + p * (PS * D / 16) + lane;
+    r.s1 = 0.f;
+  } else {
+    const void* pool = tag == IAK_TAG_INT8 ? (v ? a.v_int8 : a.k_int8) : tag == IAK_TAG_FP8 ? (v ? a.v_fp8 : a.k_fp8)
+                                                                                           : (v ? a.v_int4r : a.k_int4r);
+    const u4* at = reinterpret_cast<const u4*>(pool) + p * (PS * D / 16) + lane;
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j) r.x[j] = page_ld<u4, STREAM>(at + 64 * j);
-  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
-    const float* s = (v ? a.v_int4r_scale : a.k_int4r_scale) + 2 * p;
-    r.s0 = s[0];
-    r.s1 = s[1];
+    for (int j = 0; j < D / 32; ++j) r.x[j] = j < D / 64 ? page_ld<u4, STREAM>(at + 64 * j) : zero;
+    r.s0 = r.s1 = 0.f;
+    if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
+      const float* s = (v ? a.v_int4r_scale : a.k_int4r_scale) + 2 * p;
+      r.s0 = s[0];
+      r.s1 = s[1];
+    }
   }
 }
 
@@ -230,30 +255,24 @@ __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag,
       }
     }
   } else {
-    const bool fp8 = tag == IAK_TAG_FP8;
     const h2 sign = splat2((_Float16)rest);
+    auto bytes = [&](auto&& four) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const int f = 64 * j + lane, token = f / (D / 16), chunk = f % (D / 16) * 2;
+      for (int j = 0; j < D / 64; ++j) {
+        const int f = 64 * j + lane, token = f / (D / 16), chunk = f % (D / 16) * 2;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t o[4];
-        if (fp8) {
-          fp8x4_to_f16(r.x[j][2 * c], o[0], o[1]);
-          fp8x4_to_f16(r.x[j][2 * c + 1], o[2], o[3]);
-        } else {
-          i8x4_to_f16(r.x[j][2 * c], o[0], o[1]);
-          i8x4_to_f16(r.x[j][2 * c + 1], o[2], o[3]);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[4];
+          four(r.x[j][2 * c], o[0], o[1]);
+          four(r.x[j][2 * c + 1], o[2], o[3]);
+          const u4 h = u4{bits(as_h2(o[0]) * sign), bits(as_h2(o[1]) * sign), bits(as_h2(o[2]) * sign), bits(as_h2(o[3]) * sign)};
+          hi[v_chunk<D>(token, chunk + c)] = h;
+          look(h);
         }
-        if (rest != 1.f) {                                       // uniform, rare
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = bits(as_h2(o[i]) * sign);
-        }
-        const u4 h = u4{o[0], o[1], o[2], o[3]};
-        hi[v_chunk<D>(token, chunk + c)] = h;
-        look(h);
       }
-    }
+    };
+    if (tag == IAK_TAG_FP8) bytes([](uint32_t x, uint32_t& l, uint32_t& h) __attribute__((always_inline)) { fp8x4_to_f16(x, l, h); });
+    else bytes([](uint32_t x, uint32_t& l, uint32_t& h) __attribute__((always_inline)) { i8x4_to_f16(x, l, h); });
   }
   return CHECK && !((float)sum[0] + (float)sum[1] == 0.f);
 }
@@ -316,35 +335,57 @@ template <int PAGES> __device__ __forceinline__ int value_power(const int (&id)[
   return most < -199.f || (e <= E && e >= E - V_ROOM) ? E : e;
 }
 
-// Infinite and NaN values where a row sees them: a weight of zero would make them NaN where it does not, so the
-// products have zeros there (clean), and each is added by itself, whatever its weight. `first`: the number of the
-// pages' first token.
-__device__ __forceinline__ h8 clean(h8 x) {
-  u4 w = __builtin_bit_cast(u4, x);
+// Infinite and NaN values of V: a weight of zero would make them NaN where a row does not see them, so
+// the tiles have zeros in their place. A page that has any leaves beside its tile, for every 16-byte chunk, which
+// of its 8 values are positive (bits 0 .. 7) and which negative (8 .. 15; NaN: both), and whoever sees one
+// remembers it by channel until the end: a weight is positive, whatever its size. All of this is rare.
+template <int D> __device__ __forceinline__ void clean_tile(u4* tile, int lane) {
+  for (int f = lane; f < PS * D / 8; f += 64) {
+    u4 w = tile[f];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t e = w[i] & 0x7C007C00u;
-    w[i] &= ((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t e = w[i] & 0x7C007C00u;
+      w[i] &= ((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u);
+    }
+    tile[f] = w;
   }
-  return __builtin_bit_cast(h8, w);
 }
-template <int D, int T>
-__device__ __forceinline__ void add_special(f4 (&acc)[T][D / 16], const u4* page, int id, int first, const int (&seen)[T], int g) {
-  if (id < 0) return;
-  for (int token = 0; token < PS; ++token) {
+template <int D> __device__ __forceinline__ void put_aside(u4* tile, uint16_t* special, int lane) {
+  for (int f = lane; f < PS * D / 8; f += 64) {
+    u4 w = tile[f];
+    uint32_t bits16 = 0u;
 #pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb) {
-      const h4 v = *reinterpret_cast<const h4*>(reinterpret_cast<const char*>(page + v_chunk<D>(token, 2 * mb + (g >> 1))) + 8 * (g & 1));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float x = (float)v[q];
-        const bool special = !(fabsf(x) < __builtin_inff());
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-          if (special && first + token < seen[t]) acc[t][mb][q] += x;
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+      if ((h & 0x7C00u) == 0x7C00u) {
+        const bool nan = (h & 0x3FFu) != 0u;
+        bits16 |= (nan || h < 0x8000u ? 1u << i : 0u) | (nan || h >= 0x8000u ? 256u << i : 0u);
+        w[i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
       }
     }
+    tile[f] = w;
+    special[f] = (uint16_t)bits16;
   }
+}
+// A lane's memory: bit 4 mb + q is channel 16 mb + 4 g + q of its row.
+struct Seen16 { uint32_t plus, minus; };
+template <int D>
+__device__ __forceinline__ void remember(Seen16& x, const uint16_t* special, int tokens, int g) {
+  for (int token = 0; token < tokens; ++token)
+    for (int mb = 0; mb < D / 16; ++mb) {
+      const uint32_t s = (uint32_t)special[v_chunk<D>(token, 2 * mb + (g >> 1))] >> (4 * (g & 1));
+      x.plus |= (s & 15u) << (4 * mb);
+      x.minus |= ((s >> 8) & 15u) << (4 * mb);
+    }
+}
+template <int D> __device__ __forceinline__ void bring_back(f4 (&acc)[D / 16], const Seen16& x) {
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if ((x.plus >> (4 * mb + q)) & 1u) acc[mb][q] += __builtin_inff();
+      if ((x.minus >> (4 * mb + q)) & 1u) acc[mb][q] -= __builtin_inff();
+    }
 }
 
 }  // namespace iak

@@ -16,9 +16,6 @@ namespace iak {
 
 namespace {
 
-struct Plain { static constexpr bool value = false; };
-struct Cleaned { static constexpr bool value = true; };
-
 template <int D, bool QF32, int NW, int RT, int KIND>
 __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a) {
   static_assert(NW == 4 || NW == 8, "a wave takes a page of K and of V, or one of the two");
@@ -27,7 +24,9 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   __shared__ u4 tiles[2][2][4][PAGE];                            // [buffer][K, V][page]
   __shared__ u4 rest[WIDE ? 2 : 1][2][4][WIDE ? PAGE : 1];       // of wide pages: what their tiles leave
   __shared__ u4 none[WIDE ? PAGE : 1];                           // zeros
-  __shared__ u4 special_in[2];                                   // a word a page: V has infinite or NaN values
+  __shared__ u4 metas[128];                                      // of entry e at e % 128: page, tag, km, vl
+  __shared__ u2 factors[SCALED ? 128 : 1];                       // kf, vf
+  __shared__ int special;                                        // V has infinite or NaN values
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const MxPart part = a.shares ? mx_shared_part<4, true>(a) : mx_fixed_part(a);
@@ -58,41 +57,59 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
 
-  // entries 64 at a time: lane i holds entry i of the block, in `next` of the block after it
+  // The entries' pages and multipliers lie in LDS, 64 ahead of the walk: wave 0 looks up a block of 64
+  // in four steps of the walk, a load each.
   const int32_t* row = a.table + kvrow * a.W;
-  auto entry = [&](int k) { return page_entry<D, KIND>(a, row, e0 + k, e1); };
-  PageEntry now = entry(lane), next = entry(64 + lane);
-  auto id_of = [&](int k) {
-    const int here = __builtin_amdgcn_readlane(now.id, k & 63), after = __builtin_amdgcn_readlane(next.id, k & 63);
-    return k < 64 ? here : after;
+  auto keep = [&](int k, const PageEntry& x) __attribute__((always_inline)) {
+    metas[k & 127] = u4{(uint32_t)x.id, (uint32_t)x.tag, f2u(x.km), f2u(x.vl)};
+    if constexpr (SCALED) factors[k & 127] = u2{f2u(x.kf), f2u(x.vf)};
   };
-  auto tag_of = [&](int k) {
-    if constexpr (!SCALED) return (int)IAK_TAG_FP16;
-    const int here = __builtin_amdgcn_readlane(now.tag, k & 63), after = __builtin_amdgcn_readlane(next.tag, k & 63);
-    return k < 64 ? here : after;
+  if (w < 2) keep(64 * w + lane, page_entry<D, KIND>(a, row, e0 + 64 * w + lane, e1));
+  if (threadIdx.x == 0) special = 0;
+  __syncthreads();
+  int ahead = 0, ahead_tag = 0;
+  float ahead_k = 1.f, ahead_v = 1.f;
+  auto look_ahead = [&](int k) __attribute__((always_inline)) {  // k: entry of the walk, a multiple of 4
+    if ((k & 15) != 0 || w != 0) return;
+    const int stage = (k >> 4) & 3, e = (k & ~63) + 64 + lane;   // the block after the one at hand
+    if (k < 64) return;                                          // two blocks are there at first
+    if (stage == 0) ahead = raw_entry(row, e0 + e, e1);
+    else if (stage == 1) {
+      ahead = entry_page(a, ahead);
+      ahead_tag = raw_tag(a, ahead);
+    } else if (stage == 2) {
+      const PageTag x = page_tag<KIND>(a, ahead, ahead_tag);
+      ahead = x.id;
+      ahead_tag = x.tag;
+      page_scales<D, KIND>(a, x, ahead_k, ahead_v);
+    } else keep(e, page_multipliers<KIND>(PageTag{ahead, ahead_tag}, ahead_k, ahead_v));
   };
-  auto pick = [&](float here, float after, int k) { return k < 64 ? lane_f(here, k & 63) : lane_f(after, k & 63); };
+  auto uniform = [](uint32_t x) { return __builtin_amdgcn_readfirstlane((int)x); };
+  auto uniform_f = [](uint32_t x) { return u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)x)); };
 
   // this wave's page of a step, of K and V or of one of them: loaded a step ahead, put into LDS during
   // the step before
   const int own = w & 3, side = w >> 2;
   PageRaw<D> raw[OWN];
-  auto load = [&](int k) __attribute__((always_inline)) {
-    const int id = id_of(k), tag = tag_of(k);
+  auto load = [&](const u4& x) __attribute__((always_inline)) {
 #pragma unroll
-    for (int o = 0; o < OWN; ++o) load_page<D, KIND, false>(raw[o], a, OWN == 2 ? o == 1 : side == 1, id, tag, lane);
+    for (int o = 0; o < OWN; ++o)
+      load_page<D, KIND, false>(raw[o], a, OWN == 2 ? o == 1 : side == 1, uniform(x[0]), uniform(x[1]), lane);
   };
-  auto convert = [&](int buf, int k) __attribute__((always_inline)) {
-    const int id = id_of(k), tag = tag_of(k);
+  auto convert = [&](int buf, const u4& x, const u2& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
       const int s = OWN == 2 ? o : side;
-      const float f = !SCALED ? 1.f : s ? pick(now.vf, next.vf, k) : pick(now.kf, next.kf, k);
-      const bool odd = store_page<D, KIND, true>(raw[o], id, tag, f, tiles[buf][s][own], rest[WIDE ? buf : 0][s][own], lane);
-      const uint64_t any = __builtin_amdgcn_ballot_w64(odd);
-      if (s == 1 && lane == 0) reinterpret_cast<uint32_t*>(&special_in[buf])[own] = any != 0;
+      const bool bad = store_page<D, KIND, true>(raw[o], uniform(x[0]), uniform(x[1]), uniform_f(s ? f[1] : f[0]), tiles[buf][s][own],
+                                                 rest[WIDE ? buf : 0][s][own], lane);
+      if (s == 1 && __builtin_amdgcn_ballot_w64(bad)) {          // rare
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        clean_tile<D>(tiles[buf][1][own], lane);
+        if (lane == 0) special = 1;
+      }
     }
   };
+  const u2 one = {f2u(1.f), f2u(1.f)};
 
   f4 acc[RT][D / 16], l[RT];
   float lsum[RT], m[RT];
@@ -107,8 +124,13 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   }
 
   const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-  int k = 0, block = 0;                                          // number of entry e in the block
+  int k = 0;                                                     // number of entry e in the part
   auto step = [&](int buf, int e) __attribute__((always_inline)) {
+    u4 at[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) at[p] = metas[(k + p) & 127];
+    const u4 mine = metas[(k + 4 + own) & 127], after = metas[(k + 8 + own) & 127];
+    const u2 factor = SCALED ? factors[(k + 4 + own) & 127] : one;
     f4 s[RT][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -125,14 +147,15 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
           if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[t][j], s[t][p], 0, 0, 0);
         }
       }
-    const int id[4] = {id_of(k), id_of(k + 1), id_of(k + 2), id_of(k + 3)};
+    int id[4];
     float km[4], vl[4];
     bool wide[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      km[p] = SCALED ? pick(now.km, next.km, k + p) : 1.f;
-      vl[p] = SCALED ? pick(now.vl, next.vl, k + p) : 0.f;
-      wide[p] = WIDE && id[p] >= 0 && wide_tag(tag_of(k + p));
+      id[p] = uniform(at[p][0]);
+      km[p] = SCALED ? uniform_f(at[p][2]) : 1.f;
+      vl[p] = SCALED ? uniform_f(at[p][3]) : 0.f;
+      wide[p] = WIDE && id[p] >= 0 && wide_tag(uniform(at[p][1]));
     }
     if constexpr (WIDE) {
 #pragma unroll
@@ -146,10 +169,9 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
         }
       }
     }
-    const u4 sp = special_in[buf];
-    convert(buf ^ 1, k + 4 + own);
-    load(k + 8 + own);
-    const uint32_t special = __builtin_amdgcn_readfirstlane(sp[0] | sp[1] | sp[2] | sp[3]);
+    convert(buf ^ 1, mine, factor);
+    load(after);
+    look_ahead(k);
     const uint32_t no_nan[4] = {0u, 0u, 0u, 0u};
     hide<4, RT>(s, no_nan, id, e, seen, least, g);
     if constexpr (SCALED) {
@@ -185,20 +207,6 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
         pb[t][h] = weights(s[t][2 * h], s[t][2 * h + 1]);
         if constexpr (QF32) pl[t][h] = weights_rest(s[t][2 * h], s[t][2 * h + 1], pb[t][h]);
       }
-    auto values = [&](auto cleaned) __attribute__((always_inline)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int mb = 0; mb < D / 16; ++mb) {
-          h8 va = values_back<D>(tiles[buf][1][2 * h], tiles[buf][1][2 * h + 1], mb, c, g);
-          if constexpr (decltype(cleaned)::value) va = clean(va);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[t][h], acc[t][mb], 0, 0, 0);
-            if constexpr (QF32) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[t][h], acc[t][mb], 0, 0, 0);
-          }
-        }
-    };
     if constexpr (!SCALED) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -208,13 +216,17 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
           if constexpr (QF32) l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t][h], l[t], 0, 0, 0);
         }
     }
-    if (special == 0) {
-      values(Plain{});
-    } else {
-      values(Cleaned{});
 #pragma unroll
-      for (int p = 0; p < 4; ++p) add_special<D, RT>(acc, tiles[buf][1][p], id[p], (e + p) * PS, seen, g);
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) {
+        const h8 va = values_back<D>(tiles[buf][1][2 * h], tiles[buf][1][2 * h + 1], mb, c, g);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[t][h], acc[t][mb], 0, 0, 0);
+          if constexpr (QF32) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[t][h], acc[t][mb], 0, 0, 0);
+        }
+      }
     if constexpr (WIDE) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -230,23 +242,51 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
       }
     }
     k += 4;
-    if (k == 64) {
-      k = 0;
-      block += 64;
-      now = next;
-      next = entry(block + 64 + lane);
-    }
     __syncthreads();                                             // this buffer is free, the other one is whole
   };
   if (e0 < e1) {
-    load(own);
-    convert(0, own);
-    load(4 + own);
+    load(metas[own]);
+    convert(0, metas[own], SCALED ? factors[own] : one);
+    load(metas[4 + own]);
     __syncthreads();
     for (int e = e0; e < e1; e += 8) {
       step(0, e);
       if (e + 4 < e1) step(1, e + 4);
     }
+  }
+
+  // what V has of infinite and NaN values, in a second walk
+  if (special) {                                                 // uniform: written before the last barrier
+    uint16_t* aside = reinterpret_cast<uint16_t*>(&tiles[1][0][0][0]);
+    uint32_t* any = reinterpret_cast<uint32_t*>(&tiles[1][1][0][0]);
+    Seen16 odd[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) odd[t] = Seen16{0u, 0u};
+    for (int e = e0; e < e1; e += 4) {
+      __syncthreads();
+      if (w < 4) {
+        const PageEntry x = page_entry<D, KIND>(a, row, e + w, e1);
+        const int id = uniform((uint32_t)x.id), tag = uniform((uint32_t)x.tag);
+        PageRaw<D> r;
+        load_page<D, KIND, false>(r, a, true, id, tag, lane);
+        const bool bad = store_page<D, KIND, true>(r, id, tag, uniform_f(f2u(x.vf)), tiles[0][0][w], rest[0][0][w], lane);
+        const bool some = __builtin_amdgcn_ballot_w64(bad) != 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (some) put_aside<D>(tiles[0][0][w], aside + w * PAGE, lane);
+        if (lane == 0) any[w] = some;
+      }
+      __syncthreads();
+      for (int p = 0; p < 4; ++p) {
+        if (uniform(any[p]) == 0) continue;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const int left = seen[t] - (e + p) * PS;
+          remember<D>(odd[t], aside + p * PAGE, left < PS ? left : PS, g);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) bring_back<D>(acc[t], odd[t]);
   }
 
 #pragma unroll
@@ -293,7 +333,7 @@ template <int D, bool QF32, int NW, int RT> void launch_tiles(const PageAttn& a,
 }
 
 template <int D> void launch_chunk(const PageAttn& a, hipStream_t stream) {
-  if (a.q_dtype == IAK_DTYPE_F32) launch_tiles<D, true, 4, 2>(a, stream);
+  if (a.q_dtype == IAK_DTYPE_F32) launch_tiles<D, true, 8, 1>(a, stream);
   else if (a.tile_rows == 256) launch_tiles<D, false, 8, 2>(a, stream);
   else launch_tiles<D, false, 4, 2>(a, stream);
 }

@@ -33,6 +33,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
   constexpr int PAGE = PS * D / 8;                               // 16-byte units of a tile
   __shared__ u4 tiles[ROW_WAVES][2 * PAGE * (WIDE ? 2 : 1)];     // K's, then V's; at the end the waves' sums
   __shared__ u4 none[WIDE ? PAGE : 1];                           // zeros
+  __shared__ uint16_t special[ROW_WAVES][PAGE];
   __shared__ float part_m[ROW_WAVES][16], part_l[ROW_WAVES][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
@@ -59,25 +60,21 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
 
   // the wave's entries, 64 at a time: lane i holds number i of the block, in `next` of the block after it
   const int32_t* row = a.table + kvrow * a.W;
-  auto entry = [&](int k) {
-    const int e = e0 + wave_entry(w, k);
-    return page_entry<D, KIND>(a, row, e, e1);
-  };
+  auto entry = [&](int k) { return page_entry<D, KIND>(a, row, e0 + wave_entry(w, k), e1); };
   PageEntry now = entry(lane), next = entry(64 + lane);
-  auto of = [&](int k) {                                         // entry k of the block, k < 128
-    const PageEntry& x = k < 64 ? now : next;
-    PageEntry y;
-    y.id = __builtin_amdgcn_readlane(x.id, k & 63);
+  auto pick = [&](int here, int after, int k) {
+    const int x = __builtin_amdgcn_readlane(here, k & 63), y = __builtin_amdgcn_readlane(after, k & 63);
+    return k < 64 ? x : y;
+  };
+  auto pick_f = [&](float here, float after, int k) { return u2f((uint32_t)pick((int)f2u(here), (int)f2u(after), k)); };
+  auto of = [&](int k) __attribute__((always_inline)) {          // entry k of the block, k < 128
+    PageEntry y = {pick(now.id, next.id, k), IAK_TAG_FP16, 1.f, 1.f, 0.f, 1.f};
     if constexpr (KIND != PAGES_F16) {
-      y.tag = __builtin_amdgcn_readlane(x.tag, k & 63);
-      y.km = lane_f(x.km, k & 63);
-      y.kf = lane_f(x.kf, k & 63);
-      y.vl = lane_f(x.vl, k & 63);
-      y.vf = lane_f(x.vf, k & 63);
-    } else {
-      y.tag = IAK_TAG_FP16;
-      y.km = y.kf = y.vf = 1.f;
-      y.vl = 0.f;
+      y.tag = pick(now.tag, next.tag, k);
+      y.km = pick_f(now.km, next.km, k);
+      y.kf = pick_f(now.kf, next.kf, k);
+      y.vl = pick_f(now.vl, next.vl, k);
+      y.vf = pick_f(now.vf, next.vf, k);
     }
     return y;
   };
@@ -91,6 +88,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
   float m[1] = {M_NONE}, l[1] = {0.f};
   int E = 0;
   u4* mine = tiles[w];
+  Seen16 odd = {0u, 0u};
 
   PageRaw<D> k[2], v[2];
   PageEntry at[2];                                               // of the pair that k and v hold
@@ -147,13 +145,19 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
 
     // V in K's place
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    bool odd[2];
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-      odd[p] = store_page<D, KIND, true>(v[p], id[p], x[p].tag, x[p].vf, mine + p * PAGE, mine + (2 + p) * PAGE, lane);
+    for (int p = 0; p < 2; ++p) {
+      const bool any = store_page<D, KIND, true>(v[p], id[p], x[p].tag, x[p].vf, mine + p * PAGE, mine + (2 + p) * PAGE, lane);
+      if (__builtin_amdgcn_ballot_w64(any)) {
+        put_aside<D>(mine + p * PAGE, special[w], lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int first = (e + p) * PS;
+        remember<D>(odd, special[w], seen[0] - first < PS ? seen[0] - first : PS, g);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     load(v, true);
-    const bool special = __builtin_amdgcn_ballot_w64(odd[0] || odd[1]) != 0;
 
     const uint32_t no_nan[2] = {0u, 0u};
     hide<2, 1>(s, no_nan, id, e, seen, least, g);
@@ -179,22 +183,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
     const h8 pb = weights(s[0][0], s[0][1]);
     h8 pl;
     if constexpr (QF32) pl = weights_rest(s[0][0], s[0][1], pb);
-    if (!special) {
 #pragma unroll
-      for (int mb = 0; mb < D / 16; ++mb) {
-        const h8 va = values_back<D>(mine, mine + PAGE, mb, c, g);
-        acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[0][mb], 0, 0, 0);
-        if constexpr (QF32) acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[0][mb], 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int mb = 0; mb < D / 16; ++mb) {
-        const h8 va = clean(values_back<D>(mine, mine + PAGE, mb, c, g));
-        acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[0][mb], 0, 0, 0);
-        if constexpr (QF32) acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[0][mb], 0, 0, 0);
-      }
-#pragma unroll
-      for (int p = 0; p < 2; ++p) add_special<D, 1>(acc, mine + p * PAGE, id[p], (e + p) * PS, seen, g);
+    for (int mb = 0; mb < D / 16; ++mb) {
+      const h8 va = values_back<D>(mine, mine + PAGE, mb, c, g);
+      acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[0][mb], 0, 0, 0);
+      if constexpr (QF32) acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[0][mb], 0, 0, 0);
     }
     if constexpr (WIDE) {
       if (wide[0] || wide[1]) {
@@ -213,6 +206,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
       next = entry(block + 64 + lane);
     }
   }
+
+  if (__builtin_amdgcn_ballot_w64((odd.plus | odd.minus) != 0u)) bring_back<D>(acc[0], odd);
 
   // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
   const float sum = xsum16_32(l[0]);
