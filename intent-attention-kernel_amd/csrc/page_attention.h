@@ -28,6 +28,14 @@ __device__ __forceinline__ int row_length(const PageAttn& a, int64_t kvrow) {
   return v < listed ? v : listed;
 }
 
+// The kernel's arguments, read anew: what is used seldom would otherwise be kept in scalar registers from the
+// start, and be spilled for the walk.
+__device__ __forceinline__ const PageAttn& arguments() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PageAttn*)p;
+}
+
 // --------------------------------------------------------------------------- //
 // Entries
 // --------------------------------------------------------------------------- //
@@ -92,19 +100,17 @@ template <int D, int KIND> __device__ __forceinline__ void page_scales(const Pag
 }
 
 template <int KIND> __device__ __forceinline__ PageEntry page_multipliers(const PageTag& x, float k, float v) {
-  PageEntry e = {x.id, x.tag, 1.f, 1.f, 0.f, 1.f};
-  if (KIND == PAGES_F16 || x.tag == IAK_TAG_FP16) return e;
-  if (wide_tag(x.tag)) {
-    e.km = power_of(k);
-    v = power_of(v);
-    e.kf = 1.f / e.km;                                           // exact, as the next
-    e.vf = 1.f / v;
-  } else {
-    split_scale(k, e.km, e.kf);
-    split_scale(v, v, e.vf);
-  }
-  e.vl = __builtin_amdgcn_logf(v);
-  return e;
+  if constexpr (KIND == PAGES_F16) return PageEntry{x.id, x.tag, 1.f, 1.f, 0.f, 1.f};
+  const bool wide = wide_tag(x.tag);
+  float km, kf, vm, vf;                                          // float16 pages have scales of 1
+  split_scale(k, km, kf);
+  split_scale(v, vm, vf);
+  const float kp = power_of(k), vp = power_of(v);
+  km = wide ? kp : km;
+  vm = wide ? vp : vm;
+  kf = wide ? 1.f / kp : kf;                                     // exact
+  vf = wide ? 1.f / vp : vf;
+  return PageEntry{x.id, x.tag, km, kf, __builtin_amdgcn_logf(vm), vf};
 }
 
 template <int D, int KIND>
@@ -180,11 +186,18 @@ __device__ __forceinline__ void hi_lo(float a, float b, bool fine, uint32_t& hi,
   lo = fine ? bits(h2{(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])}) : 0u;
 }
 
+// A scale in two float16 parts; a code times the first is off by what a fused product gives exactly.
+struct ScaleParts { h2 hi, lo; uint32_t fine; };                 // fine 0: infinite or NaN, which has no second part
+__device__ __forceinline__ ScaleParts scale_parts(float s) {
+  const _Float16 h = (_Float16)s;
+  return ScaleParts{splat2(h), splat2((_Float16)(s - (float)h)), fabsf(s) < __builtin_inff() ? 0xFFFFFFFFu : 0u};
+}
+
 // The pair of codes (n & 15, n >> 4 & 15), less 8 each, of byte `byte` of w, as float16: exact.
 __device__ __forceinline__ h2 nibbles(uint32_t w, int byte) {
   const uint32_t y = __builtin_amdgcn_perm(0u, w, 0x0C000C00u | (uint32_t)byte | ((uint32_t)byte << 16));   // (b, 0, b, 0)
   const h2 n = as_h2((y & 0x00F0000Fu) | MAGIC_I4);              // 1024 + low, 1024 + 16 high
-  return h2{n[0] - (_Float16)1032.f, (n[1] - (_Float16)1152.f) * (_Float16)0.0625f};
+  return __builtin_elementwise_fma(n, h2{(_Float16)1.f, (_Float16)0.0625f}, h2{(_Float16)-1032.f, (_Float16)-72.f});
 }
 
 // The page into LDS as float16 rows (16-byte chunks at v_chunk); `lo`, written for wide pages alone: what is
@@ -211,19 +224,16 @@ __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag,
       look(r.x[j]);
     }
   } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
-    const float s = r.s0 * rest;
-    const bool fine = fabsf(s) < __builtin_inff();
+    const ScaleParts k = scale_parts(r.s0 * rest);
     const int token = lane / 4, chunk = lane % 4 * (D / 32);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       u4 h, l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const h2 n = nibbles(r.x[0][c], i);
-        uint32_t x, y;
-        hi_lo((float)n[0] * s, (float)n[1] * s, fine, x, y);
-        h[i] = x;
-        l[i] = y;
+        const h2 n = nibbles(r.x[0][c], i), x = n * k.hi;
+        h[i] = bits(x);
+        l[i] = bits(__builtin_elementwise_fma(n, k.lo, __builtin_elementwise_fma(n, k.hi, -x))) & k.fine;
       }
       const int at = v_chunk<D>(token, chunk + c);
       hi[at] = h;
@@ -278,6 +288,128 @@ __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag,
 }
 
 // --------------------------------------------------------------------------- //
+// The same by pieces, for waves that share pages: a lane has one 16-byte chunk of a page's float16 rows, whatever
+// the precision, so that all waves have the same to do. Where the pages lie, their tags and multipliers are
+// looked up ahead into LDS, from where they come as vectors: a step's worth of them, and of the pools they lie in,
+// is more than the scalar registers hold.
+// --------------------------------------------------------------------------- //
+
+constexpr uint32_t NO_PAGE = 0xFFu;
+constexpr float NO_SCALE = -200.f;      // below every float's log2
+constexpr int AHEAD = 128;             // entries at hand: entry e at e % AHEAD
+
+template <int KIND> struct Ahead {
+  u4 where[AHEAD];                     // addresses of K and of V
+  uint8_t tag[AHEAD];                  // native, or NO_PAGE
+  float km[KIND == PAGES_F16 ? 1 : AHEAD], vl[KIND == PAGES_F16 ? 1 : AHEAD];   // as in PageEntry; no page: vl NO_SCALE
+  float iv[KIND == PAGES_F16 ? 1 : AHEAD];                                      // 2^-vl, 0
+  f4 factors[2][KIND == PAGES_F16 ? 1 : AHEAD];   // of K's and V's codes; INT4: by quarters of the channels, residual: base, rest
+};
+
+template <int D, int KIND>
+__device__ __forceinline__ void put_ahead(Ahead<KIND>& t, const PageAttn& a, int e, const PageTag& x) {
+  const int at = e & (AHEAD - 1);
+  const int64_t p = x.id < 0 ? 0 : x.id;
+  const void* k = a.k_fp16;
+  const void* v = a.v_fp16;
+  int bytes = PS * D * 2;
+  if (KIND != PAGES_F16 && x.tag == IAK_TAG_INT8) { k = a.k_int8; v = a.v_int8; bytes = PS * D; }
+  if (KIND != PAGES_F16 && x.tag == IAK_TAG_FP8) { k = a.k_fp8; v = a.v_fp8; bytes = PS * D; }
+  if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4) { k = a.k_int4; v = a.v_int4; bytes = PS * D / 2; }
+  if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4_RESIDUAL) { k = a.k_int4r; v = a.v_int4r; bytes = PS * D; }
+  const uint64_t ka = reinterpret_cast<uint64_t>(k) + p * bytes, va = reinterpret_cast<uint64_t>(v) + p * bytes;
+  t.where[at] = u4{(uint32_t)ka, (uint32_t)(ka >> 32), (uint32_t)va, (uint32_t)(va >> 32)};
+  t.tag[at] = (uint8_t)(x.id < 0 ? NO_PAGE : (uint32_t)x.tag);
+  if constexpr (KIND != PAGES_F16) {
+    float ks, vs;
+    page_scales<D, KIND>(a, x, ks, vs);
+    const PageEntry y = page_multipliers<KIND>(x, ks, vs);
+    f4 kf = {y.kf, y.kf, y.kf, y.kf}, vf = {y.vf, y.vf, y.vf, y.vf};
+    if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4) {
+      const int groups = D / a.int4_group;                       // 1, 2 or 4
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        kf[q] *= load_scale(a.k_int4_scale, p * groups + q * groups / 4, a.int4_sd);
+        vf[q] *= load_scale(a.v_int4_scale, p * groups + q * groups / 4, a.int4_sd);
+      }
+    }
+    if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4_RESIDUAL) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        kf[q] *= a.k_int4r_scale[2 * p + q];
+        vf[q] *= a.v_int4r_scale[2 * p + q];
+      }
+    }
+    t.km[at] = y.km;
+    t.vl[at] = x.id < 0 ? NO_SCALE : y.vl;
+    t.iv[at] = x.id < 0 ? 0.f : __builtin_amdgcn_exp2f(-y.vl);
+    t.factors[0][at] = kf;
+    t.factors[1][at] = vf;
+  }
+}
+
+// Chunk f (of 2 D) of a page at `page`.
+template <int D, int KIND>
+__device__ __forceinline__ u4 load_piece(uint64_t page, uint32_t tag, uint32_t f) {
+  typedef __attribute__((address_space(1))) const uint8_t byte;
+  typedef __attribute__((address_space(1))) const uint32_t word;
+  typedef __attribute__((address_space(1))) const u2 pair;
+  typedef __attribute__((address_space(1))) const u4 four;
+  byte* p = reinterpret_cast<byte*>(page);
+  if (tag == NO_PAGE) return u4{0u, 0u, 0u, 0u};                 // uniform
+  if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) return *reinterpret_cast<four*>(p + 16 * f);
+  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) return u4{*reinterpret_cast<word*>(p + 4 * f), 0u, 0u, 0u};
+  const u2 x = *reinterpret_cast<pair*>(p + 8 * f);
+  return u4{x[0], x[1], 0u, 0u};
+}
+
+// Into place `at` of the tile `hi`, and what is left of wide pages into `lo`.
+template <int D, int KIND>
+__device__ __forceinline__ void store_piece(const u4& x, uint32_t tag, const f4& factors, int f, u4* hi, u4* lo, int at) {
+  if (KIND == PAGES_F16 || tag == NO_PAGE || tag == IAK_TAG_FP16) {
+    hi[at] = x;
+    return;
+  }
+  u4 h, l;
+  if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
+    const ScaleParts k = scale_parts(reinterpret_cast<const float*>(&factors)[f % (D / 8) / (D / 32)]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2 n = nibbles(x[0], i), y = n * k.hi;
+      h[i] = bits(y);
+      l[i] = bits(__builtin_elementwise_fma(n, k.lo, __builtin_elementwise_fma(n, k.hi, -y))) & k.fine;
+    }
+    lo[at] = l;
+  } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
+    const float s0 = factors[0], s1 = factors[1];
+    const bool fine = fabsf(s0) + fabsf(s1) < __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = x[i >> 1];
+      const h2 m = nibbles(w, 2 * (i & 1)), n = nibbles(w, 2 * (i & 1) + 1);
+      uint32_t y, z;
+      hi_lo(__builtin_fmaf((float)m[0], s0, (float)m[1] * s1), __builtin_fmaf((float)n[0], s0, (float)n[1] * s1), fine, y, z);
+      h[i] = y;
+      l[i] = z;
+    }
+    lo[at] = l;
+  } else {
+    const h2 sign = splat2((_Float16)factors[0]);
+    uint32_t o[4];
+    if (tag == IAK_TAG_FP8) {
+      fp8x4_to_f16(x[0], o[0], o[1]);
+      fp8x4_to_f16(x[1], o[2], o[3]);
+    } else {
+      i8x4_to_f16(x[0], o[0], o[1]);
+      i8x4_to_f16(x[1], o[2], o[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = bits(as_h2(o[i]) * sign);
+  }
+  hi[at] = h;
+}
+
+// --------------------------------------------------------------------------- //
 // The softmax of PAGES pages whose scores and weights have multipliers (hide() is mx_attention.h's)
 // --------------------------------------------------------------------------- //
 
@@ -327,28 +459,29 @@ __device__ __forceinline__ float soften_scaled(f4 (&s)[PAGES], const float (&km)
 // V's scales differ by pages: weights carry 2^(vl - E), the accumulators stand for 2^E of themselves, and E follows
 // the largest of a step's, with room below it so that it moves seldom.
 constexpr int V_ROOM = 8;
-template <int PAGES> __device__ __forceinline__ int value_power(const int (&id)[PAGES], const float (&vl)[PAGES], int E) {
-  float most = -200.f;
+template <int PAGES> __device__ __forceinline__ int value_power(const float (&vl)[PAGES], int E) {
+  float most = vl[0];
 #pragma unroll
-  for (int p = 0; p < PAGES; ++p) most = id[p] >= 0 && vl[p] > most ? vl[p] : most;
+  for (int p = 1; p < PAGES; ++p) most = fmaxf(most, vl[p]);
   const int e = __builtin_amdgcn_readfirstlane((int)floorf(most));
-  return most < -199.f || (e <= E && e >= E - V_ROOM) ? E : e;
+  return e <= (int)NO_SCALE || (e <= E && e >= E - V_ROOM) ? E : e;
 }
 
 // Infinite and NaN values of V: a weight of zero would make them NaN where a row does not see them, so
 // the tiles have zeros in their place. A page that has any leaves beside its tile, for every 16-byte chunk, which
 // of its 8 values are positive (bits 0 .. 7) and which negative (8 .. 15; NaN: both), and whoever sees one
 // remembers it by channel until the end: a weight is positive, whatever its size. All of this is rare.
-template <int D> __device__ __forceinline__ void clean_tile(u4* tile, int lane) {
-  for (int f = lane; f < PS * D / 8; f += 64) {
-    u4 w = tile[f];
+// Returns whether there was any.
+__device__ __forceinline__ bool clean_chunk(u4* chunk) {
+  u4 w = *chunk;
+  const u4 was = w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t e = w[i] & 0x7C007C00u;
-      w[i] &= ((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u);
-    }
-    tile[f] = w;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = w[i] & 0x7C007C00u;
+    w[i] &= ((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u);
   }
+  *chunk = w;
+  return ((w[0] ^ was[0]) | (w[1] ^ was[1]) | (w[2] ^ was[2]) | (w[3] ^ was[3])) != 0u;
 }
 template <int D> __device__ __forceinline__ void put_aside(u4* tile, uint16_t* special, int lane) {
   for (int f = lane; f < PS * D / 8; f += 64) {

@@ -18,15 +18,15 @@ namespace {
 
 template <int D, bool QF32, int NW, int RT, int KIND>
 __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a) {
-  static_assert(NW == 4 || NW == 8, "a wave takes a page of K and of V, or one of the two");
+  static_assert(NW == 4 || NW == 8, "pieces of pages are shared out");
   constexpr bool WIDE = KIND == PAGES_ALL, SCALED = KIND != PAGES_F16;
-  constexpr int OWN = 8 / NW, BM = 16 * RT * NW, PAGE = PS * D / 8;   // 16-byte units of a tile
+  constexpr int QUARTERS = D / 32, OWN = 8 * QUARTERS / NW;      // pieces (64 chunks) a page, and of a wave a step
+  constexpr int BM = 16 * RT * NW, PAGE = PS * D / 8;   // 16-byte units of a tile
   __shared__ u4 tiles[2][2][4][PAGE];                            // [buffer][K, V][page]
   __shared__ u4 rest[WIDE ? 2 : 1][2][4][WIDE ? PAGE : 1];       // of wide pages: what their tiles leave
   __shared__ u4 none[WIDE ? PAGE : 1];                           // zeros
-  __shared__ u4 metas[128];                                      // of entry e at e % 128: page, tag, km, vl
-  __shared__ u2 factors[SCALED ? 128 : 1];                       // kf, vf
-  __shared__ int special;                                        // V has infinite or NaN values
+  __shared__ Ahead<KIND> table;
+  __shared__ int special;                                        // bit 0: V has infinite or NaN values, bit 1: a sum has
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const MxPart part = a.shares ? mx_shared_part<4, true>(a) : mx_fixed_part(a);
@@ -57,80 +57,77 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
 
-  // The entries' pages and multipliers lie in LDS, 64 ahead of the walk: wave 0 looks up a block of 64
-  // in four steps of the walk, a load each.
-  const int32_t* row = a.table + kvrow * a.W;
-  auto keep = [&](int k, const PageEntry& x) __attribute__((always_inline)) {
-    metas[k & 127] = u4{(uint32_t)x.id, (uint32_t)x.tag, f2u(x.km), f2u(x.vl)};
-    if constexpr (SCALED) factors[k & 127] = u2{f2u(x.kf), f2u(x.vf)};
+  // Wave 0 looks up a block of 64 entries in three steps of the walk, what waits for what a step apart.
+  auto look_up = [&](int k) {
+    const PageAttn& b = arguments();
+    const int page = entry_page(b, raw_entry(b.table + kvrow * b.W, e0 + k, e1));
+    put_ahead<D, KIND>(table, b, k, page_tag<KIND>(b, page, raw_tag(b, page)));
   };
-  if (w < 2) keep(64 * w + lane, page_entry<D, KIND>(a, row, e0 + 64 * w + lane, e1));
+  if (w < 2) look_up(64 * w + lane);
   if (threadIdx.x == 0) special = 0;
   __syncthreads();
   int ahead = 0, ahead_tag = 0;
-  float ahead_k = 1.f, ahead_v = 1.f;
   auto look_ahead = [&](int k) __attribute__((always_inline)) {  // k: entry of the walk, a multiple of 4
-    if ((k & 15) != 0 || w != 0) return;
+    if ((k & 15) != 0 || w != 0 || k < 64) return;               // two blocks are there at first
     const int stage = (k >> 4) & 3, e = (k & ~63) + 64 + lane;   // the block after the one at hand
-    if (k < 64) return;                                          // two blocks are there at first
-    if (stage == 0) ahead = raw_entry(row, e0 + e, e1);
+    const PageAttn& b = arguments();
+    if (stage == 0) ahead = raw_entry(b.table + kvrow * b.W, e0 + e, e1);
     else if (stage == 1) {
-      ahead = entry_page(a, ahead);
-      ahead_tag = raw_tag(a, ahead);
-    } else if (stage == 2) {
-      const PageTag x = page_tag<KIND>(a, ahead, ahead_tag);
-      ahead = x.id;
-      ahead_tag = x.tag;
-      page_scales<D, KIND>(a, x, ahead_k, ahead_v);
-    } else keep(e, page_multipliers<KIND>(PageTag{ahead, ahead_tag}, ahead_k, ahead_v));
+      ahead = entry_page(b, ahead);
+      ahead_tag = raw_tag(b, ahead);
+    } else if (stage == 2) put_ahead<D, KIND>(table, b, e, page_tag<KIND>(b, ahead, ahead_tag));
   };
-  auto uniform = [](uint32_t x) { return __builtin_amdgcn_readfirstlane((int)x); };
-  auto uniform_f = [](uint32_t x) { return u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)x)); };
+  auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
 
-  // this wave's page of a step, of K and V or of one of them: loaded a step ahead, put into LDS during
-  // the step before
-  const int own = w & 3, side = w >> 2;
-  PageRaw<D> raw[OWN];
-  auto load = [&](const u4& x) __attribute__((always_inline)) {
-#pragma unroll
-    for (int o = 0; o < OWN; ++o)
-      load_page<D, KIND, false>(raw[o], a, OWN == 2 ? o == 1 : side == 1, uniform(x[0]), uniform(x[1]), lane);
-  };
-  auto convert = [&](int buf, const u4& x, const u2& f) __attribute__((always_inline)) {
+  bool careful = false;                                          // V's infinite and NaN values become zeros
+
+  // This wave's pieces of a step's pages: loaded a step ahead, put into LDS during the step before. Piece o of
+  // wave w is number w + NW o of (page, side, quarter).
+  auto page_of = [&](int o) { return NW <= 2 * QUARTERS ? NW * o / (2 * QUARTERS) : 2 * o + w / (2 * QUARTERS); };
+  auto side_of = [&](int o) { return NW <= QUARTERS ? NW * o / QUARTERS & 1 : w / QUARTERS & 1; };
+  const int f = w % QUARTERS * 64 + lane, place = v_chunk<D>(f / (D / 8), f % (D / 8));
+  u4 raw[OWN];
+  auto tags_of = [&](int k) { return uniform(*reinterpret_cast<const uint32_t*>(&table.tag[k & (AHEAD - 1)])); };   // of four pages
+  auto load = [&](uint32_t tags, int k) __attribute__((always_inline)) {
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
-      const int s = OWN == 2 ? o : side;
-      const bool bad = store_page<D, KIND, true>(raw[o], uniform(x[0]), uniform(x[1]), uniform_f(s ? f[1] : f[0]), tiles[buf][s][own],
-                                                 rest[WIDE ? buf : 0][s][own], lane);
-      if (s == 1 && __builtin_amdgcn_ballot_w64(bad)) {          // rare
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        clean_tile<D>(tiles[buf][1][own], lane);
-        if (lane == 0) special = 1;
-      }
+      const int p = page_of(o);
+      const u2 at = reinterpret_cast<const u2*>(&table.where[(k + p) & (AHEAD - 1)])[side_of(o)];
+      raw[o] = load_piece<D, KIND>((uint64_t)at[0] | (uint64_t)at[1] << 32, (tags >> (8 * p)) & 0xFFu, f);
     }
   };
-  const u2 one = {f2u(1.f), f2u(1.f)};
+  auto convert = [&](int buf, uint32_t tags, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int p = page_of(o), s = side_of(o);
+      store_piece<D, KIND>(raw[o], (tags >> (8 * p)) & 0xFFu, table.factors[s][SCALED ? (k + p) & (AHEAD - 1) : 0], f, tiles[buf][s][p],
+                           rest[WIDE ? buf : 0][s][p], place);
+      if (careful && s == 1 && __builtin_amdgcn_ballot_w64(clean_chunk(&tiles[buf][1][p][place])) && lane == 0) special = 1;
+    }
+  };
 
   f4 acc[RT][D / 16], l[RT];
   float lsum[RT], m[RT];
   int E = 0;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    m[t] = M_NONE;
-    lsum[t] = 0.f;
-    l[t] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] = f4{0.f, 0.f, 0.f, 0.f};
-  }
-
   const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
   int k = 0;                                                     // number of entry e in the part
+  uint32_t now = 0, soon = 0;                                    // tags of this step's pages and of the next's
   auto step = [&](int buf, int e) __attribute__((always_inline)) {
-    u4 at[4];
+    const uint32_t later = tags_of(k + 8);
+    f4 kms = {1.f, 1.f, 1.f, 1.f}, vls = {0.f, 0.f, 0.f, 0.f}, ivs = vls;
+    if constexpr (SCALED) {
+      kms = *reinterpret_cast<const f4*>(&table.km[k & (AHEAD - 1)]);
+      vls = *reinterpret_cast<const f4*>(&table.vl[k & (AHEAD - 1)]);
+      ivs = *reinterpret_cast<const f4*>(&table.iv[k & (AHEAD - 1)]);
+    }
+    int id[4];                                                   // -1: no page
+    bool wide[4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) at[p] = metas[(k + p) & 127];
-    const u4 mine = metas[(k + 4 + own) & 127], after = metas[(k + 8 + own) & 127];
-    const u2 factor = SCALED ? factors[(k + 4 + own) & 127] : one;
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t tag = (now >> (8 * p)) & 0xFFu;
+      id[p] = tag == NO_PAGE ? -1 : 0;
+      wide[p] = WIDE && wide_tag((int)tag);
+    }
     f4 s[RT][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -147,16 +144,6 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
           if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[t][j], s[t][p], 0, 0, 0);
         }
       }
-    int id[4];
-    float km[4], vl[4];
-    bool wide[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      id[p] = uniform(at[p][0]);
-      km[p] = SCALED ? uniform_f(at[p][2]) : 1.f;
-      vl[p] = SCALED ? uniform_f(at[p][3]) : 0.f;
-      wide[p] = WIDE && id[p] >= 0 && wide_tag(uniform(at[p][1]));
-    }
     if constexpr (WIDE) {
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
@@ -169,14 +156,16 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
         }
       }
     }
-    convert(buf ^ 1, mine, factor);
-    load(after);
+    convert(buf ^ 1, soon, k + 4);
+    load(later, k + 8);
     look_ahead(k);
     const uint32_t no_nan[4] = {0u, 0u, 0u, 0u};
     hide<4, RT>(s, no_nan, id, e, seen, least, g);
     if constexpr (SCALED) {
+      const float km[4] = {kms[0], kms[1], kms[2], kms[3]};
+      float vl[4] = {vls[0], vls[1], vls[2], vls[3]}, out[4];
       raise_scaled<D, 4, RT>(s, km, mult, m, lsum, acc);
-      const int to = value_power<4>(id, vl, E);
+      const int to = value_power<4>(vl, E);
       if (to != E) {                                             // uniform
 #pragma unroll
         for (int t = 0; t < RT; ++t)
@@ -186,11 +175,10 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
             for (int q = 0; q < 4; ++q) acc[t][mb][q] = __builtin_ldexpf(acc[t][mb][q], E - to);
         E = to;
       }
-      float out[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        vl[p] = id[p] < 0 ? 0.f : vl[p] - (float)E;
-        out[p] = __builtin_amdgcn_exp2f(-vl[p]);
+        vl[p] -= (float)E;
+        out[p] = __builtin_ldexpf(ivs[p], E);
       }
 #pragma unroll
       for (int t = 0; t < RT; ++t) lsum[t] += soften_scaled<4>(s[t], km, vl, out, mult[t], m[t]);
@@ -242,21 +230,55 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
       }
     }
     k += 4;
+    now = soon;
+    soon = later;
     __syncthreads();                                             // this buffer is free, the other one is whole
   };
-  if (e0 < e1) {
-    load(metas[own]);
-    convert(0, metas[own], SCALED ? factors[own] : one);
-    load(metas[4 + own]);
-    __syncthreads();
-    for (int e = e0; e < e1; e += 8) {
-      step(0, e);
-      if (e + 4 < e1) step(1, e + 4);
+  // A token that a row does not see weighs nothing, and 0 times infinity is NaN: a walk that ends in such
+  // sums is made again with zeros in their place.
+  for (int walk = 0; walk < 2; ++walk) {
+    E = 0;
+    k = 0;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      m[t] = M_NONE;
+      lsum[t] = 0.f;
+      l[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] = f4{0.f, 0.f, 0.f, 0.f};
     }
+    if (e0 < e1) {
+      now = tags_of(0);
+      soon = tags_of(4);
+      load(now, 0);
+      convert(0, now, 0);
+      load(soon, 4);
+      __syncthreads();
+      for (int e = e0; e < e1; e += 8) {
+        step(0, e);
+        if (e + 4 < e1) step(1, e + 4);
+      }
+    }
+    if (careful) break;
+    float sum = 0.f;                                             // NaN once anything is not finite
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum = __builtin_fmaf(acc[t][mb][q], 0.f, sum);
+    if (__builtin_amdgcn_ballot_w64(!(sum == 0.f)) && lane == 0) special = 2;
+    __syncthreads();
+    if (special == 0) break;                                     // uniform
+    __syncthreads();
+    careful = true;
+    if (threadIdx.x == 0) special = 0;
+    if (w < 2) look_up(64 * w + lane);
+    __syncthreads();
   }
 
   // what V has of infinite and NaN values, in a second walk
-  if (special) {                                                 // uniform: written before the last barrier
+  if (special) {                                                 // uniform: written before the last barrier, by a careful walk
     uint16_t* aside = reinterpret_cast<uint16_t*>(&tiles[1][0][0][0]);
     uint32_t* any = reinterpret_cast<uint32_t*>(&tiles[1][1][0][0]);
     Seen16 odd[RT];
@@ -265,11 +287,12 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
     for (int e = e0; e < e1; e += 4) {
       __syncthreads();
       if (w < 4) {
-        const PageEntry x = page_entry<D, KIND>(a, row, e + w, e1);
-        const int id = uniform((uint32_t)x.id), tag = uniform((uint32_t)x.tag);
+        const PageAttn& b = arguments();
+        const PageEntry x = page_entry<D, KIND>(b, b.table + kvrow * b.W, e + w, e1);
+        const int id = (int)uniform((uint32_t)x.id), tag = (int)uniform((uint32_t)x.tag);
         PageRaw<D> r;
-        load_page<D, KIND, false>(r, a, true, id, tag, lane);
-        const bool bad = store_page<D, KIND, true>(r, id, tag, uniform_f(f2u(x.vf)), tiles[0][0][w], rest[0][0][w], lane);
+        load_page<D, KIND, false>(r, b, true, id, tag, lane);
+        const bool bad = store_page<D, KIND, true>(r, id, tag, u2f(uniform(f2u(x.vf))), tiles[0][0][w], rest[0][0][w], lane);
         const bool some = __builtin_amdgcn_ballot_w64(bad) != 0;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (some) put_aside<D>(tiles[0][0][w], aside + w * PAGE, lane);
@@ -289,16 +312,18 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
     for (int t = 0; t < RT; ++t) bring_back<D>(acc[t], odd[t]);
   }
 
+  const PageAttn& z = arguments();
+  const int all = z.L * z.G;
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const int r = tile * BM + (w * RT + t) * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
+    const int r = tile * BM + (w * RT + t) * 16 + c, i = r / z.G, head = hk * z.G + (r - i * z.G);
     float sum;
     if constexpr (SCALED) sum = xsum16_32(lsum[t]);
     else sum = l[t][0];
-    if (r >= rows) continue;
-    if (a.parted) {
+    if (r >= all) continue;
+    if (z.parted) {
       const int64_t slot = (int64_t)part.part * BM + (w * RT + t) * 16 + c;
-      if (g == 0) { a.ws_m[slot] = m[t]; a.ws_l[slot] = sum; }
+      if (g == 0) { z.ws_m[slot] = m[t]; z.ws_l[slot] = sum; }
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) {
         f4 x = acc[t][mb];
@@ -306,11 +331,11 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
 #pragma unroll
           for (int q = 0; q < 4; ++q) x[q] = __builtin_ldexpf(x[q], E);
         }
-        *reinterpret_cast<f4*>(a.ws_acc + slot * D + 16 * mb + 4 * g) = x;
+        *reinterpret_cast<f4*>(z.ws_acc + slot * D + 16 * mb + 4 * g) = x;
       }
     } else {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;           // NaN stays
-      const int64_t at = b * a.osb + i * a.ost + head * a.osh + 4 * g;
+      const int64_t at = b * z.osb + i * z.ost + head * z.osh + 4 * g;
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) {
         float o[4];
@@ -319,7 +344,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
           const float x = acc[t][mb][q] * inv;
           o[q] = i < n.queries ? (SCALED ? __builtin_ldexpf(x, E) : x) : 0.f;
         }
-        store_out4(a, at + 16 * mb, o);
+        store_out4(z, at + 16 * mb, o);
       }
     }
   }

@@ -164,8 +164,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
     raise_scaled<D, 2, 1>(s, km, mult, m, l, acc);
     float vl[2] = {0.f, 0.f}, out[2] = {1.f, 1.f};
     if constexpr (KIND != PAGES_F16) {
-      const float all[2] = {x[0].vl, x[1].vl};
-      const int to = value_power<2>(id, all, E);
+      const float all[2] = {id[0] < 0 ? NO_SCALE : x[0].vl, id[1] < 0 ? NO_SCALE : x[1].vl};
+      const int to = value_power<2>(all, E);
       if (to != E) {                                             // uniform
 #pragma unroll
         for (int mb = 0; mb < D / 16; ++mb)
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        vl[p] = id[p] < 0 ? 0.f : all[p] - (float)E;
+        vl[p] = id[p] < 0 ? 0.f : x[p].vl - (float)E;
         out[p] = __builtin_amdgcn_exp2f(-vl[p]);
       }
     }

@@ -114,7 +114,7 @@ void choose_chunk(const iak_paged_chunk_args* a, int64_t rows, int W, ChunkPlan*
   const double kvrows = (double)a->batch * a->num_kv_heads;
   p->tile_rows = rows <= 64 ? 16 : (rows > 128 && !f32 ? 256 : 128);
   p->tiles = (int)((rows + p->tile_rows - 1) / p->tile_rows);
-  const double tiles = kvrows * p->tiles, round = CUS * (p->tile_rows == 16 ? 3 : 2);
+  const double tiles = kvrows * p->tiles, round = CUS * (p->tile_rows == 16 ? 3 : p->tile_rows == 256 ? 1 : 2);
   int64_t splits = a->splits > 0 ? a->splits : (int64_t)(round / tiles);
   if (splits > (W + 7) / 8 && a->splits == 0) splits = (W + 7) / 8;
   if (splits > (W + 1) / 2) splits = (W + 1) / 2;
