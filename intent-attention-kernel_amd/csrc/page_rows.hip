@@ -3,19 +3,22 @@
 // that a query sees.
 //
 // A workgroup takes a tile of 16 query rows that share a KV head (row = query token * G + head of
-// the group) and one part of the head's table entries; its waves share the entries out in pairs of
-// pages (32 tokens), one pair a step, and their sums meet in LDS at the end. A wave loads its pages
-// as whole lines and turns them into operands through LDS of its own, K and V one after the other
-// (page_attention.h), so that no wave waits for another. Lane = c + 16 g:
+// the group) and one part of the head's table entries; each of its waves takes a quarter of these, and their
+// sums meet in LDS at the end. A wave sorts its entries, 64 at a time, by precision and goes through each
+// precision's pages one by one, the next ones under way in a ring of registers (paged_pages.h, as the
+// decode does). Lane = c + 16 g; per page:
 //   scores  S^T[16 tok x 16 rows] = K . Q^T, v_mfma_f32_16x16x32_f16, channels (D/4) g .. on both sides
-//   values  O^T[D x 16 rows] += V^T[D x 32 tok] . P^T; the score result has the weights of tokens
-//           4g .. 4g+3 of both pages in the lane that the operand needs them in
+//   values  O^T[D x 16 rows] += V^T[D x 16 tok] . P^T, v_mfma_f32_16x16x16_f16; the score result has the weights
+//           of the tokens in the lane that the operand needs them in
+// K and V are exact codes, with their scales in the scores and the weights; INT4 codes times their
+// groups' scales, which need more bits than float16 has, take two products.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "iak.h"
 #include "page_attention.h"
+#include "paged_pages.h"
 #include "mx_merge.h"
 
 namespace iak {
@@ -24,18 +27,263 @@ namespace {
 
 constexpr int ROW_WAVES = 4;
 
-// Entry i of the wave's own, of those that the workgroup's waves share out in pairs.
-__device__ __forceinline__ int wave_entry(int w, int i) { return 2 * (w + ROW_WAVES * (i >> 1)) + (i & 1); }
+// A wave's rows: their queries and sums so far.
+template <int D, bool QF32> struct RowWave {
+  h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
+  f4 acc[D / 16];          // lane: row c, channels (D/16)(4g + q) + mb
+  float mult, m, l;        // of row c: what makes base-2 scores; running maximum; this lane's part of the sum
+  int E;                   // the values' sum is acc 2^E (uniform)
+  int seen, least;         // tokens that row c sees, and that all rows do
+  int g;
+};
+
+template <int D, bool QF32> __device__ __forceinline__ f4 row_scores(const RowWave<D, QF32>& w, const h8 (&ka)[D / 32], f4 s) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i], w.qhi[i], s, 0, 0, 0);
+    if constexpr (QF32) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i], w.qlo[i], s, 0, 0, 0);
+  }
+  return s;
+}
+
+// Weights of a page of base-2 scores `s`; `first`: its first token's number; PERM: score r of lane group g is
+// token 4r + g (else 4g + r); e: the exponent of V's scale.
+template <bool PERM, int D, bool QF32>
+__device__ __forceinline__ f4 row_weights(RowWave<D, QF32>& w, f4 s, int first, int e) {
+  if (first + PS > w.least) {                                    // uniform
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (first + (PERM ? 4 * r + w.g : 4 * w.g + r) >= w.seen) s[r] = -__builtin_inff();
+  }
+  const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+  const bool move = e > w.E || e < w.E - V_ROOM;                 // uniform
+  if (__builtin_amdgcn_ballot_w64(top > w.m + RESCALE_SLACK) || move) {
+    const float pm = xmax16_32(top), mn = pm > w.m + RESCALE_SLACK ? pm : w.m, alpha = __builtin_amdgcn_exp2f(w.m - mn);
+    const int by = move ? w.E - e : 0;
+    w.l *= alpha;
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w.acc[mb][q] = __builtin_ldexpf(w.acc[mb][q] * alpha, by);
+    w.m = mn;
+    w.E = move ? e : w.E;
+  }
+  const float base = P_SHIFT - w.m;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] + base);
+  w.l += (s[0] + s[1]) + (s[2] + s[3]);
+  return s;
+}
+
+// A V scale: its exponent, and what multiplies the weights of a page once E has followed it. One that is not finite
+// makes every sum NaN (0 in a careful walk).
+__device__ __forceinline__ int value_exponent(float v) { return fabsf(v) < __builtin_inff() ? scale_exp(fabsf(v)) : 0; }
+__device__ __forceinline__ float value_factor(float v, int E, bool careful) {
+  return careful && !(fabsf(v) < __builtin_inff()) ? 0.f : __builtin_ldexpf(v, -E);
+}
+
+__device__ __forceinline__ h4 half4(f4 p) {
+  return h4{(_Float16)p[0], (_Float16)p[1], (_Float16)p[2], (_Float16)p[3]};
+}
+
+// acc += V^T . (weights times their factor), with what rounding left for float32 queries.
+template <int D, bool QF32>
+__device__ __forceinline__ void row_values(RowWave<D, QF32>& w, const h4 (&va)[D / 16], f4 p, float factor) {
+  p *= factor;
+  const h4 pb = half4(p);
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] = __builtin_amdgcn_mfma_f32_16x16x16f16(va[mb], pb, w.acc[mb], 0, 0, 0);
+  if constexpr (QF32) {
+    const h4 pl = half4(f4{p[0] - (float)pb[0], p[1] - (float)pb[1], p[2] - (float)pb[2], p[3] - (float)pb[3]});
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] = __builtin_amdgcn_mfma_f32_16x16x16f16(va[mb], pl, w.acc[mb], 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ uint32_t clean_pair(uint32_t x) {
+  const uint32_t e = x & 0x7C007C00u;
+  return x & (((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u));
+}
+
+template <int D, bool QF32>
+__device__ __forceinline__ void row_page_fp16(RowWave<D, QF32>& w, const Raw16<D>& r, int first, bool careful, u4* kt, int c, int g) {
+  u4 k[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) k[i] = r.k[i];
+  k_through_lds<D / 8, D / 32>(k, kt, c, g);
+  h8 ka[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) ka[i] = __builtin_bit_cast(h8, k[i]);
+  const f4 p = row_weights<true>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * w.mult, first, 0);
+  uint32_t v[4][D / 32];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) v[t][j] = careful ? clean_pair(r.v[t][j]) : r.v[t][j];
+  h4 va[D / 16];
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb) va[mb] = rows_to_a<D>(v, mb);
+  row_values(w, va, p, value_factor(1.f, w.E, false));
+}
+
+template <int TAG, int D, bool QF32>
+__device__ __forceinline__ void row_page_byte(RowWave<D, QF32>& w, const Raw8<D>& r, int first, float ks, float vs, bool careful, u4* kt,
+                                              int c, int g) {
+  uint32_t kw[D / 16];
+  k8_words<D>(r, kw, kt, c, g);
+  auto four = [](uint32_t x, uint32_t& lo, uint32_t& hi) __attribute__((always_inline)) {
+    if constexpr (TAG == IAK_TAG_FP8) fp8x4_to_f16(x, lo, hi);
+    else i8x4_to_f16(x, lo, hi);
+  };
+  h8 ka[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t o[4];
+    four(kw[2 * i], o[0], o[1]);
+    four(kw[2 * i + 1], o[2], o[3]);
+    ka[i] = make_h8(o[0], o[1], o[2], o[3]);
+  }
+  const f4 p = row_weights<true>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * (w.mult * ks), first, value_exponent(vs));
+  uint32_t v[4][D / 32];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      four(r.v[t][j], v[t][2 * j], v[t][2 * j + 1]);
+      if (TAG == IAK_TAG_FP8 && careful) {                       // NaN codes
+        v[t][2 * j] = clean_pair(v[t][2 * j]);
+        v[t][2 * j + 1] = clean_pair(v[t][2 * j + 1]);
+      }
+    }
+  h4 va[D / 16];
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb) va[mb] = rows_to_a<D>(v, mb);
+  row_values(w, va, p, value_factor(vs, w.E, careful));
+}
+
+// base * s0 + rest * s1, both codes exact (the rest's 16 times), products apart.
+template <int D, bool QF32>
+__device__ __forceinline__ void row_page_int4r(RowWave<D, QF32>& w, const Raw8<D>& r, int first, float ks0, float ks1, float vs0, float vs1,
+                                               bool careful, u4* kt, int c, int g) {
+  uint32_t kw[D / 16];
+  k8_words<D>(r, kw, kt, c, g);
+  const uint32_t mg = magic_i4();
+  h8 kb[D / 32], kr[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t b[4], x16[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t x = kw[2 * i + h];
+      const uint32_t y01 = __builtin_amdgcn_perm(x, x, 0x01010000u), y23 = __builtin_amdgcn_perm(x, x, 0x03030202u);
+      b[2 * h] = bits(i4r_base_pair(y01, mg));
+      b[2 * h + 1] = bits(i4r_base_pair(y23, mg));
+      x16[2 * h] = bits(i4r_resid16_pair(y01, mg));
+      x16[2 * h + 1] = bits(i4r_resid16_pair(y23, mg));
+    }
+    kb[i] = make_h8(b[0], b[1], b[2], b[3]);
+    kr[i] = make_h8(x16[0], x16[1], x16[2], x16[3]);
+  }
+  const f4 none = {0.f, 0.f, 0.f, 0.f};
+  const f4 sb = row_scores(w, kb, none), sr = row_scores(w, kr, none);
+  const float k16 = ks1 * 0.0625f, v16 = vs1 * 0.0625f, most = fmaxf(fabsf(vs0), fabsf(vs1));
+  f4 s;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) s[q] = __builtin_fmaf(sb[q], ks0, sr[q] * k16) * w.mult;
+  const bool fine = fabsf(vs0) + fabsf(vs1) < __builtin_inff();
+  const f4 p = row_weights<true>(w, s, first, fine ? scale_exp(most) : 0);
+  const float f0 = careful && !fine ? 0.f : __builtin_ldexpf(vs0, -w.E), f1 = careful && !fine ? 0.f : __builtin_ldexpf(v16, -w.E);
+  h4 va[D / 16], vr[D / 16];
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb) {
+    const int j = mb >> 2, k = mb & 3;
+    const uint32_t sel = (uint32_t)k * 0x00000101u + (uint32_t)(4 + k) * 0x01010000u;   // (t_even byte k, t_odd byte k)
+    const uint32_t y01 = __builtin_amdgcn_perm(r.v[1][j], r.v[0][j], sel), y23 = __builtin_amdgcn_perm(r.v[3][j], r.v[2][j], sel);
+    va[mb] = make_h4(bits(i4r_base_pair(y01, mg)), bits(i4r_base_pair(y23, mg)));
+    vr[mb] = make_h4(bits(i4r_resid16_pair(y01, mg)), bits(i4r_resid16_pair(y23, mg)));
+  }
+  row_values(w, va, p, f0);
+  row_values(w, vr, p, f1);
+}
+
+template <int D> struct RawScaled4 {   // INT4, with the scales of the lane's channels
+  Raw4<D> x;
+  float ks, vs;
+};
+
+template <int D, bool QF32>
+__device__ __forceinline__ void row_page_int4(RowWave<D, QF32>& w, const RawScaled4<D>& rs, int first, bool careful, const h8 (&qhi)[D / 32],
+                                              const h8 (&qlo)[QF32 ? D / 32 : 1], int c) {
+  const Raw4<D>& r = rs.x;
+  const uint32_t mg = magic_i4();
+  // powers of two that bring the page's scales near 1; K's lanes differ by g, V's by c / 4
+  auto largest = [](float x) { x = fabsf(x); return x < __builtin_inff() ? x : 0.f; };
+  const int ek = scale_exp(xmax16_32(largest(rs.ks)));
+  float most = largest(rs.vs);
+  most = fmaxf(most, __shfl_xor(most, 4, 64));
+  most = fmaxf(most, __shfl_xor(most, 8, 64));
+  const int ev = __builtin_amdgcn_readfirstlane(scale_exp(most));
+  const ScaleParts ks = scale_parts(__builtin_ldexpf(rs.ks, -ek));
+  const bool fine = fabsf(rs.vs) < __builtin_inff();
+  const ScaleParts vs = scale_parts(careful && !fine ? 0.f : __builtin_ldexpf(rs.vs, -ev));
+  auto parts = [](h2 n, const ScaleParts& k, uint32_t& hi, uint32_t& lo) __attribute__((always_inline)) {
+    const h2 x = n * k.hi;
+    hi = bits(x);
+    lo = bits(__builtin_elementwise_fma(n, k.lo, __builtin_elementwise_fma(n, k.hi, -x))) & k.fine;
+  };
+  f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) parts(nib_pair(r.k[i] >> (4 * q), mg), ks, h[q], l[q]);
+    const h8 kh = make_h8(h[0], h[1], h[2], h[3]);
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qhi[i], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(make_h8(l[0], l[1], l[2], l[3]), qhi[i], s, 0, 0, 0);
+    if constexpr (QF32) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qlo[i], s, 0, 0, 0);
+  }
+  const f4 p = row_weights<false>(w, s * __builtin_ldexpf(w.mult, ek), first, ev);
+  h4 va[D / 16], vl[D / 16];
+  const uint32_t y01l = pack_lo(r.v[0], r.v[1]), y01h = pack_hi(r.v[0], r.v[1]);
+  const uint32_t y23l = pack_lo(r.v[2], r.v[3]), y23h = pack_hi(r.v[2], r.v[3]);
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    const uint32_t y01 = d < 4 ? y01l : y01h, y23 = d < 4 ? y23l : y23h;
+    uint32_t h[2], l[2];
+    parts(nib_pair(y01 >> (4 * (d & 3)), mg), vs, h[0], l[0]);
+    parts(nib_pair(y23 >> (4 * (d & 3)), mg), vs, h[1], l[1]);
+    va[d] = make_h4(h[0], h[1]);
+    vl[d] = make_h4(l[0], l[1]);
+  }
+  const float factor = __builtin_ldexpf(1.f, ev - w.E);
+  row_values(w, va, p, factor);
+  const h4 pb = half4(p * factor);
+#pragma unroll
+  for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] = __builtin_amdgcn_mfma_f32_16x16x16f16(vl[mb], pb, w.acc[mb], 0, 0, 0);
+}
+
+// What a lane's rows see of infinite and NaN values (page_attention.h), by its channels here: bit (D/16) q + mb.
+template <int D> __device__ __forceinline__ void row_remember(Seen16& x, const uint16_t* special, int tokens, int g) {
+  for (int token = 0; token < tokens; ++token)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int first = (D / 16) * (4 * g + q);
+      const uint32_t s = (uint32_t)special[v_chunk<D>(token, first / 8)] >> (first % 8), mask = (1u << (D / 16)) - 1u;
+      x.plus |= (s & mask) << (D / 16 * q);
+      x.minus |= ((s >> 8) & mask) << (D / 16 * q);
+    }
+}
+
+// Waves a SIMD: what the registers hold of rings and queries in two parts.
+template <bool QF32> constexpr int row_waves_per_simd() { return QF32 ? 2 : 3; }
 
 template <int D, bool QF32, int KIND>
-__global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const PageAttn a) {
-  constexpr bool WIDE = KIND == PAGES_ALL;
-  constexpr int PAGE = PS * D / 8;                               // 16-byte units of a tile
-  __shared__ u4 tiles[ROW_WAVES][2 * PAGE * (WIDE ? 2 : 1)];     // K's, then V's; at the end the waves' sums
-  __shared__ u4 none[WIDE ? PAGE : 1];                           // zeros
-  __shared__ uint16_t special[ROW_WAVES][PAGE];
+__global__ __launch_bounds__(64 * ROW_WAVES, row_waves_per_simd<QF32>()) void page_rows_kernel(const PageAttn a) {
+  constexpr int UNIT = 16 * D / 4;                               // 16-byte units of a wave's sums, and at least a page's K
+  __shared__ u4 lds[ROW_WAVES][UNIT];
+  __shared__ uint16_t special[ROW_WAVES][PS * D / 8];
   __shared__ float part_m[ROW_WAVES][16], part_l[ROW_WAVES][16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const MxPart part = a.shares ? mx_shared_part<2 * ROW_WAVES, false>(a) : mx_fixed_part(a);
   if (part.idle) return;                                         // uniform, as below
@@ -46,181 +294,147 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
   const int entries = mx_entries(a, n, tile * 16, 16);
   const int e0 = part.e0, e1 = e0 + part.chunk < entries ? e0 + part.chunk : entries;
   if (e0 > 0 && e0 >= e1) return;                                // the merge does not look at it
-  if constexpr (WIDE) {
-    for (int i = threadIdx.x; i < PAGE; i += 64 * ROW_WAVES) none[i] = u4{0u, 0u, 0u, 0u};
-    __syncthreads();
-  }
 
-  const int r = tile * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
-  const bool active = r < a.L * a.G, live = active && i < n.queries;
-  const int seen[1] = {live ? mx_seen(a, n, i) : 0};
-  int least = live ? seen[0] : 0x7FFFFFFF;                       // tokens below it need no mask
+  RowWave<D, QF32> w;
+  {
+    const int r = tile * 16 + c, i = r / a.G, head = hk * a.G + (r - i * a.G);
+    const bool active = r < a.L * a.G, live = active && i < n.queries;
+    w.seen = live ? mx_seen(a, n, i) : 0;
+    w.least = live ? w.seen : 0x7FFFFFFF;
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(least, o, 64); least = x < least ? x : least; }
+    for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(w.least, o, 64); w.least = x < w.least ? x : w.least; }
+    w.mult = load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, w.qhi, w.qlo);
+  }
+  w.g = g;
 
-  // the wave's entries, 64 at a time: lane i holds number i of the block, in `next` of the block after it
+  // the wave's entries: a quarter of the part's
+  const int each = (e1 - e0 + ROW_WAVES - 1) / ROW_WAVES, w0 = e0 + wv * each, w1 = w0 + each < e1 ? w0 + each : e1;
   const int32_t* row = a.table + kvrow * a.W;
-  auto entry = [&](int k) { return page_entry<D, KIND>(a, row, e0 + wave_entry(w, k), e1); };
-  PageEntry now = entry(lane), next = entry(64 + lane);
-  auto pick = [&](int here, int after, int k) {
-    const int x = __builtin_amdgcn_readlane(here, k & 63), y = __builtin_amdgcn_readlane(after, k & 63);
-    return k < 64 ? x : y;
-  };
-  auto pick_f = [&](float here, float after, int k) { return u2f((uint32_t)pick((int)f2u(here), (int)f2u(after), k)); };
-  auto of = [&](int k) __attribute__((always_inline)) {          // entry k of the block, k < 128
-    PageEntry y = {pick(now.id, next.id, k), IAK_TAG_FP16, 1.f, 1.f, 0.f, 1.f};
-    if constexpr (KIND != PAGES_F16) {
-      y.tag = pick(now.tag, next.tag, k);
-      y.km = pick_f(now.km, next.km, k);
-      y.kf = pick_f(now.kf, next.kf, k);
-      y.vl = pick_f(now.vl, next.vl, k);
-      y.vf = pick_f(now.vf, next.vf, k);
-    }
-    return y;
-  };
-
-  h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
-  const float mult[1] = {load_query<D, QF32>(a, active, b * a.qsb + i * a.qst + head * a.qsh, g, qhi, qlo)};
-
-  f4 acc[1][D / 16];
-#pragma unroll
-  for (int mb = 0; mb < D / 16; ++mb) acc[0][mb] = f4{0.f, 0.f, 0.f, 0.f};
-  float m[1] = {M_NONE}, l[1] = {0.f};
-  int E = 0;
-  u4* mine = tiles[w];
+  u4* kt = lds[wv];
+  bool careful = false;
   Seen16 odd = {0u, 0u};
-
-  PageRaw<D> k[2], v[2];
-  PageEntry at[2];                                               // of the pair that k and v hold
-  auto look_up = [&](int i) __attribute__((always_inline)) {
-    at[0] = of(i);
-    at[1] = of(i + 1);
-  };
-  auto load = [&](PageRaw<D> (&x)[2], bool side) __attribute__((always_inline)) {
+  // A token that a row does not see weighs nothing, and 0 times infinity is NaN: a walk that ends in such sums is made
+  // again with zeros in their place.
+  for (int walk = 0; walk < 2; ++walk) {
+    w.m = M_NONE;
+    w.l = 0.f;
+    w.E = 0;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) load_page<D, KIND, true>(x[p], a, side, at[p].id, at[p].tag, lane);
-  };
-
-  int number = 0, block = 0;                                     // the next pair, of the block of 64 entries
-  if (e0 + 2 * w < e1) {
-    look_up(0);
-    load(k, false);
-    load(v, true);
-  }
-  for (int e = e0 + 2 * w; e < e1; e += 2 * ROW_WAVES) {
-    const PageEntry x[2] = {at[0], at[1]};
-    const int id[2] = {x[0].id, x[1].id};
-    const bool wide[2] = {WIDE && id[0] >= 0 && wide_tag(x[0].tag), WIDE && id[1] >= 0 && wide_tag(x[1].tag)};
-    const float km[2] = {x[0].km, x[1].km};
-
-    // K into LDS and back as operands
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-      store_page<D, KIND, false>(k[p], id[p], x[p].tag, x[p].kf, mine + p * PAGE, mine + (2 + p) * PAGE, lane);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    number += 2;
-    look_up(number);                                             // the next pair: under way from here
-    load(k, false);
-    f4 s[1][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const h8 ka = __builtin_bit_cast(h8, mine[p * PAGE + v_chunk<D>(c, g * (D / 32) + j)]);
-        s[0][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[j], s[0][p], 0, 0, 0);
-        if constexpr (QF32) s[0][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[j], s[0][p], 0, 0, 0);
+    for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int block = w0; block < w1; block += 64) {
+      // lane i has entry i of the block; those of one precision are gone through together
+      const int page = entry_page(a, raw_entry(row, block + lane, w1));
+      const PageTag x = page_tag<KIND>(a, page, raw_tag(a, page));
+      auto mask = [&](int tag) { return __builtin_amdgcn_ballot_w64(x.id >= 0 && x.tag == tag); };
+      auto first = [&](int idx) { return (block + idx) * PS; };
+      float s[4] = {0.f, 0.f, 0.f, 0.f};                         // K's and V's scales; residual: base, rest of both
+      if constexpr (KIND != PAGES_F16) {
+        if (x.id >= 0 && (x.tag == IAK_TAG_INT8 || x.tag == IAK_TAG_FP8)) page_scales<D, KIND>(a, x, s[0], s[1]);
+        if (KIND == PAGES_ALL && x.id >= 0 && x.tag == IAK_TAG_INT4_RESIDUAL) {
+          s[0] = a.k_int4r_scale[2 * (int64_t)x.id];
+          s[1] = a.k_int4r_scale[2 * (int64_t)x.id + 1];
+          s[2] = a.v_int4r_scale[2 * (int64_t)x.id];
+          s[3] = a.v_int4r_scale[2 * (int64_t)x.id + 1];
+        }
       }
-    if constexpr (WIDE) {
+      auto scale = [&](int i, int idx) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(s[i]), idx)); };
+      class_loop<IAK_RING_FP16, Raw16<D>>(
+          mask(IAK_TAG_FP16), x.id,
+          [&](Raw16<D>& r, int p) {
+            load16<D>(r, page_at<_Float16>(a.k_fp16, p, PS * D * 2), page_at<_Float16>(a.v_fp16, p, PS * D * 2), c, g);
+          },
+          [&](const Raw16<D>& r, int idx) { row_page_fp16(w, r, first(idx), careful, kt, c, g); });
+      if constexpr (KIND != PAGES_F16) {
+        class_loop<IAK_RING_BYTE, Raw8<D>>(
+            mask(IAK_TAG_FP8), x.id,
+            [&](Raw8<D>& r, int p) { load8<D>(r, page_at<uint8_t>(a.k_fp8, p, PS * D), page_at<uint8_t>(a.v_fp8, p, PS * D), c, g); },
+            [&](const Raw8<D>& r, int idx) {
+              row_page_byte<IAK_TAG_FP8>(w, r, first(idx), scale(0, idx), scale(1, idx), careful, kt, c, g);
+            });
+        class_loop<IAK_RING_BYTE, Raw8<D>>(
+            mask(IAK_TAG_INT8), x.id,
+            [&](Raw8<D>& r, int p) { load8<D>(r, page_at<uint8_t>(a.k_int8, p, PS * D), page_at<uint8_t>(a.v_int8, p, PS * D), c, g); },
+            [&](const Raw8<D>& r, int idx) {
+              row_page_byte<IAK_TAG_INT8>(w, r, first(idx), scale(0, idx), scale(1, idx), careful, kt, c, g);
+            });
+      }
+      if constexpr (KIND == PAGES_ALL) {
+        class_loop<IAK_RING_BYTE, Raw8<D>>(
+            mask(IAK_TAG_INT4_RESIDUAL), x.id,
+            [&](Raw8<D>& r, int p) { load8<D>(r, page_at<uint8_t>(a.k_int4r, p, PS * D), page_at<uint8_t>(a.v_int4r, p, PS * D), c, g); },
+            [&](const Raw8<D>& r, int idx) {
+              row_page_int4r(w, r, first(idx), scale(0, idx), scale(1, idx), scale(2, idx), scale(3, idx), careful, kt, c, g);
+            });
+        const uint64_t packed = mask(IAK_TAG_INT4);
+        if (packed) {
+          h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];                // in the order of the codes' pairs
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        if (!wide[p]) continue;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const h8 ka = __builtin_bit_cast(h8, mine[(2 + p) * PAGE + v_chunk<D>(c, g * (D / 32) + j)]);
-          s[0][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[j], s[0][p], 0, 0, 0);
+          for (int i = 0; i < D / 32; ++i) {
+            qhi[i] = q_int4_order(w.qhi[i]);
+            if constexpr (QF32) qlo[i] = q_int4_order(w.qlo[i]);
+          }
+          const int groups = D / a.int4_group;
+          class_loop<IAK_RING_INT4, RawScaled4<D>>(
+              packed, x.id,
+              [&](RawScaled4<D>& r, int p) {
+                load4<D>(r.x, page_at<uint8_t>(a.k_int4, p, PS * D / 2), page_at<uint8_t>(a.v_int4, p, PS * D / 2), c, g);
+                const int64_t at = (int64_t)(p < 0 ? 0 : p) * groups;
+                r.ks = load_scale(a.k_int4_scale, at + g * groups / 4, a.int4_sd);
+                r.vs = load_scale(a.v_int4_scale, at + (c >> 2) * groups / 4, a.int4_sd);
+              },
+              [&](const RawScaled4<D>& r, int idx) { row_page_int4(w, r, first(idx), careful, qhi, qlo, c); });
         }
       }
     }
-
-    // V in K's place
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (careful) break;
+    float sum = 0.f;                                             // NaN once anything is not finite
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const bool any = store_page<D, KIND, true>(v[p], id[p], x[p].tag, x[p].vf, mine + p * PAGE, mine + (2 + p) * PAGE, lane);
-      if (__builtin_amdgcn_ballot_w64(any)) {
-        put_aside<D>(mine + p * PAGE, special[w], lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int first = (e + p) * PS;
-        remember<D>(odd, special[w], seen[0] - first < PS ? seen[0] - first : PS, g);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    load(v, true);
-
-    const uint32_t no_nan[2] = {0u, 0u};
-    hide<2, 1>(s, no_nan, id, e, seen, least, g);
-    raise_scaled<D, 2, 1>(s, km, mult, m, l, acc);
-    float vl[2] = {0.f, 0.f}, out[2] = {1.f, 1.f};
-    if constexpr (KIND != PAGES_F16) {
-      const float all[2] = {id[0] < 0 ? NO_SCALE : x[0].vl, id[1] < 0 ? NO_SCALE : x[1].vl};
-      const int to = value_power<2>(all, E);
-      if (to != E) {                                             // uniform
+    for (int mb = 0; mb < D / 16; ++mb)
 #pragma unroll
-        for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[0][mb][q] = __builtin_ldexpf(acc[0][mb][q], E - to);
-        E = to;
-      }
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        vl[p] = id[p] < 0 ? 0.f : x[p].vl - (float)E;
-        out[p] = __builtin_amdgcn_exp2f(-vl[p]);
-      }
-    }
-    l[0] += soften_scaled<2>(s[0], km, vl, out, mult[0], m[0]);
-    const h8 pb = weights(s[0][0], s[0][1]);
-    h8 pl;
-    if constexpr (QF32) pl = weights_rest(s[0][0], s[0][1], pb);
-#pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb) {
-      const h8 va = values_back<D>(mine, mine + PAGE, mb, c, g);
-      acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[0][mb], 0, 0, 0);
-      if constexpr (QF32) acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[0][mb], 0, 0, 0);
-    }
-    if constexpr (WIDE) {
-      if (wide[0] || wide[1]) {
-        const u4* p0 = wide[0] ? mine + 2 * PAGE : none;
-        const u4* p1 = wide[1] ? mine + 3 * PAGE : none;
-#pragma unroll
-        for (int mb = 0; mb < D / 16; ++mb)
-          acc[0][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values_back<D>(p0, p1, mb, c, g), pb, acc[0][mb], 0, 0, 0);
-      }
-    }
-    if (number == 64) {
-      number = 0;
-      now = next;
-      // the entries of two blocks on, past what this one and the next hold
-      block += 64;
-      next = entry(block + 64 + lane);
-    }
+      for (int q = 0; q < 4; ++q) sum = __builtin_fmaf(w.acc[mb][q], 0.f, sum);
+    if (!__builtin_amdgcn_ballot_w64(!(sum == 0.f))) break;      // uniform in the wave
+    careful = true;
   }
-
-  if (__builtin_amdgcn_ballot_w64((odd.plus | odd.minus) != 0u)) bring_back<D>(acc[0], odd);
+  if (careful) {                                                 // what V has of them, in a walk of its own
+    for (int e = w0; e < w1; ++e) {
+      const PageEntry x = page_entry<D, KIND>(a, row, e, w1);
+      const int id = __builtin_amdgcn_readfirstlane(x.id), tag = __builtin_amdgcn_readfirstlane(x.tag);
+      PageRaw<D> r;
+      load_page<D, KIND, false>(r, a, true, id, tag, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const bool bad = store_page<D, KIND, true>(r, id, tag, u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(x.vf))), kt,
+                                                 kt + PS * D / 8, lane);
+      if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      put_aside<D>(kt, special[wv], lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int left = w.seen - e * PS;
+      row_remember<D>(odd, special[wv], left < PS ? left : PS, g);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if ((odd.plus >> (D / 16 * q + mb)) & 1u) w.acc[mb][q] += __builtin_inff();
+        if ((odd.minus >> (D / 16 * q + mb)) & 1u) w.acc[mb][q] -= __builtin_inff();
+      }
+  }
 
   // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
-  const float sum = xsum16_32(l[0]);
+  const float sum = xsum16_32(w.l);
   __syncthreads();
-  if (g == 0) { part_m[w][c] = m[0]; part_l[w][c] = sum; }
-  f4* sums = reinterpret_cast<f4*>(mine);
+  if (g == 0) { part_m[wv][c] = w.m; part_l[wv][c] = sum; }
+  f4* sums = reinterpret_cast<f4*>(lds[wv]);
 #pragma unroll
-  for (int mb = 0; mb < D / 16; ++mb) {
-    f4 x;
+  for (int q = 0; q < 4; ++q)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = __builtin_ldexpf(acc[0][mb][q], E);
-    sums[c * (D / 4) + ((4 * mb + g) ^ c)] = x;
-  }
+    for (int u = 0; u < D / 64; ++u) {
+      f4 x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = __builtin_ldexpf(w.acc[4 * u + k][q], w.E);
+      sums[c * (D / 4) + (((D / 64) * (4 * g + q) + u) ^ c)] = x;
+    }
   __syncthreads();
   const int rows = a.L * a.G - tile * 16 < 16 ? a.L * a.G - tile * 16 : 16;
   for (int k2 = threadIdx.x; k2 < rows * (D / 4); k2 += 64 * ROW_WAVES) {
@@ -233,7 +447,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, 2) void page_rows_kernel(const Page
     for (int x = 0; x < ROW_WAVES; ++x) {
       const float wgt = __builtin_amdgcn_exp2f(part_m[x][cr] - M);
       L += wgt * part_l[x][cr];
-      o += reinterpret_cast<const f4*>(&tiles[x][0])[cr * (D / 4) + (u ^ cr)] * wgt;
+      o += reinterpret_cast<const f4*>(lds[x])[cr * (D / 4) + (u ^ cr)] * wgt;
     }
     if (a.parted) {
       const int64_t slot = (int64_t)part.part * 16 + cr;
