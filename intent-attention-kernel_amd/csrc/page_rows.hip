@@ -275,10 +275,10 @@ template <int D> __device__ __forceinline__ void row_remember(Seen16& x, const u
 }
 
 // Waves a SIMD: what the registers hold of rings and queries in two parts.
-template <bool QF32> constexpr int row_waves_per_simd() { return QF32 ? 2 : 3; }
+template <bool QF32, int KIND> constexpr int row_waves_per_simd() { return QF32 || KIND == PAGES_ALL ? 2 : 3; }
 
 template <int D, bool QF32, int KIND>
-__global__ __launch_bounds__(64 * ROW_WAVES, row_waves_per_simd<QF32>()) void page_rows_kernel(const PageAttn a) {
+__global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>())) void page_rows_kernel(const PageAttn a) {
   constexpr int UNIT = 16 * D / 4;                               // 16-byte units of a wave's sums, and at least a page's K
   __shared__ u4 lds[ROW_WAVES][UNIT];
   __shared__ uint16_t special[ROW_WAVES][PS * D / 8];

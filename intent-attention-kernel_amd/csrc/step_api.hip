@@ -103,26 +103,75 @@ constexpr double CUS = 256;
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
 
 struct ChunkPlan {
-  int G, kind, tile_rows, tiles, splits, chunk;
+  int G, kind, tile_rows, tiles, splits, chunk, shares;
   int64_t items;
-  size_t ws_m, ws_l, ws_acc, total;
+  size_t ws_m, ws_l, ws_acc, ws_parts, total;
 };
 
-// Which kernel, and into how many parts a row's tokens go.
+// Which kernel, and into how many parts a row's tokens go: the least cost in microseconds, of
+//   (start + entry * entries of a part) * (workgroups of the busiest CU, against one) + the merge of parts,
+// from the table's width alone, for the lengths are on the device. An entry's time is one workgroup's
+// alone on its CU; `pair`: two workgroups of a CU take that much longer than one, and more go as pairs
+// (matrix work and the L2's rate are shared; what waits for memory is not). Of 300 calls timed under
+// every kernel and number of parts (1 to 64 sequences, 4 to 1,024 rows, 400 to 16,000 tokens, equal and
+// ragged, float16 pages and mixed ones), the choice took 1.03 times the best of each at the mean;
+// by rows alone, in one round of workgroups, 1.18. head_dim 128, mixed pages: 64 rows of 16,000 tokens, 8 KV
+// heads x 2: 16 rows 58 us, 128 rows 97; 256 rows (16 sequences, 2,500 tokens): 16 rows 177 us, 256 rows 114.
+// Several sequences may be shared out by their lengths instead of split alike, where a part is at
+// least half a tile's: 16 x 8 of up to 16,384 tokens in mixed pages 107 us, split alike 125 at the best,
+// 103 and 109 if the lengths are equal. Not over many tiles of 16 rows, whose workgroups then do not
+// read the same pages at the same time (4 x 8 of 128 rows, 16,000 tokens: 231 us for 148).
+struct ChunkCost { int tile; double start, entry, pair; };
+
 void choose_chunk(const iak_paged_chunk_args* a, int64_t rows, int W, ChunkPlan* p) {
-  const bool f32 = a->q_dtype == IAK_DTYPE_F32;
-  const double kvrows = (double)a->batch * a->num_kv_heads;
-  p->tile_rows = rows <= 64 ? 16 : (rows > 128 && !f32 ? 256 : 128);
-  p->tiles = (int)((rows + p->tile_rows - 1) / p->tile_rows);
-  const double tiles = kvrows * p->tiles, round = CUS * (p->tile_rows == 16 ? 3 : p->tile_rows == 256 ? 1 : 2);
-  int64_t splits = a->splits > 0 ? a->splits : (int64_t)(round / tiles);
-  if (splits > (W + 7) / 8 && a->splits == 0) splits = (W + 7) / 8;
+  const bool f32 = a->q_dtype == IAK_DTYPE_F32, plain = p->kind == iak::PAGES_F16, big = a->head_dim == 128;
+  const double kvrows = (double)a->batch * a->num_kv_heads, LAUNCH = 8, MERGE = 5, SHARE = 10, FILL = 0.75;
+  const ChunkCost costs[3] = {
+      {16, plain ? 0. : big ? 3. : 2., big ? (plain ? 0.148 : 0.212) : (plain ? 0.135 : 0.16), big ? (plain ? 2 : 1.5) : (plain ? 1.6 : 1.4)},
+      {128, plain ? 4. : big ? 8. : 5., big ? (plain ? 0.40 : 1.12) : (plain ? 0.33 : 0.63), big ? (plain ? 1.65 : 2) : (plain ? 1.5 : 1.37)},
+      {256, plain ? 5. : big ? 8. : 6., big ? (plain ? 0.52 : 1.08) : (plain ? 0.36 : 0.68), 2}};
+  double least = -1;
+  int64_t splits = 1;
+  for (const ChunkCost& c : costs) {
+    if ((c.tile == 128 && rows <= 16) || (c.tile == 256 && (rows <= 128 || f32))) continue;   // a kernel of 256 float32 rows is not there
+    const int tiles = (int)((rows + c.tile - 1) / c.tile);
+    const double work = kvrows * tiles, entry = c.entry * (f32 ? 1.5 : 1);
+    auto load = [&](double groups) { return groups <= CUS ? 1 : std::ceil(groups / CUS) * c.pair / 2; };
+    auto keep = [&](double cost, int64_t s, int shares) {
+      if (least >= 0 && cost >= least) return;
+      least = cost;
+      splits = s;
+      p->tile_rows = c.tile;
+      p->tiles = tiles;
+      p->shares = shares;
+    };
+    const int64_t most = c.tile == 16 ? (W + 3) / 4 : (W + 15) / 16;
+    auto split = [&](int64_t s) {
+      if (s < 1 || s > most) return;
+      const double merge = s > 1 ? MERGE + kvrows * rows * (s * (double)a->head_dim * 8 / 5.5e6 + (s > 8 ? 1e-3 : 0)) : 0;
+      keep(LAUNCH + (c.start + entry * W / s) * load(work * s) + merge, s, 0);
+    };
+    if (a->splits > 0) {
+      keep(LAUNCH + (c.start + entry * W / a->splits) * load(work * a->splits), a->splits, 0);
+      continue;
+    }
+    for (int64_t s = 1; s <= 128; s *= 2) split(s);
+    split((int64_t)(CUS / work));
+    split((int64_t)(2 * CUS / work));
+    if (a->batch == 1 || work > iak::MX_SHARED_TILES || work * W > 2e9 || (c.tile == 16 && rows > 48)) continue;
+    for (int shares = c.tile == 16 ? 2 * (int)CUS : (int)CUS; shares <= 2 * CUS; shares *= 2) {
+      const double parts = shares / work;                        // of a tile, on average
+      if (parts < 2 || parts > most) continue;
+      keep(LAUNCH + (c.start + FILL * entry * W / std::floor(parts)) * load(shares) + SHARE +
+               kvrows * rows * parts * a->head_dim * 8 / 5.5e6, 1, shares);
+    }
+  }
+  const double tiles = kvrows * p->tiles;
   if (splits > (W + 1) / 2) splits = (W + 1) / 2;
-  if (splits < 1) splits = 1;
   while (splits > 1 && tiles * splits * p->tile_rows > 1.6e7) splits /= 2;
   p->chunk = (int)((W + splits - 1) / splits);
   p->splits = (W + p->chunk - 1) / p->chunk;
-  p->items = (int64_t)tiles * p->splits;
+  p->items = p->shares ? p->shares : (int64_t)tiles * p->splits;
 }
 
 iak_status validate_paged_chunk(const iak_paged_chunk_args* a, ChunkPlan* p) {
@@ -181,11 +230,12 @@ iak_status validate_paged_chunk(const iak_paged_chunk_args* a, ChunkPlan* p) {
   if (kvrows * ((rows + 15) / 16) > 1.6e7)
     return fail(IAK_EINVAL, "too many query rows for one call (%.0f tiles of 16)", kvrows * ((rows + 15) / 16));
   choose_chunk(a, rows, a->table_width > 0 ? a->table_width : 1, p);
-  if (p->splits > 1) {
+  if (p->splits > 1 || p->shares) {
     const size_t kept = (size_t)p->items * p->tile_rows;
     p->ws_l = round_up(4 * kept);
     p->ws_acc = p->ws_l + round_up(4 * kept);
-    p->total = p->ws_acc + round_up(4 * kept * (size_t)a->head_dim);
+    p->ws_parts = p->ws_acc + round_up(4 * kept * (size_t)a->head_dim);
+    p->total = p->ws_parts + (p->shares ? round_up(8 * (size_t)kvrows * p->tiles) : 0);
   }
   return IAK_OK;
 }
@@ -213,7 +263,9 @@ iak_status iak_paged_chunk(const iak_paged_chunk_args* a, void* workspace, size_
   iak::PageAttn k{};
   k.B = a->batch; k.L = a->q_len; k.Hq = a->num_q_heads; k.Hkv = a->num_kv_heads; k.G = p.G; k.D = a->head_dim;
   k.W = a->table_width; k.NP = a->num_pages;
-  k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.items = p.items; k.parted = p.total > 0;
+  k.tile_rows = p.tile_rows; k.tiles = p.tiles; k.splits = p.splits; k.chunk = p.chunk; k.shares = p.shares;
+  k.items = p.items;
+  k.parted = p.total > 0;
   k.q = a->q; k.q_dtype = a->q_dtype; k.qsb = a->q_stride_b; k.qst = a->q_stride_t; k.qsh = a->q_stride_h;
   k.out = a->out; k.out_dtype = a->out_dtype; k.osb = a->out_stride_b; k.ost = a->out_stride_t; k.osh = a->out_stride_h;
   k.table = a->page_table; k.q_lens = a->q_lens; k.counts = a->page_counts; k.bounds = a->valid_tokens;
@@ -235,6 +287,7 @@ iak_status iak_paged_chunk(const iak_paged_chunk_args* a, void* workspace, size_
   k.ws_m = reinterpret_cast<float*>(ws + p.ws_m);
   k.ws_l = reinterpret_cast<float*>(ws + p.ws_l);
   k.ws_acc = reinterpret_cast<float*>(ws + p.ws_acc);
+  k.ws_parts = reinterpret_cast<int2*>(ws + p.ws_parts);
   return launched(iak::launch_page_attention(k, reinterpret_cast<hipStream_t>(stream)), "chunk attention");
 }
 
