@@ -3,17 +3,17 @@
 //   candidate (k, v) = scores[k] + logits[k, v] - log sum_u exp(logits[k, u]),
 // best first, ties to the lowest k V + v.
 //
-//   beam_part_kernel   a workgroup takes a segment of one row of logits into registers, once: its
-//                      sum of exponentials and its `count` best by (logit, index), which no offset of
-//                      the row changes. The count-th largest of the threads' maxima bounds
-//                      those from below, so that few elements go through LDS to be ranked.
+//   beam_part_kernel   a wave streams a segment of one row of logits, once: its sum of exponentials,
+//                      and its `count` best by (logit, index), which no offset of the row changes.
+//                      What is below a running threshold costs one comparison; the rest goes
+//                      to a list in LDS, which is ranked when it is full and at the end.
 //   beam_merge_kernel  a workgroup per request: the rows' normalisers out of the segments' sums,
-//                      and the best of the segments' lists.
+//                      and the best of the segments' lists, one after the other from their heads.
 //
 // Which token comes first is a whole number, so candidates of different beams have to be compared
 // to more than 32 bits: with offsets off by 2^-24 of 30 or so, two in some 10^5 neighbours would
-// change places. exp(x) = 2^(k/16) e^r with |r| <= ln 2 / 32: the table's 2^(k/16) and the sum in
-// 64 bits, e^r - 1 in 32 (off by 2^-30), so that a normaliser is off by some 1e-9.
+// change places. exp(x) = 2^(k/32) e^r with |r| <= ln 2 / 64: the table's 2^(k/32) and the sum in
+// 64 bits, r and e^r - 1 in 32, off by some 2^-31, so that a normaliser is off by some 1e-9.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -26,7 +26,7 @@ namespace iak {
 
 namespace {
 
-constexpr int BEAM_THREADS = 256;
+constexpr int BEAM_THREADS = 256, BEAM_WAVES = BEAM_THREADS / 64;
 
 struct BeamArgs {
   int B, K, V, n;
@@ -35,8 +35,8 @@ struct BeamArgs {
   const uint8_t* finished;
   int end;
   float* out_scores; int32_t* out_parents; int32_t* out_tokens;
-  int segments, per;        // segments a row, chunks of 8 logits a thread
-  double* norms;            // [rows, segments] log of the sum of exponentials; NaN: a logit is NaN or +inf
+  int segments, per;        // segments a row (a wave each), groups of logits a segment
+  double2* norms;           // [rows, segments] base and sum of exp(logit - base); base NaN: a logit is NaN or +inf
   uint64_t* best;           // [rows, segments, n] keys, best first; 0: none
 };
 
@@ -52,286 +52,451 @@ __device__ __forceinline__ bool beam_live(const BeamArgs& a, int64_t row, float 
   return !(a.finished && a.finished[row]) && __builtin_isfinite(score);
 }
 
-typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  any4 w[sizeof(T) / 2];
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(p) + i);
-  T t[8];
-  __builtin_memcpy(t, w, sizeof(t));
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
+// The largest of the wave's values, in every lane.
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+  auto step = [&](uint32_t y) { x = y > x ? y : x; };
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));   // row_bcast:15 into rows 1 and 3
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));   // row_bcast:31 into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// The workgroup's number of keys above `key` among keys[0 .. n - 1], for each thread.
-__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
-  int r = 0;
-  for (int i = 0; i < n; ++i) r += keys[i] > key;
+// A number that at least n of the wave's values reach, and as few more as there are (0: fewer do).
+__device__ __forceinline__ uint32_t wave_nth(uint32_t x, int n) {
+  uint32_t least = 0;
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+    const int reach = __builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= (least | bit)));
+    if (reach >= n) least |= bit;
+    if (reach == n) break;
+  }
+  return least;
+}
+
+// 8 logits as they lie, and one of them.
+typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> struct Raw8 { any4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ float value(const Raw8<T>& r, int j);
+template <> __device__ __forceinline__ float value<float>(const Raw8<float>& r, int j) { return u2f(r.w[j / 4][j % 4]); }
+template <> __device__ __forceinline__ float value<_Float16>(const Raw8<_Float16>& r, int j) {
+  const uint16_t h = (uint16_t)(r.w[0][j / 2] >> (16 * (j % 2)));
+  return (float)__builtin_bit_cast(_Float16, h);
+}
+template <> __device__ __forceinline__ float value<__bf16>(const Raw8<__bf16>& r, int j) {
+  return u2f(j % 2 ? r.w[0][j / 2] & 0xFFFF0000u : r.w[0][j / 2] << 16);
+}
+// Numbers of logits go up to 2^31 and a group past it: unsigned.
+template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* row, uint32_t v, uint32_t V) {
+  Raw8<T> r;
+  if (v + 8 <= V) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(row + v) + i);
+    return r;
+  }
+  // past the row: -inf, which adds nothing to a sum
+  constexpr int BITS = 8 * sizeof(T);
+  constexpr uint32_t NONE = __is_same(T, float) ? 0xFF800000u : __is_same(T, _Float16) ? 0xFC00u : 0xFF80u;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 32 / BITS; ++j) {
+        const uint32_t u = v + (4 * i + d) * (32 / BITS) + j;
+        uint32_t bits = NONE;
+        if (u < V) {
+          if constexpr (BITS == 32) bits = __builtin_bit_cast(uint32_t, row[u]);
+          else bits = __builtin_bit_cast(uint16_t, row[u]);
+        }
+        w |= bits << (BITS * j & 31);
+      }
+      r.w[i][d] = w;
+    }
   return r;
 }
 
+// exp(x) added up in 64 bits, for |x| up to some 600 (below that: as there). k = 32 x / ln 2 rounded, as the
+// low bits of a float past 2^23; the table's entry j has -j 2^15 in its high word, so that k 2^15
+// makes it 2^(k/32).
+__device__ __forceinline__ void add_exp(float x, const uint2* table, double& sum) {
+  constexpr float TURN = 46.166241308446828f, MAGIC = 12582912.f;   // 32 / ln 2, 1.5 2^23
+  constexpr double STEP = 0.021660849392498290;                     // ln 2 / 32
+  constexpr float STEP_HIGH = (float)STEP, STEP_LOW = (float)(STEP - (double)STEP_HIGH);
+  x = fmaxf(x, -600.f);
+  const float m = __builtin_fmaf(x, TURN, MAGIC), k = m - MAGIC;
+  const float r = __builtin_fmaf(-k, STEP_LOW, __builtin_fmaf(-k, STEP_HIGH, x));
+  const float q = r * __builtin_fmaf(r, __builtin_fmaf(r, 1.f / 6, 0.5f), 1.f);   // r^4 / 24 is 2^-30 at most
+  const uint2 e = table[f2u(m) & 31];
+  const uint64_t bits = ((uint64_t)(e.y + (f2u(m) << 15)) << 32) | e.x;
+  const double t = __builtin_bit_cast(double, bits);
+  sum = __builtin_fma(t, (double)q, sum) + t;
+}
+
+// What a wave's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int BEAM_LIST = 256;   // keys of a wave's list
+
+// The list's n best, in order, to its front. -> how many it holds then.
+__device__ __forceinline__ int rank_list(uint64_t* list, int count, int n, int lane) {
+  wave_sync();
+  uint64_t own[BEAM_LIST / 64];
+  int rank[BEAM_LIST / 64];
+#pragma unroll
+  for (int i = 0; i < BEAM_LIST / 64; ++i) {
+    own[i] = lane + 64 * i < count ? list[lane + 64 * i] : 0;
+    rank[i] = 0;
+  }
+  const int sets = (count + 63) >> 6;
+  for (int i = 0; i < count; ++i) {                              // keys differ
+    const uint64_t key = list[i];
+    rank[0] += key > own[0];
+    if (sets > 1) {
+#pragma unroll
+      for (int s = 1; s < BEAM_LIST / 64; ++s) rank[s] += key > own[s];
+    }
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < BEAM_LIST / 64; ++i)
+    if (own[i] != 0 && rank[i] < n) list[rank[i]] = own[i];
+  wave_sync();
+  return count < n ? count : n;
+}
+
+// The number that stands for at least `reach` in the order.
+__device__ __forceinline__ float level(uint32_t reach) { return reach > 0x007FFFFFu ? unordered(reach) : -__builtin_inff(); }
+
 template <typename T, int PER>
-__global__ __launch_bounds__(BEAM_THREADS) void beam_part_kernel(const BeamArgs a) {
-  __shared__ double table[16];
-  __shared__ uint64_t maxima[BEAM_THREADS];
-  __shared__ uint64_t found[BEAM_MOST_COUNT * PER * 8];
-  __shared__ double wave_sum[BEAM_THREADS / 64];
-  __shared__ uint32_t wave_top[BEAM_THREADS / 64];
-  __shared__ uint64_t least;
-  __shared__ int count;
-  const int t = threadIdx.x, seg = blockIdx.x;
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
-  if (row >= (int64_t)a.B * a.K || !beam_live(a, row, a.scores[row])) return;   // uniform
-  const int b = (int)(row / a.K), k = (int)(row - (int64_t)b * a.K);
+__global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamArgs a) {
+  __shared__ uint2 table[32];
+  __shared__ uint64_t lists[BEAM_WAVES][BEAM_LIST];
+  __shared__ Raw8<T> listed[BEAM_WAVES][PER][64];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  if (t < 32) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(t * 0.03125));
+    table[t] = make_uint2((uint32_t)bits, (uint32_t)(bits >> 32) - ((uint32_t)t << 15));
+  }
+  __syncthreads();
+  const int64_t part = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * BEAM_WAVES + wave, row = part / a.segments;
+  if (row >= (int64_t)a.B * a.K || !beam_live(a, row, a.scores[row])) return;   // no barrier below
+  const int b = (int)(row / a.K), k = (int)(row - (int64_t)b * a.K), seg = (int)(part - row * a.segments);
   const T* p = reinterpret_cast<const T*>(a.logits) + b * a.sb + k * a.sk;
-  if (t < 16) table[t] = exp2(t * 0.0625);
-  if (t == 0) { least = 0; count = 0; }
+  uint64_t* list = lists[wave];
 
-  // chunk i of thread t: logits 8 (seg PER 256 + i 256 + t) ..; what lies past the row is NaN here
-  float x[PER][8];
-  const int first = seg * (PER * BEAM_THREADS * 8) + 8 * t;
-  auto index = [&](int i) { return first + i * (BEAM_THREADS * 8); };
+  // chunk i of group g: logits g 512 PER + 512 i + 8 lane ..
+  constexpr int GROUP = 512 * PER;
+  const uint32_t V = (uint32_t)a.V;
+  const int n = a.n, g0 = seg * a.per, all = (int)((V + GROUP - 1) / GROUP), g1 = g0 + a.per < all ? g0 + a.per : all;
+  Raw8<T> x[PER], next[PER];
+  auto load = [&](Raw8<T> (&r)[PER], int g) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int v = index(i);
-    if (v + 8 <= a.V) {
-      load8(p + v, x[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = v + j < a.V ? (float)p[v + j] : -__builtin_inff();
-    }
-  }
-  // the thread's maximum, and whether everything is a number or -inf
+    for (int i = 0; i < PER; ++i) r[i] = load_raw8(p, (uint32_t)g * GROUP + 512 * i + 8 * lane, V);
+  };
+  load(x, g0);
+
+  // A logit goes to the list if it reaches `least` and its key is past `bound`. Of the first
+  // group's lane maxima the n-th largest bounds the n best from below; later that of the logits
+  // which went to the list, and the list's n-th key when it was ranked.
   float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, value<T>(x[i], j));
+  uint32_t highest = (uint32_t)g0 * GROUP + 8 * lane < V ? ordered(top) : 0;
+  uint32_t reach = wave_nth(highest, n);
+  float least = level(reach);
+  uint64_t bound = 0;
+  int count = 0;
   bool bad = false;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      bad = bad || !(x[i][j] < __builtin_inff());
-      top = fmaxf(top, x[i][j]);
-    }
-  int at = -1;                                                   // its lowest place; -1: the thread has no logits
-#pragma unroll
-  for (int i = PER - 1; i >= 0; --i)
-#pragma unroll
-    for (int j = 7; j >= 0; --j)
-      if (x[i][j] == top && index(i) + j < a.V) at = index(i) + j;
-  const uint64_t mine = at < 0 ? 0 : ((uint64_t)ordered(top) << 32) | (uint32_t)~at;
-  maxima[t] = mine;
-  uint32_t high = bad ? 0xFFFFFFFFu : ordered(top);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const uint32_t y = __shfl_xor(high, o, 64); high = y > high ? y : high; }
-  if ((t & 63) == 0) wave_top[t >> 6] = high;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < BEAM_THREADS / 64; ++w) high = wave_top[w] > high ? wave_top[w] : high;
-  const int64_t part = row * a.segments + seg;
-  if (high == 0xFFFFFFFFu) {                                     // uniform: the row is not finite
-    if (t == 0) a.norms[part] = __builtin_nan("");
-    return;
-  }
-
-  // the sum of exp(x - base), relative to the power of two below the maximum's. Large logits are taken
-  // from the maximum, which loses nothing: a 32-bit number's step is 2^-8 there, and what differs by a factor counts for nothing
-  constexpr float TURN = 23.083120654223414f;                    // 16 / ln 2
-  constexpr double STEP = 0.043321698784996581;                  // ln 2 / 16
-  const float M = unordered(high);
-  const bool any = M > -__builtin_inff();
-  const float base = any && fabsf(M) > 65536.f ? M : 0.f;
-  const float peak = any ? M - base : 0.f, low = peak - 500.f;   // e^-500 of the maximum: nothing
-  const int power = (int)rintf(peak * TURN) >> 4;
   double sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float l = fmaxf(x[i][j] - base, low);
-      const float kf = rintf(l * TURN);
-      const int kk = (int)kf;
-      const float r = (float)__builtin_fma(-STEP, (double)kf, (double)l);
-      const float q = __builtin_fmaf(r, __builtin_fmaf(r, __builtin_fmaf(r, 1.f / 24, 1.f / 6), 0.5f), 1.f);
-      const double e = __builtin_ldexp(table[kk & 15], (kk >> 4) - power);
-      sum = __builtin_fma(e, (double)(r * q), sum) + e;
-    }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-  if ((t & 63) == 0) wave_sum[t >> 6] = sum;
 
-  // a bound from below for the n best: the n-th largest of the threads' maxima (0: fewer have any)
-  if (rank_of(mine, maxima, BEAM_THREADS) == a.n - 1 && mine != 0) least = mine;   // keys differ: one thread
-  __syncthreads();
-  if (t == 0) {
-    double s = 0;
+  for (int g = g0; g < g1; ++g) {
+    if (g + 1 < g1) load(next, g + 1);
+    uint32_t chunks = 0;                                         // that have logits for the list
 #pragma unroll
-    for (int w = 0; w < BEAM_THREADS / 64; ++w) s += wave_sum[w];
-    a.norms[part] = any ? log(s) + 0.69314718055994530942 * power + (double)base : -__builtin_inf();
-  }
-  const uint64_t bound = least;
-  if (mine != 0 && mine >= bound) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
+    for (int i = 0; i < PER; ++i) {
+      bool any = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int v = index(i) + j;
-        const uint64_t key = ((uint64_t)ordered(x[i][j]) << 32) | (uint32_t)~v;
-        if (v < a.V && key >= bound) found[atomicAdd(&count, 1)] = key;   // n threads at most, 8 PER of each
+        const float l = value<T>(x[i], j);
+        any = any || !(l < least);                               // NaN too
+        add_exp(l, table, sum);
       }
+      if (__builtin_amdgcn_ballot_w64(any)) {
+        chunks |= 1u << i;
+        listed[wave][i][lane] = x[i];
+      }
+    }
+    if (chunks) {                                                // uniform
+      bool ranked = false;
+      for (; chunks; chunks &= chunks - 1) {
+        const int i = __builtin_ctz(chunks);
+        const T* own = reinterpret_cast<const T*>(&listed[wave][i][lane]);   // the lane's own, in LDS for `i` and `j` vary
+        const uint32_t first = (uint32_t)g * GROUP + 512 * i + 8 * lane;
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const float l = (float)own[j];
+          if (__builtin_amdgcn_ballot_w64(!(l < least)) == 0) continue;
+          const uint32_t high = ordered(l);
+          const uint64_t key = ((uint64_t)high << 32) | ~(first + j);
+          bad = bad || !(l < __builtin_inff());
+          const bool take = l >= least && key > bound && first + j < V;
+          const uint64_t takers = __builtin_amdgcn_ballot_w64(take);
+          if (take) {
+            highest = high > highest ? high : highest;
+            list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takers >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takers, 0))] = key;
+          }
+          count += __builtin_popcountll(takers);
+          if (count > BEAM_LIST - 64) {
+            count = rank_list(list, count, n, lane);
+            bound = list[n - 1];
+            least = unordered((uint32_t)(bound >> 32));
+            ranked = true;
+          }
+        }
+      }
+      // what follows has higher numbers: of equal logits it comes after those that are in the list
+      uint32_t most = wave_nth(highest, n);
+      if (ranked && (uint32_t)(bound >> 32) + 1 > most) most = (uint32_t)(bound >> 32) + 1;
+      if (most > reach) {
+        reach = most;
+        least = level(reach);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = next[i];
   }
-  __syncthreads();
-  uint64_t* out = a.best + part * a.n;
-  const int c = count;
-  for (int i = t; i < c; i += BEAM_THREADS) {
-    const int r = rank_of(found[i], found, c);
-    if (r < a.n) out[r] = found[i];
+
+  count = rank_list(list, count, n, lane);
+  if (lane < n) a.best[part * n + lane] = lane < count ? list[lane] : 0;
+  if (__builtin_amdgcn_ballot_w64(bad)) {
+    if (lane == 0) a.norms[part] = make_double2(__builtin_nan(""), 0);
+    return;
   }
-  for (int i = c + t; i < a.n; i += BEAM_THREADS) out[i] = 0;
+  double base = 0;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  if (!(sum > 1e-40 && sum < 1e40)) {
+    // Logits too large or too small, all of them: once more from the largest, from which all that
+    // matter differ by less than half of it, so that the difference is exact.
+    const float most = count ? unordered((uint32_t)(list[0] >> 32)) : -__builtin_inff();
+    base = most;
+    sum = 0;
+    if (most > -__builtin_inff()) {
+      for (int g = g0; g < g1; ++g) {
+        load(x, g);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) add_exp(value<T>(x[i], j) - most, table, sum);
+          __builtin_amdgcn_sched_barrier(0);                     // else a chunk's conversions go ahead of another's sum
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    }
+  }
+  if (lane == 0) a.norms[part] = make_double2(base, sum);
 }
 
-// A candidate of the merge: better with the larger value, or the lower index of equal ones.
-struct Candidate { double at; int64_t index; };                 // index -1: none
-__device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
-  return x.index >= 0 && (y.index < 0 || x.at > y.at || (x.at == y.at && x.index < y.index));
+// Candidates in LDS, a wave's at a time; a value's order as an unsigned number, 0: none.
+constexpr int MERGE_STAGE = 1024;
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
+  return b ^ (b >> 63 ? ~0ull : 1ull << 63);
 }
-
-constexpr int MERGE_PER = 16;   // candidates a thread takes a round
+__device__ __forceinline__ double unordered(uint64_t o) { return __builtin_bit_cast(double, o ^ (o >> 63 ? 1ull << 63 : ~0ull)); }
 
 __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs a) {
   __shared__ double norms[BEAM_MOST_BEAMS];                      // normaliser; NaN: the beam is out of the search
   __shared__ float scores[BEAM_MOST_BEAMS];
-  __shared__ Candidate maxima[BEAM_THREADS], found[BEAM_MOST_COUNT * (MERGE_PER + 1)], kept[BEAM_MOST_COUNT];
-  __shared__ Candidate least;
-  __shared__ int count;
-  const int t = threadIdx.x, b = blockIdx.x, lane = t & 63;
+  __shared__ bool ended[BEAM_MOST_BEAMS];
+  __shared__ uint64_t stage_at[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];       // of the lists, then the wave's best so far
+  __shared__ uint32_t stage_index[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // k V + v
+  __shared__ uint8_t stage_head[BEAM_WAVES][MERGE_STAGE + 1];
+  const int t = threadIdx.x, b = blockIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), n = a.n;
   const int64_t row0 = (int64_t)b * a.K;
 
-  // a wave a beam: its normaliser out of the segments' ones
-  for (int k = t >> 6; k < a.K; k += BEAM_THREADS / 64) {        // uniform in the wave
-    const int64_t row = row0 + k;
+  // 16 threads a beam: its normaliser out of the segments' sums
+  for (int k0 = 0; k0 < a.K; k0 += BEAM_THREADS / 16) {          // uniform
+    const int k = k0 + t / 16;
+    const bool there = k < a.K;
+    const int64_t row = row0 + (there ? k : 0);
     const float score = a.scores[row];
-    double norm = __builtin_nan("");
-    if (a.finished && a.finished[row]) {
-      if (__builtin_isfinite(score)) norm = 0;
-    } else if (__builtin_isfinite(score)) {
-      double most = -__builtin_inf(), sum = 0;
-      bool fine = true;
-      for (int s = lane; s < a.segments; s += 64) {
-        const double x = a.norms[row * a.segments + s];
-        fine = fine && x == x;
-        most = fmax(most, x);
-      }
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) most = fmax(most, __shfl_xor(most, d, 64));
-      if (__builtin_amdgcn_ballot_w64(!fine) == 0 && most > -__builtin_inf()) {
-        for (int s = lane; s < a.segments; s += 64) sum += exp(a.norms[row * a.segments + s] - most);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        norm = most + log(sum);
+    const bool live = beam_live(a, row, score);
+    double most = -__builtin_inf(), sum = 0;
+    bool fine = true;
+    if (live) {
+      for (int s = t & 15; s < a.segments; s += 16) {
+        const double2 x = a.norms[row * a.segments + s];
+        fine = fine && x.x == x.x;
+        if (x.x > most) {
+          sum = most == -__builtin_inf() ? x.y : sum * exp(most - x.x) + x.y;
+          most = x.x;
+        } else if (x.x > -__builtin_inf()) {
+          sum += x.x == most ? x.y : x.y * exp(x.x - most);
+        }
       }
     }
-    if (lane == 0) { norms[k] = norm; scores[k] = score; }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const double m = __shfl_xor(most, d, 64), s = __shfl_xor(sum, d, 64);
+      fine = __shfl_xor((int)fine, d, 64) && fine;
+      const double high = m > most ? m : most, low = m > most ? most : m;
+      const double own = m > most ? s : sum, other = m > most ? sum : s;
+      sum = own + (low == high ? other : low > -__builtin_inf() ? other * exp(low - high) : 0);
+      most = high;
+    }
+    if (there && (t & 15) == 0) {
+      const bool done = a.finished && a.finished[row];
+      double norm = __builtin_nan("");
+      if (done && __builtin_isfinite(score)) norm = 0;
+      else if (live && fine && most > -__builtin_inf()) norm = most + log(sum);
+      norms[k] = norm;
+      scores[k] = score;
+      ended[k] = done;
+    }
   }
-  if (t < a.n) kept[t].index = -1;
   __syncthreads();
 
-  // Candidate c of the request: number c % n of segment c / n % segments of beam c / n / segments.
-  // A beam at its end continues with the end token alone, one out of the search with nothing:
-  // the rest of theirs is -inf, the first n of which segment 0 stands for.
+  // List l of the request: segment l % segments of beam l / segments. A beam at its end continues
+  // with the end token alone, one out of the search with nothing: the rest of theirs is -inf, the first
+  // n of which segment 0 stands for.
   const int lists = a.K * a.segments;
-  auto candidate = [&](int64_t c) {
-    Candidate r = {0, -1};
-    const int list = (int)(c / a.n), j = (int)(c - (int64_t)list * a.n), k = list / a.segments, s = list - k * a.segments;
-    const bool done = a.finished && a.finished[row0 + k];
+  uint64_t* at = stage_at[wave];
+  uint32_t* index = stage_index[wave];
+  uint8_t* head = stage_head[wave];
+  auto candidate = [&](int list, int j, uint64_t& value, uint32_t& number) {
+    const int k = list / a.segments, s = list - k * a.segments;
     const double norm = norms[k], score = scores[k];
-    if (done || !(norm == norm)) {
-      if (s != 0 || j >= a.V) return r;
-      if (norm == norm) {
-        const int v = j == 0 ? a.end : (j - 1 < a.end ? j - 1 : j);
-        r = {j == 0 ? score : -__builtin_inf(), (int64_t)k * a.V + v};
-      } else {
-        r = {-__builtin_inf(), (int64_t)k * a.V + j};
-      }
-      return r;
+    value = 0;
+    number = 0;
+    if (ended[k] || !(norm == norm)) {
+      if (s != 0 || j >= a.V) return;
+      const bool last = norm == norm;
+      value = ordered(last && j == 0 ? score : -__builtin_inf());
+      number = (uint32_t)(k * a.V + (last ? (j == 0 ? a.end : (j - 1 < a.end ? j - 1 : j)) : j));
+      return;
     }
-    const uint64_t key = a.best[((row0 + k) * a.segments + s) * a.n + j];
-    // the score last, which a large normaliser would swallow
-    if (key != 0) r = {score + ((double)unordered((uint32_t)(key >> 32)) - norm), (int64_t)k * a.V + (int)~(uint32_t)key};
-    return r;
+    const uint64_t key = a.best[((row0 + k) * a.segments + s) * n + j];
+    if (key == 0) return;
+    value = ordered(score + ((double)unordered((uint32_t)(key >> 32)) - norm));   // the score last, which a large normaliser would swallow
+    number = (uint32_t)(k * a.V) + ~(uint32_t)key;
   };
-  const int64_t total = (int64_t)lists * a.n;
-  for (int64_t c0 = 0; c0 < total; c0 += (int64_t)BEAM_THREADS * MERGE_PER) {   // uniform
-    Candidate x[MERGE_PER], top = t < a.n ? kept[t] : Candidate{0, -1};
-    const Candidate mine = top;
-#pragma unroll
-    for (int i = 0; i < MERGE_PER; ++i) {
-      const int64_t c = c0 + i * BEAM_THREADS + t;
-      x[i] = c < total ? candidate(c) : Candidate{0, -1};
-      if (better(x[i], top)) top = x[i];
-    }
-    maxima[t] = top;
-    if (t == 0) { least.index = -1; count = 0; }
-    __syncthreads();
-    int above = 0;
-    for (int i = 0; i < BEAM_THREADS; ++i) above += better(maxima[i], top);
-    if (top.index >= 0 && above == a.n - 1) least = top;
-    __syncthreads();
-    const Candidate bound = least;
-    auto take = [&](const Candidate& y) {
-      if (y.index >= 0 && !better(bound, y)) found[atomicAdd(&count, 1)] = y;
+  // The n best of `count` lists in the stage, of list l at n l, each in order, to `to`: the best head,
+  // n times. A lane has every 64th list.
+  auto merge = [&](int count, uint64_t* to_at, uint32_t* to_index) {
+    wave_sync();
+    for (int l = lane; l < count; l += 64) head[l] = 0;
+    uint64_t best = 0;
+    uint32_t number = 0;
+    int from = 0;
+    auto look = [&]() {
+      best = 0;
+      number = 0;
+      for (int l = lane; l < count; l += 64) {
+        const int j = head[l];
+        if (j >= n) continue;
+        const uint64_t v = at[l * n + j];
+        const uint32_t i = index[l * n + j];
+        if (v > best || (v == best && v != 0 && i < number)) { best = v; number = i; from = l; }
+      }
     };
-    if (top.index >= 0 && !better(bound, top)) {
-      take(mine);
-#pragma unroll
-      for (int i = 0; i < MERGE_PER; ++i) take(x[i]);
+    look();
+    uint64_t kept_at = 0;
+    uint32_t kept_index = 0;
+    for (int r = 0; r < n; ++r) {
+      const uint32_t high = wave_most((uint32_t)(best >> 32));
+      bool wins = (uint32_t)(best >> 32) == high;
+      uint64_t winners = __builtin_amdgcn_ballot_w64(wins);
+      if (winners & (winners - 1)) {
+        const uint32_t low = wave_most(wins ? (uint32_t)best : 0);
+        wins = wins && (uint32_t)best == low;
+        const uint32_t first = wave_most(wins ? ~number : 0);
+        wins = wins && ~number == first;
+        winners = __builtin_amdgcn_ballot_w64(wins);
+      }
+      const int owner = __builtin_ctzll(winners);
+      const uint32_t a0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, owner);
+      const uint32_t i0 = (uint32_t)__builtin_amdgcn_readlane((int)number, owner);
+      if (lane == r) { kept_at = ((uint64_t)high << 32) | a0; kept_index = i0; }
+      if (lane == owner) {
+        ++head[from];
+        look();
+      }
     }
-    __syncthreads();
-    const int c = count;
-    for (int i = t; i < c; i += BEAM_THREADS) {
-      const Candidate y = found[i];
-      int r = 0;
-      for (int h = 0; h < c; ++h) r += better(found[h], y);
-      if (r < a.n) kept[r] = y;
-    }
-    __syncthreads();
+    wave_sync();
+    if (lane < n) { to_at[lane] = kept_at; to_index[lane] = kept_index; }
+    wave_sync();
+  };
+  const int each = MERGE_STAGE / n;                              // lists in the stage
+  bool some = false;
+  for (int l0 = wave * each; l0 < lists; l0 += BEAM_WAVES * each) {
+    const int count = lists - l0 < each ? lists - l0 : each;
+    for (int e = lane; e < count * n; e += 64) candidate(l0 + e / n, e % n, at[e], index[e]);
+    if (some && lane < n) { at[count * n + lane] = at[MERGE_STAGE + lane]; index[count * n + lane] = index[MERGE_STAGE + lane]; }
+    merge(count + some, at + MERGE_STAGE, index + MERGE_STAGE);
+    some = true;
   }
-  if (t < a.n) {
-    const Candidate y = kept[t];
-    const int64_t k = y.index / a.V;
-    a.out_scores[(int64_t)b * a.n + t] = (float)y.at;
-    a.out_parents[(int64_t)b * a.n + t] = (int32_t)(row0 + k);
-    a.out_tokens[(int64_t)b * a.n + t] = (int32_t)(y.index - k * a.V);
+  const int waves = lists > each ? ((lists + each - 1) / each < BEAM_WAVES ? (lists + each - 1) / each : BEAM_WAVES) : 1;
+  if (waves > 1) {                                               // uniform
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = waves - 1; w >= 0; --w)
+        if (lane < n) { at[w * n + lane] = stage_at[w][MERGE_STAGE + lane]; index[w * n + lane] = stage_index[w][MERGE_STAGE + lane]; }
+      merge(waves, at + MERGE_STAGE, index + MERGE_STAGE);
+    }
+  }
+  if (wave == 0 && lane < n) {
+    const uint32_t i = index[MERGE_STAGE + lane];
+    const uint32_t k = i / (uint32_t)a.V;
+    a.out_scores[(int64_t)b * n + lane] = (float)unordered(at[MERGE_STAGE + lane]);
+    a.out_parents[(int64_t)b * n + lane] = (int32_t)(row0 + k);
+    a.out_tokens[(int64_t)b * n + lane] = (int32_t)(i - k * (uint32_t)a.V);
   }
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Chunks of 8 logits a thread: 4, or as few as give the card a workgroup a CU.
+// Chunks of 512 logits that a wave has under way, twice: as many bytes of either type.
+constexpr int beam_per_of(int bytes) { return bytes == 4 ? 2 : 4; }
+
+// Groups of logits a segment: some 16 waves a CU, and no more lists than the merge takes in a few rounds.
 int beam_per(const iak_beam_select_args& a) {
-  const int64_t rows = (int64_t)a.batch * a.beams;
-  int per = 4;
-  while (per > 1 && rows * ((a.vocab + per * BEAM_THREADS * 8 - 1) / (per * BEAM_THREADS * 8)) < 256) per /= 2;
-  return per;
+  const int64_t rows = (int64_t)a.batch * a.beams, group = 512 * beam_per_of(a.dtype == IAK_DTYPE_F32 ? 4 : 2);
+  const int64_t groups = (a.vocab + group - 1) / group;
+  int64_t segments = 4096 / rows;
+  const int64_t most = 16384 / ((int64_t)a.beams * a.count);
+  if (segments > most) segments = most;
+  if (segments > groups) segments = groups;
+  if (segments < 1) segments = 1;
+  return (int)((groups + segments - 1) / segments);
 }
 
 template <typename T> void launch_part(const BeamArgs& a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.B * a.K;
-  const uint32_t y = (uint32_t)(rows < 32768 ? rows : 32768);
-  const dim3 grid((uint32_t)a.segments, y, (uint32_t)((rows + y - 1) / y));
-  if (a.per == 4) hipLaunchKernelGGL((beam_part_kernel<T, 4>), grid, dim3(BEAM_THREADS), 0, stream, a);
-  else if (a.per == 2) hipLaunchKernelGGL((beam_part_kernel<T, 2>), grid, dim3(BEAM_THREADS), 0, stream, a);
-  else hipLaunchKernelGGL((beam_part_kernel<T, 1>), grid, dim3(BEAM_THREADS), 0, stream, a);
+  const int64_t groups = ((int64_t)a.B * a.K * a.segments + BEAM_WAVES - 1) / BEAM_WAVES;
+  const uint32_t x = (uint32_t)(groups < (1 << 20) ? groups : 1 << 20);
+  const dim3 grid(x, (uint32_t)((groups + x - 1) / x));
+  hipLaunchKernelGGL((beam_part_kernel<T, beam_per_of(sizeof(T))>), grid, dim3(BEAM_THREADS), 0, stream, a);
 }
 
 }  // namespace
 
 int beam_segments(const iak_beam_select_args& a) {
-  const int64_t each = (int64_t)beam_per(a) * BEAM_THREADS * 8;
+  const int64_t each = (int64_t)beam_per(a) * 512 * beam_per_of(a.dtype == IAK_DTYPE_F32 ? 4 : 2);
   return (int)((a.vocab + each - 1) / each);
 }
 
 size_t beam_workspace(const iak_beam_select_args& a) {
   const size_t parts = (size_t)a.batch * a.beams * beam_segments(a);
-  return up256(8 * parts) + up256(8 * parts * a.count);
+  return up256(16 * parts) + up256(8 * parts * a.count);
 }
 
 hipError_t launch_beam_select(const iak_beam_select_args& a, void* workspace, hipStream_t stream) {
@@ -344,8 +509,8 @@ hipError_t launch_beam_select(const iak_beam_select_args& a, void* workspace, hi
   k.per = beam_per(a);
   const size_t parts = (size_t)a.batch * a.beams * k.segments;
   char* p = reinterpret_cast<char*>(workspace);
-  k.norms = reinterpret_cast<double*>(p);
-  k.best = reinterpret_cast<uint64_t*>(p + up256(8 * parts));
+  k.norms = reinterpret_cast<double2*>(p);
+  k.best = reinterpret_cast<uint64_t*>(p + up256(16 * parts));
   if (a.dtype == IAK_DTYPE_F32) launch_part<float>(k, stream);
   else if (a.dtype == IAK_DTYPE_F16) launch_part<_Float16>(k, stream);
   else launch_part<__bf16>(k, stream);
