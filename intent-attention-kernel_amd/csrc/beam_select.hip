@@ -67,6 +67,7 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t x) {
 // A number that at least n of the wave's values reach, and as few more as there are (0: fewer do).
 __device__ __forceinline__ uint32_t wave_nth(uint32_t x, int n) {
   uint32_t least = 0;
+#pragma unroll 1
   for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
     const int reach = __builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= (least | bit)));
     if (reach >= n) least |= bit;
@@ -125,7 +126,7 @@ __device__ __forceinline__ void add_exp(float x, const uint2* table, double& sum
   constexpr float TURN = 46.166241308446828f, MAGIC = 12582912.f;   // 32 / ln 2, 1.5 2^23
   constexpr double STEP = 0.021660849392498290;                     // ln 2 / 32
   constexpr float STEP_HIGH = (float)STEP, STEP_LOW = (float)(STEP - (double)STEP_HIGH);
-  x = fmaxf(x, -600.f);
+  x = u2f(f2u(x) < 0xC4160000u ? f2u(x) : 0xC4160000u);             // no less than -600, in one instruction
   const float m = __builtin_fmaf(x, TURN, MAGIC), k = m - MAGIC;
   const float r = __builtin_fmaf(-k, STEP_LOW, __builtin_fmaf(-k, STEP_HIGH, x));
   const float q = r * __builtin_fmaf(r, __builtin_fmaf(r, 1.f / 6, 0.5f), 1.f);   // r^4 / 24 is 2^-30 at most
@@ -143,31 +144,44 @@ __device__ __forceinline__ void wave_sync() {
 
 constexpr int BEAM_LIST = 256;   // keys of a wave's list
 
-// The list's n best, in order, to its front. -> how many it holds then.
-__device__ __forceinline__ int rank_list(uint64_t* list, int count, int n, int lane) {
+// The list's n best, in order, to its front; `reach`: a number that n of its logits reach, in
+// `ordered`, so that only those are compared with each other. -> how many it holds then.
+__device__ __forceinline__ int rank_list(uint64_t* list, int count, int n, uint32_t reach, int lane) {
+  constexpr int SETS = BEAM_LIST / 64;
+  uint64_t own[SETS];
   wave_sync();
-  uint64_t own[BEAM_LIST / 64];
-  int rank[BEAM_LIST / 64];
 #pragma unroll
-  for (int i = 0; i < BEAM_LIST / 64; ++i) {
-    own[i] = lane + 64 * i < count ? list[lane + 64 * i] : 0;
+  for (int i = 0; i < SETS; ++i) own[i] = lane + 64 * i < count ? list[lane + 64 * i] : 0;
+  wave_sync();
+  int left = 0;
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) {
+    const bool stays = own[i] != 0 && (uint32_t)(own[i] >> 32) >= reach;
+    const uint64_t staying = __builtin_amdgcn_ballot_w64(stays);
+    if (stays) list[left + __builtin_amdgcn_mbcnt_hi((uint32_t)(staying >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)staying, 0))] = own[i];
+    left += __builtin_popcountll(staying);
+  }
+  wave_sync();
+  int rank[SETS];
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) {
+    own[i] = lane + 64 * i < left ? list[lane + 64 * i] : 0;
     rank[i] = 0;
   }
-  const int sets = (count + 63) >> 6;
-  for (int i = 0; i < count; ++i) {                              // keys differ
+  for (int i = 0; i < left; ++i) {                               // keys differ
     const uint64_t key = list[i];
     rank[0] += key > own[0];
-    if (sets > 1) {
+    if (left > 64) {
 #pragma unroll
-      for (int s = 1; s < BEAM_LIST / 64; ++s) rank[s] += key > own[s];
+      for (int s = 1; s < SETS; ++s) rank[s] += key > own[s];
     }
   }
   wave_sync();
 #pragma unroll
-  for (int i = 0; i < BEAM_LIST / 64; ++i)
+  for (int i = 0; i < SETS; ++i)
     if (own[i] != 0 && rank[i] < n) list[rank[i]] = own[i];
   wave_sync();
-  return count < n ? count : n;
+  return left < n ? left : n;
 }
 
 // The number that stands for at least `reach` in the order.
@@ -217,48 +231,60 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
   bool bad = false;
   double sum = 0;
 
+  auto put = [&](float l, uint32_t v) {                          // with room for 64
+    const uint32_t high = ordered(l);
+    const uint64_t key = ((uint64_t)high << 32) | ~v;
+    bad = bad || !(l < __builtin_inff());
+    const bool take = l >= least && key > bound && v < V;
+    const uint64_t takers = __builtin_amdgcn_ballot_w64(take);
+    if (take) {
+      highest = high > highest ? high : highest;
+      list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takers >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takers, 0))] = key;
+    }
+    count += __builtin_popcountll(takers);
+  };
   for (int g = g0; g < g1; ++g) {
     if (g + 1 < g1) load(next, g + 1);
-    uint32_t chunks = 0;                                         // that have logits for the list
+    const int before = count;
+    bool full = false;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      bool any = false;
+      const uint32_t first = (uint32_t)g * GROUP + 512 * i + 8 * lane;
+      uint64_t hits[8], any = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float l = value<T>(x[i], j);
-        any = any || !(l < least);                               // NaN too
+        hits[j] = __builtin_amdgcn_ballot_w64(!(l < least));     // NaN too
+        any |= hits[j];
         add_exp(l, table, sum);
       }
-      if (__builtin_amdgcn_ballot_w64(any)) {
-        chunks |= 1u << i;
-        listed[wave][i][lane] = x[i];
-      }
+      asm volatile("" : "+v"(sum));                              // here, not behind the loop: 16 registers a chunk
+      if (any == 0) continue;                                    // uniform, as below
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (hits[j]) {
+          if (count > BEAM_LIST - 64) full = true;
+          else put(value<T>(x[i], j), first + j);
+        }
     }
-    if (chunks) {                                                // uniform
+    if (count != before || full) {
       bool ranked = false;
-      for (; chunks; chunks &= chunks - 1) {
-        const int i = __builtin_ctz(chunks);
-        const T* own = reinterpret_cast<const T*>(&listed[wave][i][lane]);   // the lane's own, in LDS for `i` and `j` vary
-        const uint32_t first = (uint32_t)g * GROUP + 512 * i + 8 * lane;
+      if (full) {                                                // again, the list ranked as often as it is full
+        count = before;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) listed[wave][i][lane] = x[i];
 #pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          const float l = (float)own[j];
-          if (__builtin_amdgcn_ballot_w64(!(l < least)) == 0) continue;
-          const uint32_t high = ordered(l);
-          const uint64_t key = ((uint64_t)high << 32) | ~(first + j);
-          bad = bad || !(l < __builtin_inff());
-          const bool take = l >= least && key > bound && first + j < V;
-          const uint64_t takers = __builtin_amdgcn_ballot_w64(take);
-          if (take) {
-            highest = high > highest ? high : highest;
-            list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takers >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takers, 0))] = key;
-          }
-          count += __builtin_popcountll(takers);
-          if (count > BEAM_LIST - 64) {
-            count = rank_list(list, count, n, lane);
-            bound = list[n - 1];
-            least = unordered((uint32_t)(bound >> 32));
-            ranked = true;
+        for (int i = 0; i < PER; ++i) {
+          const T* own = reinterpret_cast<const T*>(&listed[wave][i][lane]);   // the lane's own, in LDS for `i` and `j` vary
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {
+            put((float)own[j], (uint32_t)g * GROUP + 512 * i + 8 * lane + j);
+            if (count > BEAM_LIST - 64) {
+              count = rank_list(list, count, n, 0, lane);
+              bound = list[n - 1];
+              least = unordered((uint32_t)(bound >> 32));
+              ranked = true;
+            }
           }
         }
       }
@@ -274,7 +300,7 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
     for (int i = 0; i < PER; ++i) x[i] = next[i];
   }
 
-  count = rank_list(list, count, n, lane);
+  count = rank_list(list, count, n, wave_nth(highest, n), lane);
   if (lane < n) a.best[part * n + lane] = lane < count ? list[lane] : 0;
   if (__builtin_amdgcn_ballot_w64(bad)) {
     if (lane == 0) a.norms[part] = make_double2(__builtin_nan(""), 0);
@@ -323,19 +349,32 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
   __shared__ uint8_t stage_head[BEAM_WAVES][MERGE_STAGE + 1];
   const int t = threadIdx.x, b = blockIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), n = a.n;
   const int64_t row0 = (int64_t)b * a.K;
+  const int lists = a.K * a.segments, each = MERGE_STAGE / n;    // of the request, and in a wave's stage
+  const bool once = lists <= each;                               // uniform: one wave merges, and all load for it
+  constexpr int OWN = MERGE_STAGE / BEAM_THREADS;
+  uint64_t keys[OWN];                                            // on their way meanwhile; of beams that are out: anything
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int e = t + i * BEAM_THREADS;
+      keys[i] = a.best[row0 * a.segments * n + (e < lists * n ? e : 0)];
+    }
+  }
 
   // 16 threads a beam: its normaliser out of the segments' sums
   for (int k0 = 0; k0 < a.K; k0 += BEAM_THREADS / 16) {          // uniform
     const int k = k0 + t / 16;
     const bool there = k < a.K;
     const int64_t row = row0 + (there ? k : 0);
+    const double2* own = a.norms + row * a.segments;
     const float score = a.scores[row];
+    double2 x = own[(t & 15) < a.segments ? t & 15 : 0];         // of a beam that is out: anything
     const bool live = beam_live(a, row, score);
     double most = -__builtin_inf(), sum = 0;
     bool fine = true;
     if (live) {
       for (int s = t & 15; s < a.segments; s += 16) {
-        const double2 x = a.norms[row * a.segments + s];
+        if (s >= 16) x = own[s];
         fine = fine && x.x == x.x;
         if (x.x > most) {
           sum = most == -__builtin_inf() ? x.y : sum * exp(most - x.x) + x.y;
@@ -369,11 +408,10 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
   // List l of the request: segment l % segments of beam l / segments. A beam at its end continues
   // with the end token alone, one out of the search with nothing: the rest of theirs is -inf, the first
   // n of which segment 0 stands for.
-  const int lists = a.K * a.segments;
   uint64_t* at = stage_at[wave];
   uint32_t* index = stage_index[wave];
   uint8_t* head = stage_head[wave];
-  auto candidate = [&](int list, int j, uint64_t& value, uint32_t& number) {
+  auto candidate = [&](int list, int j, uint64_t key, uint64_t& value, uint32_t& number) {
     const int k = list / a.segments, s = list - k * a.segments;
     const double norm = norms[k], score = scores[k];
     value = 0;
@@ -385,7 +423,6 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
       number = (uint32_t)(k * a.V + (last ? (j == 0 ? a.end : (j - 1 < a.end ? j - 1 : j)) : j));
       return;
     }
-    const uint64_t key = a.best[((row0 + k) * a.segments + s) * n + j];
     if (key == 0) return;
     value = ordered(score + ((double)unordered((uint32_t)(key >> 32)) - norm));   // the score last, which a large normaliser would swallow
     number = (uint32_t)(k * a.V) + ~(uint32_t)key;
@@ -436,16 +473,33 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
     if (lane < n) { to_at[lane] = kept_at; to_index[lane] = kept_index; }
     wave_sync();
   };
-  const int each = MERGE_STAGE / n;                              // lists in the stage
-  bool some = false;
-  for (int l0 = wave * each; l0 < lists; l0 += BEAM_WAVES * each) {
-    const int count = lists - l0 < each ? lists - l0 : each;
-    for (int e = lane; e < count * n; e += 64) candidate(l0 + e / n, e % n, at[e], index[e]);
-    if (some && lane < n) { at[count * n + lane] = at[MERGE_STAGE + lane]; index[count * n + lane] = index[MERGE_STAGE + lane]; }
-    merge(count + some, at + MERGE_STAGE, index + MERGE_STAGE);
-    some = true;
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int e = t + i * BEAM_THREADS;
+      if (e < lists * n) candidate(e / n, e % n, keys[i], stage_at[0][e], stage_index[0][e]);
+    }
+    __syncthreads();
+    if (wave == 0) merge(lists, at + MERGE_STAGE, index + MERGE_STAGE);
+  } else {
+    bool some = false;
+    for (int l0 = wave * each; l0 < lists; l0 += BEAM_WAVES * each) {
+      const int count = lists - l0 < each ? lists - l0 : each, total = count * n;
+      for (int e0 = lane; e0 < total; e0 += 64 * OWN) {
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) keys[i] = a.best[(row0 * a.segments + l0) * n + (e0 + 64 * i < total ? e0 + 64 * i : 0)];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+          const int e = e0 + 64 * i;
+          if (e < total) candidate(l0 + e / n, e % n, keys[i], at[e], index[e]);
+        }
+      }
+      if (some && lane < n) { at[total + lane] = at[MERGE_STAGE + lane]; index[total + lane] = index[MERGE_STAGE + lane]; }
+      merge(count + some, at + MERGE_STAGE, index + MERGE_STAGE);
+      some = true;
+    }
   }
-  const int waves = lists > each ? ((lists + each - 1) / each < BEAM_WAVES ? (lists + each - 1) / each : BEAM_WAVES) : 1;
+  const int rounds = (lists + each - 1) / each, waves = rounds < BEAM_WAVES ? rounds : BEAM_WAVES;
   if (waves > 1) {                                               // uniform
     __syncthreads();
     if (wave == 0) {
