@@ -180,10 +180,11 @@ __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool
 }
 
 // Two values as float16 and what is left of them. The first is cut rather than rounded: the second has it.
-__device__ __forceinline__ void hi_lo(float a, float b, bool fine, uint32_t& hi, uint32_t& lo) {
+// `fine` 0: they are not finite, and have no second part; else all bits.
+__device__ __forceinline__ void hi_lo(float a, float b, uint32_t fine, uint32_t& hi, uint32_t& lo) {
   const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
   hi = bits(h);
-  lo = fine ? bits(h2{(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])}) : 0u;
+  lo = bits(h2{(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])}) & fine;
 }
 
 // A scale in two float16 parts; a code times the first is off by what a fused product gives exactly.
@@ -242,7 +243,7 @@ __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag,
     }
   } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
     const float s0 = r.s0 * rest, s1 = r.s1 * rest;
-    const bool fine = fabsf(s0) + fabsf(s1) < __builtin_inff();
+    const uint32_t fine = fabsf(s0) + fabsf(s1) < __builtin_inff() ? 0xFFFFFFFFu : 0u;
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
       const int f = 64 * j + lane, token = f / (D / 16), chunk = f % (D / 16) * 2;
@@ -303,7 +304,8 @@ template <int KIND> struct Ahead {
   uint8_t tag[AHEAD];                  // native, or NO_PAGE
   float km[KIND == PAGES_F16 ? 1 : AHEAD], vl[KIND == PAGES_F16 ? 1 : AHEAD];   // as in PageEntry; no page: vl NO_SCALE
   float iv[KIND == PAGES_F16 ? 1 : AHEAD];                                      // 2^-vl, 0
-  f4 factors[2][KIND == PAGES_F16 ? 1 : AHEAD];   // of K's and V's codes; INT4: by quarters of the channels, residual: base, rest
+  f4 factors[2][KIND == PAGES_F16 ? 1 : AHEAD];   // of K's and V's codes, by quarters of the channels; residual: of the bases
+  float second[2][KIND == PAGES_ALL ? AHEAD : 1];                               // residual: of the residuals
 };
 
 template <int D, int KIND>
@@ -334,11 +336,10 @@ __device__ __forceinline__ void put_ahead(Ahead<KIND>& t, const PageAttn& a, int
       }
     }
     if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4_RESIDUAL) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        kf[q] *= a.k_int4r_scale[2 * p + q];
-        vf[q] *= a.v_int4r_scale[2 * p + q];
-      }
+      t.second[0][at] = kf[0] * a.k_int4r_scale[2 * p + 1];
+      t.second[1][at] = vf[0] * a.v_int4r_scale[2 * p + 1];
+      kf *= a.k_int4r_scale[2 * p];
+      vf *= a.v_int4r_scale[2 * p];
     }
     t.km[at] = y.km;
     t.vl[at] = x.id < 0 ? NO_SCALE : y.vl;
@@ -363,16 +364,16 @@ __device__ __forceinline__ u4 load_piece(uint64_t page, uint32_t tag, uint32_t f
   return u4{x[0], x[1], 0u, 0u};
 }
 
-// Into place `at` of the tile `hi`, and what is left of wide pages into `lo`.
+// Into place `at` of the tile `hi`, and what is left of wide pages into `lo`; s0, s1: the lane's factors.
 template <int D, int KIND>
-__device__ __forceinline__ void store_piece(const u4& x, uint32_t tag, const f4& factors, int f, u4* hi, u4* lo, int at) {
+__device__ __forceinline__ void store_piece(const u4& x, uint32_t tag, float s0, float s1, u4* hi, u4* lo, int at) {
   if (KIND == PAGES_F16 || tag == NO_PAGE || tag == IAK_TAG_FP16) {
     hi[at] = x;
     return;
   }
   u4 h, l;
   if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
-    const ScaleParts k = scale_parts(reinterpret_cast<const float*>(&factors)[f % (D / 8) / (D / 32)]);
+    const ScaleParts k = scale_parts(s0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const h2 n = nibbles(x[0], i), y = n * k.hi;
@@ -381,8 +382,7 @@ __device__ __forceinline__ void store_piece(const u4& x, uint32_t tag, const f4&
     }
     lo[at] = l;
   } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
-    const float s0 = factors[0], s1 = factors[1];
-    const bool fine = fabsf(s0) + fabsf(s1) < __builtin_inff();
+    const uint32_t fine = fabsf(s0) + fabsf(s1) < __builtin_inff() ? 0xFFFFFFFFu : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w = x[i >> 1];
@@ -394,7 +394,7 @@ __device__ __forceinline__ void store_piece(const u4& x, uint32_t tag, const f4&
     }
     lo[at] = l;
   } else {
-    const h2 sign = splat2((_Float16)factors[0]);
+    const h2 sign = splat2((_Float16)s0);
     uint32_t o[4];
     if (tag == IAK_TAG_FP8) {
       fp8x4_to_f16(x[0], o[0], o[1]);

@@ -16,10 +16,27 @@ namespace iak {
 
 namespace {
 
+// N operands from LDS and what each is multiplied by, the operands read ahead of their products, for
+// a read takes as long as several. (Left to itself the compiler reads each just before its own.)
+template <int N, int AHEAD_OF, typename Read, typename Multiply> __device__ __forceinline__ void products(Read&& read, Multiply&& multiply) {
+  constexpr int A = N < AHEAD_OF ? N : AHEAD_OF;
+  h8 x[A];
+#pragma unroll
+  for (int i = 0; i < A; ++i) x[i] = read(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(i, x[i % A]);
+    if (i + A < N) x[i % A] = read(i + A);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int D, bool QF32, int NW, int RT, int KIND>
 __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a) {
   static_assert(NW == 4 || NW == 8, "pieces of pages are shared out");
   constexpr bool WIDE = KIND == PAGES_ALL, SCALED = KIND != PAGES_F16;
+  constexpr int FEED = 4;
   constexpr int QUARTERS = D / 32, OWN = 8 * QUARTERS / NW;      // pieces (64 chunks) a page, and of a wave a step
   constexpr int BM = 16 * RT * NW, PAGE = PS * D / 8;   // 16-byte units of a tile
   __shared__ u4 tiles[2][2][4][PAGE];                            // [buffer][K, V][page]
@@ -88,80 +105,79 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   const int f = w % QUARTERS * 64 + lane, place = v_chunk<D>(f / (D / 8), f % (D / 8));
   u4 raw[OWN];
   auto tags_of = [&](int k) { return uniform(*reinterpret_cast<const uint32_t*>(&table.tag[k & (AHEAD - 1)])); };   // of four pages
+  // (What LDS has for all pieces is read before any is worked on: the tags' branches would have a read's
+  // wait each.)
   auto load = [&](uint32_t tags, int k) __attribute__((always_inline)) {
+    u2 at[OWN];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) at[o] = reinterpret_cast<const u2*>(&table.where[(k + page_of(o)) & (AHEAD - 1)])[side_of(o)];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o)
+      raw[o] = load_piece<D, KIND>((uint64_t)at[o][0] | (uint64_t)at[o][1] << 32, (tags >> (8 * page_of(o))) & 0xFFu, f);
+  };
+  const int quarter = f % (D / 8) / (D / 32);
+  auto convert = [&](int buf, uint32_t tags, int k) __attribute__((always_inline)) {
+    float s0[OWN], s1[OWN];
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
-      const int p = page_of(o);
-      const u2 at = reinterpret_cast<const u2*>(&table.where[(k + p) & (AHEAD - 1)])[side_of(o)];
-      raw[o] = load_piece<D, KIND>((uint64_t)at[0] | (uint64_t)at[1] << 32, (tags >> (8 * p)) & 0xFFu, f);
+      const int e = (k + page_of(o)) & (AHEAD - 1);
+      s0[o] = SCALED ? reinterpret_cast<const float*>(&table.factors[side_of(o)][SCALED ? e : 0])[quarter] : 0.f;
+      s1[o] = WIDE ? table.second[side_of(o)][WIDE ? e : 0] : 0.f;
     }
-  };
-  auto convert = [&](int buf, uint32_t tags, int k) __attribute__((always_inline)) {
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
       const int p = page_of(o), s = side_of(o);
-      store_piece<D, KIND>(raw[o], (tags >> (8 * p)) & 0xFFu, table.factors[s][SCALED ? (k + p) & (AHEAD - 1) : 0], f, tiles[buf][s][p],
-                           rest[WIDE ? buf : 0][s][p], place);
-      if (careful && s == 1 && __builtin_amdgcn_ballot_w64(clean_chunk(&tiles[buf][1][p][place])) && lane == 0) special = 1;
+      store_piece<D, KIND>(raw[o], (tags >> (8 * p)) & 0xFFu, s0[o], s1[o], tiles[buf][s][p], rest[WIDE ? buf : 0][s][p], place);
+    }
+    if (careful) {
+#pragma unroll 1
+      for (int o = 0; o < OWN; ++o)
+        if (side_of(o) == 1 && __builtin_amdgcn_ballot_w64(clean_chunk(&tiles[buf][1][page_of(o)][place])) && lane == 0) special = 1;
     }
   };
 
-  f4 acc[RT][D / 16], l[RT];
+  f4 acc[RT][D / 16], l[RT], s[RT][4];
   float lsum[RT], m[RT];
+  h8 pb[RT][2], pl[RT][QF32 ? 2 : 1];
   int E = 0;
   const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-  int k = 0;                                                     // number of entry e in the part
-  uint32_t now = 0, soon = 0;                                    // tags of this step's pages and of the next's
-  auto step = [&](int buf, int e) __attribute__((always_inline)) {
-    const uint32_t later = tags_of(k + 8);
-    f4 kms = {1.f, 1.f, 1.f, 1.f}, vls = {0.f, 0.f, 0.f, 0.f}, ivs = vls;
-    if constexpr (SCALED) {
-      kms = *reinterpret_cast<const f4*>(&table.km[k & (AHEAD - 1)]);
-      vls = *reinterpret_cast<const f4*>(&table.vl[k & (AHEAD - 1)]);
-      ivs = *reinterpret_cast<const f4*>(&table.iv[k & (AHEAD - 1)]);
+  auto wide = [&](uint32_t tags, int p) { return WIDE && wide_tag((int)((tags >> (8 * p)) & 0xFFu)); };
+
+  // s = K Q^T of a step's tokens; its operand i is channels 8 (i / 4) .. of page i % 4
+  auto read_k = [&](const u4 (&page)[PAGE], int j) __attribute__((always_inline)) {
+    return __builtin_bit_cast(h8, page[v_chunk<D>(c, g * (D / 32) + j)]);
+  };
+  auto score = [&](int p, int j, const h8& k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qhi[t][j], j == 0 ? f4{0.f, 0.f, 0.f, 0.f} : s[t][p], 0, 0, 0);
+      if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qlo[t][j], s[t][p], 0, 0, 0);
     }
-    int id[4];                                                   // -1: no page
-    bool wide[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const uint32_t tag = (now >> (8 * p)) & 0xFFu;
-      id[p] = tag == NO_PAGE ? -1 : 0;
-      wide[p] = WIDE && wide_tag((int)tag);
-    }
-    f4 s[RT][4];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int p = 0; p < 4; ++p) s[t][p] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const h8 ka = __builtin_bit_cast(h8, tiles[buf][0][p][v_chunk<D>(c, g * (D / 32) + j)]);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[t][j], s[t][p], 0, 0, 0);
-          if constexpr (QF32) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[t][j], s[t][p], 0, 0, 0);
-        }
-      }
+  };
+  auto scores_rest = [&](int buf, uint32_t tags) __attribute__((always_inline)) {
     if constexpr (WIDE) {
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        if (!wide[p]) continue;
+        if (!wide(tags, p)) continue;
+        products<D / 32, 4>([&](int j) __attribute__((always_inline)) { return __builtin_bit_cast(h8, rest[buf][0][p][v_chunk<D>(c, g * (D / 32) + j)]); },
+                            [&](int j, const h8& k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const h8 ka = __builtin_bit_cast(h8, rest[buf][0][p][v_chunk<D>(c, g * (D / 32) + j)]);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[t][j], s[t][p], 0, 0, 0);
-        }
+          for (int t = 0; t < RT; ++t) s[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qhi[t][j], s[t][p], 0, 0, 0);
+        });
       }
     }
-    convert(buf ^ 1, soon, k + 4);
-    load(later, k + 8);
-    look_ahead(k);
+  };
+  // pb = weights of the scores of tokens 16 e ..; the sums so far follow the maximum
+  auto softmax = [&](uint32_t tags, int k, int e) __attribute__((always_inline)) {
+    int id[4];                                                   // -1: no page
+#pragma unroll
+    for (int p = 0; p < 4; ++p) id[p] = ((tags >> (8 * p)) & 0xFFu) == NO_PAGE ? -1 : 0;
     const uint32_t no_nan[4] = {0u, 0u, 0u, 0u};
     hide<4, RT>(s, no_nan, id, e, seen, least, g);
     if constexpr (SCALED) {
+      const f4 kms = *reinterpret_cast<const f4*>(&table.km[k & (AHEAD - 1)]);
+      const f4 vls = *reinterpret_cast<const f4*>(&table.vl[k & (AHEAD - 1)]);
+      const f4 ivs = *reinterpret_cast<const f4*>(&table.iv[k & (AHEAD - 1)]);
       const float km[4] = {kms[0], kms[1], kms[2], kms[3]};
       float vl[4] = {vls[0], vls[1], vls[2], vls[3]}, out[4];
       raise_scaled<D, 4, RT>(s, km, mult, m, lsum, acc);
@@ -187,7 +203,6 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
 #pragma unroll
       for (int t = 0; t < RT; ++t) soften<4>(s[t], mult[t], m[t]);
     }
-    h8 pb[RT][2], pl[RT][QF32 ? 2 : 1];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -195,6 +210,21 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
         pb[t][h] = weights(s[t][2 * h], s[t][2 * h + 1]);
         if constexpr (QF32) pl[t][h] = weights_rest(s[t][2 * h], s[t][2 * h + 1], pb[t][h]);
       }
+  };
+  // acc += V^T pb of a step's tokens; its operand i is 16 channels of two pages
+  auto value = [&](int i, const h8& v) __attribute__((always_inline)) {
+    const int h = i / (D / 16), mb = i % (D / 16);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[t][h], acc[t][mb], 0, 0, 0);
+      if constexpr (QF32) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t][h], acc[t][mb], 0, 0, 0);
+    }
+  };
+  auto read_v = [&](int buf, int i) __attribute__((always_inline)) {
+    const int h = i / (D / 16), mb = i % (D / 16);
+    return values_back<D>(tiles[buf][1][2 * h], tiles[buf][1][2 * h + 1], mb, c, g);
+  };
+  auto weigh = [&]() __attribute__((always_inline)) {            // the weights' sum
     if constexpr (!SCALED) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -204,31 +234,45 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
           if constexpr (QF32) l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t][h], l[t], 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int mb = 0; mb < D / 16; ++mb) {
-        const h8 va = values_back<D>(tiles[buf][1][2 * h], tiles[buf][1][2 * h + 1], mb, c, g);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[t][h], acc[t][mb], 0, 0, 0);
-          if constexpr (QF32) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[t][h], acc[t][mb], 0, 0, 0);
-        }
-      }
+  };
+  auto values_rest = [&](int buf, uint32_t tags) __attribute__((always_inline)) {
     if constexpr (WIDE) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!wide[2 * h] && !wide[2 * h + 1]) continue;
-        const u4* p0 = wide[2 * h] ? rest[buf][1][2 * h] : none;
-        const u4* p1 = wide[2 * h + 1] ? rest[buf][1][2 * h + 1] : none;
+        const bool w0 = wide(tags, 2 * h), w1 = wide(tags, 2 * h + 1);
+        if (!w0 && !w1) continue;
+        const u4* p0 = w0 ? rest[buf][1][2 * h] : none;
+        const u4* p1 = w1 ? rest[buf][1][2 * h + 1] : none;
+        products<D / 16, FEED>([&](int mb) __attribute__((always_inline)) { return values_back<D>(p0, p1, mb, c, g); },
+                               [&](int mb, const h8& v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int mb = 0; mb < D / 16; ++mb) {
-          const h8 va = values_back<D>(p0, p1, mb, c, g);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[t][h], acc[t][mb], 0, 0, 0);
-        }
+          for (int t = 0; t < RT; ++t) acc[t][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[t][h], acc[t][mb], 0, 0, 0);
+        });
       }
     }
+  };
+  constexpr int ALL = D / 8;                                     // operands of either side
+  auto scores = [&](int buf, uint32_t tags) __attribute__((always_inline)) {
+    products<ALL, FEED>([&](int i) __attribute__((always_inline)) { return read_k(tiles[buf][0][i % 4], i / 4); },
+                        [&](int i, const h8& x) __attribute__((always_inline)) { score(i % 4, i / 4, x); });
+    scores_rest(buf, tags);
+  };
+  auto values = [&](int buf, uint32_t tags) __attribute__((always_inline)) {
+    weigh();
+    products<ALL, FEED>([&](int i) __attribute__((always_inline)) { return read_v(buf, i); },
+                        [&](int i, const h8& x) __attribute__((always_inline)) { value(i, x); });
+    values_rest(buf, tags);
+  };
+  uint32_t now = 0, soon = 0;                                    // tags of this step's pages and of the next's
+  int k = 0;                                                     // number of its first entry in the part
+  auto step = [&](int buf, int e) __attribute__((always_inline)) {
+    const uint32_t later = tags_of(k + 8);
+    scores(buf, now);
+    convert(buf ^ 1, soon, k + 4);
+    load(later, k + 8);
+    look_ahead(k);
+    softmax(now, k, e);
+    values(buf, now);
     k += 4;
     now = soon;
     soon = later;
@@ -238,7 +282,6 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   // sums is made again with zeros in their place.
   for (int walk = 0; walk < 2; ++walk) {
     E = 0;
-    k = 0;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       m[t] = M_NONE;
@@ -247,7 +290,8 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) acc[t][mb] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    if (e0 < e1) {
+    if (e0 < e1) {                                               // uniform
+      k = 0;
       now = tags_of(0);
       soon = tags_of(4);
       load(now, 0);
