@@ -133,13 +133,8 @@ template <int D> struct PageRaw {
   float s0, s1;                        // INT4: its channels' scale; residual: both
 };
 
-template <typename T, bool STREAM> __device__ __forceinline__ T page_ld(const T* p) {
-  if constexpr (STREAM) return ld_nt(p);
-  else return *p;
-}
-
 // (Every branch sets every field: a field that some leave alone is kept in memory by the compiler.)
-template <int D, int KIND, bool STREAM>
+template <int D, int KIND>
 __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool v, int id, int tag, int lane) {
   const int64_t p = id < 0 ? 0 : id;                             // uniform, as the tag
   const u4 zero = {0u, 0u, 0u, 0u};
@@ -150,7 +145,7 @@ __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool
   } else if (KIND == PAGES_F16 || tag == IAK_TAG_FP16) {
     const u4* at = reinterpret_cast<const u4*>(v ? a.v_fp16 : a.k_fp16) + p * (PS * D / 8) + lane;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) r.x[j] = page_ld<u4, STREAM>(at + 64 * j);
+    for (int j = 0; j < D / 32; ++j) r.x[j] = at[64 * j];
     r.s0 = r.s1 = 0.f;
   } else if (KIND == PAGES_ALL && tag == IAK_TAG_INT4) {
     const uint8_t* page = reinterpret_cast<const uint8_t*>(v ? a.v_int4 : a.k_int4) + p * (PS * D / 2);
@@ -169,7 +164,7 @@ __device__ __forceinline__ void load_page(PageRaw<D>& r, const PageAttn& a, bool
                                                                                            : (v ? a.v_int4r : a.k_int4r);
     const u4* at = reinterpret_cast<const u4*>(pool) + p * (PS * D / 16) + lane;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) r.x[j] = j < D / 64 ? page_ld<u4, STREAM>(at + 64 * j) : zero;
+    for (int j = 0; j < D / 32; ++j) r.x[j] = j < D / 64 ? at[64 * j] : zero;
     r.s0 = r.s1 = 0.f;
     if (KIND == PAGES_ALL && tag == IAK_TAG_INT4_RESIDUAL) {
       const float* s = (v ? a.v_int4r_scale : a.k_int4r_scale) + 2 * p;
@@ -202,15 +197,13 @@ __device__ __forceinline__ h2 nibbles(uint32_t w, int byte) {
 }
 
 // The page into LDS as float16 rows (16-byte chunks at v_chunk); `lo`, written for wide pages alone: what is
-// left. id < 0: zeros. `rest`: kf or vf of the entry. Returns whether a value is infinite or NaN in this lane (CHECK).
-template <int D, int KIND, bool CHECK>
+// left. id < 0: zeros. `rest`: kf or vf of the entry. Returns whether a value is infinite or NaN in this lane.
+template <int D, int KIND>
 __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag, float rest, u4* hi, u4* lo, int lane) {
   h2 sum = {0, 0};                     // NaN once anything is not finite
   auto look = [&](const u4& x) {
-    if constexpr (CHECK) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum = __builtin_elementwise_fma(as_h2(x[i]), h2{0, 0}, sum);
-    }
+    for (int i = 0; i < 4; ++i) sum = __builtin_elementwise_fma(as_h2(x[i]), h2{0, 0}, sum);
   };
   if (id < 0) {
 #pragma unroll
@@ -285,7 +278,7 @@ __device__ __forceinline__ bool store_page(const PageRaw<D>& r, int id, int tag,
     if (tag == IAK_TAG_FP8) bytes([](uint32_t x, uint32_t& l, uint32_t& h) __attribute__((always_inline)) { fp8x4_to_f16(x, l, h); });
     else bytes([](uint32_t x, uint32_t& l, uint32_t& h) __attribute__((always_inline)) { i8x4_to_f16(x, l, h); });
   }
-  return CHECK && !((float)sum[0] + (float)sum[1] == 0.f);
+  return !((float)sum[0] + (float)sum[1] == 0.f);
 }
 
 // --------------------------------------------------------------------------- //

@@ -335,8 +335,8 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
         const PageEntry x = page_entry<D, KIND>(b, b.table + kvrow * b.W, e + w, e1);
         const int id = (int)uniform((uint32_t)x.id), tag = (int)uniform((uint32_t)x.tag);
         PageRaw<D> r;
-        load_page<D, KIND, false>(r, b, true, id, tag, lane);
-        const bool bad = store_page<D, KIND, true>(r, id, tag, u2f(uniform(f2u(x.vf))), tiles[0][0][w], rest[0][0][w], lane);
+        load_page<D, KIND>(r, b, true, id, tag, lane);
+        const bool bad = store_page<D, KIND>(r, id, tag, u2f(uniform(f2u(x.vf))), tiles[0][0][w], rest[0][0][w], lane);
         const bool some = __builtin_amdgcn_ballot_w64(bad) != 0;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (some) put_aside<D>(tiles[0][0][w], aside + w * PAGE, lane);

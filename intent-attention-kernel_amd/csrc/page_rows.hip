@@ -400,9 +400,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
       const PageEntry x = page_entry<D, KIND>(a, row, e, w1);
       const int id = __builtin_amdgcn_readfirstlane(x.id), tag = __builtin_amdgcn_readfirstlane(x.tag);
       PageRaw<D> r;
-      load_page<D, KIND, false>(r, a, true, id, tag, lane);
+      load_page<D, KIND>(r, a, true, id, tag, lane);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const bool bad = store_page<D, KIND, true>(r, id, tag, u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(x.vf))), kt,
+      const bool bad = store_page<D, KIND>(r, id, tag, u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(x.vf))), kt,
                                                  kt + PS * D / 8, lane);
       if (!__builtin_amdgcn_ballot_w64(bad)) continue;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
