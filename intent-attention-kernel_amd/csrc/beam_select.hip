@@ -195,7 +195,7 @@ template <typename T, int PER>
 __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamArgs a) {
   __shared__ uint2 table[32];
   __shared__ uint64_t lists[BEAM_WAVES][BEAM_LIST];
-  __shared__ Raw8<T> listed[BEAM_WAVES][PER][64];
+  __shared__ __attribute__((aligned(16))) Raw8<T> listed[BEAM_WAVES][PER][64];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   if (t < 32) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(t * 0.03125));
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
   __shared__ bool ended[BEAM_MOST_BEAMS];
   __shared__ uint64_t stage_at[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];       // of the lists, then the wave's best so far
   __shared__ uint32_t stage_index[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // k V + v
-  __shared__ uint8_t stage_head[BEAM_WAVES][MERGE_STAGE + 1];
+  __shared__ __attribute__((aligned(16))) uint8_t stage_head[BEAM_WAVES][MERGE_STAGE + 1];
   const int t = threadIdx.x, b = blockIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), n = a.n;
   const int64_t row0 = (int64_t)b * a.K;
   const int lists = a.K * a.segments, each = MERGE_STAGE / n;    // of the request, and in a wave's stage
