@@ -14,6 +14,12 @@
 // to more than 32 bits: with offsets off by 2^-24 of 30 or so, two in some 10^5 neighbours would
 // change places. exp(x) = 2^(k/32) e^r with |r| <= ln 2 / 64: the table's 2^(k/32) and the sum in
 // 64 bits, r and e^r - 1 in 32, off by some 2^-31, so that a normaliser is off by some 1e-9.
+//
+// What bounds it: the logits are read once (64 x 8 x 131,072 in bfloat16, a tenth of the beams at their end: 121 MB,
+// 24 us at a copy's rate), and an exponential to 1e-9 is 15 vector instructions a logit, 28 us of
+// the card's; the part kernel takes 53, what is left being its first group (nothing to overlap with), the list's
+// upkeep and the ends of the waves. The merge takes 11 (16 steps of some 0.2 us, and the loads and
+// logarithms before them); two requests x 4 beams x 32,000: 7.3 + 6.1 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -339,36 +345,36 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
 }
 
 // Candidates in LDS, a wave's at a time; a value's order as an unsigned number, 0: none.
-constexpr int MERGE_STAGE = 1024;
+constexpr int MERGE_STAGE = 1024, MERGE_WAVES = 8, MERGE_THREADS = 64 * MERGE_WAVES;
 __device__ __forceinline__ uint64_t ordered(double x) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
   return b ^ (b >> 63 ? ~0ull : 1ull << 63);
 }
 __device__ __forceinline__ double unordered(uint64_t o) { return __builtin_bit_cast(double, o ^ (o >> 63 ? 1ull << 63 : ~0ull)); }
 
-__global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs a) {
+__global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArgs a) {
   __shared__ double norms[BEAM_MOST_BEAMS];                      // normaliser; NaN: the beam is out of the search
   __shared__ float scores[BEAM_MOST_BEAMS];
   __shared__ bool ended[BEAM_MOST_BEAMS];
-  __shared__ uint64_t stage_at[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];       // of the lists, then the wave's best so far
-  __shared__ uint32_t stage_index[BEAM_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // k V + v
-  __shared__ __attribute__((aligned(16))) uint8_t stage_head[BEAM_WAVES][MERGE_STAGE + 1];
+  __shared__ uint64_t stage_at[MERGE_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];       // of the lists, then the wave's best so far
+  __shared__ uint32_t stage_index[MERGE_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // k V + v
+  __shared__ __attribute__((aligned(16))) uint8_t stage_head[MERGE_WAVES][MERGE_STAGE + 1];
   const int t = threadIdx.x, b = blockIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), n = a.n;
   const int64_t row0 = (int64_t)b * a.K;
   const int lists = a.K * a.segments, each = MERGE_STAGE / n;    // of the request, and in a wave's stage
   const bool once = lists <= each;                               // uniform: one wave merges, and all load for it
-  constexpr int OWN = MERGE_STAGE / BEAM_THREADS;
+  constexpr int OWN = MERGE_STAGE / MERGE_THREADS;
   uint64_t keys[OWN];                                            // on their way meanwhile; of beams that are out: anything
   if (once) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      const int e = t + i * BEAM_THREADS;
+      const int e = t + i * MERGE_THREADS;
       keys[i] = a.best[row0 * a.segments * n + (e < lists * n ? e : 0)];
     }
   }
 
   // 16 threads a beam: its normaliser out of the segments' sums
-  for (int k0 = 0; k0 < a.K; k0 += BEAM_THREADS / 16) {          // uniform
+  for (int k0 = 0; k0 < a.K; k0 += MERGE_THREADS / 16) {          // uniform
     const int k = k0 + t / 16;
     const bool there = k < a.K;
     const int64_t row = row0 + (there ? k : 0);
@@ -437,10 +443,12 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
   // n times. A lane has every 64th list.
   auto merge = [&](int count, uint64_t* to_at, uint32_t* to_index) {
     wave_sync();
-    for (int l = lane; l < count; l += 64) head[l] = 0;
-    uint64_t best = 0;
-    uint32_t number = 0;
-    int from = 0;
+    const bool single = count <= 64;                             // a list a lane: its next head is read a step ahead
+    if (!single)
+      for (int l = lane; l < count; l += 64) head[l] = 0;
+    uint64_t best = 0, second = 0;
+    uint32_t number = 0, second_number = 0;
+    int from = 0, taken = 0;                                     // list of the lane's best; of a single list: how many are gone
     auto look = [&]() {
       best = 0;
       number = 0;
@@ -452,7 +460,17 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
         if (v > best || (v == best && v != 0 && i < number)) { best = v; number = i; from = l; }
       }
     };
-    look();
+    auto ahead = [&]() {                                         // entry taken + 1 of the lane's list
+      const bool more = lane < count && taken + 1 < n;
+      const int e = more ? lane * n + taken + 1 : 0;
+      second = at[e];
+      second_number = index[e];
+      if (!more) second = 0;
+    };
+    if (single) {
+      if (lane < count) { best = at[lane * n]; number = index[lane * n]; }
+      ahead();
+    } else look();
     uint64_t kept_at = 0;
     uint32_t kept_index = 0;
     for (int r = 0; r < n; ++r) {
@@ -471,8 +489,15 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
       const uint32_t i0 = (uint32_t)__builtin_amdgcn_readlane((int)number, owner);
       if (lane == r) { kept_at = ((uint64_t)high << 32) | a0; kept_index = i0; }
       if (lane == owner) {
-        ++head[from];
-        look();
+        if (single) {
+          best = second;
+          number = second_number;
+          ++taken;
+          ahead();
+        } else {
+          ++head[from];
+          look();
+        }
       }
     }
     wave_sync();
@@ -482,14 +507,14 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
   if (once) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      const int e = t + i * BEAM_THREADS;
+      const int e = t + i * MERGE_THREADS;
       if (e < lists * n) candidate(e / n, e % n, keys[i], stage_at[0][e], stage_index[0][e]);
     }
     __syncthreads();
     if (wave == 0) merge(lists, at + MERGE_STAGE, index + MERGE_STAGE);
   } else {
     bool some = false;
-    for (int l0 = wave * each; l0 < lists; l0 += BEAM_WAVES * each) {
+    for (int l0 = wave * each; l0 < lists; l0 += MERGE_WAVES * each) {
       const int count = lists - l0 < each ? lists - l0 : each, total = count * n;
       for (int e0 = lane; e0 < total; e0 += 64 * OWN) {
 #pragma unroll
@@ -505,7 +530,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_merge_kernel(const BeamArgs
       some = true;
     }
   }
-  const int rounds = (lists + each - 1) / each, waves = rounds < BEAM_WAVES ? rounds : BEAM_WAVES;
+  const int rounds = (lists + each - 1) / each, waves = rounds < MERGE_WAVES ? rounds : MERGE_WAVES;
   if (waves > 1) {                                               // uniform
     __syncthreads();
     if (wave == 0) {
@@ -528,12 +553,15 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // Chunks of 512 logits that a wave has under way, twice: as many bytes of either type.
 constexpr int beam_per_of(int bytes) { return bytes == 4 ? 2 : 4; }
 
-// Groups of logits a segment: some 16 waves a CU, and no more lists than the merge takes in a few rounds.
+// Groups of logits a segment. 4,096 segments in all are 16 waves a CU: 64 requests x 8 beams x 131,072 in
+// bfloat16 take 71.6 us, with 2,048 segments 78.8 and with 8,192 79.6. No more lists than the merge's waves hold at
+// once, for every further round of them costs count steps: 16 beams, count 32, 131,072 tokens: 56.5 us, with
+// twice as many entries 65, with half 88 (16 beams leave few waves then).
 int beam_per(const iak_beam_select_args& a) {
   const int64_t rows = (int64_t)a.batch * a.beams, group = 512 * beam_per_of(a.dtype == IAK_DTYPE_F32 ? 4 : 2);
   const int64_t groups = (a.vocab + group - 1) / group;
   int64_t segments = 4096 / rows;
-  const int64_t most = 16384 / ((int64_t)a.beams * a.count);
+  const int64_t most = MERGE_STAGE * MERGE_WAVES / ((int64_t)a.beams * a.count);
   if (segments > most) segments = most;
   if (segments > groups) segments = groups;
   if (segments < 1) segments = 1;
@@ -574,7 +602,7 @@ hipError_t launch_beam_select(const iak_beam_select_args& a, void* workspace, hi
   if (a.dtype == IAK_DTYPE_F32) launch_part<float>(k, stream);
   else if (a.dtype == IAK_DTYPE_F16) launch_part<_Float16>(k, stream);
   else launch_part<__bf16>(k, stream);
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((uint32_t)a.batch), dim3(BEAM_THREADS), 0, stream, k);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((uint32_t)a.batch), dim3(MERGE_THREADS), 0, stream, k);
   return hipGetLastError();
 }
 

@@ -12,6 +12,11 @@
 //           of the tokens in the lane that the operand needs them in
 // K and V are exact codes, with their scales in the scores and the weights; INT4 codes times their
 // groups' scales, which need more bits than float16 has, take two products.
+//
+// What bounds it: the pages' bytes. Four queries of 16 sequences over up to 16,384 tokens of mixed precision (32
+// heads over 8 of 128, 435 MB) take 104 us and 7 of merge, 4.2 TB/s; of float16 pages alone 123 us, 5.9
+// TB/s; equal lengths, mixed, 103. A short row waits for length, entry, tag, page and the waves' sums in turn:
+// 3 queries over 500 tokens 8 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -274,7 +279,9 @@ template <int D> __device__ __forceinline__ void row_remember(Seen16& x, const u
     }
 }
 
-// Waves a SIMD: what the registers hold of rings and queries in two parts.
+// Waves a SIMD: what the registers hold of rings and queries in two parts. All precisions: two (16 x 4 queries
+// over up to 16,384 tokens 108 us; three spill 62 registers, 160); float16 and bytes alone: three or two (122.9 and 122.8
+// us, 78.2 and 75.5).
 template <bool QF32, int KIND> constexpr int row_waves_per_simd() { return QF32 || KIND == PAGES_ALL ? 2 : 3; }
 
 template <int D, bool QF32, int KIND>
