@@ -18,8 +18,8 @@
 // What bounds it: the logits are read once (64 x 8 x 131,072 in bfloat16, a tenth of the beams at their end: 121 MB,
 // 24 us at a copy's rate), and an exponential to 1e-9 is 15 vector instructions a logit, 28 us of
 // the card's; the part kernel takes 53, what is left being its first group (nothing to overlap with), the list's
-// upkeep and the ends of the waves. The merge takes 11 (16 steps of some 0.2 us, and the loads and
-// logarithms before them); two requests x 4 beams x 32,000: 7.3 + 6.1 us.
+// upkeep and the ends of the waves. The merge takes 8 (16 steps of some 0.1 us, and the loads and
+// logarithms before them); two requests x 4 beams x 32,000: 7.2 + 5.9 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

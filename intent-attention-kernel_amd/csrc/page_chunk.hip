@@ -7,8 +7,8 @@
 // one barrier a step.
 //
 // What bounds it: nothing alone. 2,048 queries over 8,192 tokens of float16 pages (32 heads over 8 of 128) take
-// 254 us, 947 TFLOP/s, where a large product reaches 1,338: the matrix cores are busy 40 % of the cycles, the vector
-// instructions (softmax) 23 %, the LDS 25 %, and two waves a SIMD do not fill each other's waits. Over 16,384
+// 254 us, 947 TFLOP/s, where a large product reaches 1,338: the matrix cores are busy 44 % of the cycles, the vector
+// instructions (softmax) 26 %, the LDS 28 %, and two waves a SIMD do not fill each other's waits. Over 16,384
 // tokens of mixed pages, two sequences: 1.73 ms, 584 TFLOP/s; the vector instructions (codes to float16, multipliers in
 // the softmax) and the wide pages' second products take as long as the first products. Tried and slower: the
 // workgroup's halves in turns, one's products beside the other's softmax (chunks of mixed pages 2,270 us for 1,700,
