@@ -43,6 +43,8 @@ iak_status validate_beam_select(const iak_beam_select_args* a) {
     return fail(IAK_EINVAL, "batch %d x beams %d x vocab %d: rows and candidates have int32 numbers", a->batch, a->beams, a->vocab);
   if (a->count > (int64_t)a->beams * a->vocab)
     return fail(IAK_EINVAL, "count %d of %d x %d candidates", a->count, a->beams, a->vocab);
+  // a launch has fewer than 2^32 threads, and the merge 512 for a request
+  if (a->batch > 0x7FFFFF) return fail(IAK_EINVAL, "too many requests for one call (%d)", a->batch);
   if (a->dtype < 0 || a->dtype > 2) return fail(IAK_EINVAL, "bad dtype %d", a->dtype);
   if (a->finished && (a->end_token < 0 || a->end_token >= a->vocab))
     return fail(IAK_EINVAL, "end_token %d outside the vocabulary of %d", a->end_token, a->vocab);

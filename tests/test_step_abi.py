@@ -27,3 +27,15 @@ def test_argument_blocks_match_the_header(cname, pyname):
     assert int(got["size"]) == ctypes.sizeof(S)
     for f in fields:
         assert int(got[f]) == getattr(S, f).offset, f
+
+
+def test_more_requests_than_a_launch_has_room_for():
+    a = N.BeamSelectArgs()
+    a.beams, a.vocab, a.count = 1, 8, 1
+    a.logits = a.scores = a.out_scores = a.out_parents = a.out_tokens = 1 << 20   # not looked at
+    a.stride_b = a.stride_k = 8
+    a.batch = 0x7FFFFF
+    assert N.beam_select_workspace(a) > 0
+    a.batch = 0x800000
+    with pytest.raises(ValueError, match="too many requests"):
+        N.beam_select_workspace(a)
