@@ -28,9 +28,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, count: Optional[i
     Returns (scores float32, parents int32, tokens int32), each [B, count], the best first and equal
     ones in the order of k V + v; parents are rows of the logits as [B K, V]: b K + k. Candidates are
     compared in 64 bits. K is at most 256."""
-    if logits.dim() != 3:
-        raise ValueError(f"logits must have shape [B, K, V], got {tuple(logits.shape)}")
-    B, K, V = logits.shape
+    shape = logits.shape
+    if len(shape) != 3:
+        raise ValueError(f"logits must have shape [B, K, V], got {tuple(shape)}")
+    B, K, V = shape
     if logits.dtype not in _DT:
         raise ValueError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
     if scores.shape != (B, K) or scores.dtype is not torch.float32:
@@ -44,13 +45,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, count: Optional[i
     end = 0 if end_token is None else int(end_token)
     _check_int32(batch=B, beams=K, vocab=V, count=n, end_token=end)
     dev = _device("beam choice", logits, scores, finished)
-    if logits.stride(-1) != 1:
+    stride_b, stride_k, stride_v = logits.stride()
+    if stride_v != 1:
         logits = logits.contiguous()
+        stride_b, stride_k, _ = logits.stride()
     scores = scores.contiguous()
     finished = None if finished is None else finished.contiguous()
-    out = (torch.empty((B, max(n, 0)), dtype=torch.float32, device=dev),
-           *(torch.empty((B, max(n, 0)), dtype=torch.int32, device=dev) for _ in range(2)))
-    a = N.BeamSelectArgs(B, K, V, n, logits.data_ptr(), _DT[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(),
+    at = torch.empty((B, max(n, 0)), dtype=torch.float32, device=dev)
+    parents, tokens = (torch.empty_like(at, dtype=torch.int32) for _ in range(2))
+    out = (at, parents, tokens)
+    a = N.BeamSelectArgs(B, K, V, n, logits.data_ptr(), _DT[logits.dtype], stride_b, stride_k, scores.data_ptr(),
                          None if finished is None else finished.data_ptr(), end, *(t.data_ptr() for t in out))
     size = N.beam_select_workspace(a)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)

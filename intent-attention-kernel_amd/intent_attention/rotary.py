@@ -49,20 +49,24 @@ def append_rotated_tokens(k: torch.Tensor, v: torch.Tensor, pools: Union[PagePoo
     rounded as ``append_mxfp4_tokens`` rounds.
     Returns the rotated queries in q's dtype (in ``q_out``, which may be q), zero for i >= q_lens[b]. Inference
     only: nothing records gradients."""
-    if k.dim() != 4 or k.shape != v.shape:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape:
         raise ValueError(f"k and v must have one shape [B, L, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype not in _DT or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be float16, bfloat16 or float32, got {k.dtype} and {v.dtype}")
-    B, L, Hkv, D = k.shape
+    B, L, Hkv, D = shape
     packed = isinstance(pools, MxFp4Pools)
     if not packed and (pools.k_fp16 is None or pools.v_fp16 is None):
         raise ValueError("PagePools without float16 pages take no tokens")
     written = tuple(pools.tensors().values()) if packed else (pools.k_fp16, pools.v_fp16)
     dev = _device("rotated append", k, v, page_table, valid_tokens, inv_freq, q, q_out, q_lens, positions, page_tags, *written)
-    if q is not None and (q.dim() != 4 or q.shape[:2] != (B, L) or q.shape[3] != D or q.dtype != k.dtype):
-        raise ValueError(f"q must be {k.dtype} [{B}, {L}, Hq, {D}], got {q.dtype} {tuple(q.shape)}")
-    if q is not None and (Hkv == 0 or q.shape[2] == 0 or q.shape[2] % Hkv):
-        raise ValueError(f"query heads {q.shape[2]} must be a multiple of page-table heads {Hkv}")
+    Hq = 0
+    if q is not None:
+        Hq = q.shape[2] if q.dim() == 4 else -1
+        if q.shape != (B, L, Hq, D) or q.dtype != k.dtype:
+            raise ValueError(f"q must be {k.dtype} [{B}, {L}, Hq, {D}], got {q.dtype} {tuple(q.shape)}")
+        if Hkv == 0 or Hq == 0 or Hq % Hkv:
+            raise ValueError(f"query heads {Hq} must be a multiple of page-table heads {Hkv}")
     if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32:
         raise ValueError(f"inv_freq must be float32 [R / 2], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     if positions is not None and (positions.shape != (B, L) or positions.dtype is not torch.int32):
@@ -76,13 +80,16 @@ def append_rotated_tokens(k: torch.Tensor, v: torch.Tensor, pools: Union[PagePoo
     else:
         W = _check_metadata(page_table, valid_tokens, q_lens, B, Hkv)
         NP = pools.k_fp16.shape[0] if pools.k_fp16.dim() else -1
-        for name, t in (("k_fp16", pools.k_fp16), ("v_fp16", pools.v_fp16)):
-            _check_pool(name, t, NP, (PAGE_SIZE, D), (torch.float16,))
+        for t in written:
+            if t.dtype is not torch.float16 or t.shape != (NP, PAGE_SIZE, D) or not t.is_contiguous():
+                _check_pool("k_fp16" if t is written[0] else "v_fp16", t, NP, (PAGE_SIZE, D), (torch.float16,))
         if page_tags is not None and (page_tags.shape != (NP,) or page_tags.dtype is not torch.int32 or not page_tags.is_contiguous()):
             raise ValueError(f"page_tags must be contiguous int32 [{NP}], got {page_tags.dtype} {tuple(page_tags.shape)}")
     _check_int32(count=L, fp16_tag=fp16_tag)
-    if k.stride(-1) != 1 or v.stride(-1) != 1:
+    k_stride, v_stride = k.stride(), v.stride()
+    if k_stride[3] != 1 or v_stride[3] != 1:
         k, v = k.contiguous(), v.contiguous()
+        k_stride, v_stride = k.stride(), v.stride()
     if q is None:
         if q_out is not None:
             raise ValueError("q_out without q")
@@ -90,7 +97,7 @@ def append_rotated_tokens(k: torch.Tensor, v: torch.Tensor, pools: Union[PagePoo
         if q.stride(-1) != 1 and q_out is not q:
             q = q.contiguous()
         if q_out is None:
-            q_out = torch.empty((B, L, q.shape[2], D), dtype=q.dtype, device=dev)
+            q_out = torch.empty((B, L, Hq, D), dtype=q.dtype, device=dev)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(-1) != 1:
             raise ValueError(f"q_out must be {q.dtype} {tuple(q.shape)} with a unit last stride, got {q_out.dtype} "
                              f"{tuple(q_out.shape)}")
@@ -98,15 +105,15 @@ def append_rotated_tokens(k: torch.Tensor, v: torch.Tensor, pools: Union[PagePoo
     q_lens = None if q_lens is None else q_lens.contiguous()
     if positions is not None and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    a = N.RotaryAppendArgs(B, L, 0 if q is None else q.shape[2], Hkv, D, 2 * inv_freq.shape[0], int(bool(interleaved)), PAGE_SIZE, W, NP,
+    a = N.RotaryAppendArgs(B, L, Hq, Hkv, D, 2 * inv_freq.shape[0], int(bool(interleaved)), PAGE_SIZE, W, NP,
                            _DT[k.dtype])
     if q is not None:
         a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
         a.q_stride_b, a.q_stride_t, a.q_stride_h, _ = q.stride()
         a.q_out_stride_b, a.q_out_stride_t, a.q_out_stride_h, _ = q_out.stride()
     a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_stride_b, a.k_stride_t, a.k_stride_h, _ = k.stride()
-    a.v_stride_b, a.v_stride_t, a.v_stride_h, _ = v.stride()
+    a.k_stride_b, a.k_stride_t, a.k_stride_h, _ = k_stride
+    a.v_stride_b, a.v_stride_t, a.v_stride_h, _ = v_stride
     a.inv_freq, a.positions = inv_freq.data_ptr(), _ptr(positions)
     a.position_stride_b = 0 if positions is None else positions.stride(0)
     a.page_table, a.valid_tokens, a.q_lens = page_table.data_ptr(), valid_tokens.data_ptr(), _ptr(q_lens)
