@@ -909,7 +909,7 @@ iak_status iak_rotary_append(const iak_rotary_append_args* args, void* stream);
  * Equal candidates come in the order of k * vocab + v, those of -inf too. Candidates are compared
  * in 64 bits, with the beams' normalisers off by about 1e-9 (they decide between different beams;
  * those of one beam come in the order of their logits) and rounded to float32 at the end.
- * 1 <= count <= 64, count <= beams * vocab < 2^31, beams <= 256. Workspace:
+ * 1 <= count <= 64, count <= beams * vocab < 2^31, beams <= 256, batch < 2^23. Workspace:
  * iak_beam_select_workspace bytes, 16-byte aligned, as it comes; calls that share one on different
  * streams race. */
 typedef struct {

@@ -62,3 +62,28 @@ def test_empty_table_of_long_rows():
     s = long_case(3, 12, 1, 16, 4, 128, 1600, "all")
     s.counts[:] = 0
     s.check()
+
+
+@pytest.mark.parametrize("shape,q_dtype", [((12, 1, 16, 4, 128, 1600), "float16"), ((4, 200, 8, 2, 64, 700), "bfloat16"), ((3, 70, 8, 2, 128, 500), "float32")])
+@pytest.mark.parametrize("mix", ["fp16", "all"])
+def test_infinite_values_in_parts(shape, q_dtype, mix):
+    """Infinities and NaN of V in pages that few rows list, some past their lengths: parts with and without them are merged."""
+    s = long_case(sum(shape) + 1, *shape, mix, q_dtype, NP=400)
+    B, L, Hq, Hkv, D, W = shape
+    s.table %= 390                                               # the last ten pages: listed by hand
+    s.tags[390:] = [0, 0, 0, 0] + [0 if mix == "fp16" else t for t in (1, 3, 4, 5, 1, 0)]
+    s.host["v_fp16"][390, 3, 5], s.host["v_fp16"][391, 15, 0], s.host["v_fp16"][392, 0, D - 1] = np.inf, -np.inf, np.nan
+    s.host["v_fp16"][393] = np.inf
+    if mix == "all":
+        s.host["v_int8_scale"][394], s.host["v_fp8_scale"][395] = np.inf, np.nan
+        s.host["v_int4_scale"][396, 0], s.host["v_int4r_scale"][397, 1] = -np.inf, np.nan
+    s.valid[:] = np.maximum(s.valid, 200)
+    s.counts = -(-s.valid // 16).astype(np.int32)
+    for n, page in enumerate(range(390, 398)):
+        b, h = n % B, (n // B) % Hkv
+        entry = int(s.valid[b, h]) // 16 * (n + 1) // 9
+        s.table[b, h, entry] = page
+        s.table[(b + 1) % B, h, W - 1] = page                    # past most lengths
+    import intent_attention as ia
+    s.pools = ia.PagePools(int4_group=32, **{n: _t(x) for n, x in s.host.items()})
+    s.check()
