@@ -279,7 +279,6 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
         }
     }
     if (full || (count - seen) * 2 > n) {                        // at fewer new ones the search costs more than it saves: 66.6 and 63.8 us
-      bool ranked = false;
       if (full) {                                                // again, the list ranked as often as it is full
         count = before;
 #pragma unroll
@@ -294,19 +293,17 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
               count = rank_list(list, count, n, 0, lane);
               bound = list[n - 1];
               least = unordered((uint32_t)(bound >> 32));
-              ranked = true;
             }
           }
         }
       }
-      // what follows has higher numbers: of equal logits it comes after those that are in the list
-      uint32_t most = wave_nth(highest, n, reach);
+      // n of the list's logits reach `reach`, those equal to the n-th among them; what follows has higher numbers,
+      // so that of equal ones it comes after those that are in the list and has to be above its n-th
+      const uint32_t nth = (uint32_t)(bound >> 32), most = wave_nth(highest, n, reach);
       seen = count;
-      if (ranked && (uint32_t)(bound >> 32) + 1 > most) most = (uint32_t)(bound >> 32) + 1;
-      if (most > reach) {
-        reach = most;
-        least = level(reach);
-      }
+      if (most > reach) reach = most;
+      if (nth > reach) reach = nth;
+      least = level(reach > nth ? reach : nth + 1);              // nth 0: none was ranked yet
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) x[i] = next[i];
