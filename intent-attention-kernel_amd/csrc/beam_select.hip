@@ -129,9 +129,11 @@ template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* row,
   return r;
 }
 
-// exp(x) added up in 64 bits, for |x| up to some 600 (below that: as there). k = 32 x / ln 2 rounded, as the
+// exp(x) added up in 64 bits, for x up to ADD_EXP_MOST (from some 710 on the exponent's bits would run over, with no
+// sign of it in the sum) and down to -600 (below that: as there). k = 32 x / ln 2 rounded, as the
 // low bits of a float past 2^23; the table's entry j has -j 2^15 in its high word, so that k 2^15
 // makes it 2^(k/32).
+constexpr float ADD_EXP_MOST = 600.f;
 __device__ __forceinline__ void add_exp(float x, const uint2* table, double& sum) {
   constexpr float TURN = 46.166241308446828f, MAGIC = 12582912.f;   // 32 / ln 2, 1.5 2^23
   constexpr double STEP = 0.021660849392498290;                     // ln 2 / 32
@@ -318,10 +320,10 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
   double base = 0;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-  if (!(sum > 1e-40 && sum < 1e40)) {
-    // Logits too large or too small, all of them: once more from the largest, from which all that
+  const float most = count ? unordered((uint32_t)(list[0] >> 32)) : -__builtin_inff();
+  if (!(most <= ADD_EXP_MOST && sum > 1e-40 && sum < 1e40)) {
+    // One logit too large, or all of them too small: once more from the largest, from which all that
     // matter differ by less than half of it, so that the difference is exact.
-    const float most = count ? unordered((uint32_t)(list[0] >> 32)) : -__builtin_inff();
     base = most;
     sum = 0;
     if (most > -__builtin_inff()) {

@@ -1,4 +1,4 @@
-"""The beam choice where its lists fill with equal logits."""
+"""The beam choice where its lists fill with equal logits, and where one logit is far above the others."""
 import numpy as np
 import pytest
 
@@ -40,3 +40,31 @@ def test_next_numbers_above_many_equal(low):
         for count in (4, 17, 64):
             _check(rows[:1].view(1, 1, V), torch.tensor([[0.0]]), count)
             _check(rows[1:].view(1, 1, V), torch.tensor([[0.0]]), count)
+
+
+LARGE = [89.0, 599.0, 601.0, 709.0, 711.0, 800.0, 1000.0, 1400.0, 1419.6, 2000.0, 2839.0, 2848.0, 2900.0, 28391.0, 60000.0, 1e9]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", LARGE)
+def test_one_large_logit(top, dtype):
+    import torch
+    if dtype == "float16" and top > 65504:
+        pytest.skip("past float16's range")
+    for V in (1000, 32000):
+        x = torch.zeros(3, V)
+        x[0, V // 3] = top
+        x[1] = torch.randn(V, generator=torch.Generator().manual_seed(V))
+        x[1, V - 1] = top
+        x[2, 0] = x[2, V // 2] = top
+        x = x.to(getattr(torch, dtype))
+        _check(x.view(1, 3, V), torch.tensor([[-5.0, -4.5, -6.0]]), 8)
+        _check(x.view(3, 1, V), torch.tensor([[-5.0], [0.0], [-1.0]]), 5)
+
+
+@pytest.mark.parametrize("shift", [711.0, 1419.6, 2839.0, 2839.13, 28391.0])
+def test_rows_at_the_turns_of_the_exponent(shift):
+    """Rows all of whose logits lie where 2^(32 x / ln 2) would come round again."""
+    import torch
+    x = torch.randn(2, 2, 5000, generator=torch.Generator().manual_seed(1)) + shift
+    _check(x, torch.tensor([[-1.0, -2.0], [-1.0, -1.0]]), 9)
