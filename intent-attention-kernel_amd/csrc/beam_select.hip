@@ -1,7 +1,7 @@
 // A beam search's choice on gfx950: of each request's beams x vocabulary the `count` best
 // continuations,
 //   candidate (k, v) = scores[k] + logits[k, v] - log sum_u exp(logits[k, u]),
-// best first, ties to the lowest k V + v.
+// best first, ties to the lowest beam, of one beam's to the largest logit, then to the lowest token.
 //
 //   beam_part_kernel   a wave streams a segment of one row of logits, once: its sum of exponentials,
 //                      and its `count` best by (logit, index), which no offset of the row changes.
@@ -343,7 +343,9 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
   if (lane == 0) a.norms[part] = make_double2(base, sum);
 }
 
-// Candidates in LDS, a wave's at a time; a value's order as an unsigned number, 0: none.
+// Candidates in LDS, a wave's at a time; a value's order as an unsigned number, 0: none. Equal values come in the
+// order of their beams, within a beam in that of the logits (which 64 bits of the value need not tell apart), then
+// of the numbers.
 constexpr int MERGE_STAGE = 1024, MERGE_WAVES = 8, MERGE_THREADS = 64 * MERGE_WAVES;
 __device__ __forceinline__ uint64_t ordered(double x) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
@@ -357,6 +359,7 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
   __shared__ bool ended[BEAM_MOST_BEAMS];
   __shared__ uint64_t stage_at[MERGE_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];       // of the lists, then the wave's best so far
   __shared__ uint32_t stage_index[MERGE_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // k V + v
+  __shared__ uint32_t stage_logit[MERGE_WAVES][MERGE_STAGE + BEAM_MOST_COUNT];    // in their order
   __shared__ __attribute__((aligned(16))) uint8_t stage_head[MERGE_WAVES][MERGE_STAGE + 1];
   const int t = threadIdx.x, b = blockIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), n = a.n;
   const int64_t row0 = (int64_t)b * a.K;
@@ -421,12 +424,14 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
   // n of which segment 0 stands for.
   uint64_t* at = stage_at[wave];
   uint32_t* index = stage_index[wave];
+  uint32_t* logit = stage_logit[wave];
   uint8_t* head = stage_head[wave];
-  auto candidate = [&](int list, int j, uint64_t key, uint64_t& value, uint32_t& number) {
+  auto candidate = [&](int list, int j, uint64_t key, uint64_t& value, uint32_t& number, uint32_t& order) {
     const int k = list / a.segments, s = list - k * a.segments;
     const double norm = norms[k], score = scores[k];
     value = 0;
     number = 0;
+    order = 0;
     if (ended[k] || !(norm == norm)) {
       if (s != 0 || j >= a.V) return;
       const bool last = norm == norm;
@@ -435,43 +440,44 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
       return;
     }
     if (key == 0) return;
-    value = ordered(score + ((double)unordered((uint32_t)(key >> 32)) - norm));   // the score last, which a large normaliser would swallow
+    order = (uint32_t)(key >> 32);
+    value = ordered(score + ((double)unordered(order) - norm));   // the score last, which a large normaliser would swallow
     number = (uint32_t)(k * a.V) + ~(uint32_t)key;
   };
-  // The n best of `count` lists in the stage, of list l at n l, each in order, to `to`: the best head,
+  // The n best of `count` lists in the stage, of list l at n l, each in order, behind it: the best head,
   // n times. A lane has every 64th list.
-  auto merge = [&](int count, uint64_t* to_at, uint32_t* to_index) {
+  const uint32_t V = (uint32_t)a.V;
+  auto merge = [&](int count) {
     wave_sync();
     const bool single = count <= 64;                             // a list a lane: its next head is read a step ahead
     if (!single)
       for (int l = lane; l < count; l += 64) head[l] = 0;
     uint64_t best = 0, second = 0;
-    uint32_t number = 0, second_number = 0;
-    int from = 0, taken = 0;                                     // list of the lane's best; of a single list: how many are gone
+    int place = 0, from = 0;                                     // of the lane's best in the stage, and its list
     auto look = [&]() {
       best = 0;
-      number = 0;
       for (int l = lane; l < count; l += 64) {
-        const int j = head[l];
+        const int j = head[l], e = l * n + j;
         if (j >= n) continue;
-        const uint64_t v = at[l * n + j];
-        const uint32_t i = index[l * n + j];
-        if (v > best || (v == best && v != 0 && i < number)) { best = v; number = i; from = l; }
+        const uint64_t v = at[e];
+        bool wins = v > best;
+        if (v == best && v != 0) {
+          const uint32_t i = index[e], i0 = index[place], o = logit[e], o0 = logit[place];
+          wins = i / V == i0 / V && o != o0 ? o > o0 : i < i0;
+        }
+        if (wins) { best = v; place = e; from = l; }
       }
     };
-    auto ahead = [&]() {                                         // entry taken + 1 of the lane's list
-      const bool more = lane < count && taken + 1 < n;
-      const int e = more ? lane * n + taken + 1 : 0;
-      second = at[e];
-      second_number = index[e];
+    auto ahead = [&]() {                                         // the entry behind the lane's best
+      const bool more = lane < count && place + 1 < (lane + 1) * n;
+      second = at[more ? place + 1 : 0];
       if (!more) second = 0;
     };
     if (single) {
-      if (lane < count) { best = at[lane * n]; number = index[lane * n]; }
+      if (lane < count) { place = lane * n; best = at[place]; }
       ahead();
     } else look();
-    uint64_t kept_at = 0;
-    uint32_t kept_index = 0;
+    int kept = -1;
     for (int r = 0; r < n; ++r) {
       const uint32_t high = wave_most((uint32_t)(best >> 32));
       bool wins = (uint32_t)(best >> 32) == high;
@@ -479,19 +485,22 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
       if (winners & (winners - 1)) {
         const uint32_t low = wave_most(wins ? (uint32_t)best : 0);
         wins = wins && (uint32_t)best == low;
+        // the numbers of the first beam among them, of these the largest logit, of these the lowest number
+        const uint32_t number = index[place], order = logit[place];
+        const uint32_t past = (~wave_most(wins ? ~number : 0) / V + 1) * V;
+        wins = wins && number < past;
+        const uint32_t top = wave_most(wins ? order : 0);
+        wins = wins && order == top;
         const uint32_t first = wave_most(wins ? ~number : 0);
         wins = wins && ~number == first;
         winners = __builtin_amdgcn_ballot_w64(wins);
       }
-      const int owner = __builtin_ctzll(winners);
-      const uint32_t a0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, owner);
-      const uint32_t i0 = (uint32_t)__builtin_amdgcn_readlane((int)number, owner);
-      if (lane == r) { kept_at = ((uint64_t)high << 32) | a0; kept_index = i0; }
+      const int owner = __builtin_ctzll(winners), won = __builtin_amdgcn_readlane(place, owner);
+      if (lane == r && high != 0) kept = won;                    // high 0: there is none (-inf is above it)
       if (lane == owner) {
         if (single) {
           best = second;
-          number = second_number;
-          ++taken;
+          if (second != 0) ++place;
           ahead();
         } else {
           ++head[from];
@@ -500,17 +509,20 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
       }
     }
     wave_sync();
-    if (lane < n) { to_at[lane] = kept_at; to_index[lane] = kept_index; }
+    const uint64_t kept_at = kept < 0 ? 0 : at[kept];
+    const uint32_t kept_index = kept < 0 ? 0 : index[kept], kept_logit = kept < 0 ? 0 : logit[kept];
+    wave_sync();
+    if (lane < n) { at[MERGE_STAGE + lane] = kept_at; index[MERGE_STAGE + lane] = kept_index; logit[MERGE_STAGE + lane] = kept_logit; }
     wave_sync();
   };
   if (once) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int e = t + i * MERGE_THREADS;
-      if (e < lists * n) candidate(e / n, e % n, keys[i], stage_at[0][e], stage_index[0][e]);
+      if (e < lists * n) candidate(e / n, e % n, keys[i], stage_at[0][e], stage_index[0][e], stage_logit[0][e]);
     }
     __syncthreads();
-    if (wave == 0) merge(lists, at + MERGE_STAGE, index + MERGE_STAGE);
+    if (wave == 0) merge(lists);
   } else {
     bool some = false;
     for (int l0 = wave * each; l0 < lists; l0 += MERGE_WAVES * each) {
@@ -521,11 +533,15 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
 #pragma unroll
         for (int i = 0; i < OWN; ++i) {
           const int e = e0 + 64 * i;
-          if (e < total) candidate(l0 + e / n, e % n, keys[i], at[e], index[e]);
+          if (e < total) candidate(l0 + e / n, e % n, keys[i], at[e], index[e], logit[e]);
         }
       }
-      if (some && lane < n) { at[total + lane] = at[MERGE_STAGE + lane]; index[total + lane] = index[MERGE_STAGE + lane]; }
-      merge(count + some, at + MERGE_STAGE, index + MERGE_STAGE);
+      if (some && lane < n) {
+        at[total + lane] = at[MERGE_STAGE + lane];
+        index[total + lane] = index[MERGE_STAGE + lane];
+        logit[total + lane] = logit[MERGE_STAGE + lane];
+      }
+      merge(count + some);
       some = true;
     }
   }
@@ -534,16 +550,20 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
     __syncthreads();
     if (wave == 0) {
       for (int w = waves - 1; w >= 0; --w)
-        if (lane < n) { at[w * n + lane] = stage_at[w][MERGE_STAGE + lane]; index[w * n + lane] = stage_index[w][MERGE_STAGE + lane]; }
-      merge(waves, at + MERGE_STAGE, index + MERGE_STAGE);
+        if (lane < n) {
+          at[w * n + lane] = stage_at[w][MERGE_STAGE + lane];
+          index[w * n + lane] = stage_index[w][MERGE_STAGE + lane];
+          logit[w * n + lane] = stage_logit[w][MERGE_STAGE + lane];
+        }
+      merge(waves);
     }
   }
   if (wave == 0 && lane < n) {
     const uint32_t i = index[MERGE_STAGE + lane];
-    const uint32_t k = i / (uint32_t)a.V;
+    const uint32_t k = i / V;
     a.out_scores[(int64_t)b * n + lane] = (float)unordered(at[MERGE_STAGE + lane]);
     a.out_parents[(int64_t)b * n + lane] = (int32_t)(row0 + k);
-    a.out_tokens[(int64_t)b * n + lane] = (int32_t)(i - k * (uint32_t)a.V);
+    a.out_tokens[(int64_t)b * n + lane] = (int32_t)(i - k * V);
   }
 }
 

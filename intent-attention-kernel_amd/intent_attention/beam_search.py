@@ -27,7 +27,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, count: Optional[i
     or which is not finished and has a logit that is NaN or +inf or none above -inf.
     Returns (scores float32, parents int32, tokens int32), each [B, count], the best first and equal
     ones in the order of k V + v; parents are rows of the logits as [B K, V]: b K + k. Candidates are
-    compared in 64 bits. K is at most 256, B below 2^23."""
+    compared in 64 bits; one beam's come in the order of their logits where 64 bits do not tell them apart. K is at
+    most 256, B below 2^23."""
     shape = logits.shape
     if len(shape) != 3:
         raise ValueError(f"logits must have shape [B, K, V], got {tuple(shape)}")

@@ -1,4 +1,5 @@
-"""The beam choice where its lists fill with equal logits, and where one logit is far above the others."""
+"""The beam choice where its lists fill with equal logits, where one logit is far above the others, and where 64 bits do not tell
+candidates apart."""
 import numpy as np
 import pytest
 
@@ -68,3 +69,23 @@ def test_rows_at_the_turns_of_the_exponent(shift):
     import torch
     x = torch.randn(2, 2, 5000, generator=torch.Generator().manual_seed(1)) + shift
     _check(x, torch.tensor([[-1.0, -2.0], [-1.0, -1.0]]), 9)
+
+
+@pytest.mark.parametrize("V", [3000, 70001])
+@pytest.mark.parametrize("scores", [[-1.0, -1.0], [-1.0, -0.5], [-1e9, -1e9], [3e9, 1e9]])
+def test_one_beams_candidates_come_by_logit(V, scores):
+    """Logits so close that the candidates are equal in 64 bits: a beam's come in the order of its logits, beams in theirs."""
+    import torch
+    import intent_attention as ia
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(2, V, generator=g) * (1e-20 if abs(scores[0]) < 10 else 1e-11)
+    x[:, ::3] = 0
+    s = torch.tensor([scores])
+    for count in (5, 64):
+        got = ia.beam_select(x.view(1, 2, V).cuda(), s.cuda(), count=count)
+        # either beam's candidates are one number in 64 bits
+        k = np.repeat([0, 1], V)
+        value = np.repeat(np.asarray(scores), V)
+        order = np.lexsort((np.tile(np.arange(V), 2), -x.double().numpy().ravel(), k, -value))[:count]
+        assert got[1][0].tolist() == (order // V).tolist()
+        assert got[2][0].tolist() == (order % V).tolist()
