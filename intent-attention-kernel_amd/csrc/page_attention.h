@@ -450,14 +450,22 @@ __device__ __forceinline__ float soften_scaled(f4 (&s)[PAGES], const float (&km)
 }
 
 // V's scales differ by pages: weights carry 2^(vl - E), the accumulators stand for 2^E of themselves, and E follows
-// the largest of a step's, with room below it so that it moves seldom.
-constexpr int V_ROOM = 8;
+// the largest of a step's, with room below it so that it moves seldom. It starts at NO_POWER, where there are no sums,
+// and falls no more than V_FALL below the highest it has been: the accumulators of 2^31 tokens are below 2^62, and a fall
+// multiplies them.
+constexpr int V_ROOM = 8, V_FALL = 60, NO_POWER = 1000;
 template <int PAGES> __device__ __forceinline__ int value_power(const float (&vl)[PAGES], int E) {
   float most = vl[0];
 #pragma unroll
   for (int p = 1; p < PAGES; ++p) most = fmaxf(most, vl[p]);
   const int e = __builtin_amdgcn_readfirstlane((int)floorf(most));
   return e <= (int)NO_SCALE || (e <= E && e >= E - V_ROOM) ? E : e;
+}
+// Where E may move to, and `top`, its highest so far (at first -NO_POWER).
+__device__ __forceinline__ int moved_power(int to, int E, int& top) {
+  if (E == NO_POWER) return to;
+  top = top < E ? E : top;
+  return to < top - V_FALL ? top - V_FALL : to;
 }
 
 // Infinite and NaN values of V: a weight of zero would make them NaN where a row does not see them, so

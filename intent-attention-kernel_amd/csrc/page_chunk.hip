@@ -53,6 +53,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   __shared__ u4 none[WIDE ? PAGE : 1];                           // zeros
   __shared__ Ahead<KIND> table;
   __shared__ int special;                                        // bit 0: V has infinite or NaN values, bit 1: a sum has
+  __shared__ int power_top;                                      // the highest E so far, which is seldom asked for
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const MxPart part = a.shares ? mx_shared_part<4, true>(a) : mx_fixed_part(a);
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
     put_ahead<D, KIND>(table, b, k, page_tag<KIND>(b, page, raw_tag(b, page)));
   };
   if (w < 2) look_up(64 * w + lane);
-  if (threadIdx.x == 0) special = 0;
+  if (threadIdx.x == 0) { special = 0; power_top = -NO_POWER; }
   __syncthreads();
   int ahead = 0, ahead_tag = 0;
   auto look_ahead = [&](int k) __attribute__((always_inline)) {  // k: entry of the walk, a multiple of 4
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   f4 acc[RT][D / 16], l[RT], s[RT][4];
   float lsum[RT], m[RT];
   h8 pb[RT][2], pl[RT][QF32 ? 2 : 1];
-  int E = 0;
+  int E = NO_POWER;
   const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
   auto wide = [&](uint32_t tags, int p) { return WIDE && wide_tag((int)((tags >> (8 * p)) & 0xFFu)); };
 
@@ -190,8 +191,11 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
       const float km[4] = {kms[0], kms[1], kms[2], kms[3]};
       float vl[4] = {vls[0], vls[1], vls[2], vls[3]}, out[4];
       raise_scaled<D, 4, RT>(s, km, mult, m, lsum, acc);
-      const int to = value_power<4>(vl, E);
+      int to = value_power<4>(vl, E);
       if (to != E) {                                             // uniform
+        int highest = __builtin_amdgcn_readfirstlane(power_top);  // every wave's moves are the same, and leave the same here
+        to = moved_power(to, E, highest);
+        power_top = highest;
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
   // A token that a row does not see weighs nothing, and 0 times infinity is NaN: a walk that ends in such
   // sums is made again with zeros in their place.
   for (int walk = 0; walk < 2; ++walk) {
-    E = 0;
+    E = NO_POWER;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       m[t] = M_NONE;
@@ -325,7 +329,7 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
     if (special == 0) break;                                     // uniform
     __syncthreads();
     careful = true;
-    if (threadIdx.x == 0) special = 0;
+    if (threadIdx.x == 0) { special = 0; power_top = -NO_POWER; }
     if (w < 2) look_up(64 * w + lane);
     __syncthreads();
   }

@@ -1,0 +1,53 @@
+"""Chunk attention over pages whose V scales lie anywhere in float32's range, and infinite values with weights that vanish beside others',
+for the kernel of few query rows and that of many."""
+import numpy as np
+import pytest
+
+from test_gpu_chunk_attention import Case, _t
+
+pytestmark = pytest.mark.gpu
+
+# B, L, Hq, Hkv, W: few rows a KV head, and so many rows of so many KV heads that these go to the kernel of many
+FEW, MANY = (2, 3, 8, 2, 40), (32, 64, 16, 4, 24)
+TAG = {"int8": 1, "fp8": 3, "int4": 4, "int4r": 5}
+
+
+def _case(seed, shape, D, mix, q_dtype="float32", **kw):
+    B, L, Hq, Hkv, W = shape
+    return Case(seed, B, L, Hq, Hkv, D, W, mix, q_dtype, scale_dtype=np.float32, **kw)
+
+
+def _upload(s, *names):
+    for n in names or tuple(s.host):
+        setattr(s.pools, n, _t(s.host[n]))
+
+
+def _check_some(s, out_dtype=None, some=2, **kw):
+    """The first sequences' outputs alone (the oracle is slow)."""
+    import torch
+    got = s.run(out_dtype=None if out_dtype is None else getattr(torch, out_dtype), **kw)
+    keep = {n: getattr(s, n) for n in ("table", "counts", "valid", "q_lens", "q")}
+    for n, x in keep.items():
+        setattr(s, n, None if x is None else x[:some])
+    s.check(got[:some], **{n: x for n, x in kw.items() if n in ("causal", "sm_scale")})
+    for n, x in keep.items():
+        setattr(s, n, x)
+    return got
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("mix", ["bytes", "all"])
+def test_a_step_of_tiny_pages_between_ordinary_ones(mix, shape, D):
+    s = _case(1, shape, D, mix, "float16")
+    W = shape[-1]
+    s.tags[:] = s.rng.choice([1, 3] if mix == "bytes" else [1, 3, 4, 5], s.NP)
+    for first, size in ((8, 1e-37), (16, 1e-25)):
+        for n, x in s.host.items():
+            if n.startswith("v_") and n.endswith("_scale"):
+                x[s.table[:, :, first:first + 8]] = size
+    _upload(s)
+    assert W >= 24
+    for out in ("float32", "bfloat16"):
+        _check_some(s, out)
+    _check_some(s, "float32", splits=2)
