@@ -37,7 +37,7 @@ template <int D, bool QF32> struct RowWave {
   h8 qhi[D / 32], qlo[QF32 ? D / 32 : 1];
   f4 acc[D / 16];          // lane: row c, channels (D/16)(4g + q) + mb
   float mult, m, l;        // of row c: what makes base-2 scores; running maximum; this lane's part of the sum
-  int E;                   // the values' sum is acc 2^E (uniform)
+  int E, top;              // the values' sum is acc 2^E (uniform); the highest E that there were sums at
   int seen, least;         // tokens that row c sees, and that all rows do
   int g;
 };
@@ -52,8 +52,9 @@ template <int D, bool QF32> __device__ __forceinline__ f4 row_scores(const RowWa
 }
 
 // Weights of a page of base-2 scores `s`; `first`: its first token's number; PERM: score r of lane group g is
-// token 4r + g (else 4g + r); e: the exponent of V's scale.
-template <bool PERM, int D, bool QF32>
+// token 4r + g (else 4g + r); e: the exponent of V's scale, which E follows (as in the other kernel: moved_power; NO_POWER: not
+// this page's). FIXED: all pages' exponents are 0.
+template <bool PERM, bool FIXED, int D, bool QF32>
 __device__ __forceinline__ f4 row_weights(RowWave<D, QF32>& w, f4 s, int first, int e) {
   if (first + PS > w.least) {                                    // uniform
 #pragma unroll
@@ -61,17 +62,22 @@ __device__ __forceinline__ f4 row_weights(RowWave<D, QF32>& w, f4 s, int first, 
       if (first + (PERM ? 4 * r + w.g : 4 * w.g + r) >= w.seen) s[r] = -__builtin_inff();
   }
   const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-  const bool move = e > w.E || e < w.E - V_ROOM;                 // uniform
+  const bool move = !FIXED && e != NO_POWER && (e > w.E || e < w.E - V_ROOM);   // uniform
   if (__builtin_amdgcn_ballot_w64(top > w.m + RESCALE_SLACK) || move) {
     const float pm = xmax16_32(top), mn = pm > w.m + RESCALE_SLACK ? pm : w.m, alpha = __builtin_amdgcn_exp2f(w.m - mn);
-    const int by = move ? w.E - e : 0;
     w.l *= alpha;
 #pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb)
+    for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] *= alpha;
+    if (move) {
+      const bool none = __builtin_amdgcn_ballot_w64(w.m != M_NONE) == 0;   // no sums yet
+      const int to = moved_power(e, none ? NO_POWER : w.E, w.top);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) w.acc[mb][q] = __builtin_ldexpf(w.acc[mb][q] * alpha, by);
+      for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w.acc[mb][q] = __builtin_ldexpf(w.acc[mb][q], w.E - to);
+      w.E = to;
+    }
     w.m = mn;
-    w.E = move ? e : w.E;
   }
   const float base = P_SHIFT - w.m;
 #pragma unroll
@@ -80,9 +86,12 @@ __device__ __forceinline__ f4 row_weights(RowWave<D, QF32>& w, f4 s, int first, 
   return s;
 }
 
-// A V scale: its exponent, and what multiplies the weights of a page once E has followed it. One that is not finite
-// makes every sum NaN (0 in a careful walk).
-__device__ __forceinline__ int value_exponent(float v) { return fabsf(v) < __builtin_inff() ? scale_exp(fabsf(v)) : 0; }
+// A V scale: its exponent (NO_POWER for one that adds nothing to E), and what multiplies the weights of a page once E has
+// followed it. One that is not finite makes every sum NaN (0 in a careful walk).
+__device__ __forceinline__ int value_exponent(float v) {
+  const float a = fabsf(v);
+  return a > 0.f && a < __builtin_inff() ? (int)(f2u(a) >> 23) - 127 : NO_POWER;
+}
 __device__ __forceinline__ float value_factor(float v, int E, bool careful) {
   return careful && !(fabsf(v) < __builtin_inff()) ? 0.f : __builtin_ldexpf(v, -E);
 }
@@ -110,7 +119,7 @@ __device__ __forceinline__ uint32_t clean_pair(uint32_t x) {
   return x & (((e & 0xFFFFu) == 0x7C00u ? 0u : 0xFFFFu) | (e >> 16 == 0x7C00u ? 0u : 0xFFFF0000u));
 }
 
-template <int D, bool QF32>
+template <bool FIXED, int D, bool QF32>
 __device__ __forceinline__ void row_page_fp16(RowWave<D, QF32>& w, const Raw16<D>& r, int first, bool careful, u4* kt, int c, int g) {
   u4 k[D / 32];
 #pragma unroll
@@ -119,7 +128,7 @@ __device__ __forceinline__ void row_page_fp16(RowWave<D, QF32>& w, const Raw16<D
   h8 ka[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) ka[i] = __builtin_bit_cast(h8, k[i]);
-  const f4 p = row_weights<true>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * w.mult, first, 0);
+  const f4 p = row_weights<true, FIXED>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * w.mult, first, 0);
   uint32_t v[4][D / 32];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -128,7 +137,7 @@ __device__ __forceinline__ void row_page_fp16(RowWave<D, QF32>& w, const Raw16<D
   h4 va[D / 16];
 #pragma unroll
   for (int mb = 0; mb < D / 16; ++mb) va[mb] = rows_to_a<D>(v, mb);
-  row_values(w, va, p, value_factor(1.f, w.E, false));
+  row_values(w, va, p, FIXED ? 1.f : value_factor(1.f, w.E, false));
 }
 
 template <int TAG, int D, bool QF32>
@@ -148,7 +157,7 @@ __device__ __forceinline__ void row_page_byte(RowWave<D, QF32>& w, const Raw8<D>
     four(kw[2 * i + 1], o[2], o[3]);
     ka[i] = make_h8(o[0], o[1], o[2], o[3]);
   }
-  const f4 p = row_weights<true>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * (w.mult * ks), first, value_exponent(vs));
+  const f4 p = row_weights<true, false>(w, row_scores(w, ka, f4{0.f, 0.f, 0.f, 0.f}) * (w.mult * ks), first, value_exponent(vs));
   uint32_t v[4][D / 32];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -196,7 +205,7 @@ __device__ __forceinline__ void row_page_int4r(RowWave<D, QF32>& w, const Raw8<D
 #pragma unroll
   for (int q = 0; q < 4; ++q) s[q] = __builtin_fmaf(sb[q], ks0, sr[q] * k16) * w.mult;
   const bool fine = fabsf(vs0) + fabsf(vs1) < __builtin_inff();
-  const f4 p = row_weights<true>(w, s, first, fine ? scale_exp(most) : 0);
+  const f4 p = row_weights<true, false>(w, s, first, fine ? scale_exp(most) : 0);
   const float f0 = careful && !fine ? 0.f : __builtin_ldexpf(vs0, -w.E), f1 = careful && !fine ? 0.f : __builtin_ldexpf(v16, -w.E);
   h4 va[D / 16], vr[D / 16];
 #pragma unroll
@@ -247,7 +256,7 @@ __device__ __forceinline__ void row_page_int4(RowWave<D, QF32>& w, const RawScal
     s = __builtin_amdgcn_mfma_f32_16x16x32_f16(make_h8(l[0], l[1], l[2], l[3]), qhi[i], s, 0, 0, 0);
     if constexpr (QF32) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qlo[i], s, 0, 0, 0);
   }
-  const f4 p = row_weights<false>(w, s * __builtin_ldexpf(w.mult, ek), first, ev);
+  const f4 p = row_weights<false, false>(w, s * __builtin_ldexpf(w.mult, ek), first, ev);
   h4 va[D / 16], vl[D / 16];
   const uint32_t y01l = pack_lo(r.v[0], r.v[1]), y01h = pack_hi(r.v[0], r.v[1]);
   const uint32_t y23l = pack_lo(r.v[2], r.v[3]), y23h = pack_hi(r.v[2], r.v[3]);
@@ -326,6 +335,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
     w.m = M_NONE;
     w.l = 0.f;
     w.E = 0;
+    w.top = -NO_POWER;
 #pragma unroll
     for (int mb = 0; mb < D / 16; ++mb) w.acc[mb] = f4{0.f, 0.f, 0.f, 0.f};
     for (int block = w0; block < w1; block += 64) {
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
           [&](Raw16<D>& r, int p) {
             load16<D>(r, page_at<_Float16>(a.k_fp16, p, PS * D * 2), page_at<_Float16>(a.v_fp16, p, PS * D * 2), c, g);
           },
-          [&](const Raw16<D>& r, int idx) { row_page_fp16(w, r, first(idx), careful, kt, c, g); });
+          [&](const Raw16<D>& r, int idx) { row_page_fp16<KIND == PAGES_F16>(w, r, first(idx), careful, kt, c, g); });
       if constexpr (KIND != PAGES_F16) {
         class_loop<IAK_RING_BYTE, Raw8<D>>(
             mask(IAK_TAG_FP8), x.id,

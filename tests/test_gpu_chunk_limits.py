@@ -51,3 +51,36 @@ def test_a_step_of_tiny_pages_between_ordinary_ones(mix, shape, D):
     for out in ("float32", "bfloat16"):
         _check_some(s, out)
     _check_some(s, "float32", splits=2)
+
+
+def _largest(s, kind):
+    """|V| of no page is larger."""
+    code = {"int8": 128, "fp8": 448, "int4": 8, "int4r": 16}[kind]
+    return code * float(np.abs(s.host[f"v_{kind}_scale"]).max())
+
+
+def _far(power, kind, shape, D, **kw):
+    """V's scales times 2^power: outputs times 2^power."""
+    import torch
+    s = _case(abs(power), shape, D, kind)
+    s.tags[:] = TAG[kind]
+    near = _check_some(s, "float32", **kw)
+    size = _largest(s, kind)
+    n = f"v_{kind}_scale"
+    s.host[n] = np.ldexp(s.host[n], power).astype(np.float32)
+    assert (s.host[n] >= 2.0 ** -126).all()
+    _upload(s, n)
+    got = s.run(out_dtype=torch.float32, **kw).double()
+    assert torch.isfinite(got).all()
+    # A weight's exponent has the logarithm of the scale: below 2^7, so rounded by 2^-18 and off by 2^-17 of its own, and three
+    # roundings of sums of that size: 3 2^-17 in all, times ln 2, in either run; the rest is as small as a weight's two parts.
+    error = float((torch.ldexp(got, torch.tensor(-power, device=got.device)) - near.double()).abs().amax())
+    assert error <= 2 * 3 * 2.0 ** -17 * size, (error, size)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("power", [-110, -70, 70])
+def test_scales_far_from_one(power, kind, shape, D):
+    _far(power, kind, shape, D)
