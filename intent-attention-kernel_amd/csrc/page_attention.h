@@ -54,8 +54,15 @@ __device__ __forceinline__ void split_scale(float s, float& mult, float& rest) {
   mult = plain ? a : 1.f;
   rest = plain ? (s < 0.f ? -1.f : 1.f) : s;
 }
-// The power of two of a scale whose codes go as values.
-__device__ __forceinline__ float power_of(float s) { return s > 0.f && s < __builtin_inff() ? pow2f(scale_exp(s)) : 1.f; }
+// The exponent of a positive finite scale whose codes go as values, which go relative to that power of two; 0 for others.
+// (2^126 is the largest whose inverse is normal.)
+__device__ __forceinline__ int power_exponent(float s) {
+  const int e = (int)(f2u(s) >> 23) - 127;
+  return !(s > 0.f && s < __builtin_inff()) ? 0 : e < -126 ? -126 : e > 126 ? 126 : e;
+}
+__device__ __forceinline__ float power_of(float s) { return pow2f(power_exponent(s)); }
+// |s|, 0 for what is not finite.
+__device__ __forceinline__ float finite_size(float s) { return fabsf(s) < __builtin_inff() ? fabsf(s) : 0.f; }
 
 // The look-up in three steps, each of which waits for the one before: the entry, its page's tag, the
 // scales. (A step's loads can be under way while others work.)

@@ -205,7 +205,7 @@ __device__ __forceinline__ void row_page_int4r(RowWave<D, QF32>& w, const Raw8<D
 #pragma unroll
   for (int q = 0; q < 4; ++q) s[q] = __builtin_fmaf(sb[q], ks0, sr[q] * k16) * w.mult;
   const bool fine = fabsf(vs0) + fabsf(vs1) < __builtin_inff();
-  const f4 p = row_weights<true, false>(w, s, first, fine ? scale_exp(most) : 0);
+  const f4 p = row_weights<true, false>(w, s, first, fine ? value_exponent(most) : NO_POWER);
   const float f0 = careful && !fine ? 0.f : __builtin_ldexpf(vs0, -w.E), f1 = careful && !fine ? 0.f : __builtin_ldexpf(v16, -w.E);
   h4 va[D / 16], vr[D / 16];
 #pragma unroll
@@ -231,12 +231,12 @@ __device__ __forceinline__ void row_page_int4(RowWave<D, QF32>& w, const RawScal
   const Raw4<D>& r = rs.x;
   const uint32_t mg = magic_i4();
   // powers of two that bring the page's scales near 1; K's lanes differ by g, V's by c / 4
-  auto largest = [](float x) { x = fabsf(x); return x < __builtin_inff() ? x : 0.f; };
-  const int ek = scale_exp(xmax16_32(largest(rs.ks)));
-  float most = largest(rs.vs);
+  const int ek = power_exponent(xmax16_32(finite_size(rs.ks)));
+  float most = finite_size(rs.vs);
   most = fmaxf(most, __shfl_xor(most, 4, 64));
   most = fmaxf(most, __shfl_xor(most, 8, 64));
-  const int ev = __builtin_amdgcn_readfirstlane(scale_exp(most));
+  const int ev = __builtin_amdgcn_readfirstlane(power_exponent(most));
+  const bool some = __builtin_amdgcn_readfirstlane((int)(most > 0.f)) != 0;   // else zeros, infinities and NaN alone
   const ScaleParts ks = scale_parts(__builtin_ldexpf(rs.ks, -ek));
   const bool fine = fabsf(rs.vs) < __builtin_inff();
   const ScaleParts vs = scale_parts(careful && !fine ? 0.f : __builtin_ldexpf(rs.vs, -ev));
@@ -256,7 +256,7 @@ __device__ __forceinline__ void row_page_int4(RowWave<D, QF32>& w, const RawScal
     s = __builtin_amdgcn_mfma_f32_16x16x32_f16(make_h8(l[0], l[1], l[2], l[3]), qhi[i], s, 0, 0, 0);
     if constexpr (QF32) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qlo[i], s, 0, 0, 0);
   }
-  const f4 p = row_weights<false, false>(w, s * __builtin_ldexpf(w.mult, ek), first, ev);
+  const f4 p = row_weights<false, false>(w, s * __builtin_ldexpf(w.mult, ek), first, some ? ev : NO_POWER);
   h4 va[D / 16], vl[D / 16];
   const uint32_t y01l = pack_lo(r.v[0], r.v[1]), y01h = pack_hi(r.v[0], r.v[1]);
   const uint32_t y23l = pack_lo(r.v[2], r.v[3]), y23h = pack_hi(r.v[2], r.v[3]);
@@ -269,7 +269,7 @@ __device__ __forceinline__ void row_page_int4(RowWave<D, QF32>& w, const RawScal
     va[d] = make_h4(h[0], h[1]);
     vl[d] = make_h4(l[0], l[1]);
   }
-  const float factor = __builtin_ldexpf(1.f, ev - w.E);
+  const float factor = some ? __builtin_ldexpf(1.f, ev - w.E) : 0.f;
   row_values(w, va, p, factor);
   const h4 pb = half4(p * factor);
 #pragma unroll

@@ -84,3 +84,27 @@ def _far(power, kind, shape, D, **kw):
 @pytest.mark.parametrize("power", [-110, -70, 70])
 def test_scales_far_from_one(power, kind, shape, D):
     _far(power, kind, shape, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["int4", "int4r"])
+@pytest.mark.parametrize("power", [-110, -70, 70])
+def test_scales_far_from_one_of_4_bits(power, kind, shape, D):
+    _far(power, kind, shape, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["int4", "int4r"])
+@pytest.mark.parametrize("power", [-70, 70])
+def test_key_scales_far_from_one_of_4_bits(power, kind, shape, D):
+    import torch
+    s = _case(abs(power), shape, D, kind)
+    s.tags[:] = TAG[kind]
+    near = s.run(out_dtype=torch.float32, sm_scale=0.125)
+    n = f"k_{kind}_scale"
+    s.host[n] = np.ldexp(s.host[n], power).astype(np.float32)
+    _upload(s, n)
+    got = s.run(out_dtype=torch.float32, sm_scale=float(np.ldexp(0.125, -power)))
+    assert torch.equal(got, near)                                # powers of two cancel
