@@ -82,7 +82,7 @@ template <int KIND> __device__ __forceinline__ PageTag page_tag(const PageAttn& 
   return PageTag{known ? page : -1, known ? tag : (int)IAK_TAG_SKIP};
 }
 
-// A page's scales: INT8 and FP8 the ones, 4 bits the largest.
+// A page's scales: INT8 and FP8 the ones, 4 bits the largest finite one.
 template <int D, int KIND> __device__ __forceinline__ void page_scales(const PageAttn& a, const PageTag& x, float& k, float& v) {
   k = v = 1.f;
   if (KIND == PAGES_F16 || x.id < 0) return;
@@ -97,12 +97,12 @@ template <int D, int KIND> __device__ __forceinline__ void page_scales(const Pag
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t at = p * groups + (i < groups ? i : 0);
-      k = fmaxf(k, fabsf(load_scale(a.k_int4_scale, at, a.int4_sd)));
-      v = fmaxf(v, fabsf(load_scale(a.v_int4_scale, at, a.int4_sd)));
+      k = fmaxf(k, finite_size(load_scale(a.k_int4_scale, at, a.int4_sd)));
+      v = fmaxf(v, finite_size(load_scale(a.v_int4_scale, at, a.int4_sd)));
     }
   } else if (KIND == PAGES_ALL && x.tag == IAK_TAG_INT4_RESIDUAL) {
-    k = fmaxf(fabsf(a.k_int4r_scale[2 * p]), fabsf(a.k_int4r_scale[2 * p + 1]));
-    v = fmaxf(fabsf(a.v_int4r_scale[2 * p]), fabsf(a.v_int4r_scale[2 * p + 1]));
+    k = fmaxf(finite_size(a.k_int4r_scale[2 * p]), finite_size(a.k_int4r_scale[2 * p + 1]));
+    v = fmaxf(finite_size(a.v_int4r_scale[2 * p]), finite_size(a.v_int4r_scale[2 * p + 1]));
   }
 }
 

@@ -108,3 +108,16 @@ def test_key_scales_far_from_one_of_4_bits(power, kind, shape, D):
     _upload(s, n)
     got = s.run(out_dtype=torch.float32, sm_scale=float(np.ldexp(0.125, -power)))
     assert torch.equal(got, near)                                # powers of two cancel
+
+
+@pytest.mark.parametrize("shape", [FEW, MANY])
+def test_infinite_scales_beside_large_ones(shape):
+    """Of a page's groups one is infinite, the others past float16's range."""
+    s = _case(6, shape, 128, "int4")
+    s.tags[:] = TAG["int4"]
+    page = s.table[:, :, 2].ravel()
+    s.host["v_int4_scale"][page] = 1e5
+    s.host["v_int4_scale"][page, 1] = -np.inf
+    _upload(s)
+    _check_some(s, "float32")
+    _check_some(s, "float32", splits=2)
