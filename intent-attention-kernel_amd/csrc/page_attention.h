@@ -475,6 +475,14 @@ __device__ __forceinline__ int moved_power(int to, int E, int& top) {
   return to < top - V_FALL ? top - V_FALL : to;
 }
 
+// A row's sums as they meet others': acc 2^E may be past float32's range where its quotient by the weights' sum l is
+// not. Past 2^SUM_POWER the row's maximum is therefore counted higher by this power of two, and l (to some 2^-10, so that 2^10
+// parts add up) and acc lower.
+constexpr int SUM_POWER = 60;
+__device__ __forceinline__ int sum_power(float l, int E) {
+  return E > SUM_POWER && l > 0.f && l < __builtin_inff() ? (int)(f2u(l) >> 23) - 127 + 11 : 0;
+}
+
 // Infinite and NaN values of V: a weight of zero would make them NaN where a row does not see them, so
 // the tiles have zeros in their place. A page that has any leaves beside its tile, for every 16-byte chunk, which
 // of its 8 values are positive (bits 0 .. 7) and which negative (8 .. 15; NaN: both), and whoever sees one

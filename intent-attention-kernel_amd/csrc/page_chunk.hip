@@ -380,13 +380,14 @@ __global__ __launch_bounds__(64 * NW, 2) void page_chunk_kernel(const PageAttn a
     if (r >= all) continue;
     if (z.parted) {
       const int64_t slot = (int64_t)part.part * BM + (w * RT + t) * 16 + c;
-      if (g == 0) { z.ws_m[slot] = m[t]; z.ws_l[slot] = sum; }
+      const int by = SCALED ? sum_power(sum, E) : 0;
+      if (g == 0) { z.ws_m[slot] = m[t] + (float)by; z.ws_l[slot] = __builtin_ldexpf(sum, -by); }
 #pragma unroll
       for (int mb = 0; mb < D / 16; ++mb) {
         f4 x = acc[t][mb];
         if constexpr (SCALED) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = __builtin_ldexpf(x[q], E);
+          for (int q = 0; q < 4; ++q) x[q] = __builtin_ldexpf(x[q], E - by);
         }
         *reinterpret_cast<f4*>(z.ws_acc + slot * D + 16 * mb + 4 * g) = x;
       }

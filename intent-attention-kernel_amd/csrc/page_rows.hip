@@ -440,8 +440,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
 
   // the waves' sums meet in LDS (rows c, 16-byte units turned by c against bank conflicts)
   const float sum = xsum16_32(w.l);
+  const int by = KIND == PAGES_F16 ? 0 : sum_power(sum, w.E);
   __syncthreads();
-  if (g == 0) { part_m[wv][c] = w.m; part_l[wv][c] = sum; }
+  if (g == 0) { part_m[wv][c] = w.m + (float)by; part_l[wv][c] = __builtin_ldexpf(sum, -by); }
   f4* sums = reinterpret_cast<f4*>(lds[wv]);
 #pragma unroll
   for (int q = 0; q < 4; ++q)
@@ -449,7 +450,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
     for (int u = 0; u < D / 64; ++u) {
       f4 x;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = __builtin_ldexpf(w.acc[4 * u + k][q], w.E);
+      for (int k = 0; k < 4; ++k) x[k] = __builtin_ldexpf(w.acc[4 * u + k][q], w.E - by);
       sums[c * (D / 4) + (((D / 64) * (4 * g + q) + u) ^ c)] = x;
     }
   __syncthreads();

@@ -121,3 +121,12 @@ def test_infinite_scales_beside_large_ones(shape):
     _upload(s)
     _check_some(s, "float32")
     _check_some(s, "float32", splits=2)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["int8", "fp8", "int4", "int4r"])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_values_next_to_the_ranges_end(splits, kind, shape, D):
+    """The weighted sums, before they are divided, are past float32's range."""
+    _far({"int8": 124, "fp8": 122, "int4": 124, "int4r": 124}[kind], kind, shape, D, splits=splits)
