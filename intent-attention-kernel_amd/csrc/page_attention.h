@@ -46,13 +46,14 @@ struct PageEntry { int id, tag; float km, kf, vl, vf; };
 
 __device__ __forceinline__ bool wide_tag(int tag) { return tag == IAK_TAG_INT4 || tag == IAK_TAG_INT4_RESIDUAL; }
 
-// A page scale in a positive normal multiplier and what is left for the codes: its sign, or itself
-// where it is zero or not finite.
+// A page scale in a positive normal multiplier whose inverse is normal, and what is left for the codes: its sign (from
+// 2^126 on four times that), or itself where it is zero or not finite.
 __device__ __forceinline__ void split_scale(float s, float& mult, float& rest) {
   const float a = fabsf(s);
+  const bool most = a >= 8.50705917e37f;
   const bool plain = a >= 1.17549435e-38f && a < __builtin_inff();
-  mult = plain ? a : 1.f;
-  rest = plain ? (s < 0.f ? -1.f : 1.f) : s;
+  mult = plain ? (most ? 0.25f : 1.f) * a : 1.f;
+  rest = plain ? __builtin_copysignf(most ? 4.f : 1.f, s) : s;
 }
 // The exponent of a positive finite scale whose codes go as values, which go relative to that power of two; 0 for others.
 // (2^126 is the largest whose inverse is normal.)

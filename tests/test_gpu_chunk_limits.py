@@ -130,3 +130,20 @@ def test_infinite_scales_beside_large_ones(shape):
 def test_values_next_to_the_ranges_end(splits, kind, shape, D):
     """The weighted sums, before they are divided, are past float32's range."""
     _far({"int8": 124, "fp8": 122, "int4": 124, "int4r": 124}[kind], kind, shape, D, splits=splits)
+
+
+@pytest.mark.parametrize("shape", [FEW, MANY])
+def test_scales_at_the_ranges_end(shape):
+    """Scales from 2^126 on, whose inverse is below the normal range."""
+    import torch
+    s = _case(5, shape, 64, "int8")
+    s.tags[:] = 1
+    s.host["v_int8"] = (s.host["v_int8"] % 3 - 1).astype(np.int8)
+    s.host["v_int8_scale"][:] = np.float32(1.5 * 2.0 ** -7)
+    _upload(s)
+    near = _check_some(s, "float32")
+    for size in (1.5 * 2.0 ** 127, 1.5 * 2.0 ** 126):
+        s.host["v_int8_scale"][:] = np.float32(size)
+        _upload(s, "v_int8_scale")
+        got = s.run(out_dtype=torch.float32).double() / size
+        assert float((got - near.double() / (1.5 * 2.0 ** -7)).abs().amax()) <= 2 * 3 * 2.0 ** -17
