@@ -157,6 +157,16 @@ template <int UNIT, bool RUNS, typename A> __device__ __forceinline__ MxPart mx_
   return p;
 }
 
+// Parts' sums add up as x weight. Where a weight has vanished, what x has of infinite and NaN values stays as it is: no
+// weight is zero, and the product would be NaN.
+__device__ __forceinline__ void part_weight(f4& x, float& weight) {
+  if (weight == 0.f) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = fabsf(x[q]) < __builtin_inff() ? 0.f : x[q];
+    weight = 1.f;
+  }
+}
+
 // N query values at element offset `at`, wherever they lie: 16-byte loads, all under way at once.
 template <typename T, int N> __device__ __forceinline__ void mx_load(const T* p, float (&x)[N]) {
   T t[N];

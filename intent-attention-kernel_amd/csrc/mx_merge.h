@@ -69,8 +69,9 @@ __global__ __launch_bounds__(256) void mx_merge_kernel(const A a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (s0 + k * PARTS >= parts) break;
-      const float wgt = __builtin_amdgcn_exp2f(m4[k] - M);
+      float wgt = __builtin_amdgcn_exp2f(m4[k] - M);
       L += wgt * l4[k];
+      part_weight(o4[k], wgt);
       o += o4[k] * wgt;
     }
   }

@@ -463,9 +463,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES, (row_waves_per_simd<QF32, KIND>()))
     f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < ROW_WAVES; ++x) {
-      const float wgt = __builtin_amdgcn_exp2f(part_m[x][cr] - M);
+      float wgt = __builtin_amdgcn_exp2f(part_m[x][cr] - M);
       L += wgt * part_l[x][cr];
-      o += reinterpret_cast<const f4*>(lds[x])[cr * (D / 4) + (u ^ cr)] * wgt;
+      f4 own = reinterpret_cast<const f4*>(lds[x])[cr * (D / 4) + (u ^ cr)];
+      part_weight(own, wgt);
+      o += own * wgt;
     }
     if (a.parted) {
       const int64_t slot = (int64_t)part.part * 16 + cr;

@@ -147,3 +147,38 @@ def test_scales_at_the_ranges_end(shape):
         _upload(s, "v_int8_scale")
         got = s.run(out_dtype=torch.float32).double() / size
         assert float((got - near.double() / (1.5 * 2.0 ** -7)).abs().amax()) <= 2 * 3 * 2.0 ** -17
+
+
+@pytest.mark.parametrize("shape", [FEW, MANY])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("mix", ["fp16", "all"])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_infinite_values_with_weights_that_vanish(value, mix, splits, shape):
+    """Scores of some pages are hundreds above those of the page with the infinity, in other waves' and other parts' shares."""
+    s = _case(3, shape, 64, mix, ragged=False)
+    B, L, Hq, Hkv, W = shape
+    s.q[:] = 0
+    s.q[..., 0] = 8.0
+    s.tags[:] = 0
+    s.host["k_fp16"][:] = 0
+    for e in range(W):
+        s.host["k_fp16"][s.table[:, :, e].ravel(), :, 0] = 400.0 if e >= W // 2 else -400.0
+    at = s.table[:, :, 1].ravel()
+    s.host["v_fp16"][at, 3, 5] = value
+    _upload(s, "k_fp16", "v_fp16")
+    _check_some(s, splits=splits)
+    _check_some(s, causal=False, splits=splits)
+    # and the other way round: what is infinite outweighs the rest
+    s.host["k_fp16"][:, :, 0] *= -1
+    _upload(s, "k_fp16")
+    _check_some(s, splits=splits)
+
+
+@pytest.mark.parametrize("shape,mix", [(FEW, "all"), (MANY, "all"), (MANY, "fp16")])
+def test_runs_repeat_themselves(shape, mix):
+    import torch
+    s = _case(4, shape, 128, mix, "float16")
+    for splits in (0, 3):
+        first = s.run(splits=splits)
+        for _ in range(3):
+            assert torch.equal(first, s.run(splits=splits))
