@@ -746,7 +746,8 @@ iak_status iak_copy_pages(const iak_copy_pages_args* args, void* stream);
  *       keeps tokens that got no room from being appended over older ones.
  *   iak_fork_sequences  sequence seqs[i], which has no tokens, becomes a copy of parents[i]:
  *       it shares the parent's pages (refs + 1), except that a last page which is not full
- *       is copied (every array) into a free page, chosen in the order of (i, row).
+ *       is copied (every array) into a free page, chosen in the order of (i, row). (Without arrays
+ *       such a page holds what it held: the caller's to fill, as iak_reorder_sequences' too.)
  * Grow and fork do all of it or nothing and say which in missing[0]: 0 done; n > 0: n more
  * free pages would be needed; -1: an index outside [0, num_seqs) or listed twice among
  * seqs, a negative new_tokens, a row that would be longer than its table, a shared last page
@@ -760,10 +761,10 @@ typedef struct {
   int32_t* refs;
   int32_t count;
   const int32_t* seqs;
-  const int32_t* parents;      /* fork */
+  const int32_t* parents;      /* fork, reorder */
   const int32_t* new_tokens;   /* grow; free: may be NULL */
-  int32_t* missing;            /* grow, fork */
-  int32_t num_arrays;          /* grow, fork */
+  int32_t* missing;            /* grow, fork, reorder */
+  int32_t num_arrays;          /* grow, fork, reorder */
   iak_page_array arrays[IAK_MAX_PAGE_ARRAYS];
   int32_t* granted;            /* grow; may be NULL */
 } iak_sequences_args;

@@ -27,7 +27,10 @@ Which page goes where is a function of the arguments alone.
 ``grow_sequences``, ``fork_sequences`` and ``reorder_sequences`` do all of a call or nothing of it, and return an
 int32 [1] device tensor: 0 done, n > 0: n free pages too few, -1: refused (an index out
 of range or listed twice, a negative count, a row that would be longer than its table, a
-last page to be copied and no pools, a forked sequence that has tokens or is itself a parent). What is queued behind a call that was not done runs
+growing row whose last page others hold too and no pools, a forked sequence that has tokens or is itself a parent).
+``fork_sequences`` and ``reorder_sequences`` hand pages out without ``pools`` too: a last page that they would
+copy holds then what it held before, and is the caller's to copy (``copy_pages``) before anything reads it: where the
+pools are more tensors than a call takes. What is queued behind a call that was not done runs
 all the same: ``grow_sequences(..., granted=lens)`` leaves in ``lens`` how many tokens each
 sequence got room for, 0 then, and ``append_mxfp4_tokens(..., q_lens=lens)`` writes no more.
 Without it read the answer before tokens are appended, for they would land on older ones.
@@ -179,8 +182,8 @@ def fork_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs: t
                    missing: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Sequence ``children[i]``, which has no tokens, becomes a copy of ``parents[i]``: it shares
     the parent's pages (refs + 1), except that a last page which is not full is copied, in
-    every tensor of ``pools``, to a free page. All or nothing; returns ``missing``
-    (module docstring). A parent may be listed many times."""
+    every tensor of ``pools``, to a free page (without ``pools`` that page is the caller's to fill). All or
+    nothing; returns ``missing`` (module docstring). A parent may be listed many times."""
     a, dev, children, tensors = _sequences("page sharing", page_table, valid_tokens, refs, children, pools)
     parents = _indices("parents", parents, dev, children.shape[0])
     a.parents = parents.data_ptr()
@@ -197,8 +200,8 @@ def reorder_sequences(page_table: torch.Tensor, valid_tokens: torch.Tensor, refs
     stays as it is). Full pages are shared, and rows let go of the pages they had. A last page that
     is not full stays with one owner, the parent if it stays itself or is not among ``seqs``, else its first
     child in the call; the others get copies of it, in every tensor of ``pools``, in pages that were free
-    before the call (the lowest ids first, in the order of i, row). All or nothing; returns
-    ``missing`` (module docstring)."""
+    before the call (the lowest ids first, in the order of i, row; without ``pools`` those pages are the caller's to
+    fill). All or nothing; returns ``missing`` (module docstring)."""
     a, dev, seqs, tensors = _sequences("page sharing", page_table, valid_tokens, refs, seqs, pools)
     parents = _indices("parents", parents, dev, seqs.shape[0])
     a.parents = parents.data_ptr()
