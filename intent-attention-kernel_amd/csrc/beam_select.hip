@@ -485,13 +485,17 @@ __global__ __launch_bounds__(MERGE_THREADS) void beam_merge_kernel(const BeamArg
       if (winners & (winners - 1)) {
         const uint32_t low = wave_most(wins ? (uint32_t)best : 0);
         wins = wins && (uint32_t)best == low;
-        // the numbers of the first beam among them, of these the largest logit, of these the lowest number
+        winners = __builtin_amdgcn_ballot_w64(wins);
         const uint32_t number = index[place], order = logit[place];
-        const uint32_t past = (~wave_most(wins ? ~number : 0) / V + 1) * V;
-        wins = wins && number < past;
-        const uint32_t top = wave_most(wins ? order : 0);
-        wins = wins && order == top;
-        const uint32_t first = wave_most(wins ? ~number : 0);
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)order, __builtin_ctzll(winners));
+        if (__builtin_amdgcn_ballot_w64(wins && order != other)) {
+          // of the first beam among them the largest logit
+          const uint32_t past = (~wave_most(wins ? ~number : 0) / V + 1) * V;
+          wins = wins && number < past;
+          const uint32_t top = wave_most(wins ? order : 0);
+          wins = wins && order == top;
+        }
+        const uint32_t first = wave_most(wins ? ~number : 0);     // then the lowest number
         wins = wins && ~number == first;
         winners = __builtin_amdgcn_ballot_w64(wins);
       }
