@@ -46,12 +46,9 @@ def test_next_numbers_above_many_equal(low):
 LARGE = [89.0, 599.0, 601.0, 709.0, 711.0, 800.0, 1000.0, 1400.0, 1419.6, 2000.0, 2839.0, 2848.0, 2900.0, 28391.0, 60000.0, 1e9]
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("top", LARGE)
+@pytest.mark.parametrize("top,dtype", [(top, t) for t in TYPES for top in LARGE if t != "float16" or top <= 65504])
 def test_one_large_logit(top, dtype):
     import torch
-    if dtype == "float16" and top > 65504:
-        pytest.skip("past float16's range")
     for V in (1000, 32000):
         x = torch.zeros(3, V)
         x[0, V // 3] = top
