@@ -276,25 +276,25 @@ def build_workload(name: str, device: torch.device, seed: int = 1234, chunk_page
 
 # HBM bytes per decode-kernel launch (reads + writes) from rocprofv3 FETCH_SIZE /
 # WRITE_SIZE runs of this bench, each scaled by what the counter reads for a
-# 1 GiB device copy (--calibrate-copy): profiles/paged_decode_cfg3_hbm_traffic.txt and
-# profiles/paged_decode_cfg4_kernel_stats.txt. Each figure holds the digest of the
+# 1 GiB device copy (--calibrate-copy): profiles/paged_decode_cfg3_hbm_traffic.txt, and for
+# cfg4's writes profiles/paged_decode_cfg4_kernel_stats.txt. Each figure holds the digest of the
 # decode kernel's sources it was measured on (kernel_source_digest); a build whose
 # sources differ reports traffic null (stale) until the counters are run again.
 MEASURED_TRAFFIC = {
     "cfg3": {"bytes": 2_105_403_125 + 5_054_464, "src": "ceb1d54afdea7918",
              "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
     "cfg4": {"bytes": 189_798_155 + 2_129_920, "src": "ceb1d54afdea7918",
-             "source": "profiles/paged_decode_cfg4_kernel_stats.txt"},
+             "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
     # the same decodes reading 32-byte page descriptors (--page-descriptors) or
     # 32-byte entry records (--entry-records)
     "cfg3-desc": {"bytes": 2_079_880_235 + 5_054_464, "src": "ceb1d54afdea7918",
                   "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
     "cfg4-desc": {"bytes": 182_753_856 + 2_129_920, "src": "ceb1d54afdea7918",
-                  "source": "profiles/paged_decode_cfg4_kernel_stats.txt"},
+                  "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
     "cfg3-records": {"bytes": 2_005_617_995 + 5_054_464, "src": "ceb1d54afdea7918",
                      "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
     "cfg4-records": {"bytes": 178_933_344 + 2_129_920, "src": "ceb1d54afdea7918",
-                     "source": "profiles/paged_decode_cfg4_kernel_stats.txt"},
+                     "source": "profiles/paged_decode_cfg3_hbm_traffic.txt"},
 }
 KERNEL_SOURCES = ("paged_decode.hip", "paged_pages.h", "iak_device.h", "iak_internal.h")
 MLA_KERNEL_SOURCES = ("mla_decode.hip", "iak_device.h", "iak_internal.h")

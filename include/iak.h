@@ -822,8 +822,11 @@ iak_status iak_compact_pages(const iak_compact_pages_args* args, void* workspace
  * Tokens that a query does not see never reach it, whatever their bytes; an infinite or NaN value of one that it
  * sees reaches its channel. A query row that is not finite is NaN if it sees a token.
  * Products run on the matrix cores in float16 with float32 sums: K and V as exact codes, with
- * their scales in float32 (float32 sums of log2 in the exponential), or in two parts (4-bit pages; 21 bits); query rows
- * and weights as for iak_mx_attention. V scales of one row may differ by 2^18 without loss.
+ * their scales in float32 (float32 sums of log2 in the exponential), or in two parts (4-bit pages: 21 bits; groups
+ * whose scale is below 1/16 of the page's largest lose 2^-25 of that); query rows
+ * and weights as for iak_mx_attention (weights of 16-bit queries in 11 bits). V scales lie anywhere in float32's normal
+ * range (below it they may count as zero), those of one row may differ by 2^18 without loss. int4_group is head_dim, its
+ * half or its quarter (IAK_ENOTSUP else).
  * splits: parts a row's tokens are divided into (0: automatic). The parts meet in the workspace
  * (iak_paged_chunk_workspace bytes, 16-byte aligned, as it comes; 0: not needed); calls that share one
  * on different streams race. head_dim 64 or 128, page_size 16; pools 16-byte aligned. */

@@ -16,9 +16,9 @@
 // 64 bits, r and e^r - 1 in 32, off by some 2^-31, so that a normaliser is off by some 1e-9.
 //
 // What bounds it: the logits are read once (64 x 8 x 131,072 in bfloat16, a tenth of the beams at their end: 121 MB,
-// 24 us at a copy's rate), and an exponential to 1e-9 is 15 vector instructions a logit, 28 us of
-// the card's; the part kernel takes 53, what is left being its first group (nothing to overlap with), the list's
-// upkeep and the ends of the waves. The merge takes 8 (16 steps of some 0.1 us, and the loads and
+// 24 us at a copy's rate), with 21 vector instructions a logit (an exponential to 1e-9 is 15 of them), 37 us of
+// the card's; the part kernel takes 54, what is left being its first group (nothing to overlap with), the list's
+// upkeep and the ends of the waves. The merge takes 8.6 (16 steps of some 0.1 us, and the loads and
 // logarithms before them); two requests x 4 beams x 32,000: 7.2 + 5.9 us.
 
 #include <hip/hip_runtime.h>
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_part_kernel(const BeamAr
           else put(value<T>(x[i], j), first + j);
         }
     }
-    if (full || (count - seen) * 2 > n) {                        // at fewer new ones the search costs more than it saves: 66.6 and 63.8 us
+    if (full || (count - seen) * 2 > n) {                        // at fewer new ones the search costs more than it saves: 61.8 and 59.1 us
       if (full) {                                                // again, the list ranked as often as it is full
         count = before;
 #pragma unroll
@@ -577,9 +577,9 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 constexpr int beam_per_of(int bytes) { return bytes == 4 ? 2 : 4; }
 
 // Groups of logits a segment. 4,096 segments in all are 16 waves a CU: 64 requests x 8 beams x 131,072 in
-// bfloat16 take 71.6 us, with 2,048 segments 78.8 and with 8,192 79.6. No more lists than the merge's waves hold at
-// once, for every further round of them costs count steps: 16 beams, count 32, 131,072 tokens: 56.5 us, with
-// twice as many entries 65, with half 88 (16 beams leave few waves then).
+// bfloat16 take 59.1 us, with 2,048 segments 66.8 and with 8,192 71.5. No more lists than the merge's waves hold at
+// once, for every further round of them costs count steps: 16 beams, count 32, 131,072 tokens: 54.5 us, with
+// twice as many entries 63, with half 85 (16 beams leave few waves then).
 int beam_per(const iak_beam_select_args& a) {
   const int64_t rows = (int64_t)a.batch * a.beams, group = 512 * beam_per_of(a.dtype == IAK_DTYPE_F32 ? 4 : 2);
   const int64_t groups = (a.vocab + group - 1) / group;

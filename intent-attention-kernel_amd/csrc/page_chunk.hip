@@ -7,9 +7,9 @@
 // one barrier a step.
 //
 // What bounds it: nothing alone. 2,048 queries over 8,192 tokens of float16 pages (32 heads over 8 of 128) take
-// 254 us, 947 TFLOP/s, where a large product reaches 1,338: the matrix cores are busy 44 % of the cycles, the vector
+// 250 to 262 us from box to box, 918 to 960 TFLOP/s, where a large product reaches 1,338: the matrix cores are busy 44 % of the cycles, the vector
 // instructions (softmax) 26 %, the LDS 28 %, and two waves a SIMD do not fill each other's waits. Over 16,384
-// tokens of mixed pages, two sequences: 1.73 ms, 584 TFLOP/s; the vector instructions (codes to float16, multipliers in
+// tokens of mixed pages, two sequences: 1.74 ms, 582 TFLOP/s; the vector instructions (codes to float16, multipliers in
 // the softmax) and the wide pages' second products take as long as the first products. Tried and slower: the
 // workgroup's halves in turns, one's products beside the other's softmax (chunks of mixed pages 2,270 us for 1,700,
 // float16 ones 291 for 282), convert() behind the softmax (1,684 for 1,692: no difference).
@@ -25,8 +25,9 @@ namespace iak {
 namespace {
 
 // N operands from LDS and what each is multiplied by, the operands read ahead of their products, for
-// a read takes as long as several. (Left to itself the compiler reads each just before its own: float16 chunks as
-// above 292 us for 282; two or six ahead: 279 and 286.)
+// a read takes as long as several. (Left to itself the compiler reads each just before its own, which took 292 us
+// for 282 of float16 chunks. Two, four and six ahead: float16 chunks as above 248, 251 and 250 us, mixed ones 1,751,
+// 1,739 and 1,745: four for these.)
 template <int N, int AHEAD_OF, typename Read, typename Multiply> __device__ __forceinline__ void products(Read&& read, Multiply&& multiply) {
   constexpr int A = N < AHEAD_OF ? N : AHEAD_OF;
   h8 x[A];

@@ -15,7 +15,7 @@
 //                                      entries aside: rows become each other's copies at once
 //                reorder_apply_kernel  a workgroup per row: counts and entries where they differ (rows
 //                                      that share a beginning leave it alone), the last page. 64 x 4
-//                                      sequences of 8 rows of up to 200 entries: 8.9 + 11.4 us, two
+//                                      sequences of 8 rows of up to 200 entries: 9.7 + 11.8 us, two
 //                                      launches' latency and 14.5 MB
 //   compact      compact_count_kernel, compact_rank_kernel (which page goes where; for few pages
 //                compact_small_kernel), compact_apply_kernel (pages copied, table, counts and

@@ -289,8 +289,8 @@ template <int D> __device__ __forceinline__ void row_remember(Seen16& x, const u
 }
 
 // Waves a SIMD: what the registers hold of rings and queries in two parts. All precisions: two (16 x 4 queries
-// over up to 16,384 tokens 108 us; three spill 62 registers, 160); float16 and bytes alone: three or two (122.9 and 122.8
-// us, 78.2 and 75.5).
+// over up to 16,384 tokens 108 us; three spill 62 registers, 160). Others: three or two of float16 pages 120.9 and
+// 121.0 us (675 MB), of float16 and bytes 101.7 and 102.0.
 template <bool QF32, int KIND> constexpr int row_waves_per_simd() { return QF32 || KIND == PAGES_ALL ? 2 : 3; }
 
 template <int D, bool QF32, int KIND>

@@ -8,8 +8,9 @@
 // after the other the queries' and the keys' (with the values), for which its 8 sines and
 // cosines are the same. What bounds long calls is the bytes, short ones the launch: the prompts of 8
 // sequences (up to 4,001 tokens, 32 query heads and 8 of keys and values, 128 channels, float16) 614 MB
-// in 135 us, 4.55 TB/s; one token of 64 sequences 5.4 us. Into 4-bit blocks the 64-bit angles count: 5 x 509 tokens
-// of 16 + 4 heads x 64 in float32 14 us.
+// in 128 to 140 us, 4.4 to 4.8 TB/s (148 under the profiler, as the other figures here); one token of 64 sequences 5.3
+// us. Into 4-bit blocks the 64-bit angles count: 5 x 509 tokens
+// of 16 + 4 heads x 64 in float32 14.5 us.
 //
 // Angles reach far beyond one turn (10^6 radians), where a float32 angle is off by 0.06: turns
 // are counted in 64 bits and reduced there. For float16 pages and the queries the
@@ -29,7 +30,7 @@ namespace iak {
 namespace {
 
 constexpr int ROTARY_THREADS = 256;
-constexpr int64_t ROTARY_BUSY = 256 * 2048;   // threads that keep the card busy (prompts as below: a quarter of them 161 us, four times 152)
+constexpr int64_t ROTARY_BUSY = 256 * 2048;   // threads that keep the card busy (prompts as above 148 us, with a quarter of them 161, with four times 156)
 
 // sin(x) and cos(x) for |x| <= pi / 4, by their Taylor series: the first term left out is at most
 // 2^-25 and 2^-63.
@@ -313,8 +314,8 @@ hipError_t launch_rotary_append(const iak_rotary_append_args& c, hipStream_t str
   a.v_codes = reinterpret_cast<uint8_t*>(c.v_codes); a.v_scales = reinterpret_cast<uint8_t*>(c.v_scales);
   a.tags = c.page_tags; a.tag = c.tag;
   const int chunks = a.D / 16, heads = a.Hq + a.Hkv;
-  // 8 tokens a thread group where there are many: whole lines of a page are written at once (the prompts 145 us,
-  // one by one 151); below 16 a group could be half empty, and nothing is gained (8 tokens of 64 sequences: 17.7 us both)
+  // 8 tokens a thread group where there are many: whole lines of a page are written at once (the prompts 148 us,
+  // one by one 153); below 16 a group could be half empty, and nothing is gained (8 tokens of 64 sequences: 7.2 us both)
   a.group_bits = a.count >= 16 ? 3 : 0;
   const int64_t tokens = ((int64_t)a.count + (1 << a.group_bits) - 1) >> a.group_bits << a.group_bits;
   // a head a thread until the card has threads enough, then as few sines as keep it busy

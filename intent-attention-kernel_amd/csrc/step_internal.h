@@ -13,7 +13,7 @@
 namespace iak {
 
 constexpr int BEAM_MOST_COUNT = 64, BEAM_MOST_BEAMS = 256;
-// Workgroups (segments of the vocabulary) that a row of logits is divided into, and the workspace.
+// Waves (segments of the vocabulary) that a row of logits is divided into, and the workspace.
 int beam_segments(const iak_beam_select_args& a);
 size_t beam_workspace(const iak_beam_select_args& a);
 hipError_t launch_beam_select(const iak_beam_select_args& a, void* workspace, hipStream_t stream);

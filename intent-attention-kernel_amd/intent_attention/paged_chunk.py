@@ -124,7 +124,8 @@ def paged_chunk_attention(q: torch.Tensor, pools: PagePools, page_table: torch.T
     """Attention of the newest tokens over pages of mixed precision.
 
     q [B, L, Hq, D] or [B, Hq, D] (one token per sequence), float16, bfloat16 or float32, D = 64 or
-    128; page_table [B, Hkv, W], page_counts [B, Hkv], page_tags [NP], ``tag_map``,
+    128; of ``pools`` INT4 scales are per head, half or quarter of it (``int4_group`` D, D / 2 or D / 4; others are refused);
+    page_table [B, Hkv, W], page_counts [B, Hkv], page_tags [NP], ``tag_map``,
     ``negative_ids`` and ``map_other_tags`` as for ``paged_decode``. Token t of entry e of a row is its number
     16 e + t; a row holds min(valid_tokens, 16 page_counts) of them (``valid_tokens`` [B, Hkv],
     default: all of its pages'), the queries' own the last: query i < q_lens[b] (default L) sees
