@@ -8,7 +8,7 @@ from test_gpu_chunk_attention import Case, _t
 pytestmark = pytest.mark.gpu
 
 # B, L, Hq, Hkv, W: few rows a KV head, and so many rows of so many KV heads that these go to the kernel of many
-FEW, MANY = (2, 3, 8, 2, 40), (32, 64, 16, 4, 24)
+FEW, MANY = (2, 3, 8, 2, 40), (32, 64, 16, 4, 25)
 TAG = {"int8": 1, "fp8": 3, "int4": 4, "int4r": 5}
 
 

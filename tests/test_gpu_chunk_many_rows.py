@@ -27,7 +27,7 @@ def test_every_precision(D, mix, q_dtype):
 @pytest.mark.parametrize("mix", ["fp16", "bytes", "all"])
 @pytest.mark.parametrize("D", [64, 128])
 def test_tiles_of_128_rows(D, mix, q_dtype):
-    s = _case(8, (64, 32, 16, 4, 24), D, mix, q_dtype)
+    s = _case(8, (64, 32, 16, 4, 25), D, mix, q_dtype)
     _check_some(s)
     _check_some(s, splits=3)
 
